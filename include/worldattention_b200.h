@@ -148,6 +148,32 @@ int wa_block_sparse_forward(const wa_tensor4 *q, const wa_tensor4 *k, const wa_t
                             int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
                             int round_output_bf16, float *lse, void *stream);
 
+/* Attention of every query block over its selected key blocks, with its gradient (the training form of block_sparse_attention,
+ * block_sparse_triton.py:142-382):  S = q k^T D^-1/2,  P = softmax of S over the tokens of the listed blocks,  out = P v, and with
+ * delta = sum(dout * out)  dv = P^T dout,  dS = P (dout v^T - delta) D^-1/2,  dq = dS k,  dk = dS^T q.
+ * `Hkv` divides `H`; query head h reads key head h / (H / Hkv).  Lists: `[B, H, ceil(Lq / block_size)]` rows, `index_stride` ids apart,
+ * of which the first `num` count; an id that is listed twice counts once, one outside the key blocks not at all.  A
+ * row without a key gives out = 0, lse = -inf and takes no part in the gradients.  `block_sizes` (device int32 per key block, or null): only the
+ * first so many tokens of a block are keys.  One dtype for all tensors; sums, statistics and gradients are accumulated in float32 (bf16:
+ * probabilities and dS are rounded to bf16 as factors of the products).  No atomics on values: equal calls give equal bits.
+ * `lse` float32 `[B, H, Lq]`, natural logarithm: written by the forward call (or null), read by the backward call.
+ * bf16 with head_dim 128 and blocks of 64 or 128 tokens runs on the tensor cores; head_dim is at most 256. */
+typedef struct wa_selected_params {
+    int32_t B, H, Hkv, D, Lq, Lkv, block_size, index_stride;
+    wa_tensor4 q, k, v, out;            /* forward; backward reads all four */
+    wa_tensor4 dout, dq, dk, dv;        /* backward */
+    const int32_t *index, *num, *block_sizes;
+    float *lse;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *status_mirror;             /* page-locked host word, or null: the site code (401 to 499) of a bounded wait that ran out */
+} wa_selected_params;
+size_t wa_selected_params_size(void);
+/* 0 for arguments that the call itself refuses. */
+size_t wa_selected_workspace_bytes(const wa_selected_params *p, int backward);
+int wa_selected_forward(const wa_selected_params *p, void *stream);
+int wa_selected_backward(const wa_selected_params *p, void *stream);
+
 /* compress_kv (attention.py:64-110) on `[B, L, H, D]` views.  out_k/out_v receive
  * `[B, sum_seg rank_seg, H, D]`; `proj_*` are `[proj_rank, proj_cols]` row-major. */
 int wa_compress_kv(const wa_tensor4 *k, const wa_tensor4 *v, const wa_tensor4 *out_k,
@@ -304,6 +330,17 @@ int wa_ln_modulate(const void *x, void *out, long long rows, int C, float eps, c
 int wa_gated_residual(const void *x, const void *y, void *out, long long rows, int C, const void *gate, long long mod_stride,
                       int tokens_per_frame, void *stream);
 
+/* Rotary embedding of up to four `[B, L, heads[t], D]` tensors (one dtype, one B, L and D) whose tokens have a position of their
+ * own on each of `axes` (at most 8) axes; axis a turns the next axis_pairs[a] pairs of a head by the angles whose (cos, sin) stand in row
+ * positions[b, l, a] of `table` (device float32 `[table_rows, sum of axis_pairs, 2]`).  causal_rope_apply (causal_model.py:34-62) is the case
+ * of one grid for all samples.  A pair is two neighbouring channels (interleaved) or channels i and i + pairs; channels
+ * behind the turned ones are copied.  `inverse` turns back, which is the gradient.  A position outside the table makes the
+ * pairs of its axis NaN.  `positions`: device int32, its last axis contiguous, strides in elements (0 between samples: one
+ * set for all).  `out` may be `x`. */
+int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const int32_t *heads, int tensors, int B, int L, int D,
+                  const int32_t *positions, int64_t position_stride_b, int64_t position_stride_l, const int32_t *axis_pairs, int axes,
+                  const float *table, int table_rows, int interleaved, int inverse, void *stream);
+
 /* ---------------------------------------------------------------------------------------------
  * HKV retrieval -- pipeline/hkv/retrieval.py, rope.py, cache.py
  * ------------------------------------------------------------------------------------------- */
@@ -393,6 +430,20 @@ int wa_hkv_install_pages(const wa_hkv_install *p, const void *device_table, cons
  * launch runs out: pages and slots are then incomplete.  wa_compress_status reads the same code from the device. */
 int wa_hkv_install_pages_mirrored(const wa_hkv_install *p, const void *device_table, const float *rotations, int32_t *status_mirror,
                                   void *stream);
+
+/* Moves of cache pages in place (no counterpart in the reference, whose window rolls through clones, causal_model.py:331-360):
+ * page dst[i] becomes what page src[i] was, or zeros where src[i] is -1, for all n moves at once (a page may be read by several
+ * moves and be overwritten by another), in every tensor.  A page is `page_tokens` token rows; the last page of a tensor may be
+ * shorter, and a move between a whole and a shorter page moves the rows that both have.  All arrays are host arrays; they are
+ * read before the function returns.  WA_ERR_ARG: a page that some tensor does not have, or that is the destination of two moves.
+ * The tensors must not share memory. */
+typedef struct wa_page_tensor {
+    void *ptr;                          /* token 0 of sample 0 */
+    int64_t batch_stride, token_stride; /* bytes */
+    int64_t tokens, row_bytes;          /* of a sample; contiguous bytes of a token */
+    int32_t batch, page_tokens;
+} wa_page_tensor;
+int wa_hkv_move_pages(const wa_page_tensor *tensors, int n_tensors, const int32_t *dst, const int32_t *src, int n, void *stream);
 
 /* Promotion of cold pages (the `.to(device)` of cache.py:229-231 for chunks that live in host memory): one
  * asynchronous host-to-device copy per record of the HOST array `host_records` (src = page-locked host memory,

@@ -52,6 +52,18 @@ class PageCopy(C.Structure):
                 ("dst_stride", C.c_int64), ("n_tokens", C.c_int32), ("rot", C.c_int32)]
 
 
+class SelectedParams(C.Structure):  # wa_selected_params
+    _fields_ = [(n, C.c_int32) for n in ("B", "H", "Hkv", "D", "Lq", "Lkv", "block_size", "index_stride")] + \
+               [(n, Tensor4) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + \
+               [(n, C.c_void_p) for n in ("index", "num", "block_sizes", "lse", "workspace")] + \
+               [("workspace_bytes", C.c_size_t), ("status_mirror", C.c_void_p)]
+
+
+class PageTensor(C.Structure):      # wa_page_tensor
+    _fields_ = [("ptr", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64), ("tokens", C.c_int64), ("row_bytes", C.c_int64),
+                ("batch", C.c_int32), ("page_tokens", C.c_int32)]
+
+
 class HkvInstall(C.Structure):      # wa_hkv_install
     _fields_ = [(n, C.c_int32) for n in ("pages", "tensors", "segments", "B", "H", "D", "frame", "block_size", "proj_rank", "proj_cols",
                                          "n_temporal")] + \
@@ -96,6 +108,12 @@ SIGNATURES = {
     "wa_gated_residual": [_vp, _vp, _vp, _i64, _i, _vp, _i64, _i, _vp],
     "wa_qk_norm_rope": [_T4P, _T4P, _i, _i, _i, _i, _vp, _i, _f, _vp, _i, _i, _i, _i, _vp],
     "wa_qk_norm_rope_at": [_T4P, _T4P, _i, _i, _i, _i, _vp, _i, _f, _vp, _i, _vp, _i, _i, _vp],
+    "wa_selected_params_size": [],
+    "wa_selected_workspace_bytes": [_vp, _i],
+    "wa_selected_forward": [_vp, _vp],
+    "wa_selected_backward": [_vp, _vp],
+    "wa_axial_rope": [_T4P, _T4P, _vp, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _i, _vp, _i, _i, _i, _vp],
+    "wa_hkv_move_pages": [_vp, _i, _vp, _vp, _i, _vp],
     "wa_hkv_page_centroids": [_T4P, _i, _i, _i, _i, _vp, _i, _vp, _i, _i, _i, _vp, _vp],
     "wa_hkv_score_topk": [_vp, _vp, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp],
     "wa_hkv_score_topk_layers": [_vp, _vp, _i, _i, _i, _i, C.c_longlong, _f, _i, _vp, _vp, _vp, _vp],
@@ -110,7 +128,7 @@ SIGNATURES = {
     "wa_hkv_clear_rows": [_vp, _i, _i, _i, _i, _vp],
     "wa_hkv_gather_pages": [_vp, _i, _i, _i, _i, _i, _vp, _i, _vp],
 }
-_RESTYPES = {"wa_last_error": C.c_char_p, "wa_hkv_install_table_bytes": C.c_size_t, "wa_hsa_workspace_bytes": C.c_size_t, "wa_hsa_params_size": C.c_size_t, "wa_kv_append_workspace_bytes": C.c_size_t,
+_RESTYPES = {"wa_last_error": C.c_char_p, "wa_hkv_install_table_bytes": C.c_size_t, "wa_hsa_workspace_bytes": C.c_size_t, "wa_hsa_params_size": C.c_size_t, "wa_selected_params_size": C.c_size_t, "wa_selected_workspace_bytes": C.c_size_t, "wa_kv_append_workspace_bytes": C.c_size_t,
              "wa_launch_count": C.c_ulonglong}
 
 _lib: Optional[C.CDLL] = None

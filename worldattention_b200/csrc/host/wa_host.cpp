@@ -19,6 +19,7 @@
 #include <list>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../../include/worldattention_b200.h"
 
@@ -37,6 +38,11 @@ decltype(&wa_kv_append_workspace_bytes) f_append_bytes;
 decltype(&wa_kv_append_compress) f_append;
 decltype(&wa_ln_modulate) f_ln;
 decltype(&wa_gated_residual) f_residual;
+decltype(&wa_axial_rope) f_axial;
+decltype(&wa_hkv_move_pages) f_move_pages;
+decltype(&wa_selected_workspace_bytes) f_selected_bytes;
+decltype(&wa_selected_forward) f_selected_forward;
+decltype(&wa_selected_backward) f_selected_backward;
 PyObject *py_out_of_memory = nullptr;                                 // torch.OutOfMemoryError
 PyObject *py_status_word = nullptr, *py_raise_if_failed = nullptr;   // _lib.status_word(index) -> address, _lib.raise_if_failed(index)
 
@@ -490,6 +496,246 @@ PyObject *gated_residual(PyObject *const *a, Py_ssize_t n) {
     return THPVariable_Wrap(std::move(out));
 }
 
+// A sequence's elements, for the time of a call
+struct Sequence {
+    PyObject *o;
+    Sequence(PyObject *seq, const char *what) : o(PySequence_Fast(seq, what)) {
+        if (!o) throw PyFailure();
+    }
+    ~Sequence() { Py_DECREF(o); }
+    Sequence(const Sequence &) = delete;
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(o); }
+    PyObject *operator[](Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(o, i); }
+};
+int small_integer(PyObject *o, const char *what) {
+    const long long v = integer(o);
+    if (v < INT_MIN || v > INT_MAX) fail(PyExc_ValueError, std::string(what) + " must fit 32 bits");
+    return (int)v;
+}
+
+// ---- attention over selected blocks (hsa/selected.py): q [B, Lq, H, D], k, v [B, Lkv, Hkv, D], index [B, H, Nq, S], num [B, H, Nq], block, block_sizes|None ----
+struct SelectedCall {
+    wa_selected_params p{};
+    Tensor keep[9];
+    c10::Device dev{c10::kCUDA, 0};
+    bool nothing = false;              // no query or no key: no launch
+
+    explicit SelectedCall(PyObject *const *a) {
+        bool seen = false;
+        const char *names[] = {"q", "k", "v", "index", "num"};
+        for (int i = 0; i < 5; ++i) require_cuda(tensor(a[i], names[i]), dev, seen);
+        const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &v = THPVariable_Unpack(a[2]);
+        const Tensor &index = THPVariable_Unpack(a[3]), &num = THPVariable_Unpack(a[4]);
+        const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
+        if (sizes) require_cuda(*sizes, dev, seen);
+        if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4) fail(PyExc_ValueError, "q, k and v must be [B, L, H, D] tensors");
+        const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), D = q.size(3), Lkv = k.size(1), Hkv = k.size(2);
+        for (const int64_t x : {B, Lq, H, D, Lkv, Hkv})
+            if (x > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
+        if (k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D)
+            fail(PyExc_ValueError, "k and v must be [B, Lkv, Hkv, D] with q's B and D, got q " + shape_of(q) + ", k " + shape_of(k) + ", v " + shape_of(v));
+        if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) fail(PyExc_ValueError, "q, k and v must have one dtype");
+        dtype_code(q.scalar_type());
+        if (H == 0 || Hkv == 0 || H % Hkv) fail(PyExc_ValueError, std::to_string(H) + " query heads do not divide among " + std::to_string(Hkv) + " key heads");
+        const int block = small_integer(a[5], "block_size");
+        if (block <= 0) fail(PyExc_ValueError, "block_size must be positive, got " + std::to_string(block));
+        const int64_t nq = (Lq + block - 1) / block, nkv = (Lkv + block - 1) / block;
+        if (index.dim() != 4 || index.size(0) != B || index.size(1) != H || index.size(2) != nq || num.dim() != 3 || num.size(0) != B || num.size(1) != H || num.size(2) != nq)
+            fail(PyExc_ValueError, "index must be [B, H, Nq, ids] and num [B, H, Nq] with Nq = " + std::to_string(nq) + " query blocks, got " + shape_of(index) + " and " + shape_of(num));
+        if (index.scalar_type() != at::kInt || num.scalar_type() != at::kInt) fail(PyExc_ValueError, "index and num must be int32");
+        if (sizes && (sizes->dim() != 1 || sizes->size(0) != nkv || sizes->scalar_type() != at::kInt))
+            fail(PyExc_ValueError, "block_sizes must be int32 [" + std::to_string(nkv) + "], got shape " + shape_of(*sizes));
+        nothing = B == 0 || Lq == 0 || Lkv == 0 || D == 0 || index.size(3) == 0;
+        p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.D = (int)D; p.Lq = (int)Lq; p.Lkv = (int)Lkv; p.block_size = block;
+        if (index.size(3) > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
+        p.index_stride = (int)index.size(3);
+        if (nothing) return;
+        p.q = view4(q, keep[0]); p.k = view4(k, keep[1]); p.v = view4(v, keep[2]);
+        keep[3] = index.contiguous(); keep[4] = num.contiguous();
+        p.index = keep[3].data_ptr<int32_t>(); p.num = keep[4].data_ptr<int32_t>();
+        if (sizes) {
+            keep[5] = sizes->contiguous();
+            p.block_sizes = keep[5].data_ptr<int32_t>();
+        }
+        p.status_mirror = const_cast<int32_t *>(reinterpret_cast<volatile int32_t *>(status_word(dev.index())));
+    }
+    // the workspace lives in the caching allocator for the time of the call: recycled in the stream's order, a graph's own while one is captured
+    Tensor workspace_for(bool backward) {
+        const size_t bytes = f_selected_bytes(&p, backward);
+        if (bytes == 0) check(backward ? f_selected_backward(&p, nullptr) : f_selected_forward(&p, nullptr));      // says why
+        Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = bytes;
+        return ws;
+    }
+};
+wa_tensor4 result4(const Tensor &t) { return wa_tensor4{t.data_ptr(), dtype_code(t.scalar_type()), 0, t.stride(0), t.stride(1), t.stride(2)}; }
+
+// -> (out [B, Lq, H, D], lse float32 [B, H, Lq])
+PyObject *selected_forward(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 7);
+    SelectedCall c(a);
+    raise_if_failed(c.dev.index());
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Tensor &q = THPVariable_Unpack(a[0]);
+    const auto options = q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+    Tensor out, lse;
+    if (c.nothing) {
+        out = at::zeros(q.sizes(), q.options().requires_grad(false));
+        lse = at::full({c.p.B, c.p.H, c.p.Lq}, -INFINITY, q.options().dtype(at::kFloat).requires_grad(false));
+    } else {
+        out = at::empty(q.sizes(), options);
+        lse = at::empty({c.p.B, c.p.H, c.p.Lq}, options.dtype(at::kFloat));
+        c.p.out = result4(out);
+        c.p.lse = lse.data_ptr<float>();
+        const Tensor ws = c.workspace_for(false);
+        check(f_selected_forward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+    }
+    PyObject *pair = PyTuple_New(2);
+    if (!pair) throw PyFailure();
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+    return pair;
+}
+
+// ..., out, lse, dout -> (dq, dk, dv)
+PyObject *selected_backward(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 10);
+    SelectedCall c(a);
+    raise_if_failed(c.dev.index());
+    bool seen = true;
+    const char *names[] = {"out", "lse", "dout"};
+    for (int i = 0; i < 3; ++i) require_cuda(tensor(a[7 + i], names[i]), c.dev, seen);
+    c10::cuda::CUDAGuard guard(c.dev);
+    const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &out = THPVariable_Unpack(a[7]), &dout = THPVariable_Unpack(a[9]);
+    if (out.sizes() != q.sizes() || dout.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || dout.scalar_type() != q.scalar_type())
+        fail(PyExc_ValueError, "out and dout must have q's shape and dtype");
+    Tensor grad[3];
+    for (int i = 0; i < 3; ++i) {
+        const Tensor &x = i == 0 ? q : k;
+        const auto options = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+        grad[i] = c.nothing ? at::zeros(x.sizes(), x.options().requires_grad(false)) : at::empty(x.sizes(), options);
+    }
+    if (!c.nothing) {
+        c.p.out = view4(out, c.keep[6]);
+        c.p.dout = view4(dout, c.keep[7]);
+        c.keep[8] = THPVariable_Unpack(a[8]).contiguous();
+        if (c.keep[8].scalar_type() != at::kFloat || c.keep[8].numel() != (int64_t)c.p.B * c.p.H * c.p.Lq) fail(PyExc_ValueError, "lse must be float32 [B, H, Lq]");
+        c.p.lse = c.keep[8].data_ptr<float>();
+        c.p.dq = result4(grad[0]); c.p.dk = result4(grad[1]); c.p.dv = result4(grad[2]);
+        const Tensor ws = c.workspace_for(true);
+        check(f_selected_backward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+    }
+    PyObject *three = PyTuple_New(3);
+    if (!three) throw PyFailure();
+    for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(three, i, THPVariable_Wrap(std::move(grad[i])));
+    return three;
+}
+
+// ---- axial_rope(tensors, positions int32 [L, A] or [B, L, A], table float32 [rows, pairs, 2], pairs of each axis, interleaved, inverse) -> list of tensors ----
+PyObject *axial_rope(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 6);
+    const Sequence xs(a[0], "expected a tensor or a tuple of tensors"), axes(a[3], "axes must be a sequence of integers");
+    const Tensor &pos0 = tensor(a[1], "positions"), &table0 = tensor(a[2], "table");
+    constexpr int MOST = 4;
+    if (xs.size() < 1 || xs.size() > MOST) fail(PyExc_ValueError, "expected one to four tensors, got " + std::to_string(xs.size()));
+    c10::Device dev(c10::kCUDA, 0);
+    bool seen = false;
+    for (Py_ssize_t t = 0; t < xs.size(); ++t) require_cuda(tensor(xs[t], "every element"), dev, seen);
+    require_cuda(pos0, dev, seen);
+    require_cuda(table0, dev, seen);
+    const Tensor &x0 = THPVariable_Unpack(xs[0]);
+    if (x0.dim() != 4) fail(PyExc_ValueError, "expected [B, L, H, D] tensors, got shape " + shape_of(x0));
+    const int64_t B = x0.size(0), L = x0.size(1), D = x0.size(3);
+    if (B > INT_MAX || L > INT_MAX || D > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
+    const int64_t A = axes.size();
+    int pairs[8];
+    if (A < 1 || A > 8) fail(PyExc_ValueError, "expected one to eight axes, got " + std::to_string(A));
+    int64_t sum = 0;
+    for (int64_t i = 0; i < A; ++i) sum += pairs[i] = small_integer(axes[i], "axes");
+    if (table0.dim() != 3 || table0.size(2) != 2 || table0.size(0) < 1 || table0.scalar_type() != at::kFloat)
+        fail(PyExc_ValueError, "table must be float32 [rows, pairs, 2], got shape " + shape_of(table0));
+    if (table0.size(1) != sum || 2 * sum > D)
+        fail(PyExc_ValueError, "the axes turn " + std::to_string(sum) + " pairs, the table has " + std::to_string(table0.size(1)) + " and a head " + std::to_string(D / 2));
+    const bool shared = pos0.dim() == 2;
+    if (pos0.scalar_type() != at::kInt || (!shared && pos0.dim() != 3) || pos0.size(-1) != A || pos0.size(-2) != L || (!shared && pos0.size(0) != B))
+        fail(PyExc_ValueError, "positions must be int32 [L, axes] or [B, L, axes] for tensors of shape " + shape_of(x0) + ", got shape " + shape_of(pos0));
+    c10::cuda::CUDAGuard guard(dev);
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const Tensor pos = pos0.stride(-1) == 1 || A == 1 ? pos0 : pos0.contiguous(), table = table0.contiguous();
+    wa_tensor4 in[MOST], out[MOST];
+    int32_t heads[MOST];
+    Tensor keep[MOST], result[MOST];
+    for (Py_ssize_t t = 0; t < xs.size(); ++t) {
+        const Tensor &x = THPVariable_Unpack(xs[t]);
+        if (x.dim() != 4 || x.size(0) != B || x.size(1) != L || x.size(3) != D || x.scalar_type() != x0.scalar_type())
+            fail(PyExc_ValueError, "the tensors must share batch, length, head_dim and dtype, got shapes " + shape_of(x0) + " and " + shape_of(x));
+        if (x.size(2) > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
+        in[t] = view4(x, keep[t]);
+        result[t] = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+        out[t] = wa_tensor4{result[t].data_ptr(), in[t].dtype, 0, result[t].stride(0), result[t].stride(1), result[t].stride(2)};
+        heads[t] = (int32_t)x.size(2);
+    }
+    check(f_axial(in, out, heads, (int)xs.size(), (int)B, (int)L, (int)D, pos.data_ptr<int32_t>(), shared ? 0 : pos.stride(0), pos.stride(-2), pairs, (int)A,
+                  table.data_ptr<float>(), (int)std::min<int64_t>(table.size(0), INT_MAX), a[4] == Py_True, a[5] == Py_True, stream));
+    PyObject *list = PyList_New(xs.size());
+    if (!list) throw PyFailure();
+    for (Py_ssize_t t = 0; t < xs.size(); ++t) PyList_SET_ITEM(list, t, THPVariable_Wrap(std::move(result[t])));
+    return list;
+}
+
+// ---- move_pages(tensors [B, tokens, ...], destination pages, source pages or None, tokens of a page: one or one per tensor) ----
+PyObject *move_pages(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 4);
+    const Sequence xs(a[0], "expected a sequence of tensors"), to(a[1], "destination must be a sequence of page numbers"),
+        from(a[2], "source must be a sequence of page numbers or None");
+    if (to.size() != from.size())
+        fail(PyExc_ValueError, "destination and source must be equally long, got " + std::to_string(to.size()) + " and " + std::to_string(from.size()));
+    const bool one = PyIndex_Check(a[3]);
+    std::vector<int32_t> dst(to.size()), src(from.size());
+    for (Py_ssize_t i = 0; i < to.size(); ++i) {
+        dst[i] = small_integer(to[i], "page numbers");
+        src[i] = from[i] == Py_None ? -1 : small_integer(from[i], "page numbers");
+        if (dst[i] < 0 || (src[i] < 0 && from[i] != Py_None)) fail(PyExc_ValueError, "page numbers must not be negative");
+    }
+    std::vector<wa_page_tensor> tensors(xs.size());
+    std::vector<int> lengths;
+    if (one) {
+        lengths.assign(xs.size(), small_integer(a[3], "page_tokens"));
+    } else {
+        const Sequence each(a[3], "page_tokens must be an integer or a sequence of integers");
+        if (each.size() != xs.size()) fail(PyExc_ValueError, "page_tokens must name a length for each tensor");
+        for (Py_ssize_t t = 0; t < each.size(); ++t) lengths.push_back(small_integer(each[t], "page_tokens"));
+    }
+    c10::Device dev(c10::kCUDA, 0);
+    bool seen = false;
+    for (Py_ssize_t t = 0; t < xs.size(); ++t) {
+        const Tensor &x = tensor(xs[t], "every element");
+        require_cuda(x, dev, seen);
+        if (x.dim() < 2) fail(PyExc_ValueError, "expected [B, tokens, ...] tensors, got shape " + shape_of(x));
+        if (lengths[t] <= 0) fail(PyExc_ValueError, "page_tokens must be positive");
+        if (x.requires_grad() && at::GradMode::is_enabled())
+            fail(PyExc_RuntimeError, "pages are moved in place: a tensor that requires a gradient cannot be moved with gradients enabled");
+        int64_t row = 1;
+        for (int64_t d = x.dim() - 1; d >= 2; --d) {
+            if (x.size(d) != 1 && x.stride(d) != row) fail(PyExc_ValueError, "the axes behind the tokens must be contiguous");
+            row *= x.size(d);
+        }
+        if (x.size(0) > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
+        const int64_t size = x.element_size();
+        tensors[t] = wa_page_tensor{x.numel() ? x.data_ptr() : nullptr, x.stride(0) * size, x.stride(1) * size, x.size(1), row * size, (int32_t)x.size(0), lengths[t]};
+    }
+    if (xs.size() == 0) Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(dev);
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    check(f_move_pages(tensors.data(), (int)tensors.size(), dst.data(), src.data(), (int)dst.size(), stream));
+    for (Py_ssize_t t = 0; t < xs.size(); ++t) {        // what autograd saved of them before is no longer there
+        const Tensor &x = THPVariable_Unpack(xs[t]);
+        if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+}
+
 // ---- tensor_table(tensors) -> bytes: twelve int64 per tensor -------------------------------------
 // address, device index (-1: host), scalar type, dimensions, the first four sizes, the first four strides.  A prompt switch looks
 // at some hundred tensors; asked for one attribute at a time from Python that took longer than the copies.
@@ -568,6 +814,11 @@ PyObject *bind(PyObject *const *a, Py_ssize_t n) {
     get("wa_kv_append_compress", f_append);
     get("wa_ln_modulate", f_ln);
     get("wa_gated_residual", f_residual);
+    get("wa_axial_rope", f_axial);
+    get("wa_hkv_move_pages", f_move_pages);
+    get("wa_selected_workspace_bytes", f_selected_bytes);
+    get("wa_selected_forward", f_selected_forward);
+    get("wa_selected_backward", f_selected_backward);
     if (PyErr_Occurred()) throw PyFailure();
     PyObject *torch_module = PyImport_ImportModule("torch");
     py_out_of_memory = torch_module ? PyObject_GetAttrString(torch_module, "OutOfMemoryError") : nullptr;
@@ -600,7 +851,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 #define WA_ENTRY(name) {#name, (PyCFunction)(void (*)(void))entry<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {WA_ENTRY(bind), WA_ENTRY(hsa_forward), WA_ENTRY(run_forward), WA_ENTRY(qk_norm_rope), WA_ENTRY(append_kv), WA_ENTRY(ln_modulate),
-                         WA_ENTRY(gated_residual), WA_ENTRY(tensor_table), WA_ENTRY(read_on_stream), {nullptr, nullptr, 0, nullptr}};
+                         WA_ENTRY(gated_residual), WA_ENTRY(axial_rope), WA_ENTRY(selected_forward), WA_ENTRY(selected_backward), WA_ENTRY(move_pages), WA_ENTRY(tensor_table), WA_ENTRY(read_on_stream), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -23,6 +23,7 @@ struct GenericAttnParams {
     int out_dtype;
     long long osb, osl, osh;
     int H, Lq, Lkv, D;
+    int kv_group = 1;   // query heads that share a key head
     int q_block;    // query rows per routing block
     int q_tile;     // query rows per CTA (<= GA_QT, divides the work inside one routing block)
     int tiles_per_block;
@@ -77,8 +78,9 @@ generic_attention_kernel(GenericAttnParams p) {
     const long long meta = ((long long)b * p.H + h) * (long long)((p.Lq + p.q_block - 1) / p.q_block) + qb;
     const int n_sel = p.dense ? p.n_kv_blocks : max(0, min(p.num[meta], p.index_stride));
     const int32_t *ids = p.dense ? nullptr : p.index + meta * (long long)p.index_stride;
-    const long long kbase = (long long)b * p.k.sb + (long long)h * p.k.sh;
-    const long long vbase = (long long)b * p.v.sb + (long long)h * p.v.sh;
+    const int hk = h / p.kv_group;
+    const long long kbase = (long long)b * p.k.sb + (long long)hk * p.k.sh;
+    const long long vbase = (long long)b * p.v.sb + (long long)hk * p.v.sh;
 
     for (int s = 0; s < n_sel; ++s) {
         int id = p.dense ? s : ids[s];
@@ -315,7 +317,8 @@ split_attention_kernel(GenericAttnParams p) {
     const long long meta = ((long long)b * p.H + h) * (long long)((p.Lq + p.q_block - 1) / p.q_block) + qb;
     const int n_sel = p.dense ? p.n_kv_blocks : max(0, min(p.num[meta], p.index_stride));
     const int32_t *ids = p.dense ? nullptr : p.index + meta * (long long)p.index_stride;
-    const long long kbase = (long long)b * p.k.sb + (long long)h * p.k.sh, vbase = (long long)b * p.v.sb + (long long)h * p.v.sh;
+    const int hk = h / p.kv_group;
+    const long long kbase = (long long)b * p.k.sb + (long long)hk * p.k.sh, vbase = (long long)b * p.v.sb + (long long)hk * p.v.sh;
     const long long total = (long long)n_sel * p.kv_block;
     const bool rows_mine = 16 * rg < rows_here;
     unsigned any_key = 0;   // this warp's half had a real key
@@ -889,7 +892,7 @@ using namespace wa;
 namespace wa {
 int block_sparse_run(const wa_tensor4 *q, const wa_tensor4 *k, const wa_tensor4 *v, const wa_tensor4 *out, int B, int H, int Lq, int Lkv, int D,
                      int block_size, const int32_t *index, const int32_t *num, int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
-                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream) {
+                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream, int kv_group) {
     const char *what = "wa_block_sparse_forward";
     int rc;
     if ((rc = check_view(q, what, "q")) || (rc = check_view(k, what, "k")) || (rc = check_view(v, what, "v")) ||
@@ -908,6 +911,7 @@ int block_sparse_run(const wa_tensor4 *q, const wa_tensor4 *k, const wa_tensor4 
     p.scale = (float)(1.0 / sqrt((double)D));
     p.lse = lse;
     p.order = order; p.ahead = ahead;
+    p.kv_group = kv_group;
     return launch_generic_attention(p, B, ceil_div(Lq, block_size), stream, what);
 }
 
@@ -939,7 +943,7 @@ extern "C" int wa_block_sparse_forward(const wa_tensor4 *q, const wa_tensor4 *k,
                                        int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
                                        int round_output_bf16, float *lse, void *stream) {
     return block_sparse_run(q, k, v, out, B, H, Lq, Lkv, D, block_size, index, num, index_stride, block_sizes, round_inputs_bf16,
-                            round_output_bf16, lse, nullptr, false, (cudaStream_t)stream);
+                            round_output_bf16, lse, nullptr, false, (cudaStream_t)stream, 1);
 }
 
 extern "C" int wa_linear_branch(const wa_tensor4 *q, const wa_tensor4 *k_coarse, const wa_tensor4 *v_coarse,

@@ -1,0 +1,241 @@
+// Rotary embedding of tokens that each have a position of their own on several axes (time, height, width).
+//
+//     (a, b) -> (a cos - b sin, a sin + b cos),     cos, sin = table[positions[token, axis of the pair], pair]
+//
+// wa_qk_norm_rope (causal_rope_apply, wan/modules/causal_model.py:34-62) lays all samples of a batch out on one grid; here samples
+// of different grids, text between pictures and single tokens share a call.  The gradient is the same turn with -sin.
+// Arithmetic in float32, one rounding at the end.
+//
+// Bound: HBM, each value read once and written once.  A token is one warp's work: a lane looks the cosines and sines of its pairs up
+// once (they come from L2) and keeps them for all heads of q and k, whose 16-byte vectors are four at a time in flight.
+// Calls of few tokens spread the heads over more warps.
+#include "wa_common.cuh"
+
+namespace wa {
+
+constexpr int AR_TENSORS = 4, AR_AXES = 8, AR_WARPS = 8;
+
+struct AxialRope {
+    View4 x[AR_TENSORS];
+    void *out[AR_TENSORS];
+    long long ob[AR_TENSORS], ol[AR_TENSORS], oh[AR_TENSORS];
+    int heads[AR_TENSORS];
+    int tensors, D, pairs, axes, rows;
+    int end[AR_AXES];                 // first pair behind each axis
+    long long tokens;                 // of the batch
+    int L;
+    const int32_t *positions;
+    long long psb, psl;               // elements between samples (0: the same for all) and between tokens
+    const float2 *table;              // [rows, pairs] (cos, sin)
+    float sign;                       // of the angle
+    int groups, per_warp;             // vector form: head groups of all tensors, and how many of them a warp takes
+};
+
+// cos and sin of a pair; a position outside the table gives NaN, so that it shows in the result instead of some row's angle
+__device__ __forceinline__ float2 ar_turn(const AxialRope &p, const int32_t *pos, int pair) {
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < AR_AXES - 1; ++a) axis += a < p.axes - 1 && pair >= p.end[a];
+    const int row = __ldg(pos + axis);
+    if ((unsigned)row >= (unsigned)p.rows) return make_float2(NAN, NAN);
+    const float2 t = __ldg(p.table + (long long)row * p.pairs + pair);
+    return make_float2(t.x, t.y * p.sign);
+}
+
+template <typename T> struct ArVec;
+template <> struct ArVec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(uint4 w, float (&f)[8]) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            u[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+};
+template <> struct ArVec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(uint4 w, float (&f)[4]) {
+        f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+
+// `INTER`: a pair is two neighbouring channels, and a lane's vector holds whole pairs.  Otherwise a pair is channels i and i + pairs,
+// and a lane takes the two vectors that hold its pairs' halves.  Channels behind the turned ones are copied.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(AR_WARPS * 32)
+axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
+    using V = ArVec<T>;
+    constexpr int N = V::N, TURNS = INTER ? N / 2 : N, AT_ONCE = INTER ? 4 : 2;
+    pdl_wait();
+    const long long token = (long long)blockIdx.x * AR_WARPS + (threadIdx.x >> 5);
+    if (token >= p.tokens) return;
+    const int lane = threadIdx.x & 31;
+    const int b = (int)(token / p.L), l = (int)(token - (long long)b * p.L);
+    const int32_t *pos = p.positions + b * p.psb + l * p.psl;
+    const int per_head = (INTER ? p.D : p.pairs) / N, at_once = 32 / per_head;      // lanes a head takes, heads a warp takes at a time
+    const int sub = lane / per_head, c = lane - sub * per_head;                     // head within the group, vector within the head
+    float2 turn[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        const int pair = c * TURNS + i;
+        turn[i] = sub < at_once && pair < p.pairs ? ar_turn(p, pos, pair) : make_float2(1.f, 0.f);
+    }
+    const int first = blockIdx.y * p.per_warp, last = min(first + p.per_warp, p.groups);
+    for (int g0 = first; g0 < last; g0 += AT_ONCE) {
+        const T *src[AT_ONCE];
+        T *dst[AT_ONCE];
+        uint4 v[AT_ONCE], w[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            src[u] = nullptr;
+            int g = g0 + u, t = 0;
+            if (g < last) {
+                while (t < p.tensors - 1 && g >= (p.heads[t] + at_once - 1) / at_once) g -= (p.heads[t] + at_once - 1) / at_once, ++t;
+                const int h = g * at_once + sub;
+                if (sub < at_once && h < p.heads[t]) {
+                    src[u] = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh + c * N;
+                    dst[u] = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t] + c * N;
+                    v[u] = *reinterpret_cast<const uint4 *>(src[u]);
+                    if (!INTER) w[u] = *reinterpret_cast<const uint4 *>(src[u] + p.pairs);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (!src[u]) continue;
+            float x[N], y[N], r[N], s[N];
+            V::get(v[u], x);
+            if (INTER) {
+#pragma unroll
+                for (int i = 0; i < TURNS; ++i) {
+                    const bool turned = c * TURNS + i < p.pairs;
+                    r[2 * i] = turned ? fmaf(x[2 * i], turn[i].x, -x[2 * i + 1] * turn[i].y) : x[2 * i];
+                    r[2 * i + 1] = turned ? fmaf(x[2 * i], turn[i].y, x[2 * i + 1] * turn[i].x) : x[2 * i + 1];
+                }
+                *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
+            } else {
+                V::get(w[u], y);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    r[i] = fmaf(x[i], turn[i].x, -y[i] * turn[i].y);
+                    s[i] = fmaf(x[i], turn[i].y, y[i] * turn[i].x);
+                }
+                *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
+                *reinterpret_cast<uint4 *>(dst[u] + p.pairs) = V::put(s);
+                // channels behind the turned ones
+                for (int d = 2 * p.pairs; d < p.D - c * N; d += p.pairs)
+                    *reinterpret_cast<uint4 *>(dst[u] + d) = *reinterpret_cast<const uint4 *>(src[u] + d);
+            }
+        }
+    }
+}
+
+// Any head_dim and alignment: a thread per pair or single channel.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(256)
+axial_rope_kernel(const __grid_constant__ AxialRope p) {
+    pdl_wait();
+    const int slots = p.D - p.pairs;                 // pairs, then the channels behind them
+    long long heads = 0;
+    for (int t = 0; t < p.tensors; ++t) heads += p.heads[t];
+    const long long all = p.tokens * heads * slots;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
+        const long long row = e / slots, token = row / heads;
+        const int slot = (int)(e - row * slots), b = (int)(token / p.L), l = (int)(token - (long long)b * p.L);
+        int h = (int)(row - token * heads), t = 0;
+        while (h >= p.heads[t]) h -= p.heads[t++];
+        const T *src = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh;
+        T *dst = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t];
+        if (slot >= p.pairs) {
+            dst[slot + p.pairs] = src[slot + p.pairs];
+            continue;
+        }
+        const float2 turn = ar_turn(p, p.positions + b * p.psb + l * p.psl, slot);
+        const int i = INTER ? 2 * slot : slot, j = INTER ? i + 1 : i + p.pairs;
+        const float x = (float)src[i], y = (float)src[j];
+        dst[i] = (T)fmaf(x, turn.x, -y * turn.y);
+        dst[j] = (T)fmaf(x, turn.y, y * turn.x);
+    }
+}
+
+}  // namespace wa
+
+using namespace wa;
+
+extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const int32_t *heads, int tensors, int B, int L, int D,
+                             const int32_t *positions, int64_t position_stride_b, int64_t position_stride_l, const int32_t *axis_pairs, int axes,
+                             const float *table, int table_rows, int interleaved, int inverse, void *stream) {
+    const char *what = "wa_axial_rope";
+    WA_REQUIRE(x && out && heads && axis_pairs, WA_ERR_ARG, "%s: null pointer", what);
+    WA_REQUIRE(tensors > 0 && tensors <= AR_TENSORS, WA_ERR_UNSUPPORTED, "%s: takes 1 to %d tensors, got %d", what, AR_TENSORS, tensors);
+    WA_REQUIRE(axes > 0 && axes <= AR_AXES, WA_ERR_UNSUPPORTED, "%s: takes 1 to %d axes, got %d", what, AR_AXES, axes);
+    WA_REQUIRE(B >= 0 && L >= 0 && D > 0 && table_rows > 0, WA_ERR_ARG, "%s: sizes must be positive", what);
+    AxialRope p{};
+    p.tensors = tensors; p.D = D; p.axes = axes; p.rows = table_rows; p.L = L; p.tokens = (long long)B * L;
+    p.positions = positions; p.psb = position_stride_b; p.psl = position_stride_l;
+    p.table = (const float2 *)table; p.sign = inverse ? -1.f : 1.f;
+    long long pairs = 0;
+    for (int a = 0; a < axes; ++a) {
+        WA_REQUIRE(axis_pairs[a] >= 0, WA_ERR_ARG, "%s: an axis has %d pairs", what, axis_pairs[a]);
+        pairs += axis_pairs[a];
+        WA_REQUIRE(2 * pairs <= D, WA_ERR_ARG, "%s: more pairs than half the %d channels of a head", what, D);
+        p.end[a] = (int)pairs;
+    }
+    WA_REQUIRE(pairs > 0, WA_ERR_ARG, "%s: no axis has a pair", what);
+    p.pairs = (int)pairs;
+    const int dtype = x[0].dtype;
+    WA_REQUIRE(valid_dtype(dtype), WA_ERR_ARG, "%s: bad dtype %d", what, dtype);
+    const int n = 16 / (int)dtype_size(dtype), unit = interleaved ? D : (int)pairs;      // channels of a vector; of what a head's lanes share
+    bool vec = D % n == 0 && unit % n == 0 && unit / n <= 32;
+    if (!interleaved) vec = vec && (D - 2 * pairs) % n == 0;
+    long long all_heads = 0, groups = 0;
+    for (int t = 0; t < tensors; ++t) {
+        WA_REQUIRE(x[t].dtype == dtype && out[t].dtype == dtype, WA_ERR_ARG, "%s: the tensors must have one dtype", what);
+        WA_REQUIRE(heads[t] >= 0, WA_ERR_ARG, "%s: sizes must be positive", what);
+        WA_REQUIRE((x[t].ptr && out[t].ptr) || p.tokens * heads[t] == 0, WA_ERR_ARG, "%s: null pointer", what);
+        p.x[t] = make_view(&x[t]);
+        p.out[t] = out[t].ptr; p.ob[t] = out[t].stride_b; p.ol[t] = out[t].stride_l; p.oh[t] = out[t].stride_h;
+        p.heads[t] = heads[t];
+        all_heads += heads[t];
+        if (vec) groups += ceil_div(heads[t], 32 / (unit / n));
+        const uintptr_t places = (uintptr_t)x[t].ptr | (uintptr_t)out[t].ptr;
+        const int64_t steps = x[t].stride_b | x[t].stride_l | x[t].stride_h | out[t].stride_b | out[t].stride_l | out[t].stride_h;
+        vec = vec && places % 16 == 0 && steps % n == 0;
+    }
+    if (p.tokens == 0 || all_heads == 0) return 0;
+    WA_REQUIRE(positions && table, WA_ERR_ARG, "%s: null pointer", what);
+    WA_REQUIRE((uintptr_t)table % 8 == 0 && (uintptr_t)positions % 4 == 0, WA_ERR_ALIGN, "%s: the table must be 8-byte aligned", what);
+    cudaError_t e;
+    if (vec) {
+        const long long ctas = (p.tokens + AR_WARPS - 1) / AR_WARPS;
+        WA_REQUIRE(ctas < (1ll << 31) && groups < (1 << 20), WA_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
+        // all heads of a token by one warp once there are warps enough for the chip (the look-ups are then shared by all heads); else spread
+        p.groups = (int)groups;
+        const long long spread = (148ll * 16 + p.tokens - 1) / p.tokens;
+        p.per_warp = (int)(groups / spread);
+        if (p.per_warp < 1) p.per_warp = 1;
+        const dim3 grid((unsigned)ctas, (unsigned)ceil_div(p.groups, p.per_warp));
+        WA_REQUIRE(grid.y <= 65535, WA_ERR_UNSUPPORTED, "%s: too many heads", what);
+        const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_vec_kernel<__nv_bfloat16, true> : axial_rope_vec_kernel<__nv_bfloat16, false>)
+                                             : (interleaved ? axial_rope_vec_kernel<float, true> : axial_rope_vec_kernel<float, false>);
+        e = launch_dependent(kernel, grid, dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
+    } else {
+        const long long want = (p.tokens * all_heads * (D - pairs) + 255) / 256, most = 32ll * sm_count();
+        const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_kernel<__nv_bfloat16, true> : axial_rope_kernel<__nv_bfloat16, false>)
+                                             : (interleaved ? axial_rope_kernel<float, true> : axial_rope_kernel<float, false>);
+        e = launch_dependent(kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, (cudaStream_t)stream, p);
+    }
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
+}

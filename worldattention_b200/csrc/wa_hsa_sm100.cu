@@ -136,7 +136,11 @@ static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget exceeded");
 // 1560 tokens, cold L2: instruction cache hits 81 %, 1.33 of the cycles between issues without an instruction, special-function unit 30 %).
 // Softmax without a row maximum per tile, straight-line exponentials for full tiles and rolled epilogues made that 91 %, 0.45 and
 // 38 %, and the launch 72 -> 65 us.  The copies of K and V are not the bound: L2 hands tiles out at 18 TB/s, twice what the kernel asks for.
-template <int BLK, bool PAIR>   // routing block size: 128, or 64 (see Params::blk)
+//
+// SEL: the sparse branch alone, for wa_selected_forward: no slots, no gate tile, its result rounded once into `out` and its normalisers into
+// `lse_sparse`; lists `list_stride` ids apart, `kv_group` query heads to a key head.  No polynomial: the normaliser is an output and the
+// gradient's probabilities are made from it, so its exponentials keep the special-function unit's error.
+template <int BLK, bool PAIR, bool SEL = false>   // routing block size: 128, or 64 (see Params::blk)
 __global__ void __launch_bounds__(THREADS, 1)
 hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kc,
@@ -198,7 +202,9 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const uint32_t tmem_s = tmem, tmem_o = tmem + S_BUFS * TILE;   // S buffer b at tmem_s + b * TILE
     WA_TRACE_DECL;
     WA_TRACE(0);
-    const int lin_tiles = (p.Lc + TILE - 1) / TILE;
+    const int lin_tiles = SEL ? 0 : (p.Lc + TILE - 1) / TILE;
+    constexpr int GATE_TILES = SEL ? 0 : 1;      // an item's tiles behind those of keys
+    const int list_stride = SEL ? p.list_stride : p.Nkv;
 
     // The softmax threads keep 32 scores of two rows, the packed probabilities, the parked sparse result and the gate values in registers; the
     // other four warps need few.  Shift the register file accordingly (whole warpgroups, as the instruction requires).
@@ -224,7 +230,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 // out to have any or not -- and Q's load leaves before the answers are there (a launch begins with this chain).
                 const int item = at < p.n_items ? p.order[at] : -1;
                 int n_sel = 0, n_sel2 = 0, n_both = 0;      // PAIR: of the item's first and second query block; tiles for both
-                int qb = 0, h = 0, b = 0, first = 0, first2 = 0, other = 0;
+                int qb = 0, h = 0, hk = 0, b = 0, first = 0, first2 = 0, other = 0;
                 const int32_t *ids = p.index;
                 const uint32_t qs = jcount % Q_STAGES, q_phase = ((jcount / Q_STAGES) & 1u) ^ 1u;
                 auto load_q = [&]() {
@@ -237,15 +243,16 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 if (item >= 0) {
                     const int bh = item / p.q_items;
                     qb = item - bh * p.q_items, b = bh / p.H, h = bh - b * p.H;
+                    hk = SEL ? h / p.kv_group : h;
                     const long long row0 = PAIR ? (long long)bh * p.Nq + 2 * qb : item;      // routing row of the (first) query block
                     const bool second = PAIR && 2 * qb + 1 < p.Nq;
-                    ids += row0 * p.Nkv;
+                    ids += row0 * list_stride;
                     n_sel = p.num[row0];
                     if (second) n_sel2 = p.num[row0 + 1];
                     if (PAIR) n_both = p.both[item];
                     first = ids[0];
-                    if (BLK != TILE) first2 = ids[min(1, p.Nkv - 1)];
-                    if (second) other = ids[p.Nkv];
+                    if (BLK != TILE) first2 = ids[min(1, list_stride - 1)];
+                    if (second) other = ids[list_stride];
                     q_sent = mbar_test(&bar->q_empty[qs], q_phase);
                     if (q_sent) load_q();
                     n_sel = max(0, min(n_sel, p.Nkv));
@@ -269,13 +276,13 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     if (BLK == TILE) return make_int2(ids[t], 0);
                     if (!PAIR) return make_int2(ids[2 * t], ids[min(2 * t + 1, n_sel - 1)]);
                     if (t < n_both) return make_int2(ids[2 * t], ids[2 * t + 1]);
-                    return make_int2(t + n_both < n_sel ? ids[t + n_both] : INT_MAX, t + n_both < n_sel2 ? ids[p.Nkv + t + n_both] : INT_MAX);
+                    return make_int2(t + n_both < n_sel ? ids[t + n_both] : INT_MAX, t + n_both < n_sel2 ? ids[list_stride + t + n_both] : INT_MAX);
                 };
                 auto block_row = [&](int id) { return PAIR && id == INT_MAX ? p.Nkv : max(0, min(id, p.Nkv - 1)); };
                 int2 next = make_int2(first, n_sel > 1 ? first2 : first);
                 if (PAIR && n_both == 0) next = make_int2(n_sel > 0 ? first : INT_MAX, n_sel2 > 0 ? other : INT_MAX);
                 const int n_kv = n_st + lin_tiles;
-                WA_STATS_ITEM(n_kv + 1);
+                WA_STATS_ITEM(n_kv + GATE_TILES);
 
                 if (!q_sent) {
                     ok = mbar_wait(&bar->q_empty[qs], q_phase, abort_flag, sink, 12);
@@ -293,8 +300,8 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     mbar_expect_tx(&bar->v_full[vs], TILE_BYTES);
                     if (tv < n_st) {
                         const int id = bar->blocks[tv & 7].x, id2 = bar->blocks[tv & 7].y;
-                        tma_load_5d(vdst, &tm_v, &bar->v_full[vs], 0, id * BLK, 0, h, b);      // both halves of the channels
-                        if (BLK == HALF) tma_load_5d(vdst + HALF_BYTES, &tm_v, &bar->v_full[vs], 0, id2 * HALF, 0, h, b);
+                        tma_load_5d(vdst, &tm_v, &bar->v_full[vs], 0, id * BLK, 0, hk, b);      // both halves of the channels
+                        if (BLK == HALF) tma_load_5d(vdst + HALF_BYTES, &tm_v, &bar->v_full[vs], 0, id2 * HALF, 0, hk, b);
                     } else {
                         tma_load_5d(vdst, &tm_vc, &bar->v_full[vs], 0, (tv - n_st) * TILE, 0, h, b);
                     }
@@ -302,7 +309,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 };
                 auto v_free = [&]() { return mbar_test(&bar->v_empty[vcount % V_STAGES], ((vcount / V_STAGES) & 1u) ^ 1u); };
 
-                for (int t = 0; t <= n_kv && ok; ++t) {
+                for (int t = 0; t < n_kv + GATE_TILES && ok; ++t) {
                     const uint32_t ks = kcount % KV_STAGES, kpar = ((kcount / KV_STAGES) & 1u) ^ 1u;
                     // wait for the K stage; V tiles whose K tile is out already go out as their stages come back
                     if (!mbar_test(&bar->k_empty[ks], kpar)) {
@@ -348,12 +355,12 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     mbar_expect_tx(&bar->k_full[ks], TILE_BYTES);
                     if (t < n_st) {
                         if (BLK == TILE) {
-                            tma_load_5d(kdst, &tm_k, &bar->k_full[ks], 0, id * TILE, 0, h, b);
+                            tma_load_5d(kdst, &tm_k, &bar->k_full[ks], 0, id * TILE, 0, hk, b);
                         } else {   // 64-row boxes: rows 0..63 of each half-tile from the first block, 64..127 from the second
-                            tma_load_5d(kdst, &tm_k, &bar->k_full[ks], 0, id * HALF, 0, h, b);
-                            tma_load_5d(kdst + HALF_BYTES / 2, &tm_k, &bar->k_full[ks], 0, id2 * HALF, 0, h, b);
-                            tma_load_5d(kdst + HALF_BYTES, &tm_k, &bar->k_full[ks], 0, id * HALF, 1, h, b);
-                            tma_load_5d(kdst + HALF_BYTES + HALF_BYTES / 2, &tm_k, &bar->k_full[ks], 0, id2 * HALF, 1, h, b);
+                            tma_load_5d(kdst, &tm_k, &bar->k_full[ks], 0, id * HALF, 0, hk, b);
+                            tma_load_5d(kdst + HALF_BYTES / 2, &tm_k, &bar->k_full[ks], 0, id2 * HALF, 0, hk, b);
+                            tma_load_5d(kdst + HALF_BYTES, &tm_k, &bar->k_full[ks], 0, id * HALF, 1, hk, b);
+                            tma_load_5d(kdst + HALF_BYTES + HALF_BYTES / 2, &tm_k, &bar->k_full[ks], 0, id2 * HALF, 1, hk, b);
                         }
                     } else if (t < n_kv) {
                         const int c = (t - n_st) * TILE;
@@ -438,7 +445,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             ok = __all_sync(0xffffffffu, mbar_wait(&bar->q_full[qs], (jcount / Q_STAGES) & 1u, abort_flag, sink, 3));
             if (!ok) break;
             const uint64_t qd = smem_desc(smem_u32(q_s + qs * TILE_BYTES), 16, 1024);
-            for (int t = 0; t <= n_kv && ok; ++t) ok = issue_qk(qd, t == n_kv);
+            for (int t = 0; t < n_kv + GATE_TILES && ok; ++t) ok = issue_qk(qd, t == n_kv);
             ++jcount;
         }
     } else if (warp == 11) {
@@ -502,7 +509,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 __syncwarp();
                 WA_TRACE(7);
             }
-            ++g;   // the gate tile
+            g += GATE_TILES;
             ++jcount;
         }
     } else if (warp == 10) {
@@ -588,7 +595,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             float ls_spA = 0.f, ls_spB = 0.f;   // the sparse branch's log-sum-exp (packed records write both in one store)
 
 #pragma unroll 1   // one copy of each kind of tile: two gain 1.2 us of 92 on repeated inputs and lose 2.4 of 102 on changing ones
-            for (int phase = 0; phase < 2 && ok; ++phase) {
+            for (int phase = 0; phase < (SEL ? 1 : 2) && ok; ++phase) {
                 const int t0 = phase == 0 ? 0 : n_sel, t1 = phase == 0 ? n_sel : n_kv;
                 float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;   // l: this thread's columns only
                 bool started = false;      // every row of the warp has a reference point that should do for the next tile
@@ -716,7 +723,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                             for (int c = 0; c < halves; ++c) {
                                 tmem_wait_ld16(lo);
                                 TMEM_LDQ16(s_addr + 64 * c + 32, hi);
-                                exp32(lo, pk1, std::true_type());
+                                exp32(lo, pk1, std::bool_constant<!SEL>());
                                 tmem_wait_ld16(hi);
                                 if (c + 1 < halves) TMEM_LDQ16(s_addr + 64 * c + 64, lo);
                                 exp32(hi, pk1 + 8, std::false_type());
@@ -822,7 +829,14 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 const float invA = lA > 0.f ? 1.0f / lA : 0.f, invB = lB > 0.f ? 1.0f / lB : 0.f;
                 const float lsA = lA > 0.f ? (mA + log2f(lA)) * 0.6931471805599453f : -INFINITY;
                 const float lsB = lB > 0.f ? (mB + log2f(lB)) * 0.6931471805599453f : -INFINITY;
-                if (phase == 0) {
+                if (SEL) {
+                    inv_linA = invA;
+                    inv_linB = invB;
+                    if (p.lse_sparse && c2 == 0) {
+                        if (okA) p.lse_sparse[lseA] = lsA;
+                        if (okB) p.lse_sparse[lseB] = lsB;
+                    }
+                } else if (phase == 0) {
                     inv_spA = invA;
                     inv_spB = invB;
                     ls_spA = lsA;
@@ -856,11 +870,18 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             auto tile_off = [&](int row, int j) -> int {
                 return (j >> 3) * HALF_BYTES + row * 128 + (((j & 7) ^ (row & 7)) << 4) + 4 * c2;
             };
-            if (ok) {
+            if (SEL && ok) {
+                // the output is staged where Q lies: its products are done with it (o_done follows them), or, without a key, it has landed
+                ok = n_sel > 0 ? __all_sync(0xffffffffu, mbar_wait(&bar->o_done, ph_od, abort_flag, sink, 9))
+                               : __all_sync(0xffffffffu, mbar_wait(&bar->q_full[qs], (jcount / Q_STAGES) & 1u, abort_flag, sink, 9));
+                if (n_sel > 0) ph_od ^= 1u;
+                tc_fence_after();
+            }
+            if (!SEL && ok) {
                 WA_TRACE(18);
                 ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[gbuf], ((sg + n_kv) / S_BUFS) & 1u, abort_flag, sink, 10));
             }
-            if (ok) {
+            if (!SEL && ok) {
                 tc_fence_after();
                 WA_TRACE(13);
                 if (!p.part_linear) {
@@ -915,7 +936,29 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     WA_TRACE(12);
                 }
             }
-            if (ok && p.part_linear) {
+            if (SEL && ok) {
+                // rows without a key are zeros, whatever the accumulator holds
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {   // 32 columns at a time
+                    uint32_t o[16] = {};
+                    if (n_sel > 0) {
+                        TMEM_LDQ16(tmem_o + lane_addr + c * 32, o);
+                        tmem_wait_ld();
+                        if (c == 3) {
+                            tc_fence_before();
+                            warp_arrive(&bar->o_free);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool keyA = inv_linA != 0.f, keyB = inv_linB != 0.f;
+                        __nv_bfloat162 ra = __floats2bfloat162_rn(keyA ? __uint_as_float(o[4 * j]) * inv_linA : 0.f, keyA ? __uint_as_float(o[4 * j + 1]) * inv_linA : 0.f);
+                        __nv_bfloat162 rb = __floats2bfloat162_rn(keyB ? __uint_as_float(o[4 * j + 2]) * inv_linB : 0.f, keyB ? __uint_as_float(o[4 * j + 3]) * inv_linB : 0.f);
+                        *reinterpret_cast<uint32_t *>(q_stage + tile_off(rowA, 4 * c + j)) = *reinterpret_cast<uint32_t *>(&ra);
+                        *reinterpret_cast<uint32_t *>(q_stage + tile_off(rowB, 4 * c + j)) = *reinterpret_cast<uint32_t *>(&rb);
+                    }
+                }
+            } else if (ok && p.part_linear) {
                 // Partial outputs leave as whole rows: a quad holds 32 bytes of a row per step, and stores of that size are
                 // what a peer's buffer takes worst over NVLink.  The Q stage is free by now (every score product of the item
                 // has landed), so each warp turns its 16 rows x 64 columns of float32 around in 4 KB of it (32-byte pieces
@@ -1012,7 +1055,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&bar->out_ready[qs]);
             WA_TRACE(10);
-            sg += n_kv + 1;
+            sg += n_kv + GATE_TILES;
             ++jcount;
         }
         tc_fence_before();
@@ -1035,7 +1078,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 // share their blocks have far fewer of them than their counts say.
 constexpr int PL_WARPS = 8;
 __global__ void __launch_bounds__(PL_WARPS * 32)
-pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__ num, int Nq, int Nkv, int q_items, int n_items,
+pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__ num, int Nq, int Nkv, int stride, int q_items, int n_items,
                   int32_t *__restrict__ lists, int32_t *both, int ctas, SchedJob job) {
     extern __shared__ uint32_t pl_smem[];
     __shared__ int hist[SCHED_BINS], warp_tot[32], last_cta;
@@ -1049,7 +1092,7 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
         int n[2], distinct[2] = {0, 0}, shared = 0;
         for (int w = lane; w < words; w += 32) bits[0][w] = bits[1][w] = 0u;
         __syncwarp();
-        auto id_of = [&](int side, int i) { return max(0, min(index[(row0 + side) * Nkv + i], Nkv - 1)); };
+        auto id_of = [&](int side, int i) { return max(0, min(index[(row0 + side) * stride + i], Nkv - 1)); };
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
             n[side] = side == 0 || two ? max(0, min(num[row0 + side], Nkv)) : 0;
@@ -1072,11 +1115,11 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
         }
         const bool plain = distinct[0] != n[0] || distinct[1] != n[1];
         const int n_both = plain ? 0 : shared;
-        int32_t *own = lists + row0 * Nkv;
+        int32_t *own = lists + row0 * stride;
         if (plain) {
 #pragma unroll
             for (int side = 0; side < 2; ++side)
-                for (int i = lane; i < n[side]; i += 32) own[(long long)side * Nkv + i] = id_of(side, i);
+                for (int i = lane; i < n[side]; i += 32) own[(long long)side * stride + i] = id_of(side, i);
         } else {
             int at[3] = {0, n_both, n_both};            // next place of a block of both, of the first row's others, of the second's
             for (int w0 = 0; w0 < words; w0 += 32) {
@@ -1096,7 +1139,7 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
                     for (uint32_t m = part[k]; m; m &= m - 1, ++pos) {
                         const int id = (w0 + lane) * 32 + __ffs(m) - 1;
                         if (k != 2) own[pos] = id;
-                        if (k != 1 && two) own[Nkv + pos] = id;
+                        if (k != 1 && two) own[stride + pos] = id;
                     }
                 }
             }
@@ -1346,7 +1389,7 @@ int hsa_sm100_launch(const wa_hsa_params *p, int Lc, const wa_tensor4 *kc, const
     if (pair) {
         const size_t smem = (size_t)PL_WARPS * 2 * ((Nkv + 31) / 32) * sizeof(uint32_t);   // at most 32 KB beside 17 KB for the order
         const cudaError_t e = launch_dependent(pair_lists_kernel, dim3(ceil_div(n_items, PL_WARPS)), dim3(PL_WARPS * 32), smem, stream, index, num, Nq,
-                                               Nkv, q_items, n_items, lists, both, n_items < max_grid() ? n_items : max_grid(), job);
+                                               Nkv, Nkv, q_items, n_items, lists, both, n_items < max_grid() ? n_items : max_grid(), job);
         if (e != cudaSuccess) return fail((int)e, "wa_hsa_forward(pairs): %s", cudaGetErrorString(e));
         if ((rc = check_launch("wa_hsa_forward(pairs)"))) return rc;
         index = lists;
@@ -1423,6 +1466,96 @@ int hsa_sm100_launch_linear(const wa_hsa_params *p, int Lc, const wa_tensor4 *kc
                                     nullptr, nullptr, stream);
     profile_pause(false);
     return rc;
+}
+
+// ---- the sparse branch alone (wa_selected_forward) -------------------------------------------------
+namespace sm100 {
+struct SelectedWs {
+    size_t order, counter, both, lists, total;
+};
+static bool selected_paired(const wa_selected_params *p) {       // as hsa_sm100_sched_job has it
+    return p->block_size == HALF && (long long)p->Lkv <= 16384ll * HALF && (long long)p->B * p->H * ceil_div(p->Lq, p->block_size) > max_grid();
+}
+static SelectedWs selected_ws(const wa_selected_params *p) {
+    SelectedWs w{};
+    size_t c = 0;
+    const size_t items = (size_t)p->B * p->H * ceil_div(p->Lq, p->block_size);
+    w.order = c; c = align_up(c + items * sizeof(int32_t), 256);
+    w.counter = c; c = align_up(c + 3 * sizeof(int), 256);
+    if (p->block_size == HALF) {
+        w.both = c; c = align_up(c + items * sizeof(int32_t), 256);
+        w.lists = c; c = align_up(c + items * p->index_stride * sizeof(int32_t), 256);
+    }
+    w.total = c;
+    return w;
+}
+}  // namespace sm100
+
+bool selected_sm100_tensors(const wa_selected_params *p) {
+    using namespace sm100;
+    return p->D == TILE && (p->block_size == TILE || p->block_size == HALF) && !p->block_sizes && view_ok(&p->q) && view_ok(&p->k) && view_ok(&p->v) &&
+           (long long)p->B * p->H * ceil_div(p->Lq, p->block_size) <= (1 << 24) && device_is_sm100() && encode_fn() != nullptr;
+}
+bool selected_sm100_forward_supported(const wa_selected_params *p) { return selected_sm100_tensors(p) && sm100::view_ok(&p->out); }
+size_t selected_sm100_forward_bytes(const wa_selected_params *p) { return sm100::selected_ws(p).total; }
+
+int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, void *workspace, cudaStream_t stream) {
+    using namespace sm100;
+    const char *what = "wa_selected_forward(tcgen05)";
+    const SelectedWs w = selected_ws(p);
+    char *ws = (char *)workspace;
+    const int blk = p->block_size, Nq = ceil_div(p->Lq, blk), Nkv = ceil_div(p->Lkv, blk);
+    const bool pair = selected_paired(p);
+    SchedJob job{};
+    job.order = (int32_t *)(ws + w.order);
+    job.work_counter = (int *)(ws + w.counter);
+    job.error_flag = job.work_counter + 1;
+    job.pairs_done = job.work_counter + 2;
+    job.paired = pair;
+    job.by_head = pair && 4ll * p->B * p->Hkv * p->Lkv * p->D > (64ll << 20);
+
+    CUtensorMap tq, tk, tv, tout;
+    int rc;
+    if ((rc = make_map_4d(&tq, &p->q, p->B, p->Lq, p->H, "q"))) return rc;
+    if ((rc = make_map_5d(&tk, &p->k, p->B, p->Lkv, p->Hkv, "k", blk, blk == TILE ? 2 : 1))) return rc;
+    if ((rc = make_map_5d(&tv, &p->v, p->B, p->Lkv, p->Hkv, "v", blk, 2))) return rc;
+    if ((rc = make_map_4d(&tout, &p->out, p->B, p->Lq, p->H, "out", pair ? TILE : blk))) return rc;
+    static PerDeviceOnce attr_set;
+    if (!attr_set.done()) {
+        cudaError_t e = cudaSuccess;
+        for (auto kernel : {hsa_fwd_sm100_kernel<TILE, false, true>, hsa_fwd_sm100_kernel<HALF, false, true>, hsa_fwd_sm100_kernel<HALF, true, true>})
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(pair_lists_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * 1024);
+        if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+        attr_set.mark();
+    }
+    const int rows = p->B * p->H * Nq, q_items = pair ? (Nq + 1) / 2 : Nq, n_items = p->B * p->H * q_items;
+    schedule_kernel<<<1, 1024, 0, stream>>>(num, rows, Nkv, job);
+    if ((rc = check_launch(what))) return rc;
+    Params kp{};
+    kp.both = (const int32_t *)(ws + w.both);
+    if (pair) {
+        const size_t smem = (size_t)PL_WARPS * 2 * ((Nkv + 31) / 32) * sizeof(uint32_t);
+        const cudaError_t e = launch_dependent(pair_lists_kernel, dim3(ceil_div(n_items, PL_WARPS)), dim3(PL_WARPS * 32), smem, stream, index, num, Nq, Nkv,
+                                               p->index_stride, q_items, n_items, (int32_t *)(ws + w.lists), (int32_t *)(ws + w.both),
+                                               n_items < max_grid() ? n_items : max_grid(), job);
+        if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+        if ((rc = check_launch(what))) return rc;
+        index = (const int32_t *)(ws + w.lists);
+    }
+    kp.B = p->B; kp.H = p->H; kp.Lq = p->Lq; kp.Lkv = p->Lkv; kp.Nq = Nq; kp.Nkv = Nkv;
+    kp.n_items = n_items; kp.q_items = q_items; kp.blk = blk;
+    kp.index = index; kp.num = num; kp.order = job.order; kp.work_counter = job.work_counter; kp.error_flag = job.error_flag;
+    kp.status_mirror = p->status_mirror;
+    kp.scale_log2 = (float)(pow((double)TILE, -0.5) * 1.4426950408889634);
+    kp.lse_sparse = p->lse;
+    kp.lse_st = 1; kp.lse_sh = p->Lq; kp.lse_sb = (long long)p->H * p->Lq;
+    kp.list_stride = p->index_stride; kp.kv_group = p->H / p->Hkv;
+    const auto kernel = blk == TILE ? hsa_fwd_sm100_kernel<TILE, false, true> : pair ? hsa_fwd_sm100_kernel<HALF, true, true> : hsa_fwd_sm100_kernel<HALF, false, true>;
+    // (the maps of the slots and of the gate's weights are not used)
+    const cudaError_t e = launch_dependent(kernel, dim3(n_items < max_grid() ? n_items : max_grid()), dim3(THREADS), SMEM_BYTES, stream, tq, tk, tv, tk, tv, tq, tout, kp);
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
 }
 
 }  // namespace wa

@@ -1,0 +1,295 @@
+// Moves of cache pages in place: new[d_i] = old[s_i] for all i at once, or zeros, in all tensors of a call.
+//
+// Copying, forking, moving together and clearing pages are all of this form; the roll of a key/value window (wan/modules/
+// causal_model.py:331-360) is the one that moves every page to the front.  No scratch and no order between thread blocks is needed:
+// whatever happens to one 16-byte piece of a page happens to the same piece of every page, independently of all other pieces.  So
+// a thread takes a piece (its place within a page) and runs a short list of page numbers over it: load from the source pages,
+// store to the destinations.  The host puts a list into an order in which no page is overwritten before it has been read for the last
+// time (a page that is read by several comes after them, a ring of pages keeps one piece in registers), and splits it
+// into parts that share no page that is both read and written; parts run side by side.
+//
+// Bound: HBM, every moved page is read once and written once.  Eight loads of a thread are in flight at a time.
+// Page numbers and tensors travel as launch parameters: nothing is copied to the device, and the call can be captured.
+#include <algorithm>
+#include <new>
+#include <numeric>
+#include <vector>
+
+#include "wa_common.cuh"
+
+namespace wa {
+
+constexpr int PM_CLEAR = -1, PM_SAVED = -2, PM_SAVE = -3;      // sources that are no page: zeros, the kept piece; keep a piece of `dst`
+constexpr int PM_THREADS = 256, PM_PIECES = 2, PM_AT_ONCE = 4;  // pieces of a thread, moves whose loads are in flight together
+
+struct PageTensor {
+    char *ptr;
+    long long batch_stride, row_stride, page_stride;            // bytes
+    long long rows;                                             // tokens of a sample
+    int page_rows, row_pieces;                                  // tokens of a page, pieces of a token
+    int batch;
+};
+
+template <int TENSORS, int MOVES>
+struct PageMoves {
+    PageTensor tensor[TENSORS];
+    int2 move[MOVES];                  // (destination, source)
+    int part[MOVES + 1];               // first move of each part
+    int tensors, last_of[TENSORS];     // last_of: first launch row behind each tensor's (samples of all tensors are the grid's z)
+};
+
+template <typename Piece, int TENSORS, int MOVES>
+__global__ void __launch_bounds__(PM_THREADS)
+move_pages_kernel(const __grid_constant__ PageMoves<TENSORS, MOVES> p) {
+    pdl_wait();
+    int t = 0;
+    while ((int)blockIdx.z >= p.last_of[t]) ++t;
+    const PageTensor &x = p.tensor[t];
+    const unsigned pieces = (unsigned)x.page_rows * (unsigned)x.row_pieces;      // below 2^31
+    const unsigned first = blockIdx.x * (unsigned)(PM_THREADS * PM_PIECES) + threadIdx.x;
+    if (first >= pieces) return;
+    char *base = x.ptr + (blockIdx.z - (t ? p.last_of[t - 1] : 0)) * x.batch_stride;
+    long long at[PM_PIECES];
+    int row[PM_PIECES];
+#pragma unroll
+    for (int u = 0; u < PM_PIECES; ++u) {
+        const unsigned e = first + u * PM_THREADS, r = e / (unsigned)x.row_pieces;
+        row[u] = e < pieces ? (int)r : INT32_MAX;
+        at[u] = (long long)r * x.row_stride + (long long)(e - r * (unsigned)x.row_pieces) * (long long)sizeof(Piece);
+    }
+    const auto rows_of = [&](int page) {        // the last page may be shorter
+        const long long left = x.rows - (long long)page * x.page_rows;
+        return (int)(left < x.page_rows ? left : x.page_rows);
+    };
+    Piece kept[PM_PIECES] = {};
+    int kept_rows = 0;
+    const int end = p.part[blockIdx.y + 1];
+    for (int m0 = p.part[blockIdx.y]; m0 < end; m0 += PM_AT_ONCE) {
+        Piece v[PM_AT_ONCE][PM_PIECES];
+        int rows[PM_AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < PM_AT_ONCE; ++i) {
+            rows[i] = 0;
+            if (m0 + i < end) {
+                const int2 m = p.move[m0 + i];
+                const int page = m.y >= 0 ? m.y : m.x, mine = rows_of(page);
+                rows[i] = m.y == PM_SAVE ? 0 : m.y == PM_SAVED ? min(kept_rows, mine) : min(rows_of(m.x), mine);
+                const bool load = m.y >= 0 || m.y == PM_SAVE;
+                const char *src = base + (long long)page * x.page_stride;
+#pragma unroll
+                for (int u = 0; u < PM_PIECES; ++u) {
+                    v[i][u] = m.y == PM_SAVED ? kept[u] : Piece{};
+                    if (load && row[u] < mine) v[i][u] = *reinterpret_cast<const Piece *>(src + at[u]);
+                    if (m.y == PM_SAVE) kept[u] = v[i][u];
+                }
+                if (m.y == PM_SAVE) kept_rows = mine;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PM_AT_ONCE; ++i) {
+            if (rows[i] == 0) continue;
+            char *dst = base + (long long)p.move[m0 + i].x * x.page_stride;
+#pragma unroll
+            for (int u = 0; u < PM_PIECES; ++u)
+                if (row[u] < rows[i]) *reinterpret_cast<Piece *>(dst + at[u]) = v[i][u];
+        }
+    }
+}
+
+struct PagePlan {
+    std::vector<int2> move;
+    std::vector<int> part, hole;       // of each move: its part, and the page that the kept piece may be put back to behind it (-1: none is kept)
+};
+
+// The order described above.  `pages`: one more than the largest page number.
+static PagePlan plan_moves(const int32_t *dst, const int32_t *src, int n, int pages) {
+    std::vector<int> op(pages, -1), readers(pages, 0), root(pages);
+    std::iota(root.begin(), root.end(), 0);
+    auto find = [&](int a) {
+        while (root[a] != a) a = root[a] = root[root[a]];
+        return a;
+    };
+    for (int i = 0; i < n; ++i)
+        if (dst[i] != src[i]) op[dst[i]] = i;
+    for (int i = 0; i < n; ++i)
+        if (dst[i] != src[i] && src[i] >= 0) {
+            ++readers[src[i]];
+            if (op[src[i]] >= 0) root[find(dst[i])] = find(src[i]);
+        }
+    PagePlan plan;
+    std::vector<char> done(n, 0);
+    auto emit = [&](int d, int s, int hole) {
+        plan.move.push_back(make_int2(d, s));
+        plan.part.push_back(find(d));
+        plan.hole.push_back(hole);
+    };
+    for (int i = 0; i < n; ++i) {              // from pages that nothing reads
+        int j = i;
+        while (j >= 0 && dst[j] != src[j] && !done[j] && readers[dst[j]] == 0) {
+            done[j] = 1;
+            emit(dst[j], src[j] < 0 ? PM_CLEAR : src[j], -1);
+            const int s = src[j];
+            j = s >= 0 && --readers[s] == 0 ? op[s] : -1;
+        }
+    }
+    for (int i = 0; i < n; ++i) {              // what is left are rings
+        if (done[i] || dst[i] == src[i]) continue;
+        emit(dst[i], PM_SAVE, dst[i]);
+        for (int j = i; !done[j]; j = op[src[j]]) {
+            done[j] = 1;
+            const bool closes = src[j] == dst[i];
+            emit(dst[j], closes ? PM_SAVED : src[j], closes ? -1 : src[j]);
+        }
+    }
+    // part by part, in the order above within each
+    std::vector<int> by(plan.move.size());
+    std::iota(by.begin(), by.end(), 0);
+    std::stable_sort(by.begin(), by.end(), [&](int a, int b) { return plan.part[a] < plan.part[b]; });
+    PagePlan sorted;
+    for (int i : by) {
+        sorted.move.push_back(plan.move[i]);
+        sorted.part.push_back(plan.part[i]);
+        sorted.hole.push_back(plan.hole[i]);
+    }
+    return sorted;
+}
+
+template <typename Piece, int TENSORS, int MOVES>
+static int launch_moves(const wa_page_tensor *tensors, int n_tensors, const PagePlan &plan, int whole_pages, cudaStream_t stream, const char *what) {
+    const int total = (int)plan.move.size();
+    // a tensor at a time is added as long as there is room; all lists run over a group of tensors before the next group
+    for (int t0 = 0; t0 < n_tensors;) {
+        PageMoves<TENSORS, MOVES> p{};
+        long long widest = 0, rows = 0;
+        int t = t0;
+        for (; t < n_tensors && p.tensors < TENSORS; ++t) {
+            const wa_page_tensor &x = tensors[t];
+            if (rows + x.batch > 65535 && p.tensors > 0) break;
+            WA_REQUIRE(x.batch <= 65535, WA_ERR_UNSUPPORTED, "%s: more than 65535 samples", what);
+            PageTensor &y = p.tensor[p.tensors];
+            y.ptr = (char *)x.ptr; y.batch_stride = x.batch_stride; y.row_stride = x.token_stride; y.page_stride = x.token_stride * x.page_tokens;
+            y.rows = x.tokens; y.page_rows = x.page_tokens; y.row_pieces = (int)(x.row_bytes / (int64_t)sizeof(Piece)); y.batch = x.batch;
+            rows += x.batch;
+            p.last_of[p.tensors++] = (int)rows;
+            widest = std::max(widest, (long long)y.page_rows * y.row_pieces);
+        }
+        t0 = t;
+        if (widest == 0 || rows == 0) continue;
+        WA_REQUIRE(widest < (1ll << 31) - PM_THREADS * PM_PIECES, WA_ERR_UNSUPPORTED, "%s: pages of more than 2^31 pieces", what);
+        const long long gx = (widest + PM_THREADS * PM_PIECES - 1) / (PM_THREADS * PM_PIECES);
+        int reopen = -1;                       // page that holds the kept piece of a ring that the launch before cut
+        for (int m = 0; m < total;) {
+            int n = 0, parts = 0;
+            if (reopen >= 0) p.move[n++] = make_int2(reopen, PM_SAVE);
+            reopen = -1;
+            const int begin = m;
+            int stop = std::min(total, m + MOVES - n);
+            if (stop < total && plan.hole[stop - 1] >= 0) {
+                // a ring is cut: its kept piece goes to a page that is free by then, one that is whole in every tensor
+                --stop;
+                while (stop > begin && plan.hole[stop - 1] >= whole_pages) --stop;
+                WA_REQUIRE(stop > begin, WA_ERR_UNSUPPORTED, "%s: a ring of moves through too many shortened pages", what);
+            }
+            for (; m < stop; ++m) {
+                if (m == begin || plan.part[m] != plan.part[m - 1]) p.part[parts++] = m == begin ? 0 : n;
+                p.move[n++] = plan.move[m];
+            }
+            if (m < total && plan.hole[m - 1] >= 0) {
+                reopen = plan.hole[m - 1];
+                p.move[n++] = make_int2(reopen, PM_SAVED);
+            }
+            p.part[parts] = n;
+            const cudaError_t e = launch_dependent(move_pages_kernel<Piece, TENSORS, MOVES>, dim3((unsigned)gx, parts, (unsigned)rows), dim3(PM_THREADS), 0, stream, p);
+            if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+            const int rc = check_launch(what);
+            if (rc) return rc;
+        }
+    }
+    return 0;
+}
+
+template <typename Piece>
+static int launch_moves(const wa_page_tensor *tensors, int n_tensors, const PagePlan &plan, int whole_pages, cudaStream_t stream, const char *what) {
+    // parameters are copied with every launch: a small call has small ones
+    if (n_tensors <= 8 && plan.move.size() <= 32) return launch_moves<Piece, 8, 32>(tensors, n_tensors, plan, whole_pages, stream, what);
+    return launch_moves<Piece, 128, 1024>(tensors, n_tensors, plan, whole_pages, stream, what);
+}
+
+// Token rows of a tensor do not overlap: of its two axes the one with the larger stride steps over all of the other.
+static bool rows_apart(const wa_page_tensor &x) {
+    int64_t inner = x.token_stride, n_inner = x.tokens, outer = x.batch_stride, n_outer = x.batch;
+    if (n_inner <= 1 || (n_outer > 1 && outer < inner)) std::swap(inner, outer), std::swap(n_inner, n_outer);
+    if (n_inner > 1 && inner < x.row_bytes) return false;
+    return n_outer <= 1 || outer >= (n_inner > 1 ? (n_inner - 1) * inner : 0) + x.row_bytes;
+}
+
+// Tensors that lie apart, or whose rows alternate (keys and values of a token side by side, two samples of one cache).
+static bool tensors_apart(const wa_page_tensor *tensors, int n) {
+    struct Span { uintptr_t from, to; const wa_page_tensor *x; };
+    std::vector<Span> spans;
+    for (int t = 0; t < n; ++t) {
+        const wa_page_tensor &x = tensors[t];
+        if (x.tokens * x.row_bytes * x.batch == 0) continue;
+        const uintptr_t from = (uintptr_t)x.ptr;
+        spans.push_back({from, from + (uintptr_t)((x.batch - 1) * x.batch_stride + (x.tokens - 1) * x.token_stride + x.row_bytes), &x});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    for (size_t i = 0; i < spans.size(); ++i)
+        for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to; ++j) {
+            const wa_page_tensor &a = *spans[i].x, &b = *spans[j].x;
+            const int64_t step = a.tokens > 1 ? a.token_stride : b.token_stride;
+            if (step <= 0 || (a.tokens > 1 && a.token_stride != step) || (b.tokens > 1 && b.token_stride != step) || (a.batch > 1 && a.batch_stride % step) ||
+                (b.batch > 1 && b.batch_stride % step))
+                return false;
+            const int64_t off = (int64_t)((spans[j].from - spans[i].from) % (uintptr_t)step);
+            if (off < a.row_bytes || off + b.row_bytes > step) return false;
+        }
+    return true;
+}
+
+static int move_pages(const wa_page_tensor *tensors, int n_tensors, const int32_t *dst, const int32_t *src, int n, cudaStream_t stream) {
+    const char *what = "wa_hkv_move_pages";
+    WA_REQUIRE(n_tensors >= 0 && n >= 0, WA_ERR_ARG, "%s: sizes must not be negative", what);
+    if (n == 0 || n_tensors == 0) return 0;
+    WA_REQUIRE(tensors && dst && src, WA_ERR_ARG, "%s: null pointer", what);
+    int64_t pages = INT32_MAX, whole = INT32_MAX;
+    uintptr_t bits = 0;
+    for (int t = 0; t < n_tensors; ++t) {
+        const wa_page_tensor &x = tensors[t];
+        WA_REQUIRE(x.batch >= 0 && x.tokens >= 0 && x.row_bytes >= 0 && x.page_tokens > 0, WA_ERR_ARG, "%s: sizes must be positive", what);
+        WA_REQUIRE(x.ptr || x.tokens * x.row_bytes * x.batch == 0, WA_ERR_ARG, "%s: null pointer", what);
+        WA_REQUIRE(x.row_bytes < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: rows of more than 2^31 bytes", what);
+        WA_REQUIRE(rows_apart(x), WA_ERR_ARG, "%s: the tokens of a tensor must not overlap", what);
+        pages = std::min(pages, (x.tokens + x.page_tokens - 1) / x.page_tokens);
+        whole = std::min(whole, x.tokens / x.page_tokens);
+        bits |= (uintptr_t)x.ptr | (uintptr_t)x.batch_stride | (uintptr_t)x.token_stride | (uintptr_t)x.row_bytes;
+    }
+    WA_REQUIRE(tensors_apart(tensors, n_tensors), WA_ERR_ARG, "%s: two tensors share memory", what);
+    int most = 0;
+    for (int i = 0; i < n; ++i) {
+        WA_REQUIRE(dst[i] >= 0 && dst[i] < pages && src[i] >= -1 && src[i] < pages, WA_ERR_ARG, "%s: move %d of page %d to page %d leaves the %lld pages of a tensor",
+                   what, i, src[i], dst[i], (long long)pages);
+        most = std::max(most, std::max(dst[i], src[i]) + 1);
+    }
+    std::vector<char> taken(most, 0);
+    for (int i = 0; i < n; ++i) {
+        WA_REQUIRE(!taken[dst[i]], WA_ERR_ARG, "%s: page %d is the destination of two moves", what, dst[i]);
+        taken[dst[i]] = 1;
+    }
+    const PagePlan plan = plan_moves(dst, src, n, most);
+    if (plan.move.empty()) return 0;
+    const int whole_pages = (int)std::min<int64_t>(whole, INT32_MAX);
+    if (bits % 16 == 0) return launch_moves<uint4>(tensors, n_tensors, plan, whole_pages, stream, what);
+    if (bits % 4 == 0) return launch_moves<uint32_t>(tensors, n_tensors, plan, whole_pages, stream, what);
+    return launch_moves<unsigned char>(tensors, n_tensors, plan, whole_pages, stream, what);
+}
+
+}  // namespace wa
+
+extern "C" int wa_hkv_move_pages(const wa_page_tensor *tensors, int n_tensors, const int32_t *dst, const int32_t *src, int n, void *stream) {
+    try {
+        return wa::move_pages(tensors, n_tensors, dst, src, n, (cudaStream_t)stream);
+    } catch (const std::bad_alloc &) {
+        return wa::fail(WA_ERR_ARG, "wa_hkv_move_pages: out of host memory");
+    }
+}

@@ -1,0 +1,26 @@
+// Attention over selected key blocks with its gradient: what its translation units share.
+#pragma once
+#include "wa_internal.cuh"
+
+namespace wa {
+
+// Device pieces of a call's workspace.
+struct SelectedPlan {
+    int Nq, Nkv, group, words, row_words;      // query / key blocks, query heads of a key head, words of a bit per key block / per query block
+    size_t index, num;                         // [B, H, Nq, index_stride] clean lists, [B, H, Nq] their lengths
+    size_t rows;                               // backward: [B, Hkv, Nkv, group, row_words] which query blocks of which head list a key block
+    size_t stats;                              // backward: [B, H, (Nq + 1) * block] (log-sum-exp in powers of two, sum of dout * out) of a query row
+    size_t tuned;                              // what the tensor-core kernels need
+    size_t total;
+};
+
+// one query row of `stats`: rows that are no query's (behind the last one) have an infinite normaliser, which makes their probabilities zero
+inline size_t selected_stats_rows(const wa_selected_params *p, int Nq) { return (size_t)(Nq + 1) * p->block_size; }
+
+// bf16, head_dim 128, blocks of 64 or 128 tokens.  wa_hsa_sm100.cu:
+bool selected_sm100_tensors(const wa_selected_params *p);                 // q, k, v, blocks and device
+bool selected_sm100_forward_supported(const wa_selected_params *p);
+size_t selected_sm100_forward_bytes(const wa_selected_params *p);
+int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, void *workspace, cudaStream_t stream);
+
+}  // namespace wa

@@ -331,6 +331,7 @@ struct Params {
     int lse_packed;
     int peer_rows, peer_self;
     long long peer_delta[8];
+    int list_stride, kv_group;   // SEL: ids between two lists, query heads of a key head
 };
 
 struct ItemDesc {

@@ -9,9 +9,10 @@ from .attention import (
 )
 from .block_sparse_torch import block_sparse_attention_reference
 from .routing import BlockRouting, block_attention_map, block_mean_pool, build_block_routing
+from .selected import selected_attention
 
 __all__ = [
     "HSAAttention", "hsa_attention", "compress_kv", "resolve_backend", "hsa_parameter_names",
     "require_trained_hsa", "block_sparse_attention_reference", "BlockRouting", "build_block_routing",
-    "block_attention_map", "block_mean_pool",
+    "block_attention_map", "block_mean_pool", "selected_attention",
 ]

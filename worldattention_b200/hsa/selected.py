@@ -1,0 +1,52 @@
+"""Attention over selected key blocks with its gradient, for training and for single tokens.
+
+`selected_attention` is the differentiable form of the sparse branch: what `build_block_routing` (or any other choice of blocks)
+selected is attended to, `[B, L, H, D]` tensors are read in place, heads may share keys, and the gradient reaches q, k and v as the
+reference's Triton autograd function does (wan/modules/hsa/block_sparse_triton.py:142-382).
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+__all__ = ["selected_attention"]
+
+
+class _SelectedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, index, num, block_size, block_sizes):
+        out, lse = _lib.host().selected_forward(q, k, v, index, num, block_size, block_sizes)
+        ctx.save_for_backward(q, k, v, index, num, block_sizes, out, lse)
+        ctx.block_size = block_size
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, index, num, block_sizes, out, lse = ctx.saved_tensors
+        grads = _lib.host().selected_backward(q, k, v, index, num, ctx.block_size, block_sizes, out, lse, dout)
+        return tuple(g if needed else None for g, needed in zip(grads, ctx.needs_input_grad)) + (None,) * 4
+
+
+def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index: torch.Tensor, num: torch.Tensor, block_size: int, *,
+                       block_sizes: torch.Tensor | None = None, return_lse: bool = False):
+    """Softmax attention of each query block over the key blocks listed for it -> `[B, Lq, H, D]`; differentiable in q, k and v.
+
+    `q` `[B, Lq, H, D]`, `k` and `v` `[B, Lkv, Hkv, D]`, one dtype (float32 or bfloat16); H is a multiple of Hkv, and query head h reads key
+    head `h // (H // Hkv)`.  Any strides with a contiguous last axis are read in place.  `index` `[B, H, Nq, S]` and `num` `[B, H, Nq]` (int32,
+    `Nq = ceil(Lq / block_size)`) are the lists, as `build_block_routing` gives them: the first `num` ids of a row.  Lists are taken
+    as sets: an id named twice counts once, an id that is no key block counts nothing.  Rows whose list is empty give zeros (and
+    -inf as log-sum-exp) and have no part in the gradients.  `block_sizes` (int32 `[Nkv]`): only the first so many
+    tokens of a block are keys, as in `block_sparse_attention`; what lies behind them is not read.
+
+    `return_lse`: also the natural-log normalisers, float32 `[B, H, Lq]` (not differentiable).  Sums and statistics are float32; in bf16 the
+    probabilities and dS are rounded to bf16 where they are factors of a product.  Equal calls give equal bits, gradients included.  The
+    gradient of the gradient is not offered.
+    """
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _SelectedAttention.apply(q, k, v, index, num, block_size, block_sizes)
+    else:
+        out, lse = _lib.host().selected_forward(q, k, v, index, num, block_size, block_sizes)
+    return (out, lse) if return_lse else out

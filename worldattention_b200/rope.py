@@ -3,6 +3,9 @@
 `causal_rope_apply` keeps the reference's signature (wan/modules/causal_model.py:34-62); `qk_norm_rope` fuses the
 RMSNorm in front of it (wan/modules/model.py:70-86), which the reference applies to q and k just before.  One kernel
 launch per tensor, no float64 copy of the tokens, no loop over samples.
+
+`axial_rope` is the rotary embedding for tokens that have positions of their own (samples of different grids in one batch, text
+between pictures, single tokens), for q and k in one launch, with its gradient.
 """
 from __future__ import annotations
 
@@ -10,7 +13,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["causal_rope_apply", "qk_norm_rope"]
+__all__ = ["causal_rope_apply", "qk_norm_rope", "axial_rope"]
 
 
 def _table(freqs: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -55,3 +58,58 @@ def qk_norm_rope(x: torch.Tensor, norm_weight: torch.Tensor | None, eps: float, 
 def causal_rope_apply(x: torch.Tensor, grid_sizes, freqs: torch.Tensor, start_frame: int = 0) -> torch.Tensor:
     """Rotary embedding of `[B, L, H, D]` tokens laid out as a (frames, height, width) grid that starts at `start_frame`."""
     return qk_norm_rope(x, None, 0.0, grid_sizes, freqs, start_frame)
+
+
+class _AxialRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, table, axes, interleaved, inverse, *xs):
+        ctx.save_for_backward(positions, table)
+        ctx.how = axes, interleaved, inverse
+        ctx.set_materialize_grads(False)
+        return tuple(_lib.host().axial_rope(xs, positions, table, axes, interleaved, inverse))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, table = ctx.saved_tensors
+        axes, interleaved, inverse = ctx.how
+        there = [g for g, needed in zip(grads, ctx.needs_input_grad[5:]) if g is not None and needed]
+        turned = iter(_turn(there, positions, table, axes, interleaved, not inverse) if there else ())
+        return (None,) * 5 + tuple(next(turned) if g is not None and needed else None for g, needed in zip(grads, ctx.needs_input_grad[5:]))
+
+
+def _turn(xs, positions, table, axes, interleaved, inverse):
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        return _AxialRope.apply(positions, table, axes, interleaved, inverse, *xs)
+    return _lib.host().axial_rope(xs, positions, table, axes, interleaved, inverse)
+
+
+def axial_rope(x, positions: torch.Tensor, table: torch.Tensor, *, axes=None, interleaved: bool = True):
+    """Rotary embedding of `[B, L, H, D]` tokens at positions of their own on several axes; differentiable in `x`.
+
+    `x` is a tensor, or a tuple of up to four that share B, L and D (q and k: one launch).  `positions` `[L, A]` or `[B, L, A]`
+    holds each token's place on each of the A axes (int32; other integers are converted), `table` the angles: float32
+    `[rows, pairs, 2]` cosines and sines, or a complex table `[rows, pairs]` as `causal_rope_apply` takes, which is converted
+    in every call.  `axes` says how many consecutive pairs each axis turns (default: all of them for one axis, and for three
+    the time, height and width bands of `causal_rope_apply`).  A pair is two neighbouring channels, or with `interleaved=False`
+    channels i and i + pairs.  Channels behind `2 * pairs` are copied.  A token whose position on an axis lies outside the
+    table gets NaN in the pairs of that axis (nothing is read back to the host to refuse it).
+
+    Float32 arithmetic, rounded once.  New tensors are returned, contiguous; a tuple for a tuple.
+    """
+    alone = isinstance(x, torch.Tensor)
+    xs = (x,) if alone else tuple(x)
+    if torch.is_complex(table):
+        table = torch.view_as_real(table.resolve_conj())
+    if table.dtype != torch.float32:
+        table = table.float()
+    if positions.dtype != torch.int32:
+        if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
+            raise ValueError(f"positions must be integers, got {positions.dtype}")
+        positions = positions.clamp(-1, table.shape[0]).int()        # (what lies outside the table stays outside)
+    if axes is None:
+        pairs, n = table.shape[1], positions.shape[-1]
+        if n not in (1, 3):
+            raise ValueError(f"axes is needed for {n} axes: how many pairs does each of them turn?")
+        axes = (pairs,) if n == 1 else (pairs - 2 * (pairs // 3), pairs // 3, pairs // 3)
+    out = _turn(xs, positions, table, tuple(axes), bool(interleaved), False)
+    return out[0] if alone else tuple(out)
