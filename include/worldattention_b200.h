@@ -166,7 +166,7 @@ typedef struct wa_selected_params {
     float *lse;
     void *workspace;
     size_t workspace_bytes;
-    int32_t *status_mirror;             /* page-locked host word, or null: the site code (401 to 499) of a bounded wait that ran out */
+    int32_t *status_mirror;             /* page-locked host word, or null: the site code of a bounded wait that ran out (401 to 499: gradient) */
 } wa_selected_params;
 size_t wa_selected_params_size(void);
 /* 0 for arguments that the call itself refuses. */

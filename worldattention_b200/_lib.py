@@ -247,6 +247,8 @@ def raise_if_failed(device: torch.device) -> None:
         word.zero_()
         if 301 <= code <= 309:
             raise RuntimeError(f"an earlier HKV install on {device} gave up at wait site {code}; the installed pages and slots are invalid")
+        if 401 <= code <= 499:
+            raise RuntimeError(f"an earlier gradient of an attention over selected blocks on {device} gave up at wait site {code}; its gradients are invalid")
         kernel = "block-pooling (TMA stream)" if code in (201, 202) else "tcgen05 attention"
         raise RuntimeError(f"an earlier {kernel} launch of an HSA forward on {device} gave up at wait site {code}; "
                            "its output is invalid")

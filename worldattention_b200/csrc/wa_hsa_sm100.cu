@@ -22,7 +22,7 @@
 #include <cstdlib>
 #include <type_traits>
 
-#include "wa_internal.cuh"
+#include "wa_selected.cuh"
 #include "wa_sm100_ptx.cuh"
 
 namespace wa {
@@ -1491,6 +1491,9 @@ static SelectedWs selected_ws(const wa_selected_params *p) {
 }
 }  // namespace sm100
 
+int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int H, const char *name, int rows, int halves) {
+    return sm100::make_map_5d(map, t, B, L, H, name, rows, halves);
+}
 bool selected_sm100_tensors(const wa_selected_params *p) {
     using namespace sm100;
     return p->D == TILE && (p->block_size == TILE || p->block_size == HALF) && !p->block_sizes && view_ok(&p->q) && view_ok(&p->k) && view_ok(&p->v) &&

@@ -272,7 +272,8 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
         w.stats = c; c = align_up(c + (size_t)p->B * p->H * selected_stats_rows(p, w.Nq) * sizeof(float2), 256);
     }
     w.tuned = c;
-    if (!backward && selected_sm100_forward_supported(p)) c = align_up(c + selected_sm100_forward_bytes(p), 256);
+    if (backward ? selected_sm100_backward_supported(p) : selected_sm100_forward_supported(p))
+        c = align_up(c + (backward ? selected_sm100_backward_bytes(p) : selected_sm100_forward_bytes(p)), 256);
     w.total = c;
     return w;
 }
@@ -368,6 +369,7 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
                                            padded, all, stats);
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     if ((rc = check_launch(what))) return rc;
+    if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, ws + w.tuned, stream);
     SelectedGrad g{};
     g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v); g.dout = make_view(&p->dout);
     g.dq = p->dq.ptr; g.dqb = p->dq.stride_b; g.dql = p->dq.stride_l; g.dqh = p->dq.stride_h;

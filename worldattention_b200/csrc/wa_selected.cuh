@@ -1,5 +1,7 @@
 // Attention over selected key blocks with its gradient: what its translation units share.
 #pragma once
+#include <cuda.h>
+
 #include "wa_internal.cuh"
 
 namespace wa {
@@ -22,5 +24,12 @@ bool selected_sm100_tensors(const wa_selected_params *p);                 // q, 
 bool selected_sm100_forward_supported(const wa_selected_params *p);
 size_t selected_sm100_forward_bytes(const wa_selected_params *p);
 int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, void *workspace, cudaStream_t stream);
+// a [B, L, H, 128] view as a map of boxes of `rows` tokens and one or both halves of the channels
+int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int H, const char *name, int rows, int halves);
+// wa_selected_sm100.cu:
+bool selected_sm100_backward_supported(const wa_selected_params *p);
+size_t selected_sm100_backward_bytes(const wa_selected_params *p);
+int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float2 *stats, void *workspace,
+                            cudaStream_t stream);
 
 }  // namespace wa

@@ -1,0 +1,587 @@
+// Gradient of attention over selected key blocks on the tensor cores of sm_100a: bf16, head_dim 128, blocks of 64 or 128 tokens.
+//
+// Two launches of one kernel.  Each owns 64 rows of one side at a time -- the first 64 key tokens, for dK and dV, the second 64 query rows,
+// for dQ -- and meets 128 rows of the other side per step: a block of 128, or two of 64 that need not be neighbours (nor, with shared
+// keys, of one query head).  With F1, F2 the owned rows and G1, G2 the met ones (keys: F = k, v and G = q, dout; queries: F = q, dout and G = k, v)
+//     S = G1 F1^T   dP = G2 F2^T                      [128 met rows x 64 owned ones]
+//     P = 2^(S c - lse)   dS = P (dP - delta)
+//     dV^T += G2^T P   dK^T (or dQ^T) += G1^T dS      [128 channels x 64 owned rows]
+// so all four products have 128 rows and 64 columns, the met tile is the first operand of all of them as it lies (row-major for the
+// scores, transposed for the sums), and P and dS, which a thread holds by rows, are second operands that go to shared memory the
+// way they are.  The met rows' lists: bits per key block, or the clean ids of a query block.  Every sum is made in one CTA in
+// the order of its list: no atomics, equal calls give equal bits; the price is that S and dP are computed in both launches.
+//
+// One persistent CTA of ten warps per SM: warps 0-7 turn scores into P and dS and write finished sums out, warp 8 walks the lists and
+// issues the loads, warp 9 issues the products.  Scores of step u + 1 are issued before the sums of step u, so that they
+// run while the warps work on step u; tensor memory holds two steps' scores and the sums of two owned tiles (2 x 128 + 2 x 128 columns).
+//
+// Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
+#include "wa_selected.cuh"
+#include "wa_sm100_ptx.cuh"
+
+namespace wa {
+namespace sm100 {
+
+constexpr int SB_OWN = 64;                              // owned rows of an item
+constexpr int SB_OWN_BYTES = SB_OWN * TILE * 2;         // 16 KB: [half of the channels][row][64 channels]
+constexpr int SB_P_BYTES = TILE * SB_OWN * 2;           // 16 KB: [met row][64 owned rows]
+constexpr int SB_DESCS = 4;
+constexpr int SB_THREADS = 320;
+
+template <bool KEYS> struct SbRing {
+    static constexpr int SLOTS = KEYS ? 4 : 5;          // met tiles (32 KB each): G1 and G2 of a step take one each
+    static constexpr int FACTORS = KEYS ? 2 : 1;        // P and dS, or dS alone
+    static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + 2 * FACTORS * SB_P_BYTES + 3072;
+};
+
+enum { SB_FIRST = 1, SB_LAST = 2, SB_EMPTY = 4, SB_END = 8 };
+struct SbDesc {
+    int item, flags;
+    int real[2];         // queries' launch: real tokens of the met rows 0..63 and 64..127
+};
+
+struct SbBarriers {
+    // keys: of the met rows, [two steps][128]; queries: of the owned rows, [four items][64] -- when an item's are loaded, the warps may still be two
+    // items behind
+    float2 stats[2 * TILE];
+    uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
+    uint64_t f_full, f_empty, stats_full[4];
+    uint64_t full[5], empty[5];
+    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], p_free[2];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    SbDesc desc[SB_DESCS];
+};
+static_assert(sizeof(SbBarriers) <= 3072, "barrier block exceeds its shared-memory budget");
+static_assert(SbRing<true>::SMEM <= 227 * 1024 && SbRing<false>::SMEM <= 227 * 1024, "shared memory budget exceeded");
+
+struct SbParams {
+    int H, Hkv, group, Lq, Lkv, Nq, Nkv;
+    int owned, items;                 // owned tiles of a head; of all heads
+    int list_stride, row_words;
+    long long padded;                 // rows of `stats` of a head
+    const int32_t *index, *num;       // queries
+    const uint32_t *rows;             // keys
+    const float2 *stats;
+    __nv_bfloat16 *d1, *d2;           // dV; dK or dQ
+    long long d1b, d1l, d1h, d2b, d2l, d2h;
+    float scale, scale_log2;
+    int *work_counter, *error_flag, *status_mirror;
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+
+// What an owned tile meets, one id at a time, by a whole warp: 32 words of bits or 32 ids in its lanes' registers.
+template <bool KEYS>
+struct SbList {
+    const uint32_t *bits;
+    const int32_t *ids;
+    int n, at, words_per_head;
+    uint32_t mine;
+    unsigned left;
+    __device__ void begin(const SbParams &p, long long list, int lane) {
+        at = 0;
+        if (KEYS) {
+            words_per_head = p.row_words;
+            n = p.group * p.row_words;
+            bits = p.rows + list * n;
+        } else {
+            n = p.num[list];
+            ids = p.index + list * p.list_stride;
+        }
+        fetch(lane);
+    }
+    __device__ void fetch(int lane) {
+        if (KEYS) {
+            mine = at + lane < n ? bits[at + lane] : 0u;
+            left = __ballot_sync(0xffffffffu, mine != 0u);
+        } else {
+            mine = at + lane < n ? (uint32_t)ids[at + lane] : 0u;
+            left = __ballot_sync(0xffffffffu, at + lane < n);
+        }
+    }
+    // -1: no more.  keys: head within the group in the upper, query block in the lower 32 bits
+    __device__ long long next(int lane) {
+        while (left == 0u) {
+            at += 32;
+            if (at >= n) return -1;
+            fetch(lane);
+        }
+        const int src = __ffs(left) - 1;
+        const uint32_t word = __shfl_sync(0xffffffffu, mine, src);
+        if (!KEYS) {
+            left &= left - 1;
+            return (long long)word;
+        }
+        if (lane == src) mine &= mine - 1;
+        if ((word & (word - 1)) == 0u) left &= left - 1;
+        const int w = at + src, head = w / words_per_head;
+        return ((long long)head << 32) | (unsigned)((w - head * words_per_head) * 32 + __ffs(word) - 1);
+    }
+};
+
+template <bool KEYS, int BLK>
+__global__ void __launch_bounds__(SB_THREADS, 1)
+selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
+                           const __grid_constant__ CUtensorMap tm_g2, const SbParams p) {
+    using Ring = SbRing<KEYS>;
+    constexpr int SLOTS = Ring::SLOTS;
+    constexpr int PER = BLK / SB_OWN;                    // owned tiles of a block
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *f_s = smem, *g_s = f_s + 2 * SB_OWN_BYTES, *p_s = g_s + SLOTS * TILE_BYTES;      // p_s: [two steps][P, dS]
+    SbBarriers *bar = reinterpret_cast<SbBarriers *>(p_s + 2 * Ring::FACTORS * SB_P_BYTES);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    volatile int *abort_flag = &bar->abort_flag;
+    const FailSink sink{p.error_flag, p.status_mirror};
+
+    if (threadIdx.x == 0) {
+        bar->abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;
+        for (int i = 0; i < SB_DESCS; ++i) {
+            mbar_init(&bar->desc_full[i], 1);
+            mbar_init(&bar->desc_empty[i], 1 + 8);       // product warp and the eight others
+        }
+        mbar_init(&bar->f_full, 1);
+        mbar_init(&bar->f_empty, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&bar->stats_full[i], 1);
+        for (int i = 0; i < SLOTS; ++i) {
+            mbar_init(&bar->full[i], 1);
+            mbar_init(&bar->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar->s_full[i], 1);
+            mbar_init(&bar->dp_full[i], 1);
+            mbar_init(&bar->p_full[i], 8);
+            mbar_init(&bar->ds_full[i], 8);
+            mbar_init(&bar->p_free[i], 1);
+            mbar_init(&bar->acc_full[i], 1);
+            mbar_init(&bar->acc_empty[i], 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem_base;
+    // columns: S of two steps, dP of two steps, then the sums of two items (each dV^T, dK^T or dQ^T)
+    const uint32_t tm_s = tmem, tm_dp = tmem + 2 * SB_OWN, tm_acc = tmem + 4 * SB_OWN;
+
+    if (warp == 8) {
+        // ================= lists and loads =================
+        const bool leader = elect_one();
+        uint32_t descs = 0, tiles = 0, items = 0, steps = 0;       // so many so far
+        bool ok = true;
+        int at = blockIdx.x;
+        auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+        auto tell = [&](int item, int flags, int real0, int real1) {
+            const uint32_t d = descs % SB_DESCS;
+            if (!wait(&bar->desc_empty[d], ((descs / SB_DESCS) & 1u) ^ 1u, 401)) return false;
+            if (leader) {
+                bar->desc[d].item = item;
+                bar->desc[d].flags = flags;
+                bar->desc[d].real[0] = real0;
+                bar->desc[d].real[1] = real1;
+                mbar_arrive(&bar->desc_full[d]);
+            }
+            __syncwarp();
+            ++descs;
+            return true;
+        };
+        while (ok) {
+            if (at >= p.items) {
+                tell(0, SB_END, 0, 0);
+                break;
+            }
+            const int item = at;
+            int next_at = 0;
+            if (lane == 0) next_at = (int)gridDim.x + atomicAdd(p.work_counter, 1);
+            const int tile = item % p.owned, head = item / p.owned;      // head: (batch, head) of the owned side
+            const int b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
+            const int hk = KEYS ? h : h / p.group;
+            SbList<KEYS> list;
+            list.begin(p, (long long)head * (KEYS ? p.Nkv : p.Nq) + tile / PER, lane);
+            long long ahead = list.next(lane);
+            if (ahead < 0) {
+                ok = tell(item, SB_EMPTY, 0, 0);
+            } else {
+                // the owned tile: its last score products of the item before are done
+                ok = wait(&bar->f_empty, (items & 1u) ^ 1u, 402);
+                if (ok && leader) {
+                    mbar_expect_tx(&bar->f_full, 2 * SB_OWN_BYTES);
+                    tma_load_5d(f_s, &tm_f1, &bar->f_full, 0, tile * SB_OWN, 0, h, b);
+                    tma_load_5d(f_s + SB_OWN_BYTES, &tm_f2, &bar->f_full, 0, tile * SB_OWN, 0, h, b);
+                    if (!KEYS) {
+                        mbar_expect_tx(&bar->stats_full[items & 3u], SB_OWN * 8);
+                        bulk_load(bar->stats + (items & 3u) * SB_OWN, p.stats + (long long)head * p.padded + tile * SB_OWN, SB_OWN * 8, &bar->stats_full[items & 3u]);
+                    }
+                }
+                __syncwarp();
+                ++items;
+                int flags = SB_FIRST;
+                while (ok && ahead >= 0) {
+                    const long long one = ahead, two = BLK == SB_OWN ? list.next(lane) : -1;
+                    ahead = BLK == SB_OWN && two < 0 ? -1 : list.next(lane);
+                    if (ahead < 0) flags |= SB_LAST;
+                    // rows and heads of the two halves; what is missing lies behind the last block and loads as zeros
+                    const int blocks = KEYS ? p.Nq : p.Nkv;
+                    const int i0 = (int)(one & 0xffffffff), i1 = two < 0 ? blocks : (int)(two & 0xffffffff);
+                    const int h0 = KEYS ? h * p.group + (int)(one >> 32) : hk, h1 = KEYS ? (two < 0 ? h0 : h * p.group + (int)(two >> 32)) : hk;
+                    int real0 = SB_OWN, real1 = SB_OWN;
+                    if (!KEYS) {
+                        const int n = p.Lkv - i0 * BLK;
+                        real0 = min(n, SB_OWN);
+                        real1 = BLK == TILE ? max(0, min(n - SB_OWN, SB_OWN)) : two < 0 ? 0 : min(p.Lkv - i1 * BLK, SB_OWN);
+                    }
+                    ok = tell(item, flags, real0, real1);
+                    flags = 0;
+#pragma unroll
+                    for (int g = 0; g < 2 && ok; ++g) {
+                        const uint32_t slot = tiles % SLOTS;
+                        ok = wait(&bar->empty[slot], ((tiles / SLOTS) & 1u) ^ 1u, 403);
+                        if (ok && leader) {
+                            uint8_t *dst = g_s + slot * TILE_BYTES;
+                            uint64_t *full = &bar->full[slot];
+                            const CUtensorMap *map = g == 0 ? &tm_g1 : &tm_g2;
+                            const bool with_stats = KEYS && g == 0;
+                            mbar_expect_tx(full, TILE_BYTES + (with_stats ? TILE * 8 : 0));
+                            if (BLK == TILE) {
+                                tma_load_5d(dst, map, full, 0, i0 * TILE, 0, h0, b);
+                            } else {
+                                tma_load_5d(dst, map, full, 0, i0 * BLK, 0, h0, b);
+                                tma_load_5d(dst + HALF_BYTES / 2, map, full, 0, i1 * BLK, 0, h1, b);
+                                tma_load_5d(dst + HALF_BYTES, map, full, 0, i0 * BLK, 1, h0, b);
+                                tma_load_5d(dst + HALF_BYTES + HALF_BYTES / 2, map, full, 0, i1 * BLK, 1, h1, b);
+                            }
+                            if (with_stats) {
+                                // (the statistics of step u - 2 have been read: its sums, which come after them, freed this slot)
+                                float2 *to = bar->stats + (steps & 1u) * TILE;
+                                const float2 *row = p.stats + ((long long)b * p.H) * p.padded;
+                                bulk_load(to, row + h0 * p.padded + (long long)i0 * BLK, BLK * 8, full);
+                                if (BLK != TILE) bulk_load(to + SB_OWN, row + h1 * p.padded + (long long)i1 * BLK, BLK * 8, full);
+                            }
+                        }
+                        __syncwarp();
+                        ++tiles;
+                    }
+                    ++steps;
+                }
+            }
+            at = __shfl_sync(0xffffffffu, next_at, 0);
+        }
+        if (*abort_flag) {      // given up: copies on their way land within microseconds, the block's shared memory is kept for a millisecond
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) { }
+        }
+    } else if (warp == 9) {
+        // ================= products =================
+        const bool leader = elect_one();
+        constexpr uint32_t SCORE = instr_desc(false, SB_OWN), SUM = instr_desc(true, SB_OWN) | (1u << 15);      // both operands of the sums are transposed
+        uint32_t descs = 0, items = 0, scored = 0, summed = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+        int pending = -1;                 // flags of the step whose sums are still to be issued
+        uint32_t sum_items = 0;           // items whose sums have begun
+        auto sums = [&]() {
+            const uint32_t buf = summed & 1u, s1 = (2 * summed) % SLOTS, s2 = (2 * summed + 1) % SLOTS;
+            if (pending & SB_FIRST) {
+                if (!wait(&bar->acc_empty[sum_items & 1u], ((sum_items >> 1) & 1u) ^ 1u, 411)) return false;
+                ++sum_items;
+            }
+            const uint32_t acc = tm_acc + ((sum_items - 1) & 1u) * 2 * SB_OWN;
+            const bool fresh = pending & SB_FIRST;
+            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES;
+            if (KEYS) {
+                if (!wait(&bar->p_full[buf], (summed >> 1) & 1u, 412)) return false;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t a = smem_desc(smem_u32(g_s + s2 * TILE_BYTES), HALF_BYTES, 1024), bd = smem_desc(smem_u32(factors), HALF_BYTES, 1024);
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mma_ss(acc, a + (uint64_t)((kk * 2048) >> 4), bd + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
+                    tc_commit(&bar->empty[s2]);
+                }
+                __syncwarp();
+            }
+            if (!wait(&bar->ds_full[buf], (summed >> 1) & 1u, 413)) return false;
+            tc_fence_after();
+            if (leader) {
+                const uint64_t a = smem_desc(smem_u32(g_s + s1 * TILE_BYTES), HALF_BYTES, 1024);
+                const uint64_t bd = smem_desc(smem_u32(factors + (KEYS ? SB_P_BYTES : 0)), HALF_BYTES, 1024);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ss(acc + SB_OWN, a + (uint64_t)((kk * 2048) >> 4), bd + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
+                tc_commit(&bar->empty[s1]);
+                tc_commit(&bar->p_free[buf]);
+                if (pending & SB_LAST) tc_commit(&bar->acc_full[(sum_items - 1) & 1u]);
+            }
+            __syncwarp();
+            ++summed;
+            pending = -1;
+            return true;
+        };
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            // (where the next step is not there yet, the sums do not wait for it)
+            if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&bar->desc_full[d], (descs / SB_DESCS) & 1u))) ok = sums();
+            if (ok) ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 414);
+            if (!ok) break;
+            const int flags = bar->desc[d].flags;
+            __syncwarp();
+            if (leader) mbar_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_EMPTY) continue;
+            if (!(flags & SB_END)) {
+                if (flags & SB_FIRST) {
+                    ok = wait(&bar->f_full, items & 1u, 415);
+                    ++items;
+                }
+                const uint32_t buf = scored & 1u, s1 = (2 * scored) % SLOTS, s2 = (2 * scored + 1) % SLOTS;
+                if (ok && pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&bar->full[s1], ((2 * scored) / SLOTS) & 1u))) ok = sums();
+                // the scores of step u - 2 have been read: their P and dS, which come after, are what its sums waited for
+#pragma unroll
+                for (int g = 0; g < 2 && ok; ++g) {
+                    const uint32_t slot = g == 0 ? s1 : s2;
+                    ok = wait(&bar->full[slot], ((2 * scored + g) / SLOTS) & 1u, 416);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint64_t a = smem_desc(smem_u32(g_s + slot * TILE_BYTES), 16, 1024), f = smem_desc(smem_u32(f_s + g * SB_OWN_BYTES), 16, 1024);
+                        const uint32_t to = (g == 0 ? tm_s : tm_dp) + buf * SB_OWN;
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            mma_ss(to, a + (uint64_t)(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4), f + (uint64_t)(((kk >> 2) * (SB_OWN_BYTES / 2) + (kk & 3) * 32) >> 4), SCORE, kk > 0);
+                        tc_commit(g == 0 ? &bar->s_full[buf] : &bar->dp_full[buf]);
+                        if (!KEYS && g == 1) tc_commit(&bar->empty[slot]);       // values take no part in dQ's sum
+                        if (g == 1 && (flags & SB_LAST)) tc_commit(&bar->f_empty);
+                    }
+                    __syncwarp();
+                }
+                ++scored;
+            }
+            if (ok && pending >= 0) ok = sums();
+            if (flags & SB_END) break;
+            pending = flags;
+        }
+    } else {
+        // ================= P, dS and the finished sums =================
+        // a thread holds one met row (tensor-memory lane) and 32 owned ones (columns); warps w and w + 4 share the lanes
+        const int quarter = warp & 3, side = warp >> 2, row = quarter * 32 + lane;
+        const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
+        uint32_t descs = 0, steps = 0, items = 0;
+        int waiting = -1;                  // item whose sums are still to be written out
+        uint32_t written = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+        // one of an item's sums: channel `row` of 32 owned rows to memory, 64 consecutive bytes per warp and owned row
+        auto put = [&](int item, const uint32_t (&v)[32], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
+            const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H;
+            const int b = head / heads, h = head - b * heads, first = tile * SB_OWN + side * 32;
+            const int n = min(32, (KEYS ? p.Lkv : p.Lq) - first);
+            __nv_bfloat16 *at = to + b * sb + (long long)first * sl + h * sh + row;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j < n) at[j * sl] = __float2bfloat16_rn(__uint_as_float(v[j]) * scale);
+        };
+        auto finish = [&]() {
+            const uint32_t a = written & 1u;
+            if (!wait(&bar->acc_full[a], (written >> 1) & 1u, 421)) return false;
+            tc_fence_after();
+            uint32_t v[32];
+            const uint32_t acc = tm_acc + a * 2 * SB_OWN + side * 32 + lane_addr;
+            if (KEYS) {
+                TMEM_LD32(acc, v);
+                tmem_wait_ld32(v);
+                put(waiting, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
+            }
+            TMEM_LD32(acc + SB_OWN, v);
+            tmem_wait_ld32(v);
+            tc_fence_before();
+            warp_arrive(&bar->acc_empty[a]);
+            put(waiting, v, p.d2, p.d2b, p.d2l, p.d2h, p.scale);
+            ++written;
+            waiting = -1;
+            return true;
+        };
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 422);
+            if (!ok) break;
+            const SbDesc desc = bar->desc[d];
+            warp_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (desc.flags & SB_END) {
+                if (waiting >= 0) finish();
+                break;
+            }
+            if (desc.flags & SB_EMPTY) {
+                uint32_t zero[32] = {};
+                if (KEYS) put(desc.item, zero, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
+                put(desc.item, zero, p.d2, p.d2b, p.d2l, p.d2h, 1.0f);
+                continue;
+            }
+            if (desc.flags & SB_FIRST) {
+                if (!KEYS) ok = wait(&bar->stats_full[items & 3u], (items >> 2) & 1u, 423);
+                ++items;
+            }
+            const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
+            float norm = 0.f, delta = 0.f;
+            const float4 *own = reinterpret_cast<const float4 *>(bar->stats + ((items - 1) & 3u) * SB_OWN) + side * 16;      // queries: two owned rows each
+            if (KEYS && ok) {
+                ok = wait(&bar->full[slot], ((2 * steps) / SLOTS) & 1u, 424);
+                const float2 st = bar->stats[buf * TILE + row];
+                norm = st.x;
+                delta = st.y;
+            }
+            const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
+            if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 425);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t v[32];
+            float pr[32];
+            TMEM_LD32(tm_s + buf * SB_OWN + side * 32 + lane_addr, v);
+            tmem_wait_ld32(v);
+            const float c = p.scale_log2;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float n0 = norm, n1 = norm;
+                if (!KEYS) {
+                    const float4 st = own[j >> 1];
+                    n0 = st.x;
+                    n1 = st.z;
+                }
+                pr[j] = ex2(fmaf(__uint_as_float(v[j]), c, -n0));
+                pr[j + 1] = ex2(fmaf(__uint_as_float(v[j + 1]), c, -n1));
+                if (!KEYS && !real) pr[j] = pr[j + 1] = 0.f;
+            }
+            // the sums of step u - 2 have read the factors that lie here
+            ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 426);
+            if (!ok) break;
+            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES + row * 128;
+            auto store = [&](uint8_t *to, auto value) {       // 32 columns of the row as four 16-byte pieces, swizzled by row
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const __nv_bfloat162 x = __floats2bfloat162_rn(value(8 * q + 2 * e), value(8 * q + 2 * e + 1));
+                        w[e] = *reinterpret_cast<const uint32_t *>(&x);
+                    }
+                    *reinterpret_cast<uint4 *>(to + (((side * 4 + q) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            };
+            if (KEYS) {
+                store(factors, [&](int j) { return pr[j]; });
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                warp_arrive(&bar->p_full[buf]);
+            }
+            ok = wait(&bar->dp_full[buf], (steps >> 1) & 1u, 427);
+            if (!ok) break;
+            tc_fence_after();
+            TMEM_LD32(tm_dp + buf * SB_OWN + side * 32 + lane_addr, v);
+            tmem_wait_ld32(v);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float d0 = delta, d1 = delta;
+                if (!KEYS) {
+                    const float4 st = own[j >> 1];
+                    d0 = st.y;
+                    d1 = st.w;
+                }
+                pr[j] *= __uint_as_float(v[j]) - d0;
+                pr[j + 1] *= __uint_as_float(v[j + 1]) - d1;
+                if (!KEYS && !real) pr[j] = pr[j + 1] = 0.f;
+            }
+            store(factors + (KEYS ? SB_P_BYTES : 0), [&](int j) { return pr[j]; });
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_fence_before();
+            warp_arrive(&bar->ds_full[buf]);
+            ++steps;
+            if (waiting >= 0) ok = finish();
+            if (desc.flags & SB_LAST) waiting = desc.item;
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+static bool aligned_view(const wa_tensor4 *t) {
+    return t->ptr && (uintptr_t)t->ptr % 16 == 0 && t->stride_h % 8 == 0 && t->stride_l % 8 == 0 && t->stride_b % 8 == 0 && t->stride_h > 0 && t->stride_l > 0;
+}
+
+template <bool KEYS, int BLK>
+static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t stream) {
+    const char *what = "wa_selected_backward(tcgen05)";
+    const wa_tensor4 &f1 = KEYS ? p->k : p->q, &f2 = KEYS ? p->v : p->dout, &g1 = KEYS ? p->q : p->k, &g2 = KEYS ? p->dout : p->v;
+    const int Lf = KEYS ? p->Lkv : p->Lq, Hf = KEYS ? p->Hkv : p->H, Lg = KEYS ? p->Lq : p->Lkv, Hg = KEYS ? p->H : p->Hkv;
+    CUtensorMap maps[4];
+    int rc;
+    if ((rc = selected_sm100_map(&maps[0], &f1, p->B, Lf, Hf, "the owned rows", SB_OWN, 2))) return rc;
+    if ((rc = selected_sm100_map(&maps[1], &f2, p->B, Lf, Hf, "the owned rows", SB_OWN, 2))) return rc;
+    if ((rc = selected_sm100_map(&maps[2], &g1, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
+    if ((rc = selected_sm100_map(&maps[3], &g2, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
+    const auto kernel = selected_grad_sm100_kernel<KEYS, BLK>;
+    static PerDeviceOnce attr_set;
+    if (!attr_set.done()) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SbRing<KEYS>::SMEM);
+        if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+        attr_set.mark();
+    }
+    kp.owned = ceil_div(Lf, SB_OWN);
+    kp.items = p->B * Hf * kp.owned;
+    const wa_tensor4 &d2 = KEYS ? p->dk : p->dq;
+    kp.d1 = (__nv_bfloat16 *)p->dv.ptr; kp.d1b = p->dv.stride_b; kp.d1l = p->dv.stride_l; kp.d1h = p->dv.stride_h;
+    kp.d2 = (__nv_bfloat16 *)d2.ptr; kp.d2b = d2.stride_b; kp.d2l = d2.stride_l; kp.d2h = d2.stride_h;
+    kp.work_counter += KEYS ? 0 : 1;
+    const int sms = sm_count();
+    const cudaError_t e = launch_dependent(kernel, dim3(kp.items < sms ? kp.items : sms), dim3(SB_THREADS), SbRing<KEYS>::SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
+}
+
+}  // namespace sm100
+
+bool selected_sm100_backward_supported(const wa_selected_params *p) {
+    using namespace sm100;
+    return selected_sm100_tensors(p) && aligned_view(&p->dout) && (long long)p->B * p->H * (ceil_div(p->Lq, SB_OWN) + 1ll) <= (1 << 24) &&
+           (long long)p->B * p->Hkv * (ceil_div(p->Lkv, SB_OWN) + 1ll) <= (1 << 24);
+}
+size_t selected_sm100_backward_bytes(const wa_selected_params *) { return 256; }       // two work counters and the failure flag
+
+int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float2 *stats, void *workspace,
+                            cudaStream_t stream) {
+    using namespace sm100;
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
+    if (e != cudaSuccess) return fail((int)e, "wa_selected_backward(tcgen05): %s", cudaGetErrorString(e));
+    SbParams kp{};
+    kp.H = p->H; kp.Hkv = p->Hkv; kp.group = p->H / p->Hkv; kp.Lq = p->Lq; kp.Lkv = p->Lkv;
+    kp.Nq = ceil_div(p->Lq, p->block_size); kp.Nkv = ceil_div(p->Lkv, p->block_size);
+    kp.list_stride = p->index_stride; kp.row_words = ceil_div(kp.Nq, 32);
+    kp.padded = (long long)selected_stats_rows(p, kp.Nq);
+    kp.index = index; kp.num = num; kp.rows = rows; kp.stats = stats;
+    kp.scale = (float)pow((double)TILE, -0.5);
+    kp.scale_log2 = (float)(pow((double)TILE, -0.5) * 1.4426950408889634);
+    kp.work_counter = (int *)workspace;
+    kp.error_flag = kp.work_counter + 2;
+    kp.status_mirror = p->status_mirror;
+    int rc;
+    if (p->block_size == TILE) return (rc = launch_owned<true, TILE>(p, kp, stream)) ? rc : launch_owned<false, TILE>(p, kp, stream);
+    return (rc = launch_owned<true, HALF>(p, kp, stream)) ? rc : launch_owned<false, HALF>(p, kp, stream);
+}
+
+}  // namespace wa
