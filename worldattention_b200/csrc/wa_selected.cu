@@ -49,28 +49,72 @@ selected_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restri
 }
 
 // ---- row statistics of the gradient -----------------------------------------------------------------
-// (log-sum-exp times log2(e), sum of dout * out) of every query row, and (inf, 0) for the rows behind the last one and for rows without a key.
-// A warp per row; reads dout and out once.
-template <typename T>
+// See selected_stat.  Reads dout and out once: `LANES` lanes take a row, 16 bytes each (LANES = 0: a warp, one channel at a time, any layout), and
+// four rows are on their way at a time.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
-selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, long long all, float2 *__restrict__ stats) {
+selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, long long all, float *__restrict__ stats) {
+    constexpr int WIDE = LANES ? LANES : 32, AT_ONCE = LANES ? 4 : 1, N = 16 / sizeof(T), EACH = 256 / WIDE;
     pdl_wait();
-    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);      // (b, token, h), heads innermost as in memory
-    if (row >= all) return;
-    const int lane = threadIdx.x & 31;
-    const int h = (int)(row % H), l = (int)(row / H % padded);
-    const long long b = row / H / padded;
-    float sum = 0.f, norm = INFINITY;
-    if (l < Lq) {
-        const T *o = (const T *)out.ptr + b * out.sb + (long long)l * out.sl + (long long)h * out.sh;
-        const T *g = (const T *)dout.ptr + b * dout.sb + (long long)l * dout.sl + (long long)h * dout.sh;
-        for (int d = lane; d < D; d += 32) sum = fmaf((float)o[d], (float)g[d], sum);
-        sum = warp_sum(sum);
-        const float natural = lse[(b * H + h) * Lq + l];
-        if (natural == -INFINITY) sum = 0.f;               // nothing was listed: no key sees this row
-        else norm = natural * 1.4426950408889634f;
+    const int sub = threadIdx.x / WIDE, lane = threadIdx.x % WIDE;
+    long long row[AT_ONCE];                       // (b, token, h), heads innermost as in memory
+    long long b[AT_ONCE];
+    int h[AT_ONCE], l[AT_ONCE];
+    float sum[AT_ONCE], natural[AT_ONCE];
+    uint4 x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+        row[u] = ((long long)blockIdx.x * AT_ONCE + u) * EACH + sub;
+        const long long token = row[u] / H;
+        h[u] = (int)(row[u] - token * H);
+        b[u] = token / padded;
+        l[u] = (int)(token - b[u] * padded);
+        sum[u] = 0.f;
+        if (row[u] >= all || l[u] >= Lq) continue;
+        natural[u] = __ldg(lse + (b[u] * H + h[u]) * Lq + l[u]);
+        const T *o = (const T *)out.ptr + b[u] * out.sb + (long long)l[u] * out.sl + (long long)h[u] * out.sh;
+        const T *g = (const T *)dout.ptr + b[u] * dout.sb + (long long)l[u] * dout.sl + (long long)h[u] * dout.sh;
+        if (LANES) {
+            x[u] = __ldg(reinterpret_cast<const uint4 *>(o) + lane);
+            y[u] = __ldg(reinterpret_cast<const uint4 *>(g) + lane);
+        } else {
+            for (int d = lane; d < D; d += 32) sum[u] = fmaf((float)o[d], (float)g[d], sum[u]);
+        }
     }
-    if (lane == 0) stats[(b * H + h) * padded + l] = make_float2(norm, sum);
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+        const bool there = row[u] < all && l[u] < Lq;
+        if (LANES && there) {
+            const T *a = reinterpret_cast<const T *>(&x[u]), *c = reinterpret_cast<const T *>(&y[u]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum[u] = fmaf((float)a[e], (float)c[e], sum[u]);
+        }
+#pragma unroll
+        for (int o = WIDE / 2; o > 0; o >>= 1) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+        if (lane == 0 && row[u] < all) {
+            // a row behind the last one, or one that nothing is listed for: no key sees it
+            const bool seen = there && natural[u] != -INFINITY;
+            float *to = stats + (b[u] * H + h[u]) * padded * 2 + selected_stat(l[u]);
+            to[0] = seen ? -1.4426950408889634f * natural[u] : -INFINITY;
+            to[64] = seen ? sum[u] : 0.f;
+        }
+    }
+}
+
+template <typename T>
+static int launch_stats(const wa_selected_params *p, int padded, float *stats, cudaStream_t stream) {
+    const char *what = "wa_selected_backward";
+    const auto pieces = [](const wa_tensor4 &t) {       // rows of whole 16-byte pieces
+        constexpr int n = 16 / sizeof(T);
+        return (uintptr_t)t.ptr % 16 == 0 && t.stride_b % n == 0 && t.stride_l % n == 0 && t.stride_h % n == 0;
+    };
+    const int bytes = p->D * (int)sizeof(T), lanes = pieces(p->out) && pieces(p->dout) && (bytes == 512 || bytes == 256 || bytes == 128) ? bytes / 16 : 0;
+    const long long all = (long long)p->B * p->H * padded, each = lanes ? 4 * (256 / lanes) : 8, ctas = (all + each - 1) / each;
+    WA_REQUIRE(ctas < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+    const auto kernel = lanes == 32 ? selected_stats_kernel<T, 32> : lanes == 16 ? selected_stats_kernel<T, 16> : lanes == 8 ? selected_stats_kernel<T, 8> : selected_stats_kernel<T, 0>;
+    const cudaError_t e = launch_dependent(kernel, dim3((unsigned)ctas), dim3(256), 0, stream, make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq, p->D, padded, all, stats);
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
 }
 
 // ---- gradient, any shape ------------------------------------------------------------------------------
@@ -85,7 +129,7 @@ struct SelectedGrad {
     int H, group, Lq, Lkv, D, block, stride, Nq, Nkv, row_words, padded, tiles;
     const int32_t *index, *num, *block_sizes;
     const uint32_t *rows;
-    const float2 *stats;
+    const float *stats;
     float scale;
 };
 
@@ -116,8 +160,9 @@ selected_grad_kernel(const SelectedGrad p) {
         }
     };
     const auto bring_stats = [&](int h, int from, int end) {
+        const float *stats = p.stats + ((long long)b * p.H + h) * p.padded * 2;
         for (int r = threadIdx.x; r < T; r += 256)
-            st[r] = from + r < end ? p.stats[((long long)b * p.H + h) * p.padded + from + r] : make_float2(INFINITY, 0.f);
+            st[r] = from + r < end ? make_float2(stats[selected_stat(from + r)], stats[selected_stat(from + r) + 64]) : make_float2(-INFINITY, 0.f);
     };
     bring(f1, KEYS ? p.k : p.q, KEYS ? hk : blockIdx.y, first, own_real);
     bring(f2, KEYS ? p.v : p.dout, KEYS ? hk : blockIdx.y, first, own_real);
@@ -169,7 +214,7 @@ selected_grad_kernel(const SelectedGrad p) {
                 const int f = ty * R + i, g = tx + 16 * j;
                 const float2 row = st[KEYS ? g : f];
                 const bool there = first + f < own_real && from + g < end;
-                const float pr = there ? exp2f(fmaf(s[i][j], to_log2, -row.x)) : 0.f;
+                const float pr = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
                 ps[f * LP + g] = pr;
                 ds[f * LP + g] = there ? pr * (dp[i][j] - row.y) * p.scale : 0.f;
             }
@@ -269,7 +314,7 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     w.num = c; c = align_up(c + lists * sizeof(int32_t), 256);
     if (backward) {
         w.rows = c; c = align_up(c + (size_t)p->B * p->H * w.Nkv * w.row_words * sizeof(uint32_t), 256);
-        w.stats = c; c = align_up(c + (size_t)p->B * p->H * selected_stats_rows(p, w.Nq) * sizeof(float2), 256);
+        w.stats = c; c = align_up(c + (size_t)p->B * p->H * selected_stats_rows(p, w.Nq) * 2 * sizeof(float), 256);
     }
     w.tuned = c;
     if (backward ? selected_sm100_backward_supported(p) : selected_sm100_forward_supported(p))
@@ -360,15 +405,11 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
     if ((rc = selected_lists(p, w, true, ws, stream, what))) return rc;
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
     const uint32_t *rows = (const uint32_t *)(ws + w.rows);
-    float2 *stats = (float2 *)(ws + w.stats);
-    const int padded = (int)selected_stats_rows(p, w.Nq);
-    const long long all = (long long)p->B * p->H * padded, ctas = (all + 7) / 8;
-    WA_REQUIRE(ctas < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
-    const auto stats_kernel = p->q.dtype == WA_BF16 ? selected_stats_kernel<__nv_bfloat16> : selected_stats_kernel<float>;
-    const cudaError_t e = launch_dependent(stats_kernel, dim3((unsigned)ctas), dim3(256), 0, stream, make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq, p->D,
-                                           padded, all, stats);
-    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
-    if ((rc = check_launch(what))) return rc;
+    float *stats = (float *)(ws + w.stats);
+    const size_t stats_rows = selected_stats_rows(p, w.Nq);
+    WA_REQUIRE(stats_rows < (1ull << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+    const int padded = (int)stats_rows;
+    if ((rc = p->q.dtype == WA_BF16 ? launch_stats<__nv_bfloat16>(p, padded, stats, stream) : launch_stats<float>(p, padded, stats, stream))) return rc;
     if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, ws + w.tuned, stream);
     SelectedGrad g{};
     g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v); g.dout = make_view(&p->dout);

@@ -11,13 +11,15 @@ struct SelectedPlan {
     int Nq, Nkv, group, words, row_words;      // query / key blocks, query heads of a key head, words of a bit per key block / per query block
     size_t index, num;                         // [B, H, Nq, index_stride] clean lists, [B, H, Nq] their lengths
     size_t rows;                               // backward: [B, Hkv, Nkv, group, row_words] which query blocks of which head list a key block
-    size_t stats;                              // backward: [B, H, (Nq + 1) * block] (log-sum-exp in powers of two, sum of dout * out) of a query row
+    size_t stats;                              // backward: [B, H, selected_stats_rows] statistics of a query row, see selected_stat
     size_t tuned;                              // what the tensor-core kernels need
     size_t total;
 };
 
-// one query row of `stats`: rows that are no query's (behind the last one) have an infinite normaliser, which makes their probabilities zero
-inline size_t selected_stats_rows(const wa_selected_params *p, int Nq) { return (size_t)(Nq + 1) * p->block_size; }
+// Statistics of the query rows, 64 rows together: 64 times minus the log-sum-exp in powers of two, then 64 sums of dout * out.  Rows that are no
+// query's (behind the last one, and a block more) have an infinite normaliser, which makes their probabilities zero.
+inline size_t selected_stats_rows(const wa_selected_params *p, int Nq) { return align_up((size_t)(Nq + 1) * p->block_size, 64); }
+__host__ __device__ inline long long selected_stat(long long row) { return (row >> 6) * 128 + (row & 63); }      // the sum lies 64 behind
 
 // bf16, head_dim 128, blocks of 64 or 128 tokens.  wa_hsa_sm100.cu:
 bool selected_sm100_tensors(const wa_selected_params *p);                 // q, k, v, blocks and device
@@ -29,7 +31,7 @@ int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int 
 // wa_selected_sm100.cu:
 bool selected_sm100_backward_supported(const wa_selected_params *p);
 size_t selected_sm100_backward_bytes(const wa_selected_params *p);
-int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float2 *stats, void *workspace,
+int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats, void *workspace,
                             cudaStream_t stream);
 
 }  // namespace wa

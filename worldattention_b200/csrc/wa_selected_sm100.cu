@@ -4,16 +4,16 @@
 // for dQ -- and meets 128 rows of the other side per step: a block of 128, or two of 64 that need not be neighbours (nor, with shared
 // keys, of one query head).  With F1, F2 the owned rows and G1, G2 the met ones (keys: F = k, v and G = q, dout; queries: F = q, dout and G = k, v)
 //     S = G1 F1^T   dP = G2 F2^T                      [128 met rows x 64 owned ones]
-//     P = 2^(S c - lse)   dS = P (dP - delta)
+//     P = 2^(S c - lse)   dS = P (dP - delta)         (lse and delta of the query row: 128 of a step's, or 64 of an item's)
 //     dV^T += G2^T P   dK^T (or dQ^T) += G1^T dS      [128 channels x 64 owned rows]
 // so all four products have 128 rows and 64 columns, the met tile is the first operand of all of them as it lies (row-major for the
 // scores, transposed for the sums), and P and dS, which a thread holds by rows, are second operands that go to shared memory the
 // way they are.  The met rows' lists: bits per key block, or the clean ids of a query block.  Every sum is made in one CTA in
 // the order of its list: no atomics, equal calls give equal bits; the price is that S and dP are computed in both launches.
 //
-// One persistent CTA of ten warps per SM: warps 0-7 turn scores into P and dS and write finished sums out, warp 8 walks the lists and
-// issues the loads, warp 9 issues the products.  Scores of step u + 1 are issued before the sums of step u, so that they
-// run while the warps work on step u; tensor memory holds two steps' scores and the sums of two owned tiles (2 x 128 + 2 x 128 columns).
+// One persistent CTA of eleven warps per SM: warps 0-7 turn scores into P and dS and write finished sums out, warp 8 walks the lists and
+// issues the loads, warp 9 issues the scores' products and warp 10 the sums'.  Tensor memory holds two steps' scores and the sums of two owned
+// tiles (2 x 128 + 2 x 128 columns).
 //
 // Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
 #include "wa_selected.cuh"
@@ -26,7 +26,7 @@ constexpr int SB_OWN = 64;                              // owned rows of an item
 constexpr int SB_OWN_BYTES = SB_OWN * TILE * 2;         // 16 KB: [half of the channels][row][64 channels]
 constexpr int SB_P_BYTES = TILE * SB_OWN * 2;           // 16 KB: [met row][64 owned rows]
 constexpr int SB_DESCS = 4;
-constexpr int SB_THREADS = 320;
+constexpr int SB_THREADS = 352;
 
 template <bool KEYS> struct SbRing {
     static constexpr int SLOTS = KEYS ? 4 : 5;          // met tiles (32 KB each): G1 and G2 of a step take one each
@@ -41,13 +41,13 @@ struct SbDesc {
 };
 
 struct SbBarriers {
-    // keys: of the met rows, [two steps][128]; queries: of the owned rows, [four items][64] -- when an item's are loaded, the warps may still be two
-    // items behind
-    float2 stats[2 * TILE];
+    // 64 rows' (-normaliser) and their deltas.  keys: of the met rows, [two steps][two]; queries: of the owned rows, [four items] -- when an
+    // item's are loaded, the warps may still be two items behind
+    float stats[4 * TILE];
     uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
     uint64_t f_full, f_empty, stats_full[4];
     uint64_t full[5], empty[5];
-    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], p_free[2];
+    uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
     uint64_t acc_full[2], acc_empty[2];
     uint32_t tmem_base;
     int abort_flag;
@@ -63,7 +63,7 @@ struct SbParams {
     long long padded;                 // rows of `stats` of a head
     const int32_t *index, *num;       // queries
     const uint32_t *rows;             // keys
-    const float2 *stats;
+    const float *stats;
     __nv_bfloat16 *d1, *d2;           // dV; dK or dQ
     long long d1b, d1l, d1h, d2b, d2l, d2h;
     float scale, scale_log2;
@@ -148,7 +148,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         bar->abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
-            mbar_init(&bar->desc_empty[i], 1 + 8);       // product warp and the eight others
+            mbar_init(&bar->desc_empty[i], 2 + 8);       // the warps that issue products and the eight others
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
@@ -159,9 +159,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar->s_full[i], 1);
-            mbar_init(&bar->dp_full[i], 1);
-            mbar_init(&bar->p_full[i], 8);
-            mbar_init(&bar->ds_full[i], 8);
+            mbar_init(&bar->s_free[i], 4);
+            mbar_init(&bar->p_full[i], 4);
             mbar_init(&bar->p_free[i], 1);
             mbar_init(&bar->acc_full[i], 1);
             mbar_init(&bar->acc_empty[i], 8);
@@ -226,7 +225,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     tma_load_5d(f_s + SB_OWN_BYTES, &tm_f2, &bar->f_full, 0, tile * SB_OWN, 0, h, b);
                     if (!KEYS) {
                         mbar_expect_tx(&bar->stats_full[items & 3u], SB_OWN * 8);
-                        bulk_load(bar->stats + (items & 3u) * SB_OWN, p.stats + (long long)head * p.padded + tile * SB_OWN, SB_OWN * 8, &bar->stats_full[items & 3u]);
+                        bulk_load(bar->stats + (items & 3u) * TILE, p.stats + ((long long)head * p.padded + tile * SB_OWN) * 2, SB_OWN * 8, &bar->stats_full[items & 3u]);
                     }
                 }
                 __syncwarp();
@@ -268,10 +267,10 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                             }
                             if (with_stats) {
                                 // (the statistics of step u - 2 have been read: its sums, which come after them, freed this slot)
-                                float2 *to = bar->stats + (steps & 1u) * TILE;
-                                const float2 *row = p.stats + ((long long)b * p.H) * p.padded;
-                                bulk_load(to, row + h0 * p.padded + (long long)i0 * BLK, BLK * 8, full);
-                                if (BLK != TILE) bulk_load(to + SB_OWN, row + h1 * p.padded + (long long)i1 * BLK, BLK * 8, full);
+                                float *to = bar->stats + (steps & 1u) * 2 * TILE;
+                                const float *row = p.stats + ((long long)b * p.H) * p.padded * 2;
+                                bulk_load(to, row + (h0 * p.padded + (long long)i0 * BLK) * 2, BLK * 8, full);
+                                if (BLK != TILE) bulk_load(to + TILE, row + (h1 * p.padded + (long long)i1 * BLK) * 2, BLK * 8, full);
                             }
                         }
                         __syncwarp();
@@ -287,98 +286,100 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             while (clock64() - t0 < 2000000) { }
         }
     } else if (warp == 9) {
-        // ================= products =================
+        // ================= scores =================
+        // One thread blocks for about as long as its products run, so that its waits and commits are time in which the tensor pipe idles; the scores
+        // and the sums are issued by warps of their own, and each covers the other's.
         const bool leader = elect_one();
-        constexpr uint32_t SCORE = instr_desc(false, SB_OWN), SUM = instr_desc(true, SB_OWN) | (1u << 15);      // both operands of the sums are transposed
-        uint32_t descs = 0, items = 0, scored = 0, summed = 0;
+        constexpr uint32_t SCORE = instr_desc(false, SB_OWN);
+        uint32_t descs = 0, items = 0, steps = 0;
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
-        int pending = -1;                 // flags of the step whose sums are still to be issued
-        uint32_t sum_items = 0;           // items whose sums have begun
-        auto sums = [&]() {
-            const uint32_t buf = summed & 1u, s1 = (2 * summed) % SLOTS, s2 = (2 * summed + 1) % SLOTS;
-            if (pending & SB_FIRST) {
-                if (!wait(&bar->acc_empty[sum_items & 1u], ((sum_items >> 1) & 1u) ^ 1u, 411)) return false;
-                ++sum_items;
-            }
-            const uint32_t acc = tm_acc + ((sum_items - 1) & 1u) * 2 * SB_OWN;
-            const bool fresh = pending & SB_FIRST;
-            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES;
-            if (KEYS) {
-                if (!wait(&bar->p_full[buf], (summed >> 1) & 1u, 412)) return false;
-                tc_fence_after();
-                if (leader) {
-                    const uint64_t a = smem_desc(smem_u32(g_s + s2 * TILE_BYTES), HALF_BYTES, 1024), bd = smem_desc(smem_u32(factors), HALF_BYTES, 1024);
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        mma_ss(acc, a + (uint64_t)((kk * 2048) >> 4), bd + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
-                    tc_commit(&bar->empty[s2]);
-                }
-                __syncwarp();
-            }
-            if (!wait(&bar->ds_full[buf], (summed >> 1) & 1u, 413)) return false;
-            tc_fence_after();
-            if (leader) {
-                const uint64_t a = smem_desc(smem_u32(g_s + s1 * TILE_BYTES), HALF_BYTES, 1024);
-                const uint64_t bd = smem_desc(smem_u32(factors + (KEYS ? SB_P_BYTES : 0)), HALF_BYTES, 1024);
-#pragma unroll
-                for (int kk = 0; kk < 8; ++kk)
-                    mma_ss(acc + SB_OWN, a + (uint64_t)((kk * 2048) >> 4), bd + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
-                tc_commit(&bar->empty[s1]);
-                tc_commit(&bar->p_free[buf]);
-                if (pending & SB_LAST) tc_commit(&bar->acc_full[(sum_items - 1) & 1u]);
-            }
-            __syncwarp();
-            ++summed;
-            pending = -1;
-            return true;
-        };
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
-            // (where the next step is not there yet, the sums do not wait for it)
-            if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&bar->desc_full[d], (descs / SB_DESCS) & 1u))) ok = sums();
-            if (ok) ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 414);
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 411);
             if (!ok) break;
             const int flags = bar->desc[d].flags;
             __syncwarp();
             if (leader) mbar_arrive(&bar->desc_empty[d]);
             ++descs;
-            if (flags & SB_EMPTY) continue;
-            if (!(flags & SB_END)) {
-                if (flags & SB_FIRST) {
-                    ok = wait(&bar->f_full, items & 1u, 415);
-                    ++items;
-                }
-                const uint32_t buf = scored & 1u, s1 = (2 * scored) % SLOTS, s2 = (2 * scored + 1) % SLOTS;
-                if (ok && pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&bar->full[s1], ((2 * scored) / SLOTS) & 1u))) ok = sums();
-                // the scores of step u - 2 have been read: their P and dS, which come after, are what its sums waited for
-#pragma unroll
-                for (int g = 0; g < 2 && ok; ++g) {
-                    const uint32_t slot = g == 0 ? s1 : s2;
-                    ok = wait(&bar->full[slot], ((2 * scored + g) / SLOTS) & 1u, 416);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint64_t a = smem_desc(smem_u32(g_s + slot * TILE_BYTES), 16, 1024), f = smem_desc(smem_u32(f_s + g * SB_OWN_BYTES), 16, 1024);
-                        const uint32_t to = (g == 0 ? tm_s : tm_dp) + buf * SB_OWN;
-#pragma unroll
-                        for (int kk = 0; kk < 8; ++kk)
-                            mma_ss(to, a + (uint64_t)(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4), f + (uint64_t)(((kk >> 2) * (SB_OWN_BYTES / 2) + (kk & 3) * 32) >> 4), SCORE, kk > 0);
-                        tc_commit(g == 0 ? &bar->s_full[buf] : &bar->dp_full[buf]);
-                        if (!KEYS && g == 1) tc_commit(&bar->empty[slot]);       // values take no part in dQ's sum
-                        if (g == 1 && (flags & SB_LAST)) tc_commit(&bar->f_empty);
-                    }
-                    __syncwarp();
-                }
-                ++scored;
-            }
-            if (ok && pending >= 0) ok = sums();
             if (flags & SB_END) break;
-            pending = flags;
+            if (flags & SB_EMPTY) continue;
+            if (flags & SB_FIRST) {
+                ok = wait(&bar->f_full, items & 1u, 412);
+                ++items;
+            }
+            const uint32_t buf = steps & 1u;
+#pragma unroll
+            for (int g = 0; g < 2 && ok; ++g) {
+                const uint32_t slot = (2 * steps + g) % SLOTS;
+                ok = wait(&bar->full[slot], ((2 * steps + g) / SLOTS) & 1u, 413);
+                if (ok && g == 0) ok = wait(&bar->s_free[buf], ((steps >> 1) & 1u) ^ 1u, 414);      // the scores of step u - 2 have been read
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t a = smem_desc(smem_u32(g_s + slot * TILE_BYTES), 16, 1024), f = smem_desc(smem_u32(f_s + g * SB_OWN_BYTES), 16, 1024);
+                    const uint32_t to = (g == 0 ? tm_s : tm_dp) + buf * SB_OWN;
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        mma_ss(to, a + (uint64_t)(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4), f + (uint64_t)(((kk >> 2) * (SB_OWN_BYTES / 2) + (kk & 3) * 32) >> 4), SCORE, kk > 0);
+                    if (g == 1) tc_commit(&bar->s_full[buf]);
+                    if (!KEYS && g == 1) tc_commit(&bar->empty[slot]);       // values take no part in dQ's sum
+                    if (g == 1 && (flags & SB_LAST)) tc_commit(&bar->f_empty);
+                }
+                __syncwarp();
+            }
+            ++steps;
+        }
+    } else if (warp == 10) {
+        // ================= sums =================
+        const bool leader = elect_one();
+        constexpr uint32_t SUM = instr_desc(true, SB_OWN) | (1u << 15);      // both operands transposed
+        uint32_t descs = 0, items = 0, steps = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 415);
+            if (!ok) break;
+            const int flags = bar->desc[d].flags;
+            __syncwarp();
+            if (leader) mbar_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+            if (flags & SB_EMPTY) continue;
+            const bool fresh = flags & SB_FIRST;
+            if (fresh) {
+                ok = wait(&bar->acc_empty[items & 1u], ((items >> 1) & 1u) ^ 1u, 416);
+                ++items;
+            }
+            const uint32_t buf = steps & 1u, s1 = (2 * steps) % SLOTS, s2 = (2 * steps + 1) % SLOTS, last = (items - 1) & 1u;
+            const uint32_t acc = tm_acc + last * 2 * SB_OWN;
+            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES;
+            auto add = [&](uint32_t to, uint32_t slot, const uint8_t *factor) {
+                const uint64_t a = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024), f = smem_desc(smem_u32(factor), HALF_BYTES, 1024);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) mma_ss(to, a + (uint64_t)((kk * 2048) >> 4), f + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
+            };
+            if (ok) ok = wait(&bar->p_full[buf], (steps >> 1) & 1u, 417);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+                if (KEYS) add(acc, s2, factors);
+                add(acc + SB_OWN, s1, factors + (KEYS ? SB_P_BYTES : 0));
+                // (the factors were made from both scores: those have read their tiles too)
+                tc_commit(&bar->empty[s1]);
+                if (KEYS) tc_commit(&bar->empty[s2]);
+                tc_commit(&bar->p_free[buf]);
+                if (flags & SB_LAST) tc_commit(&bar->acc_full[last]);
+            }
+            __syncwarp();
+            ++steps;
         }
     } else {
         // ================= P, dS and the finished sums =================
-        // a thread holds one met row (tensor-memory lane) and 32 owned ones (columns); warps w and w + 4 share the lanes
+        // Two groups of four warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
+        // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and takes its 64 columns 16 at a time, the next
+        // 16 on their way, in a loop short enough for the instruction cache.  Finished sums are written by both groups, 32 columns each.
         const int quarter = warp & 3, side = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
         uint32_t descs = 0, steps = 0, items = 0;
@@ -437,81 +438,86 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 if (!KEYS) ok = wait(&bar->stats_full[items & 3u], (items >> 2) & 1u, 423);
                 ++items;
             }
-            const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
-            float norm = 0.f, delta = 0.f;
-            const float4 *own = reinterpret_cast<const float4 *>(bar->stats + ((items - 1) & 3u) * SB_OWN) + side * 16;      // queries: two owned rows each
-            if (KEYS && ok) {
-                ok = wait(&bar->full[slot], ((2 * steps) / SLOTS) & 1u, 424);
-                const float2 st = bar->stats[buf * TILE + row];
-                norm = st.x;
-                delta = st.y;
-            }
-            const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
-            if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 425);
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t v[32];
-            float pr[32];
-            TMEM_LD32(tm_s + buf * SB_OWN + side * 32 + lane_addr, v);
-            tmem_wait_ld32(v);
-            const float c = p.scale_log2;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                float n0 = norm, n1 = norm;
-                if (!KEYS) {
-                    const float4 st = own[j >> 1];
-                    n0 = st.x;
-                    n1 = st.z;
+            if ((steps & 1u) == (uint32_t)side && ok) {
+                const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
+                // (-normaliser, delta) of the met row, or of the owned rows: 64 of one, 64 of the other
+                const float *st = bar->stats + (KEYS ? buf * 2 * TILE + (row >> 6) * TILE + (row & 63) : ((items - 1) & 3u) * TILE);
+                float2 norm = make_float2(0.f, 0.f), delta = norm;
+                if (KEYS) {
+                    ok = wait(&bar->full[slot], ((2 * steps) / SLOTS) & 1u, 424);
+                    norm = make_float2(st[0], st[0]);
+                    delta = make_float2(-st[SB_OWN], -st[SB_OWN]);
                 }
-                pr[j] = ex2(fmaf(__uint_as_float(v[j]), c, -n0));
-                pr[j + 1] = ex2(fmaf(__uint_as_float(v[j + 1]), c, -n1));
-                if (!KEYS && !real) pr[j] = pr[j + 1] = 0.f;
-            }
-            // the sums of step u - 2 have read the factors that lie here
-            ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 426);
-            if (!ok) break;
-            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES + row * 128;
-            auto store = [&](uint8_t *to, auto value) {       // 32 columns of the row as four 16-byte pieces, swizzled by row
+                // queries: rows that are no keys
+                const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
+                // the sums of step u - 2 have read the factors that lie here
+                if (ok) ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
+                if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 426);
+                if (!ok) break;
+                tc_fence_after();
+                uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES + row * 128;
+                const uint32_t s_at = tm_s + buf * SB_OWN + lane_addr, dp_at = tm_dp + buf * SB_OWN + lane_addr;
+                const float2 c = make_float2(p.scale_log2, p.scale_log2);
+                uint32_t sv[2][16], dv[2][16];
+                // 16 columns: P and dS to shared memory, two 16-byte pieces of each, swizzled by row
+                auto turn = [&](const uint32_t (&x)[16], const uint32_t (&y)[16], int col) {
+                    uint32_t pw[8], dw[8];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t w[4];
+                    for (int j = 0; j < 16; j += 4) {
+                        float4 n4 = make_float4(norm.x, norm.x, norm.x, norm.x), d4;
+                        if (!KEYS) {
+                            n4 = *reinterpret_cast<const float4 *>(st + col + j);
+                            d4 = *reinterpret_cast<const float4 *>(st + SB_OWN + col + j);
+                        }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const __nv_bfloat162 x = __floats2bfloat162_rn(value(8 * q + 2 * e), value(8 * q + 2 * e + 1));
-                        w[e] = *reinterpret_cast<const uint32_t *>(&x);
+                        for (int e = 0; e < 4; e += 2) {
+                            const float2 n = e == 0 ? make_float2(n4.x, n4.y) : make_float2(n4.z, n4.w);
+                            const float2 d = KEYS ? delta : e == 0 ? make_float2(-d4.x, -d4.y) : make_float2(-d4.z, -d4.w);
+                            const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[j + e]), __uint_as_float(x[j + e + 1])), c, n);
+                            float2 pr = make_float2(ex2(z.x), ex2(z.y));
+                            float2 ds = __fmul2_rn(pr, __fadd2_rn(make_float2(__uint_as_float(y[j + e]), __uint_as_float(y[j + e + 1])), d));
+                            if (!KEYS && !real) ds = make_float2(0.f, 0.f);
+                            const __nv_bfloat162 hp = __floats2bfloat162_rn(pr.x, pr.y), hd = __floats2bfloat162_rn(ds.x, ds.y);
+                            if (KEYS) pw[(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
+                            dw[(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hd);
+                        }
                     }
-                    *reinterpret_cast<uint4 *>(to + (((side * 4 + q) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint8_t *to = factors + ((((col >> 3) + q) ^ (row & 7)) << 4);
+                        if (KEYS) *reinterpret_cast<uint4 *>(to) = make_uint4(pw[4 * q], pw[4 * q + 1], pw[4 * q + 2], pw[4 * q + 3]);
+                        *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dw[4 * q], dw[4 * q + 1], dw[4 * q + 2], dw[4 * q + 3]);
+                    }
+                };
+                TMEM_LD16(s_at, sv[0]);
+                TMEM_LD16(dp_at, dv[0]);
+#pragma unroll 1
+                for (int col = 0; col < SB_OWN; col += 32) {
+                    tmem_wait_ld16(sv[0]);
+                    tmem_wait_ld16(dv[0]);
+                    TMEM_LD16(s_at + col + 16, sv[1]);
+                    TMEM_LD16(dp_at + col + 16, dv[1]);
+                    turn(sv[0], dv[0], col);
+                    tmem_wait_ld16(sv[1]);
+                    tmem_wait_ld16(dv[1]);
+                    if (col + 32 < SB_OWN) {
+                        TMEM_LD16(s_at + col + 32, sv[0]);
+                        TMEM_LD16(dp_at + col + 32, dv[0]);
+                    } else {
+                        tc_fence_before();
+                        warp_arrive(&bar->s_free[buf]);
+                    }
+                    turn(sv[1], dv[1], col + 16);
                 }
-            };
-            if (KEYS) {
-                store(factors, [&](int j) { return pr[j]; });
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&bar->p_full[buf]);
+                if (waiting >= 0) ok = finish();
             }
-            ok = wait(&bar->dp_full[buf], (steps >> 1) & 1u, 427);
-            if (!ok) break;
-            tc_fence_after();
-            TMEM_LD32(tm_dp + buf * SB_OWN + side * 32 + lane_addr, v);
-            tmem_wait_ld32(v);
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                float d0 = delta, d1 = delta;
-                if (!KEYS) {
-                    const float4 st = own[j >> 1];
-                    d0 = st.y;
-                    d1 = st.w;
-                }
-                pr[j] *= __uint_as_float(v[j]) - d0;
-                pr[j + 1] *= __uint_as_float(v[j + 1]) - d1;
-                if (!KEYS && !real) pr[j] = pr[j + 1] = 0.f;
-            }
-            store(factors + (KEYS ? SB_P_BYTES : 0), [&](int j) { return pr[j]; });
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            tc_fence_before();
-            warp_arrive(&bar->ds_full[buf]);
             ++steps;
-            if (waiting >= 0) ok = finish();
-            if (desc.flags & SB_LAST) waiting = desc.item;
+            if (desc.flags & SB_LAST) {
+                if (ok && waiting >= 0) ok = finish();       // (an item of one step, which the other group took)
+                waiting = desc.item;
+            }
         }
         tc_fence_before();
     }
@@ -563,7 +569,7 @@ bool selected_sm100_backward_supported(const wa_selected_params *p) {
 }
 size_t selected_sm100_backward_bytes(const wa_selected_params *) { return 256; }       // two work counters and the failure flag
 
-int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float2 *stats, void *workspace,
+int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats, void *workspace,
                             cudaStream_t stream) {
     using namespace sm100;
     const cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
