@@ -11,8 +11,8 @@
 // way they are.  The met rows' lists: bits per key block, or the clean ids of a query block.  Every sum is made in one CTA in
 // the order of its list: no atomics, equal calls give equal bits; the price is that S and dP are computed in both launches.
 //
-// One persistent CTA of eleven warps per SM: warps 0-7 turn scores into P and dS and write finished sums out, warp 8 walks the lists and
-// issues the loads, warp 9 issues the scores' products and warp 10 the sums'.  Tensor memory holds two steps' scores and the sums of two owned
+// One persistent CTA of nineteen warps per SM: sixteen turn scores into P and dS and write finished sums out, one walks the lists and
+// issues the loads, one issues the scores' products and one the sums'.  Tensor memory holds two steps' scores and the sums of two owned
 // tiles (2 x 128 + 2 x 128 columns).
 //
 // Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
@@ -26,7 +26,8 @@ constexpr int SB_OWN = 64;                              // owned rows of an item
 constexpr int SB_OWN_BYTES = SB_OWN * TILE * 2;         // 16 KB: [half of the channels][row][64 channels]
 constexpr int SB_P_BYTES = TILE * SB_OWN * 2;           // 16 KB: [met row][64 owned rows]
 constexpr int SB_DESCS = 4;
-constexpr int SB_THREADS = 352;
+constexpr int SB_WORKERS = 16;                          // warps that make P and dS
+constexpr int SB_THREADS = (SB_WORKERS + 3) * 32;
 
 template <bool KEYS> struct SbRing {
     static constexpr int SLOTS = KEYS ? 4 : 5;          // met tiles (32 KB each): G1 and G2 of a step take one each
@@ -148,7 +149,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         bar->abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
-            mbar_init(&bar->desc_empty[i], 2 + 8);       // the warps that issue products and the eight others
+            mbar_init(&bar->desc_empty[i], 2 + SB_WORKERS);       // the warps that issue products, and the workers
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
@@ -159,15 +160,15 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar->s_full[i], 1);
-            mbar_init(&bar->s_free[i], 4);
-            mbar_init(&bar->p_full[i], 4);
+            mbar_init(&bar->s_free[i], SB_WORKERS / 2);
+            mbar_init(&bar->p_full[i], SB_WORKERS / 2);
             mbar_init(&bar->p_free[i], 1);
             mbar_init(&bar->acc_full[i], 1);
-            mbar_init(&bar->acc_empty[i], 8);
+            mbar_init(&bar->acc_empty[i], SB_WORKERS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == SB_WORKERS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -179,7 +180,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     // columns: S of two steps, dP of two steps, then the sums of two items (each dV^T, dK^T or dQ^T)
     const uint32_t tm_s = tmem, tm_dp = tmem + 2 * SB_OWN, tm_acc = tmem + 4 * SB_OWN;
 
-    if (warp == 8) {
+    if (warp == SB_WORKERS) {
         // ================= lists and loads =================
         const bool leader = elect_one();
         uint32_t descs = 0, tiles = 0, items = 0, steps = 0;       // so many so far
@@ -285,7 +286,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             const long long t0 = clock64();
             while (clock64() - t0 < 2000000) { }
         }
-    } else if (warp == 9) {
+    } else if (warp == SB_WORKERS + 1) {
         // ================= scores =================
         // One thread blocks for about as long as its products run, so that its waits and commits are time in which the tensor pipe idles; the scores
         // and the sums are issued by warps of their own, and each covers the other's.
@@ -330,7 +331,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             }
             ++steps;
         }
-    } else if (warp == 10) {
+    } else if (warp == SB_WORKERS + 2) {
         // ================= sums =================
         const bool leader = elect_one();
         constexpr uint32_t SUM = instr_desc(true, SB_OWN) | (1u << 15);      // both operands transposed
@@ -377,39 +378,39 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         }
     } else {
         // ================= P, dS and the finished sums =================
-        // Two groups of four warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
-        // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and takes its 64 columns 16 at a time, the next
-        // 16 on their way, in a loop short enough for the instruction cache.  Finished sums are written by both groups, 32 columns each.
-        const int quarter = warp & 3, side = warp >> 2, row = quarter * 32 + lane;
+        // Two groups of eight warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
+        // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and 32 of its 64 columns, 16 at a time.
+        // Finished sums are written by all warps, 16 columns each.
+        const int quarter = warp & 3, half = (warp >> 2) & 1, group = warp >> 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
         uint32_t descs = 0, steps = 0, items = 0;
         int waiting = -1;                  // item whose sums are still to be written out
         uint32_t written = 0;
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
-        // one of an item's sums: channel `row` of 32 owned rows to memory, 64 consecutive bytes per warp and owned row
-        auto put = [&](int item, const uint32_t (&v)[32], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
+        // one of an item's sums: channel `row` of 16 owned rows to memory, 64 consecutive bytes per warp and owned row
+        auto put = [&](int item, const uint32_t (&v)[16], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
             const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H;
-            const int b = head / heads, h = head - b * heads, first = tile * SB_OWN + side * 32;
-            const int n = min(32, (KEYS ? p.Lkv : p.Lq) - first);
+            const int b = head / heads, h = head - b * heads, first = tile * SB_OWN + part * 16;
+            const int n = min(16, (KEYS ? p.Lkv : p.Lq) - first);
             __nv_bfloat16 *at = to + b * sb + (long long)first * sl + h * sh + row;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 16; ++j)
                 if (j < n) at[j * sl] = __float2bfloat16_rn(__uint_as_float(v[j]) * scale);
         };
         auto finish = [&]() {
             const uint32_t a = written & 1u;
             if (!wait(&bar->acc_full[a], (written >> 1) & 1u, 421)) return false;
             tc_fence_after();
-            uint32_t v[32];
-            const uint32_t acc = tm_acc + a * 2 * SB_OWN + side * 32 + lane_addr;
+            uint32_t v[16];
+            const uint32_t acc = tm_acc + a * 2 * SB_OWN + part * 16 + lane_addr;
             if (KEYS) {
-                TMEM_LD32(acc, v);
-                tmem_wait_ld32(v);
+                TMEM_LD16(acc, v);
+                tmem_wait_ld16(v);
                 put(waiting, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
             }
-            TMEM_LD32(acc + SB_OWN, v);
-            tmem_wait_ld32(v);
+            TMEM_LD16(acc + SB_OWN, v);
+            tmem_wait_ld16(v);
             tc_fence_before();
             warp_arrive(&bar->acc_empty[a]);
             put(waiting, v, p.d2, p.d2b, p.d2l, p.d2h, p.scale);
@@ -429,7 +430,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 break;
             }
             if (desc.flags & SB_EMPTY) {
-                uint32_t zero[32] = {};
+                uint32_t zero[16] = {};
                 if (KEYS) put(desc.item, zero, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
                 put(desc.item, zero, p.d2, p.d2b, p.d2l, p.d2h, 1.0f);
                 continue;
@@ -438,7 +439,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 if (!KEYS) ok = wait(&bar->stats_full[items & 3u], (items >> 2) & 1u, 423);
                 ++items;
             }
-            if ((steps & 1u) == (uint32_t)side && ok) {
+            if ((steps & 1u) == (uint32_t)group && ok) {
                 const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
                 // (-normaliser, delta) of the met row, or of the owned rows: 64 of one, 64 of the other
                 const float *st = bar->stats + (KEYS ? buf * 2 * TILE + (row >> 6) * TILE + (row & 63) : ((items - 1) & 3u) * TILE);
@@ -458,7 +459,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES + row * 128;
                 const uint32_t s_at = tm_s + buf * SB_OWN + lane_addr, dp_at = tm_dp + buf * SB_OWN + lane_addr;
                 const float2 c = make_float2(p.scale_log2, p.scale_log2);
-                uint32_t sv[2][16], dv[2][16];
+                uint32_t sv[16], dv[16];
                 // 16 columns: P and dS to shared memory, two 16-byte pieces of each, swizzled by row
                 auto turn = [&](const uint32_t (&x)[16], const uint32_t (&y)[16], int col) {
                     uint32_t pw[8], dw[8];
@@ -489,25 +490,17 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                         *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dw[4 * q], dw[4 * q + 1], dw[4 * q + 2], dw[4 * q + 3]);
                     }
                 };
-                TMEM_LD16(s_at, sv[0]);
-                TMEM_LD16(dp_at, dv[0]);
 #pragma unroll 1
-                for (int col = 0; col < SB_OWN; col += 32) {
-                    tmem_wait_ld16(sv[0]);
-                    tmem_wait_ld16(dv[0]);
-                    TMEM_LD16(s_at + col + 16, sv[1]);
-                    TMEM_LD16(dp_at + col + 16, dv[1]);
-                    turn(sv[0], dv[0], col);
-                    tmem_wait_ld16(sv[1]);
-                    tmem_wait_ld16(dv[1]);
-                    if (col + 32 < SB_OWN) {
-                        TMEM_LD16(s_at + col + 32, sv[0]);
-                        TMEM_LD16(dp_at + col + 32, dv[0]);
-                    } else {
+                for (int col = half * 32; col < half * 32 + 32; col += 16) {
+                    TMEM_LD16(s_at + col, sv);
+                    TMEM_LD16(dp_at + col, dv);
+                    tmem_wait_ld16(sv);
+                    tmem_wait_ld16(dv);
+                    if (col & 16) {
                         tc_fence_before();
                         warp_arrive(&bar->s_free[buf]);
                     }
-                    turn(sv[1], dv[1], col + 16);
+                    turn(sv, dv, col);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&bar->p_full[buf]);
@@ -523,7 +516,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     }
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == SB_WORKERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 static bool aligned_view(const wa_tensor4 *t) {
