@@ -6,9 +6,8 @@
 // of different grids, text between pictures and single tokens share a call.  The gradient is the same turn with -sin.
 // Arithmetic in float32, one rounding at the end.
 //
-// Bound: HBM, each value read once and written once.  A token is one warp's work: a lane looks the cosines and sines of its pairs up
-// once (they come from L2) and keeps them for all heads of q and k, whose 16-byte vectors are four at a time in flight.
-// Calls of few tokens spread the heads over more warps.
+// Bound: HBM, each value read once and written once.  A warp takes 2 KB of a token: its loads leave first, then the lanes look the cosines and sines
+// of their pairs up (from L2, or from what a warp beside fetched for other heads of the token).
 #include "wa_common.cuh"
 
 namespace wa {
@@ -28,8 +27,10 @@ struct AxialRope {
     long long psb, psl;               // elements between samples (0: the same for all) and between tokens
     const float2 *table;              // [rows, pairs] (cos, sin)
     float sign;                       // of the angle
-    int groups, per_warp;             // vector form: head groups of all tensors, and how many of them a warp takes
+    int groups, groups_of[AR_TENSORS], parts;     // vector form: head groups of all tensors and of each, warps of a token
 };
+
+constexpr int ar_groups(bool interleaved) { return interleaved ? 4 : 2; }        // head groups of a warp: four vectors of a lane
 
 // cos and sin of a pair; a position outside the table gives NaN, so that it shows in the result instead of some row's angle
 __device__ __forceinline__ float2 ar_turn(const AxialRope &p, const int32_t *pos, int pair) {
@@ -76,67 +77,64 @@ template <typename T, bool INTER>
 __global__ void __launch_bounds__(AR_WARPS * 32)
 axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
     using V = ArVec<T>;
-    constexpr int N = V::N, TURNS = INTER ? N / 2 : N, AT_ONCE = INTER ? 4 : 2;
+    constexpr int N = V::N, TURNS = INTER ? N / 2 : N, AT_ONCE = ar_groups(INTER);
     pdl_wait();
-    const long long token = (long long)blockIdx.x * AR_WARPS + (threadIdx.x >> 5);
+    const long long work = (long long)blockIdx.x * AR_WARPS + (threadIdx.x >> 5), token = work / p.parts;
     if (token >= p.tokens) return;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, part = (int)(work - token * p.parts);
     const int b = (int)(token / p.L), l = (int)(token - (long long)b * p.L);
-    const int32_t *pos = p.positions + b * p.psb + l * p.psl;
-    const int per_head = (INTER ? p.D : p.pairs) / N, at_once = 32 / per_head;      // lanes a head takes, heads a warp takes at a time
+    const int per_head = (INTER ? p.D : p.pairs) / N, at_once = 32 / per_head;      // lanes a head takes, heads a group holds
     const int sub = lane / per_head, c = lane - sub * per_head;                     // head within the group, vector within the head
+    const T *src[AT_ONCE];
+    T *dst[AT_ONCE];
+    uint4 v[AT_ONCE], w[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+        src[u] = nullptr;
+        int g = part * AT_ONCE + u, t = 0;
+        if (g < p.groups) {
+            while (t < p.tensors - 1 && g >= p.groups_of[t]) g -= p.groups_of[t++];
+            const int h = g * at_once + sub;
+            if (sub < at_once && h < p.heads[t]) {
+                src[u] = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh + c * N;
+                dst[u] = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t] + c * N;
+                v[u] = *reinterpret_cast<const uint4 *>(src[u]);
+                if (!INTER) w[u] = *reinterpret_cast<const uint4 *>(src[u] + p.pairs);
+            }
+        }
+    }
+    const int32_t *pos = p.positions + b * p.psb + l * p.psl;
     float2 turn[TURNS];
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
         const int pair = c * TURNS + i;
         turn[i] = sub < at_once && pair < p.pairs ? ar_turn(p, pos, pair) : make_float2(1.f, 0.f);
     }
-    const int first = blockIdx.y * p.per_warp, last = min(first + p.per_warp, p.groups);
-    for (int g0 = first; g0 < last; g0 += AT_ONCE) {
-        const T *src[AT_ONCE];
-        T *dst[AT_ONCE];
-        uint4 v[AT_ONCE], w[AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            src[u] = nullptr;
-            int g = g0 + u, t = 0;
-            if (g < last) {
-                while (t < p.tensors - 1 && g >= (p.heads[t] + at_once - 1) / at_once) g -= (p.heads[t] + at_once - 1) / at_once, ++t;
-                const int h = g * at_once + sub;
-                if (sub < at_once && h < p.heads[t]) {
-                    src[u] = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh + c * N;
-                    dst[u] = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t] + c * N;
-                    v[u] = *reinterpret_cast<const uint4 *>(src[u]);
-                    if (!INTER) w[u] = *reinterpret_cast<const uint4 *>(src[u] + p.pairs);
-                }
+    for (int u = 0; u < AT_ONCE; ++u) {
+        if (!src[u]) continue;
+        float x[N], y[N], r[N], s[N];
+        V::get(v[u], x);
+        if (INTER) {
+#pragma unroll
+            for (int i = 0; i < TURNS; ++i) {
+                const bool turned = c * TURNS + i < p.pairs;
+                r[2 * i] = turned ? fmaf(x[2 * i], turn[i].x, -x[2 * i + 1] * turn[i].y) : x[2 * i];
+                r[2 * i + 1] = turned ? fmaf(x[2 * i], turn[i].y, x[2 * i + 1] * turn[i].x) : x[2 * i + 1];
             }
-        }
+            *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
+        } else {
+            V::get(w[u], y);
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            if (!src[u]) continue;
-            float x[N], y[N], r[N], s[N];
-            V::get(v[u], x);
-            if (INTER) {
-#pragma unroll
-                for (int i = 0; i < TURNS; ++i) {
-                    const bool turned = c * TURNS + i < p.pairs;
-                    r[2 * i] = turned ? fmaf(x[2 * i], turn[i].x, -x[2 * i + 1] * turn[i].y) : x[2 * i];
-                    r[2 * i + 1] = turned ? fmaf(x[2 * i], turn[i].y, x[2 * i + 1] * turn[i].x) : x[2 * i + 1];
-                }
-                *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
-            } else {
-                V::get(w[u], y);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    r[i] = fmaf(x[i], turn[i].x, -y[i] * turn[i].y);
-                    s[i] = fmaf(x[i], turn[i].y, y[i] * turn[i].x);
-                }
-                *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
-                *reinterpret_cast<uint4 *>(dst[u] + p.pairs) = V::put(s);
-                // channels behind the turned ones
-                for (int d = 2 * p.pairs; d < p.D - c * N; d += p.pairs)
-                    *reinterpret_cast<uint4 *>(dst[u] + d) = *reinterpret_cast<const uint4 *>(src[u] + d);
+            for (int i = 0; i < N; ++i) {
+                r[i] = fmaf(x[i], turn[i].x, -y[i] * turn[i].y);
+                s[i] = fmaf(x[i], turn[i].y, y[i] * turn[i].x);
             }
+            *reinterpret_cast<uint4 *>(dst[u]) = V::put(r);
+            *reinterpret_cast<uint4 *>(dst[u] + p.pairs) = V::put(s);
+            // channels behind the turned ones
+            for (int d = 2 * p.pairs; d < p.D - c * N; d += p.pairs)
+                *reinterpret_cast<uint4 *>(dst[u] + d) = *reinterpret_cast<const uint4 *>(src[u] + d);
         }
     }
 }
@@ -208,7 +206,7 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
         p.out[t] = out[t].ptr; p.ob[t] = out[t].stride_b; p.ol[t] = out[t].stride_l; p.oh[t] = out[t].stride_h;
         p.heads[t] = heads[t];
         all_heads += heads[t];
-        if (vec) groups += ceil_div(heads[t], 32 / (unit / n));
+        if (vec) groups += p.groups_of[t] = ceil_div(heads[t], 32 / (unit / n));
         const uintptr_t places = (uintptr_t)x[t].ptr | (uintptr_t)out[t].ptr;
         const int64_t steps = x[t].stride_b | x[t].stride_l | x[t].stride_h | out[t].stride_b | out[t].stride_l | out[t].stride_h;
         vec = vec && places % 16 == 0 && steps % n == 0;
@@ -218,18 +216,14 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
     WA_REQUIRE((uintptr_t)table % 8 == 0 && (uintptr_t)positions % 4 == 0, WA_ERR_ALIGN, "%s: the table must be 8-byte aligned", what);
     cudaError_t e;
     if (vec) {
-        const long long ctas = (p.tokens + AR_WARPS - 1) / AR_WARPS;
+        const int each = ar_groups(interleaved != 0);
+        const long long parts = (groups + each - 1) / each, ctas = (p.tokens * parts + AR_WARPS - 1) / AR_WARPS;
         WA_REQUIRE(ctas < (1ll << 31) && groups < (1 << 20), WA_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
-        // all heads of a token by one warp once there are warps enough for the chip (the look-ups are then shared by all heads); else spread
         p.groups = (int)groups;
-        const long long spread = (148ll * 16 + p.tokens - 1) / p.tokens;
-        p.per_warp = (int)(groups / spread);
-        if (p.per_warp < 1) p.per_warp = 1;
-        const dim3 grid((unsigned)ctas, (unsigned)ceil_div(p.groups, p.per_warp));
-        WA_REQUIRE(grid.y <= 65535, WA_ERR_UNSUPPORTED, "%s: too many heads", what);
+        p.parts = (int)parts;
         const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_vec_kernel<__nv_bfloat16, true> : axial_rope_vec_kernel<__nv_bfloat16, false>)
                                              : (interleaved ? axial_rope_vec_kernel<float, true> : axial_rope_vec_kernel<float, false>);
-        e = launch_dependent(kernel, grid, dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
+        e = launch_dependent(kernel, dim3((unsigned)ctas), dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
     } else {
         const long long want = (p.tokens * all_heads * (D - pairs) + 255) / 256, most = 32ll * sm_count();
         const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_kernel<__nv_bfloat16, true> : axial_rope_kernel<__nv_bfloat16, false>)

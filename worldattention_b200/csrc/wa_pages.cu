@@ -8,7 +8,10 @@
 // time (a page that is read by several comes after them, a ring of pages keeps one piece in registers), and splits it
 // into parts that share no page that is both read and written; parts run side by side.
 //
-// Bound: HBM, every moved page is read once and written once.  Eight loads of a thread are in flight at a time.
+// Bound: HBM, every moved page is read once and written once.  A thread has four pieces of one move in flight and makes the moves of a part one
+// after the other: the loads of several moves at a time touch as many more pages, which DRAM takes badly (60 tensors of 21 pages of 4.8 MB,
+// 12 moved together and 9 cleared, 9.5 GB: loads of four moves 2440 us, of two 1597, of one 1451 = 6.5 TB/s, what a plain copy reaches; a window of two
+// tensors rolled by 3 of 21 frames: 78, 64 and 66).
 // Page numbers and tensors travel as launch parameters: nothing is copied to the device, and the call can be captured.
 #include <algorithm>
 #include <new>
@@ -20,7 +23,7 @@
 namespace wa {
 
 constexpr int PM_CLEAR = -1, PM_SAVED = -2, PM_SAVE = -3;      // sources that are no page: zeros, the kept piece; keep a piece of `dst`
-constexpr int PM_THREADS = 256, PM_PIECES = 2, PM_AT_ONCE = 4;  // pieces of a thread, moves whose loads are in flight together
+constexpr int PM_THREADS = 256, PM_PIECES = 4;                   // pieces of a thread, whose loads are in flight together
 
 struct PageTensor {
     char *ptr;
@@ -64,35 +67,28 @@ move_pages_kernel(const __grid_constant__ PageMoves<TENSORS, MOVES> p) {
     Piece kept[PM_PIECES] = {};
     int kept_rows = 0;
     const int end = p.part[blockIdx.y + 1];
-    for (int m0 = p.part[blockIdx.y]; m0 < end; m0 += PM_AT_ONCE) {
-        Piece v[PM_AT_ONCE][PM_PIECES];
-        int rows[PM_AT_ONCE];
+    for (int i = p.part[blockIdx.y]; i < end; ++i) {
+        const int2 m = p.move[i];
+        const int page = m.y >= 0 ? m.y : m.x, mine = rows_of(page);
+        const bool load = m.y >= 0 || m.y == PM_SAVE;
+        const char *src = base + (long long)page * x.page_stride;
+        Piece v[PM_PIECES];
 #pragma unroll
-        for (int i = 0; i < PM_AT_ONCE; ++i) {
-            rows[i] = 0;
-            if (m0 + i < end) {
-                const int2 m = p.move[m0 + i];
-                const int page = m.y >= 0 ? m.y : m.x, mine = rows_of(page);
-                rows[i] = m.y == PM_SAVE ? 0 : m.y == PM_SAVED ? min(kept_rows, mine) : min(rows_of(m.x), mine);
-                const bool load = m.y >= 0 || m.y == PM_SAVE;
-                const char *src = base + (long long)page * x.page_stride;
-#pragma unroll
-                for (int u = 0; u < PM_PIECES; ++u) {
-                    v[i][u] = m.y == PM_SAVED ? kept[u] : Piece{};
-                    if (load && row[u] < mine) v[i][u] = *reinterpret_cast<const Piece *>(src + at[u]);
-                    if (m.y == PM_SAVE) kept[u] = v[i][u];
-                }
-                if (m.y == PM_SAVE) kept_rows = mine;
-            }
+        for (int u = 0; u < PM_PIECES; ++u) {
+            v[u] = m.y == PM_SAVED ? kept[u] : Piece{};
+            if (load && row[u] < mine) v[u] = *reinterpret_cast<const Piece *>(src + at[u]);
         }
+        if (m.y == PM_SAVE) {
 #pragma unroll
-        for (int i = 0; i < PM_AT_ONCE; ++i) {
-            if (rows[i] == 0) continue;
-            char *dst = base + (long long)p.move[m0 + i].x * x.page_stride;
-#pragma unroll
-            for (int u = 0; u < PM_PIECES; ++u)
-                if (row[u] < rows[i]) *reinterpret_cast<Piece *>(dst + at[u]) = v[i][u];
+            for (int u = 0; u < PM_PIECES; ++u) kept[u] = v[u];
+            kept_rows = mine;
+            continue;
         }
+        const int rows = min(m.y == PM_SAVED ? kept_rows : mine, rows_of(m.x));
+        char *dst = base + (long long)m.x * x.page_stride;
+#pragma unroll
+        for (int u = 0; u < PM_PIECES; ++u)
+            if (row[u] < rows) *reinterpret_cast<Piece *>(dst + at[u]) = v[u];
     }
 }
 

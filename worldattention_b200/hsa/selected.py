@@ -20,11 +20,14 @@ class _SelectedAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, index, num, block_sizes, out, lse)
         ctx.block_size = block_size
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 7
         q, k, v, index, num, block_sizes, out, lse = ctx.saved_tensors
         grads = _lib.host().selected_backward(q, k, v, index, num, ctx.block_size, block_sizes, out, lse, dout)
         return tuple(g if needed else None for g, needed in zip(grads, ctx.needs_input_grad)) + (None,) * 4
