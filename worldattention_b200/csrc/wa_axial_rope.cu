@@ -27,7 +27,7 @@ struct AxialRope {
     long long psb, psl;               // elements between samples (0: the same for all) and between tokens
     const float2 *table;              // [rows, pairs] (cos, sin)
     float sign;                       // of the angle
-    int groups, groups_of[AR_TENSORS], parts;     // vector form: head groups of all tensors and of each, warps of a token
+    int groups, groups_of[AR_TENSORS];     // vector form: head groups of all tensors and of each
 };
 
 constexpr int ar_groups(bool interleaved) { return interleaved ? 4 : 2; }        // head groups of a warp: four vectors of a lane
@@ -41,6 +41,35 @@ __device__ __forceinline__ float2 ar_turn(const AxialRope &p, const int32_t *pos
     if ((unsigned)row >= (unsigned)p.rows) return make_float2(NAN, NAN);
     const float2 t = __ldg(p.table + (long long)row * p.pairs + pair);
     return make_float2(t.x, t.y * p.sign);
+}
+
+// the same for `N` consecutive pairs; they mostly are of one axis or two (behind the last pair: no turn)
+template <int N>
+__device__ __forceinline__ void ar_turns(const AxialRope &p, const int32_t *pos, int first, float2 (&turn)[N]) {
+    const int last = min(first + N, p.pairs) - 1;
+    int a0 = 0, a1 = 0;
+#pragma unroll
+    for (int a = 0; a < AR_AXES - 1; ++a)
+        if (a < p.axes - 1) {
+            a0 += first >= p.end[a];
+            a1 += last >= p.end[a];
+        }
+    if (first <= last && a1 - a0 <= 1) {
+        const int r0 = __ldg(pos + a0), r1 = __ldg(pos + a1), border = p.end[a0];
+        const bool in0 = (unsigned)r0 < (unsigned)p.rows, in1 = (unsigned)r1 < (unsigned)p.rows;
+        const float2 *t0 = p.table + (long long)(in0 ? r0 : 0) * p.pairs + first, *t1 = p.table + (long long)(in1 ? r1 : 0) * p.pairs + first;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool one = first + i < border;
+            turn[i] = make_float2(1.f, 0.f);
+            if (first + i <= last) turn[i] = __ldg((one ? t0 : t1) + i);
+            turn[i].y *= p.sign;
+            if (!(one ? in0 : in1) && first + i <= last) turn[i] = make_float2(NAN, NAN);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) turn[i] = first + i <= last ? ar_turn(p, pos, first + i) : make_float2(1.f, 0.f);
+    }
 }
 
 template <typename T> struct ArVec;
@@ -79,10 +108,10 @@ axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
     using V = ArVec<T>;
     constexpr int N = V::N, TURNS = INTER ? N / 2 : N, AT_ONCE = ar_groups(INTER);
     pdl_wait();
-    const long long work = (long long)blockIdx.x * AR_WARPS + (threadIdx.x >> 5), token = work / p.parts;
-    if (token >= p.tokens) return;
-    const int lane = threadIdx.x & 31, part = (int)(work - token * p.parts);
-    const int b = (int)(token / p.L), l = (int)(token - (long long)b * p.L);
+    // (no division: the samples are the grid's z, the parts of a token its y)
+    const int l = blockIdx.x * AR_WARPS + (threadIdx.x >> 5), b = blockIdx.z, part = blockIdx.y;
+    if (l >= p.L) return;
+    const int lane = threadIdx.x & 31;
     const int per_head = (INTER ? p.D : p.pairs) / N, at_once = 32 / per_head;      // lanes a head takes, heads a group holds
     const int sub = lane / per_head, c = lane - sub * per_head;                     // head within the group, vector within the head
     const T *src[AT_ONCE];
@@ -105,11 +134,7 @@ axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
     }
     const int32_t *pos = p.positions + b * p.psb + l * p.psl;
     float2 turn[TURNS];
-#pragma unroll
-    for (int i = 0; i < TURNS; ++i) {
-        const int pair = c * TURNS + i;
-        turn[i] = sub < at_once && pair < p.pairs ? ar_turn(p, pos, pair) : make_float2(1.f, 0.f);
-    }
+    ar_turns<TURNS>(p, pos, sub < at_once ? c * TURNS : p.pairs, turn);
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
         if (!src[u]) continue;
@@ -215,15 +240,12 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
     WA_REQUIRE(positions && table, WA_ERR_ARG, "%s: null pointer", what);
     WA_REQUIRE((uintptr_t)table % 8 == 0 && (uintptr_t)positions % 4 == 0, WA_ERR_ALIGN, "%s: the table must be 8-byte aligned", what);
     cudaError_t e;
-    if (vec) {
+    if (vec && B <= 65535 && groups <= 65535) {
         const int each = ar_groups(interleaved != 0);
-        const long long parts = (groups + each - 1) / each, ctas = (p.tokens * parts + AR_WARPS - 1) / AR_WARPS;
-        WA_REQUIRE(ctas < (1ll << 31) && groups < (1 << 20), WA_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
         p.groups = (int)groups;
-        p.parts = (int)parts;
         const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_vec_kernel<__nv_bfloat16, true> : axial_rope_vec_kernel<__nv_bfloat16, false>)
                                              : (interleaved ? axial_rope_vec_kernel<float, true> : axial_rope_vec_kernel<float, false>);
-        e = launch_dependent(kernel, dim3((unsigned)ctas), dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
+        e = launch_dependent(kernel, dim3(ceil_div(L, AR_WARPS), (unsigned)((groups + each - 1) / each), B), dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
     } else {
         const long long want = (p.tokens * all_heads * (D - pairs) + 255) / 256, most = 32ll * sm_count();
         const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_kernel<__nv_bfloat16, true> : axial_rope_kernel<__nv_bfloat16, false>)

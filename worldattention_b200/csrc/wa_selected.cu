@@ -48,6 +48,248 @@ selected_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restri
     if (lane == 0) clean_num[list] = at;
 }
 
+// ---- a few query rows ----------------------------------------------------------------------------------
+// Single tokens, or up to eight rows of one query block, bf16 with head_dim 128: no tensor-core tile would be filled, and what counts is how soon the
+// listed keys and values are read.  A cluster of up to eight CTAs shares a (batch, head)'s list.  Four tokens are half a warp's step: each
+// token's 256 bytes are its 16 lanes' 16-byte loads, four of keys and four of values on their way at a time (eight of each take the registers of
+// a third CTA per SM: 12.9 -> 18.5 us); scores by shuffles, a running maximum and sum per half warp, and the halves, warps and CTAs are joined at the end in a fixed order through shared memory and the
+// cluster's.  Every CTA cleans the list for itself (a launch less).  Float32 throughout, nothing is rounded but the result.
+constexpr int SR_WARPS = 8, SR_STEP = 4, SR_IDS = 1024, SR_WORDS = 1024;      // tokens of a step; longest list and bitmap (32 768 key blocks)
+
+__device__ __forceinline__ float sr_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void sr_unpack(uint4 w, float (&f)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+}
+
+template <int R>
+__global__ void __launch_bounds__(SR_WARPS * 32)
+selected_rows_kernel(View4 q, View4 k, View4 v, void *out, long long osb, long long osl, long long osh, float *__restrict__ lse, const int32_t *__restrict__ index,
+                     const int32_t *__restrict__ num, int stride, int H, int group, int Lq, int Lkv, int block, int Nkv, float scale_log2) {
+    extern __shared__ uint32_t sr_smem[];
+    int32_t *ids = reinterpret_cast<int32_t *>(sr_smem);                   // [stride]
+    uint32_t *bits = sr_smem + stride;                                       // [words]
+    __shared__ float top_s[SR_WARPS][R], sum_s[SR_WARPS][R], acc_s[SR_WARPS][R][128];
+    __shared__ float top_c[R], sum_c[R], acc_c[R][128];                      // the CTA's
+    __shared__ int count;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, c = (lane & 15) * 8;
+    const int h = blockIdx.y, b = blockIdx.z, hk = h / group, words = (Nkv + 31) >> 5;
+    const long long list = (long long)b * H + h;
+    // the query rows, scaled; rows that are none stay zero
+    float qf[R][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (r < Lq) w = *reinterpret_cast<const uint4 *>((const __nv_bfloat16 *)q.ptr + b * q.sb + r * q.sl + h * q.sh + c);
+        sr_unpack(w, qf[r]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qf[r][e] *= scale_log2;
+    }
+    for (int w = threadIdx.x; w < words; w += SR_WARPS * 32) bits[w] = 0u;
+    __syncthreads();
+    if (warp == 0) {
+        const int n = max(0, min(num[list], stride));
+        int at = 0;
+        for (int i = 0; i < n; i += 32) {
+            const int id = i + lane < n ? index[list * stride + i + lane] : -1;
+            const bool there = (unsigned)id < (unsigned)Nkv;
+            const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1 - lane);
+            const bool take = there && lane == __ffs(same) - 1 && !((bits[id >> 5] >> (id & 31)) & 1u);
+            __syncwarp();
+            const unsigned all = __ballot_sync(0xffffffffu, take);
+            if (take) {
+                ids[at + __popc(all & ((1u << lane) - 1u))] = id;
+                atomicOr(&bits[id >> 5], 1u << (id & 31));
+            }
+            at += __popc(all);
+            __syncwarp();
+        }
+        if (lane == 0) count = at;
+    }
+    __syncthreads();
+    float top[R], sum[R], acc[R][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        top[r] = -INFINITY;
+        sum[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[r][e] = 0.f;
+    }
+    const __nv_bfloat16 *kp = (const __nv_bfloat16 *)k.ptr + b * k.sb + hk * k.sh + c, *vp = (const __nv_bfloat16 *)v.ptr + b * v.sb + hk * v.sh + c;
+    const int per_block = block / SR_STEP, steps = count * per_block;        // (block is 64 or 128)
+    const int step0 = (blockIdx.x * SR_WARPS + warp) * 2, all_steps = gridDim.x * SR_WARPS * 2;
+    for (int s0 = step0; s0 < steps; s0 += all_steps) {                       // both halves of a warp stay together
+        const int s = s0 + half;
+        const int e0 = s < steps ? s / per_block : 0, token0 = s < steps ? ids[e0] * block + (s - e0 * per_block) * SR_STEP : Lkv;
+        uint4 kw[SR_STEP], vw[SR_STEP];
+#pragma unroll
+        for (int t = 0; t < SR_STEP; ++t) {
+            kw[t] = vw[t] = make_uint4(0u, 0u, 0u, 0u);
+            if (token0 + t < Lkv) {
+                kw[t] = __ldg(reinterpret_cast<const uint4 *>(kp + (token0 + t) * k.sl));
+                vw[t] = __ldg(reinterpret_cast<const uint4 *>(vp + (token0 + t) * v.sl));
+            }
+        }
+        float z[R][SR_STEP];
+#pragma unroll
+        for (int t = 0; t < SR_STEP; ++t) {
+            float kf[8];
+            sr_unpack(kw[t], kf);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float d = qf[r][0] * kf[0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e) d = fmaf(qf[r][e], kf[e], d);
+                z[r][t] = d;
+            }
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int t = 0; t < SR_STEP; ++t) z[r][t] += __shfl_xor_sync(0xffffffffu, z[r][t], o);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float high = top[r];
+#pragma unroll
+            for (int t = 0; t < SR_STEP; ++t) {
+                if (token0 + t >= Lkv) z[r][t] = -INFINITY;
+                high = fmaxf(high, z[r][t]);
+            }
+            const float at = high == -INFINITY ? 0.f : high, back = sr_exp2(top[r] - at);      // (nothing seen yet: 2^-inf = 0)
+            top[r] = high;
+            sum[r] *= back;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][e] *= back;
+#pragma unroll
+            for (int t = 0; t < SR_STEP; ++t) {
+                z[r][t] = sr_exp2(z[r][t] - at);
+                sum[r] += z[r][t];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < SR_STEP; ++t) {
+            float vf[8];
+            sr_unpack(vw[t], vf);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(z[r][t], vf[e], acc[r][e]);
+        }
+    }
+    // halves of a warp
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float other = __shfl_xor_sync(0xffffffffu, top[r], 16), high = fmaxf(top[r], other), at = high == -INFINITY ? 0.f : high;
+        const float mine = sr_exp2(top[r] - at);
+        sum[r] *= mine;
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            acc[r][e] *= mine;
+            acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], 16);
+            if (half == 0) acc_s[warp][r][c + e] = acc[r][e];
+        }
+        if (lane == 0) top_s[warp][r] = high, sum_s[warp][r] = sum[r];
+    }
+    __syncthreads();
+    // warps of the CTA
+    for (int i = threadIdx.x; i < R * 128; i += SR_WARPS * 32) {
+        const int r = i >> 7, d = i & 127;
+        float high = -INFINITY, total = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < SR_WARPS; ++w) high = fmaxf(high, top_s[w][r]);
+        const float at = high == -INFINITY ? 0.f : high;
+#pragma unroll
+        for (int w = 0; w < SR_WARPS; ++w) {
+            const float f = sr_exp2(top_s[w][r] - at);
+            total = fmaf(sum_s[w][r], f, total);
+            x = fmaf(acc_s[w][r][d], f, x);
+        }
+        acc_c[r][d] = x;
+        if (d == 0) top_c[r] = high, sum_c[r] = total;
+    }
+    // CTAs of the cluster: CTA j joins rows j, j + CTAs, ...
+    const int ctas = gridDim.x;
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    const auto far = [](const float *p, int cta) {
+        float x;
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+        return x;
+    };
+    for (int r = blockIdx.x; r < Lq; r += ctas) {
+        const int d = threadIdx.x;
+        if (d >= 128) continue;
+        float tops[8], high = -INFINITY, total = 0.f, x = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tops[j] = j < ctas ? far(&top_c[r], j) : -INFINITY, high = fmaxf(high, tops[j]);
+        const float at = high == -INFINITY ? 0.f : high;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < ctas) {
+                const float f = sr_exp2(tops[j] - at);
+                total = fmaf(far(&sum_c[r], j), f, total);
+                x = fmaf(far(&acc_c[r][d], j), f, x);
+            }
+        // (no key: zero and -inf; a sum that is not a number stays one)
+        ((__nv_bfloat16 *)out)[b * osb + r * osl + h * osh + d] = __float2bfloat16_rn(total == 0.f ? 0.f : x / total);
+        if (lse && d == 0) lse[list * Lq + r] = total == 0.f ? -INFINITY : (high + log2f(total)) * 0.6931471805599453f;
+    }
+    if (ctas > 1) {      // the others may still be reading
+        asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    }
+}
+
+static bool selected_few_rows(const wa_selected_params *p) {
+    const auto pieces = [](const wa_tensor4 &t) { return (uintptr_t)t.ptr % 16 == 0 && t.stride_b % 8 == 0 && t.stride_l % 8 == 0 && t.stride_h % 8 == 0; };
+    return p->q.dtype == WA_BF16 && p->D == 128 && p->Lq <= 8 && (p->block_size == 64 || p->block_size == 128) && !p->block_sizes && p->index_stride <= SR_IDS &&
+           ceil_div(p->Lkv, p->block_size) <= 32 * SR_WORDS && pieces(p->q) && pieces(p->k) && pieces(p->v);
+}
+
+static int launch_few_rows(const wa_selected_params *p, cudaStream_t stream) {
+    const char *what = "wa_selected_forward";
+    const int Nkv = ceil_div(p->Lkv, p->block_size);
+    // as many CTAs for a list as it has work for, up to about four for every SM (4 x 12 lists of 32 blocks: 8 CTAs each 12.9 us, 4 14.2)
+    int ctas = 8;
+    const long long lists = (long long)p->B * p->H, steps = (long long)p->index_stride * p->block_size / SR_STEP;
+    while (ctas > 1 && (lists * ctas > 4ll * sm_count() || (long long)ctas * SR_WARPS * 2 > steps)) ctas >>= 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas, p->H, p->B);
+    cfg.blockDim = dim3(SR_WARPS * 32);
+    cfg.dynamicSmemBytes = ((size_t)p->index_stride + ceil_div(Nkv, 32)) * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    const float scale = (float)(1.4426950408889634 / sqrt(128.0));
+    const auto kernel = p->Lq == 1 ? selected_rows_kernel<1> : p->Lq == 2 ? selected_rows_kernel<2> : p->Lq <= 4 ? selected_rows_kernel<4> : selected_rows_kernel<8>;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, make_view(&p->q), make_view(&p->k), make_view(&p->v), p->out.ptr, (long long)p->out.stride_b,
+                                             (long long)p->out.stride_l, (long long)p->out.stride_h, p->lse, p->index, p->num, p->index_stride, p->H, p->H / p->Hkv, p->Lq,
+                                             p->Lkv, p->block_size, Nkv, scale);
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
+}
+
 // ---- row statistics of the gradient -----------------------------------------------------------------
 // See selected_stat.  Reads dout and out once: `LANES` lanes take a row, 16 bytes each (LANES = 0: a warp, one channel at a time, any layout), and
 // four rows are on their way at a time.
@@ -118,29 +360,35 @@ static int launch_stats(const wa_selected_params *p, int padded, float *stats, c
 }
 
 // ---- gradient, any shape ------------------------------------------------------------------------------
-// One CTA owns T rows of one side -- dQ: queries, dK/dV: keys -- and meets the rows of the other side T at a time: T x T scores and
-// dP from shared memory, P and dS back to shared memory, and from there into the owned rows' sums in registers.  256 threads, 4 x 4
-// (T = 64) or 2 x 2 (T = 32, head_dim above 128) of the T x T and as many owned rows by 4 * NM columns of the sums; all reads are 16 bytes.
+// One CTA owns 32 rows of one side -- dQ: queries, dK/dV: keys -- and meets the rows of the other side TG at a time: 32 x TG scores and
+// dP from shared memory, P and dS back to shared memory, and from there into the owned rows' sums in registers.  256 threads, 2 x TG / 16 of
+// the scores and 2 owned rows by 4 * NM columns of the sums each; all reads are 16 bytes.  The next rows to meet are on their way while some are at
+// work: asynchronous copies of aligned float32 rows, plain loads of anything else.
+// Bound: shared-memory reads, 10 of 16 bytes per warp for 32 multiply-adds (with 64 owned rows and 4 x 4 scores of a thread 6 for as many, but half
+// the CTAs and no room for the rows to come: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64, 157 + 240 us).
 struct SelectedGrad {
     View4 q, k, v, dout;
     void *dq, *dk, *dv;
     int dtype;
     long long dqb, dql, dqh, dkb, dkl, dkh, dvb, dvl, dvh;
     int H, group, Lq, Lkv, D, block, stride, Nq, Nkv, row_words, padded, tiles;
+    int async;                        // rows of whole 16-byte pieces of float32
     const int32_t *index, *num, *block_sizes;
     const uint32_t *rows;
     const float *stats;
     float scale;
 };
+constexpr int SG_OWN = 32;
 
-template <int T, int NM, bool KEYS>      // NM: 64-column steps of head_dim
+template <int TG, int NM, bool KEYS>      // NM: 64-column steps of head_dim
 __global__ void __launch_bounds__(256)
 selected_grad_kernel(const SelectedGrad p) {
-    constexpr int W = 64 * NM, LD = W + 4, R = T / 16, LP = T + 4;
+    constexpr int T = SG_OWN, W = 64 * NM, LD = W + 4, R = T / 16, C = TG / 16, LP = TG + 4;
     extern __shared__ __align__(16) float sg_smem[];
-    float *f1 = sg_smem, *f2 = f1 + T * LD, *g1 = f2 + T * LD, *g2 = g1 + T * LD;      // owned: q, dout or k, v; met: the other two
-    float *ps = g2 + T * LD, *ds = ps + T * LP;
-    float2 *st = reinterpret_cast<float2 *>(ds + T * LP);                               // statistics of the T query rows
+    float *f1 = sg_smem, *f2 = f1 + T * LD, *met = f2 + T * LD;               // owned: q, dout or k, v; met: [two buffers][the other two]
+    float *ps = met + 4 * TG * LD, *ds = ps + T * LP;
+    float2 *st = reinterpret_cast<float2 *>(ds + T * LP);                     // [two buffers] statistics of the query rows
+    constexpr int ST = TG > T ? TG : T;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int blk = blockIdx.x / p.tiles, first = blk * p.block + (blockIdx.x % p.tiles) * T, b = blockIdx.z;
     const int hk = KEYS ? blockIdx.y : blockIdx.y / p.group;
@@ -152,21 +400,67 @@ selected_grad_kernel(const SelectedGrad p) {
     const int own_real = KEYS ? min(own_end, blk * p.block + keys_of(blk)) : own_end;         // rows that count
     if (first >= own_end) return;
 
-    const auto bring = [&](float *to, const View4 &x, int h, int from, int end) {
+    const auto bring = [&](float *to, const View4 &x, int h, int from, int end, int rows) {
         const long long base = b * x.sb + (long long)h * x.sh;
-        for (int e = threadIdx.x; e < T * W; e += 256) {
-            const int r = e / W, d = e % W;
-            to[r * LD + d] = from + r < end && d < p.D ? load_elem(x.ptr, x.dtype, base + (long long)(from + r) * x.sl + d) : 0.f;
+        if (p.async) {
+            for (int e = threadIdx.x; e < rows * (W / 4); e += 256) {
+                const int r = e / (W / 4), d = e % (W / 4) * 4;
+                const bool there = from + r < end && d < p.D;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + r * LD + d)),
+                             "l"((const float *)x.ptr + (there ? base + (long long)(from + r) * x.sl + d : 0)), "r"(there ? 16 : 0) : "memory");
+            }
+        } else {
+#pragma unroll 4
+            for (int e = threadIdx.x; e < rows * W; e += 256) {
+                const int r = e / W, d = e % W;
+                to[r * LD + d] = from + r < end && d < p.D ? load_elem(x.ptr, x.dtype, base + (long long)(from + r) * x.sl + d) : 0.f;
+            }
         }
     };
-    const auto bring_stats = [&](int h, int from, int end) {
+    const auto bring_stats = [&](float2 *to, int h, int from, int end, int rows) {
         const float *stats = p.stats + ((long long)b * p.H + h) * p.padded * 2;
-        for (int r = threadIdx.x; r < T; r += 256)
-            st[r] = from + r < end ? make_float2(stats[selected_stat(from + r)], stats[selected_stat(from + r) + 64]) : make_float2(-INFINITY, 0.f);
+        for (int r = threadIdx.x; r < rows; r += 256)
+            to[r] = from + r < end ? make_float2(stats[selected_stat(from + r)], stats[selected_stat(from + r) + 64]) : make_float2(-INFINITY, 0.f);
     };
-    bring(f1, KEYS ? p.k : p.q, KEYS ? hk : blockIdx.y, first, own_real);
-    bring(f2, KEYS ? p.v : p.dout, KEYS ? hk : blockIdx.y, first, own_real);
-    if (!KEYS) bring_stats(blockIdx.y, first, own_real);
+    bring(f1, KEYS ? p.k : p.q, KEYS ? hk : blockIdx.y, first, own_real, T);
+    bring(f2, KEYS ? p.v : p.dout, KEYS ? hk : blockIdx.y, first, own_real, T);
+    if (!KEYS) bring_stats(st, blockIdx.y, first, own_real, T);
+
+    // the rows to meet, TG at a time: those of the listed blocks in the order of the list
+    struct Rows { int h, from, end; };
+    int at = -1, left_from = 0, left_end = 0, head = 0;
+    uint32_t word = 0;
+    const long long list = KEYS ? (((long long)b * (p.H / p.group) + hk) * p.Nkv + blk) * p.group * p.row_words : ((long long)b * p.H + blockIdx.y) * p.Nq + blk;
+    const int n = KEYS ? p.group * p.row_words : p.num[list];
+    const auto next = [&](Rows &to) {
+        while (left_from >= left_end) {
+            if (KEYS) {
+                while (word == 0u) {
+                    if (++at >= n) return false;
+                    word = p.rows[list + at];
+                }
+                const int i = (at % p.row_words) * 32 + __ffs(word) - 1;
+                word &= word - 1;
+                head = hk * p.group + at / p.row_words;
+                left_from = i * p.block;
+                left_end = min(left_from + p.block, p.Lq);
+            } else {
+                if (++at >= n) return false;
+                const int id = p.index[list * p.stride + at];
+                head = blockIdx.y;
+                left_from = id * p.block;
+                left_end = left_from + keys_of(id);
+            }
+        }
+        to = Rows{head, left_from, min(left_from + TG, left_end)};
+        left_from += TG;
+        return true;
+    };
+    const auto bring_met = [&](int buf, const Rows &r) {
+        bring(met + 2 * buf * TG * LD, KEYS ? p.q : p.k, KEYS ? r.h : hk, r.from, r.end, TG);
+        bring(met + (2 * buf + 1) * TG * LD, KEYS ? p.dout : p.v, KEYS ? r.h : hk, r.from, r.end, TG);
+        if (KEYS) bring_stats(st + buf * ST, r.h, r.from, r.end, TG);
+    };
 
     float4 sum1[R][NM], sum2[R][NM];         // of the owned rows: dV (KEYS), dK or dQ
 #pragma unroll
@@ -176,28 +470,34 @@ selected_grad_kernel(const SelectedGrad p) {
     const float to_log2 = p.scale * 1.4426950408889634f;
     const int depth = (p.D + 3) & ~3;
 
-    const auto meet = [&](int h, int from, int end) {       // rows from .. end of the other side
+    Rows now, then;
+    bool more = next(now);
+    if (more) bring_met(0, now);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int buf = 0; more; buf ^= 1, now = then) {
+        more = next(then);
+        if (more) bring_met(buf ^ 1, then);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
-        bring(g1, KEYS ? p.q : p.k, KEYS ? h : hk, from, end);
-        bring(g2, KEYS ? p.dout : p.v, KEYS ? h : hk, from, end);
-        if (KEYS) bring_stats(h, from, end);
-        __syncthreads();
-        float s[R][R], dp[R][R];
+        const float *g1 = met + 2 * buf * TG * LD, *g2 = g1 + TG * LD;
+        float s[R][C], dp[R][C];
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < R; ++j) s[i][j] = dp[i][j] = 0.f;
-        const auto dots = [&](float (&acc)[R][R], const float *f, const float *g) {
+            for (int j = 0; j < C; ++j) s[i][j] = dp[i][j] = 0.f;
+        const auto dots = [&](float (&acc)[R][C], const float *f, const float *g) {
+#pragma unroll 2
             for (int d = 0; d < depth; d += 4) {
-                float4 x[R], y[R];
+                float4 x[R], y[C];
 #pragma unroll
                 for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4 *>(f + (ty * R + i) * LD + d);
 #pragma unroll
-                for (int j = 0; j < R; ++j) y[j] = *reinterpret_cast<const float4 *>(g + (tx + 16 * j) * LD + d);
+                for (int j = 0; j < C; ++j) y[j] = *reinterpret_cast<const float4 *>(g + (tx + 16 * j) * LD + d);
 #pragma unroll
                 for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int j = 0; j < R; ++j) {
+                    for (int j = 0; j < C; ++j) {
                         acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
                         acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
                         acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
@@ -210,17 +510,18 @@ selected_grad_kernel(const SelectedGrad p) {
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
+            for (int j = 0; j < C; ++j) {
                 const int f = ty * R + i, g = tx + 16 * j;
-                const float2 row = st[KEYS ? g : f];
-                const bool there = first + f < own_real && from + g < end;
+                const float2 row = st[KEYS ? buf * ST + g : f];
+                const bool there = first + f < own_real && now.from + g < now.end;
                 const float pr = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
-                ps[f * LP + g] = pr;
+                if (KEYS) ps[f * LP + g] = pr;
                 ds[f * LP + g] = there ? pr * (dp[i][j] - row.y) * p.scale : 0.f;
             }
         __syncthreads();
         const auto add = [&](float4 (&acc)[R][NM], const float *w, const float *x) {
-            for (int g = 0; g < T; g += 4) {
+#pragma unroll 2
+            for (int g = 0; g < TG; g += 4) {
                 float4 a[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4 *>(w + (ty * R + i) * LP + g);
@@ -242,20 +543,7 @@ selected_grad_kernel(const SelectedGrad p) {
         };
         if (KEYS) add(sum1, ps, g2);
         add(sum2, ds, g1);
-    };
-    if (KEYS) {
-        const uint32_t *bits = p.rows + (((long long)b * (p.H / p.group) + hk) * p.Nkv + blk) * p.group * p.row_words;
-        for (int w = 0; w < p.group * p.row_words; ++w)
-            for (uint32_t left = bits[w]; left; left &= left - 1) {
-                const int i = (w % p.row_words) * 32 + __ffs(left) - 1, end = min((i + 1) * p.block, p.Lq);
-                for (int from = i * p.block; from < end; from += T) meet(hk * p.group + w / p.row_words, from, min(from + T, end));
-            }
-    } else {
-        const long long list = ((long long)b * p.H + blockIdx.y) * p.Nq + blk;
-        for (int n = 0; n < p.num[list]; ++n) {
-            const int id = p.index[list * p.stride + n], end = id * p.block + keys_of(id);
-            for (int from = id * p.block; from < end; from += T) meet(blockIdx.y, from, min(from + T, end));
-        }
+        __syncthreads();
     }
     const auto write = [&](const float4 (&acc)[R][NM], void *to, long long sb, long long sl, int h, long long sh) {
 #pragma unroll
@@ -279,24 +567,24 @@ selected_grad_kernel(const SelectedGrad p) {
     }
 }
 
-template <int T, int NM>
+template <int TG, int NM>
 static int launch_grad(SelectedGrad p, int B, int Hkv, cudaStream_t stream) {
     const char *what = "wa_selected_backward";
-    constexpr size_t smem = (size_t)(4 * T * (64 * NM + 4) + 2 * T * (T + 4)) * 4 + T * 8;
+    constexpr size_t smem = (size_t)((2 * SG_OWN + 4 * TG) * (64 * NM + 4) + 2 * SG_OWN * (TG + 4)) * 4 + 2 * (TG > SG_OWN ? TG : SG_OWN) * 8;
     static PerDeviceOnce attr_set;
     if (!attr_set.done()) {
-        cudaError_t e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(selected_grad_kernel<TG, NM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(selected_grad_kernel<TG, NM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
-    p.tiles = ceil_div(p.block, T);
+    p.tiles = ceil_div(p.block, SG_OWN);
     const long long kx = (long long)p.Nkv * p.tiles, qx = (long long)p.Nq * p.tiles;
     WA_REQUIRE(kx < (1ll << 31) && qx < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: grid too large", what);
     int rc;
-    selected_grad_kernel<T, NM, true><<<dim3((unsigned)kx, Hkv, B), 256, smem, stream>>>(p);
+    selected_grad_kernel<TG, NM, true><<<dim3((unsigned)kx, Hkv, B), 256, smem, stream>>>(p);
     if ((rc = check_launch(what))) return rc;
-    selected_grad_kernel<T, NM, false><<<dim3((unsigned)qx, p.H, B), 256, smem, stream>>>(p);
+    selected_grad_kernel<TG, NM, false><<<dim3((unsigned)qx, p.H, B), 256, smem, stream>>>(p);
     return check_launch(what);
 }
 
@@ -310,6 +598,10 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     w.row_words = ceil_div(w.Nq, 32);
     const size_t lists = (size_t)p->B * p->H * w.Nq;
     size_t c = 0;
+    if (!backward && selected_few_rows(p)) {       // needs none
+        w.total = 256;
+        return w;
+    }
     w.index = c; c = align_up(c + lists * p->index_stride * sizeof(int32_t), 256);
     w.num = c; c = align_up(c + lists * sizeof(int32_t), 256);
     if (backward) {
@@ -385,6 +677,7 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     const SelectedPlan w = selected_plan(p, false);
     WA_REQUIRE(p->workspace && p->workspace_bytes >= w.total, WA_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes, got %zu", what, w.total, p->workspace_bytes);
     WA_REQUIRE((uintptr_t)p->workspace % 256 == 0, WA_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", what);
+    if (selected_few_rows(p)) return launch_few_rows(p, stream);
     char *ws = (char *)p->workspace;
     if ((rc = selected_lists(p, w, false, ws, stream, what))) return rc;
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
@@ -421,7 +714,11 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
     g.Nq = w.Nq; g.Nkv = w.Nkv; g.row_words = w.row_words; g.padded = padded;
     g.index = index; g.num = num; g.block_sizes = p->block_sizes; g.rows = rows; g.stats = stats;
     g.scale = (float)(1.0 / sqrt((double)p->D));
+    const auto pieces = [](const wa_tensor4 &t) {
+        return t.dtype == WA_F32 && (uintptr_t)t.ptr % 16 == 0 && t.stride_b % 4 == 0 && t.stride_l % 4 == 0 && t.stride_h % 4 == 0;
+    };
+    g.async = p->D % 4 == 0 && pieces(p->q) && pieces(p->k) && pieces(p->v) && pieces(p->dout);
     if (p->D <= 64) return launch_grad<64, 1>(g, p->B, p->Hkv, stream);
-    if (p->D <= 128) return launch_grad<64, 2>(g, p->B, p->Hkv, stream);
+    if (p->D <= 128) return launch_grad<32, 2>(g, p->B, p->Hkv, stream);
     return launch_grad<32, 4>(g, p->B, p->Hkv, stream);
 }
