@@ -48,6 +48,26 @@ selected_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restri
     if (lane == 0) clean_num[list] = at;
 }
 
+// ---- work order of the gradient ------------------------------------------------------------------------
+// Query blocks by the length of their lists and key blocks by the number of query blocks that list them, heaviest first: with a few items per SM
+// whichever comes last otherwise works alone (see selected_ordered).  One CTA each.
+__global__ void __launch_bounds__(1024)
+selected_order_kernel(const int32_t *__restrict__ num, const uint32_t *__restrict__ rows, int q_items, int k_items, int words, int most_q, int most_k,
+                      int32_t *__restrict__ q_order, int32_t *__restrict__ k_order) {
+    __shared__ int hist[SCHED_BINS], warp_tot[32], unused[2];
+    pdl_wait();
+    if (blockIdx.x == 0) {
+        sort_items([&](int i) { return __ldg(num + i); }, q_items, most_q, hist, warp_tot, q_order, unused, unused + 1);
+    } else {
+        const auto listed = [&](int i) {
+            int n = 0;
+            for (int w = 0; w < words; ++w) n += __popc(__ldg(rows + (long long)i * words + w));
+            return n;
+        };
+        sort_items(listed, k_items, most_k, hist, warp_tot, k_order, unused, unused + 1);
+    }
+}
+
 // ---- a few query rows ----------------------------------------------------------------------------------
 // Single tokens, or up to eight rows of one query block, bf16 with head_dim 128: no tensor-core tile would be filled, and what counts is how soon the
 // listed keys and values are read.  A cluster of up to eight CTAs shares a (batch, head)'s list.  Four tokens are half a warp's step: each
@@ -360,12 +380,12 @@ static int launch_stats(const wa_selected_params *p, int padded, float *stats, c
 }
 
 // ---- gradient, any shape ------------------------------------------------------------------------------
-// One CTA owns 32 rows of one side -- dQ: queries, dK/dV: keys -- and meets the rows of the other side TG at a time: 32 x TG scores and
-// dP from shared memory, P and dS back to shared memory, and from there into the owned rows' sums in registers.  256 threads, 2 x TG / 16 of
-// the scores and 2 owned rows by 4 * NM columns of the sums each; all reads are 16 bytes.  The next rows to meet are on their way while some are at
-// work: asynchronous copies of aligned float32 rows, plain loads of anything else.
-// Bound: shared-memory reads, 10 of 16 bytes per warp for 32 multiply-adds (with 64 owned rows and 4 x 4 scores of a thread 6 for as many, but half
-// the CTAs and no room for the rows to come: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64, 157 + 240 us).
+// One CTA owns T rows of one side -- dQ: queries, dK/dV: keys -- and meets the rows of the other side T at a time (T = 64, 32 for head_dim above
+// 128).  A warp has T / 8 of the owned rows to itself: its lanes take T / 32 met rows each for the scores and dP, P and dS go through
+// shared memory of the warp's own, and for the sums a lane has 4 channels of each 128.  So an owned row is one address for all lanes, a met row one for
+// each, both 16 bytes: 16 wavefronts of shared memory for 64 multiply-adds of a warp (scores), 24 for 128 (sums), below what the multiply-adds take.
+// (16 x 16 threads with 2 x 2 scores each were bound by shared memory: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64 a row: TIMES)
+// The next rows to meet are on their way while some are at work: asynchronous copies of aligned float32 rows, plain loads of anything else.
 struct SelectedGrad {
     View4 q, k, v, dout;
     void *dq, *dk, *dv;
@@ -374,24 +394,25 @@ struct SelectedGrad {
     int H, group, Lq, Lkv, D, block, stride, Nq, Nkv, row_words, padded, tiles;
     int async;                        // rows of whole 16-byte pieces of float32
     const int32_t *index, *num, *block_sizes;
+    const int32_t *q_order, *k_order; // or null: as they come
     const uint32_t *rows;
     const float *stats;
     float scale;
 };
-constexpr int SG_OWN = 32;
-
-template <int TG, int NM, bool KEYS>      // NM: 64-column steps of head_dim
+template <int T, int NM, bool KEYS>      // NM: 128-column steps of head_dim
 __global__ void __launch_bounds__(256)
 selected_grad_kernel(const SelectedGrad p) {
-    constexpr int T = SG_OWN, W = 64 * NM, LD = W + 4, R = T / 16, C = TG / 16, LP = TG + 4;
+    constexpr int W = 128 * NM, LD = W + 4, R = T / 8, C = T / 32, LP = T + 4;      // R: owned rows of a warp, C: met rows of a lane
     extern __shared__ __align__(16) float sg_smem[];
     float *f1 = sg_smem, *f2 = f1 + T * LD, *met = f2 + T * LD;               // owned: q, dout or k, v; met: [two buffers][the other two]
-    float *ps = met + 4 * TG * LD, *ds = ps + T * LP;
-    float2 *st = reinterpret_cast<float2 *>(ds + T * LP);                     // [two buffers] statistics of the query rows
-    constexpr int ST = TG > T ? TG : T;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int blk = blockIdx.x / p.tiles, first = blk * p.block + (blockIdx.x % p.tiles) * T, b = blockIdx.z;
-    const int hk = KEYS ? blockIdx.y : blockIdx.y / p.group;
+    float *factors = met + 4 * T * LD;                                        // P, then dS
+    float2 *st = reinterpret_cast<float2 *>(factors + T * LP);                // [two buffers] statistics of the query rows
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int blocks = KEYS ? p.Nkv : p.Nq, heads = KEYS ? p.H / p.group : p.H;
+    const int32_t *order = KEYS ? p.k_order : p.q_order;
+    const int item = order ? order[blockIdx.x / p.tiles] : blockIdx.x / p.tiles, own_head = item / blocks;
+    const int blk = item - own_head * blocks, first = blk * p.block + (blockIdx.x % p.tiles) * T, b = own_head / heads, h = own_head - b * heads;
+    const int hk = KEYS ? h : h / p.group;
     const auto keys_of = [&](int id) {       // real tokens of a key block
         const int n = min(p.block, p.Lkv - id * p.block);
         return p.block_sizes ? max(0, min(n, p.block_sizes[id])) : n;
@@ -400,10 +421,10 @@ selected_grad_kernel(const SelectedGrad p) {
     const int own_real = KEYS ? min(own_end, blk * p.block + keys_of(blk)) : own_end;         // rows that count
     if (first >= own_end) return;
 
-    const auto bring = [&](float *to, const View4 &x, int h, int from, int end, int rows) {
-        const long long base = b * x.sb + (long long)h * x.sh;
+    const auto bring = [&](float *to, const View4 &x, int head, int from, int end) {
+        const long long base = b * x.sb + (long long)head * x.sh;
         if (p.async) {
-            for (int e = threadIdx.x; e < rows * (W / 4); e += 256) {
+            for (int e = threadIdx.x; e < T * (W / 4); e += 256) {
                 const int r = e / (W / 4), d = e % (W / 4) * 4;
                 const bool there = from + r < end && d < p.D;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + r * LD + d)),
@@ -411,26 +432,26 @@ selected_grad_kernel(const SelectedGrad p) {
             }
         } else {
 #pragma unroll 4
-            for (int e = threadIdx.x; e < rows * W; e += 256) {
+            for (int e = threadIdx.x; e < T * W; e += 256) {
                 const int r = e / W, d = e % W;
                 to[r * LD + d] = from + r < end && d < p.D ? load_elem(x.ptr, x.dtype, base + (long long)(from + r) * x.sl + d) : 0.f;
             }
         }
     };
-    const auto bring_stats = [&](float2 *to, int h, int from, int end, int rows) {
-        const float *stats = p.stats + ((long long)b * p.H + h) * p.padded * 2;
-        for (int r = threadIdx.x; r < rows; r += 256)
+    const auto bring_stats = [&](float2 *to, int head, int from, int end) {
+        const float *stats = p.stats + ((long long)b * p.H + head) * p.padded * 2;
+        for (int r = threadIdx.x; r < T; r += 256)
             to[r] = from + r < end ? make_float2(stats[selected_stat(from + r)], stats[selected_stat(from + r) + 64]) : make_float2(-INFINITY, 0.f);
     };
-    bring(f1, KEYS ? p.k : p.q, KEYS ? hk : blockIdx.y, first, own_real, T);
-    bring(f2, KEYS ? p.v : p.dout, KEYS ? hk : blockIdx.y, first, own_real, T);
-    if (!KEYS) bring_stats(st, blockIdx.y, first, own_real, T);
+    bring(f1, KEYS ? p.k : p.q, h, first, own_real);
+    bring(f2, KEYS ? p.v : p.dout, h, first, own_real);
+    if (!KEYS) bring_stats(st, h, first, own_real);
 
-    // the rows to meet, TG at a time: those of the listed blocks in the order of the list
+    // the rows to meet, T at a time: those of the listed blocks in the order of the list
     struct Rows { int h, from, end; };
     int at = -1, left_from = 0, left_end = 0, head = 0;
     uint32_t word = 0;
-    const long long list = KEYS ? (((long long)b * (p.H / p.group) + hk) * p.Nkv + blk) * p.group * p.row_words : ((long long)b * p.H + blockIdx.y) * p.Nq + blk;
+    const long long list = KEYS ? (long long)item * p.group * p.row_words : (long long)item;
     const int n = KEYS ? p.group * p.row_words : p.num[list];
     const auto next = [&](Rows &to) {
         while (left_from >= left_end) {
@@ -447,19 +468,19 @@ selected_grad_kernel(const SelectedGrad p) {
             } else {
                 if (++at >= n) return false;
                 const int id = p.index[list * p.stride + at];
-                head = blockIdx.y;
+                head = h;
                 left_from = id * p.block;
                 left_end = left_from + keys_of(id);
             }
         }
-        to = Rows{head, left_from, min(left_from + TG, left_end)};
-        left_from += TG;
+        to = Rows{head, left_from, min(left_from + T, left_end)};
+        left_from += T;
         return true;
     };
     const auto bring_met = [&](int buf, const Rows &r) {
-        bring(met + 2 * buf * TG * LD, KEYS ? p.q : p.k, KEYS ? r.h : hk, r.from, r.end, TG);
-        bring(met + (2 * buf + 1) * TG * LD, KEYS ? p.dout : p.v, KEYS ? r.h : hk, r.from, r.end, TG);
-        if (KEYS) bring_stats(st + buf * ST, r.h, r.from, r.end, TG);
+        bring(met + 2 * buf * T * LD, KEYS ? p.q : p.k, KEYS ? r.h : hk, r.from, r.end);
+        bring(met + (2 * buf + 1) * T * LD, KEYS ? p.dout : p.v, KEYS ? r.h : hk, r.from, r.end);
+        if (KEYS) bring_stats(st + buf * T, r.h, r.from, r.end);
     };
 
     float4 sum1[R][NM], sum2[R][NM];         // of the owned rows: dV (KEYS), dK or dQ
@@ -480,7 +501,7 @@ selected_grad_kernel(const SelectedGrad p) {
         asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
-        const float *g1 = met + 2 * buf * TG * LD, *g2 = g1 + TG * LD;
+        const float *g1 = met + 2 * buf * T * LD, *g2 = g1 + T * LD;
         float s[R][C], dp[R][C];
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -489,106 +510,122 @@ selected_grad_kernel(const SelectedGrad p) {
         const auto dots = [&](float (&acc)[R][C], const float *f, const float *g) {
 #pragma unroll 2
             for (int d = 0; d < depth; d += 4) {
-                float4 x[R], y[C];
+                float4 y[C];
 #pragma unroll
-                for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4 *>(f + (ty * R + i) * LD + d);
+                for (int j = 0; j < C; ++j) y[j] = *reinterpret_cast<const float4 *>(g + (lane + 32 * j) * LD + d);
 #pragma unroll
-                for (int j = 0; j < C; ++j) y[j] = *reinterpret_cast<const float4 *>(g + (tx + 16 * j) * LD + d);
-#pragma unroll
-                for (int i = 0; i < R; ++i)
+                for (int i = 0; i < R; ++i) {
+                    const float4 x = *reinterpret_cast<const float4 *>(f + (warp * R + i) * LD + d);
 #pragma unroll
                     for (int j = 0; j < C; ++j) {
-                        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-                        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-                        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-                        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+                        acc[i][j] = fmaf(x.x, y[j].x, acc[i][j]);
+                        acc[i][j] = fmaf(x.y, y[j].y, acc[i][j]);
+                        acc[i][j] = fmaf(x.z, y[j].z, acc[i][j]);
+                        acc[i][j] = fmaf(x.w, y[j].w, acc[i][j]);
                     }
+                }
             }
         };
         dots(s, f1, g1);
         dots(dp, f2, g2);
+        float *mine = factors + warp * R * LP;
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int j = 0; j < C; ++j) {
-                const int f = ty * R + i, g = tx + 16 * j;
-                const float2 row = st[KEYS ? buf * ST + g : f];
+                const int f = warp * R + i, g = lane + 32 * j;
+                const float2 row = st[KEYS ? buf * T + g : f];
                 const bool there = first + f < own_real && now.from + g < now.end;
-                const float pr = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
-                if (KEYS) ps[f * LP + g] = pr;
-                ds[f * LP + g] = there ? pr * (dp[i][j] - row.y) * p.scale : 0.f;
+                s[i][j] = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
+                dp[i][j] = there ? s[i][j] * (dp[i][j] - row.y) * p.scale : 0.f;
             }
-        __syncthreads();
-        const auto add = [&](float4 (&acc)[R][NM], const float *w, const float *x) {
-#pragma unroll 2
-            for (int g = 0; g < TG; g += 4) {
-                float4 a[R];
+        const auto add = [&](float4 (&acc)[R][NM], const float (&factor)[R][C], const float *x) {
+            __syncwarp();
 #pragma unroll
-                for (int i = 0; i < R; ++i) a[i] = *reinterpret_cast<const float4 *>(w + (ty * R + i) * LP + g);
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < C; ++j) mine[i * LP + lane + 32 * j] = factor[i][j];
+            __syncwarp();
+#pragma unroll 2
+            for (int g = 0; g < T; g += 4) {
+                float4 y[4][NM];
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int m = 0; m < NM; ++m) {
-                        const float4 y = *reinterpret_cast<const float4 *>(x + (g + u) * LD + 64 * m + 4 * tx);
+                    for (int m = 0; m < NM; ++m) y[u][m] = *reinterpret_cast<const float4 *>(x + (g + u) * LD + 128 * m + 4 * lane);
 #pragma unroll
-                        for (int i = 0; i < R; ++i) {
-                            const float c = u == 0 ? a[i].x : u == 1 ? a[i].y : u == 2 ? a[i].z : a[i].w;
-                            acc[i][m].x = fmaf(c, y.x, acc[i][m].x);
-                            acc[i][m].y = fmaf(c, y.y, acc[i][m].y);
-                            acc[i][m].z = fmaf(c, y.z, acc[i][m].z);
-                            acc[i][m].w = fmaf(c, y.w, acc[i][m].w);
+                for (int i = 0; i < R; ++i) {
+                    const float4 a = *reinterpret_cast<const float4 *>(mine + i * LP + g);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float c = u == 0 ? a.x : u == 1 ? a.y : u == 2 ? a.z : a.w;
+#pragma unroll
+                        for (int m = 0; m < NM; ++m) {
+                            acc[i][m].x = fmaf(c, y[u][m].x, acc[i][m].x);
+                            acc[i][m].y = fmaf(c, y[u][m].y, acc[i][m].y);
+                            acc[i][m].z = fmaf(c, y[u][m].z, acc[i][m].z);
+                            acc[i][m].w = fmaf(c, y[u][m].w, acc[i][m].w);
                         }
                     }
+                }
             }
         };
-        if (KEYS) add(sum1, ps, g2);
-        add(sum2, ds, g1);
+        if (KEYS) add(sum1, s, g2);
+        add(sum2, dp, g1);
         __syncthreads();
     }
-    const auto write = [&](const float4 (&acc)[R][NM], void *to, long long sb, long long sl, int h, long long sh) {
+    const auto write = [&](const float4 (&acc)[R][NM], void *to, long long sb, long long sl, long long sh) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int r = first + ty * R + i;
+            const int r = first + warp * R + i;
             if (r >= own_end) continue;
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
                 const float v[4] = {acc[i][m].x, acc[i][m].y, acc[i][m].z, acc[i][m].w};
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (64 * m + 4 * tx + u < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + 64 * m + 4 * tx + u, v[u]);
+                    if (128 * m + 4 * lane + u < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + 128 * m + 4 * lane + u, v[u]);
             }
         }
     };
     if (KEYS) {
-        write(sum1, p.dv, p.dvb, p.dvl, hk, p.dvh);
-        write(sum2, p.dk, p.dkb, p.dkl, hk, p.dkh);
+        write(sum1, p.dv, p.dvb, p.dvl, p.dvh);
+        write(sum2, p.dk, p.dkb, p.dkl, p.dkh);
     } else {
-        write(sum2, p.dq, p.dqb, p.dql, blockIdx.y, p.dqh);
+        write(sum2, p.dq, p.dqb, p.dql, p.dqh);
     }
 }
 
-template <int TG, int NM>
+template <int T, int NM>
 static int launch_grad(SelectedGrad p, int B, int Hkv, cudaStream_t stream) {
     const char *what = "wa_selected_backward";
-    constexpr size_t smem = (size_t)((2 * SG_OWN + 4 * TG) * (64 * NM + 4) + 2 * SG_OWN * (TG + 4)) * 4 + 2 * (TG > SG_OWN ? TG : SG_OWN) * 8;
+    constexpr size_t smem = (size_t)(6 * T * (128 * NM + 4) + T * (T + 4)) * 4 + 2 * T * 8;
+    static_assert(smem <= 227 * 1024, "shared memory budget exceeded");
     static PerDeviceOnce attr_set;
     if (!attr_set.done()) {
-        cudaError_t e = cudaFuncSetAttribute(selected_grad_kernel<TG, NM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(selected_grad_kernel<TG, NM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
-    p.tiles = ceil_div(p.block, SG_OWN);
-    const long long kx = (long long)p.Nkv * p.tiles, qx = (long long)p.Nq * p.tiles;
+    p.tiles = ceil_div(p.block, T);
+    const long long kx = (long long)B * Hkv * p.Nkv * p.tiles, qx = (long long)B * p.H * p.Nq * p.tiles;
     WA_REQUIRE(kx < (1ll << 31) && qx < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: grid too large", what);
     int rc;
-    selected_grad_kernel<TG, NM, true><<<dim3((unsigned)kx, Hkv, B), 256, smem, stream>>>(p);
+    selected_grad_kernel<T, NM, true><<<(unsigned)kx, 256, smem, stream>>>(p);
     if ((rc = check_launch(what))) return rc;
-    selected_grad_kernel<TG, NM, false><<<dim3((unsigned)qx, p.H, B), 256, smem, stream>>>(p);
+    selected_grad_kernel<T, NM, false><<<(unsigned)qx, 256, smem, stream>>>(p);
     return check_launch(what);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
+// Heaviest first where there are more items than SMs but their tensors fit L2 side by side: the order over all heads mixes the heads, which larger calls
+// pay for with what the CTAs of one head would find in L2.  (Three frames of 390 tokens, 12 heads, float32: TIMES2; TIMES3)
+static bool selected_ordered(const wa_selected_params *p, const SelectedPlan &w) {
+    const long long bytes = 2ll * dtype_size(p->q.dtype) * p->B * p->D * ((long long)p->H * p->Lq + (long long)p->Hkv * p->Lkv);
+    return (long long)p->B * p->H * w.Nq > sm_count() && (long long)p->B * p->H * w.Nq <= (1 << 20) && (long long)p->B * p->Hkv * w.Nkv <= (1 << 20) && bytes <= 64ll << 20;
+}
+
 static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     SelectedPlan w{};
     w.Nq = ceil_div(p->Lq, p->block_size);
@@ -604,8 +641,12 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     }
     w.index = c; c = align_up(c + lists * p->index_stride * sizeof(int32_t), 256);
     w.num = c; c = align_up(c + lists * sizeof(int32_t), 256);
+    if (selected_ordered(p, w)) w.q_order = c, c = align_up(c + lists * sizeof(int32_t), 256);
     if (backward) {
         w.rows = c; c = align_up(c + (size_t)p->B * p->H * w.Nkv * w.row_words * sizeof(uint32_t), 256);
+        if (selected_ordered(p, w)) {
+            w.k_order = c; c = align_up(c + (size_t)p->B * p->Hkv * w.Nkv * sizeof(int32_t), 256);
+        }
         w.stats = c; c = align_up(c + (size_t)p->B * p->H * selected_stats_rows(p, w.Nq) * 2 * sizeof(float), 256);
     }
     w.tuned = c;
@@ -634,6 +675,15 @@ static int selected_check(const wa_selected_params *p, bool backward, const char
     WA_REQUIRE(p->index && p->num, WA_ERR_ARG, "%s: index / num is null", what);
     WA_REQUIRE(p->lse || !backward, WA_ERR_ARG, "%s: lse is null", what);
     return 0;
+}
+
+// blocks of the queries, and for the gradient those of the keys, heaviest first
+static int selected_order(const wa_selected_params *p, const SelectedPlan &w, bool backward, char *ws, cudaStream_t stream, const char *what) {
+    const cudaError_t e = launch_dependent(selected_order_kernel, dim3(backward ? 2 : 1), dim3(1024), 0, stream, (const int32_t *)(ws + w.num),
+                                           (const uint32_t *)(ws + w.rows), p->B * p->H * w.Nq, p->B * p->Hkv * w.Nkv, w.group * w.row_words, w.Nkv,
+                                           w.group * w.Nq, (int32_t *)(ws + w.q_order), (int32_t *)(ws + w.k_order));
+    if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
 }
 
 static int selected_lists(const wa_selected_params *p, const SelectedPlan &w, bool backward, char *ws, cudaStream_t stream, const char *what) {
@@ -682,8 +732,10 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     if ((rc = selected_lists(p, w, false, ws, stream, what))) return rc;
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
     if (selected_sm100_forward_supported(p)) return selected_sm100_forward(p, index, num, ws + w.tuned, stream);
+    const bool ordered = p->D == 128 && selected_ordered(p, w);       // (the kernel of other head_dims takes its rows as they come)
+    if (ordered && (rc = selected_order(p, w, false, ws, stream, what))) return rc;
     return block_sparse_run(&p->q, &p->k, &p->v, &p->out, p->B, p->H, p->Lq, p->Lkv, p->D, p->block_size, index, num, p->index_stride, p->block_sizes, 0, 0,
-                            p->lse, nullptr, false, stream, w.group);
+                            p->lse, ordered ? (const int32_t *)(ws + w.q_order) : nullptr, false, stream, w.group);
 }
 
 extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) {
@@ -703,7 +755,13 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
     WA_REQUIRE(stats_rows < (1ull << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
     const int padded = (int)stats_rows;
     if ((rc = p->q.dtype == WA_BF16 ? launch_stats<__nv_bfloat16>(p, padded, stats, stream) : launch_stats<float>(p, padded, stats, stream))) return rc;
-    if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, ws + w.tuned, stream);
+    int32_t *q_order = nullptr, *k_order = nullptr;
+    if (selected_ordered(p, w)) {
+        q_order = (int32_t *)(ws + w.q_order);
+        k_order = (int32_t *)(ws + w.k_order);
+        if ((rc = selected_order(p, w, true, ws, stream, what))) return rc;
+    }
+    if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, q_order, k_order, ws + w.tuned, stream);
     SelectedGrad g{};
     g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v); g.dout = make_view(&p->dout);
     g.dq = p->dq.ptr; g.dqb = p->dq.stride_b; g.dql = p->dq.stride_l; g.dqh = p->dq.stride_h;
@@ -712,13 +770,11 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
     g.dtype = p->q.dtype;
     g.H = p->H; g.group = w.group; g.Lq = p->Lq; g.Lkv = p->Lkv; g.D = p->D; g.block = p->block_size; g.stride = p->index_stride;
     g.Nq = w.Nq; g.Nkv = w.Nkv; g.row_words = w.row_words; g.padded = padded;
-    g.index = index; g.num = num; g.block_sizes = p->block_sizes; g.rows = rows; g.stats = stats;
+    g.index = index; g.num = num; g.block_sizes = p->block_sizes; g.rows = rows; g.stats = stats; g.q_order = q_order; g.k_order = k_order;
     g.scale = (float)(1.0 / sqrt((double)p->D));
     const auto pieces = [](const wa_tensor4 &t) {
         return t.dtype == WA_F32 && (uintptr_t)t.ptr % 16 == 0 && t.stride_b % 4 == 0 && t.stride_l % 4 == 0 && t.stride_h % 4 == 0;
     };
     g.async = p->D % 4 == 0 && pieces(p->q) && pieces(p->k) && pieces(p->v) && pieces(p->dout);
-    if (p->D <= 64) return launch_grad<64, 1>(g, p->B, p->Hkv, stream);
-    if (p->D <= 128) return launch_grad<32, 2>(g, p->B, p->Hkv, stream);
-    return launch_grad<32, 4>(g, p->B, p->Hkv, stream);
+    return p->D <= 128 ? launch_grad<64, 1>(g, p->B, p->Hkv, stream) : launch_grad<32, 2>(g, p->B, p->Hkv, stream);
 }

@@ -63,6 +63,7 @@ struct SbParams {
     int list_stride, row_words;
     long long padded;                 // rows of `stats` of a head
     const int32_t *index, *num;       // queries
+    const int32_t *q_order, *k_order; // blocks of the owned side, heaviest first, or null: as they come
     const uint32_t *rows;             // keys
     const float *stats;
     __nv_bfloat16 *d1, *d2;           // dV; dK or dQ
@@ -206,9 +207,18 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 tell(0, SB_END, 0, 0);
                 break;
             }
-            const int item = at;
+            int item = at;
+            if (const int32_t *order = KEYS ? p.k_order : p.q_order) {
+                const int blk = order[at / PER], head = blk / (KEYS ? p.Nkv : p.Nq);      // (batch, head) of the block
+                item = head * p.owned + (blk - head * (KEYS ? p.Nkv : p.Nq)) * PER + at % PER;
+                if (item >= (head + 1) * p.owned) item = -1;                             // the last block has one tile
+            }
             int next_at = 0;
             if (lane == 0) next_at = (int)gridDim.x + atomicAdd(p.work_counter, 1);
+            if (item < 0) {
+                at = __shfl_sync(0xffffffffu, next_at, 0);
+                continue;
+            }
             const int tile = item % p.owned, head = item / p.owned;      // head: (batch, head) of the owned side
             const int b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
             const int hk = KEYS ? h : h / p.group;
@@ -542,7 +552,7 @@ static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t s
         attr_set.mark();
     }
     kp.owned = ceil_div(Lf, SB_OWN);
-    kp.items = p->B * Hf * kp.owned;
+    kp.items = (KEYS ? kp.k_order : kp.q_order) ? p->B * Hf * ceil_div(Lf, BLK) * (BLK / SB_OWN) : p->B * Hf * kp.owned;
     const wa_tensor4 &d2 = KEYS ? p->dk : p->dq;
     kp.d1 = (__nv_bfloat16 *)p->dv.ptr; kp.d1b = p->dv.stride_b; kp.d1l = p->dv.stride_l; kp.d1h = p->dv.stride_h;
     kp.d2 = (__nv_bfloat16 *)d2.ptr; kp.d2b = d2.stride_b; kp.d2l = d2.stride_l; kp.d2h = d2.stride_h;
@@ -562,8 +572,8 @@ bool selected_sm100_backward_supported(const wa_selected_params *p) {
 }
 size_t selected_sm100_backward_bytes(const wa_selected_params *) { return 256; }       // two work counters and the failure flag
 
-int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats, void *workspace,
-                            cudaStream_t stream) {
+int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats,
+                            const int32_t *q_order, const int32_t *k_order, void *workspace, cudaStream_t stream) {
     using namespace sm100;
     const cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
     if (e != cudaSuccess) return fail((int)e, "wa_selected_backward(tcgen05): %s", cudaGetErrorString(e));
@@ -572,7 +582,7 @@ int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, c
     kp.Nq = ceil_div(p->Lq, p->block_size); kp.Nkv = ceil_div(p->Lkv, p->block_size);
     kp.list_stride = p->index_stride; kp.row_words = ceil_div(kp.Nq, 32);
     kp.padded = (long long)selected_stats_rows(p, kp.Nq);
-    kp.index = index; kp.num = num; kp.rows = rows; kp.stats = stats;
+    kp.index = index; kp.num = num; kp.rows = rows; kp.stats = stats; kp.q_order = q_order; kp.k_order = k_order;
     kp.scale = (float)pow((double)TILE, -0.5);
     kp.scale_log2 = (float)(pow((double)TILE, -0.5) * 1.4426950408889634);
     kp.work_counter = (int *)workspace;
