@@ -610,7 +610,7 @@ PyObject *selected_backward(PyObject *const *a, Py_ssize_t n) {
     const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &out = THPVariable_Unpack(a[7]), &dout = THPVariable_Unpack(a[9]);
     if (out.sizes() != q.sizes() || dout.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || dout.scalar_type() != q.scalar_type())
         fail(PyExc_ValueError, "out and dout must have q's shape and dtype");
-    Tensor grad[3];
+    Tensor grad[3], laid;
     for (int i = 0; i < 3; ++i) {
         const Tensor &x = i == 0 ? q : k;
         const auto options = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
@@ -618,7 +618,10 @@ PyObject *selected_backward(PyObject *const *a, Py_ssize_t n) {
     }
     if (!c.nothing) {
         c.p.out = view4(out, c.keep[6]);
-        c.p.dout = view4(dout, c.keep[7]);
+        // (a gradient without memory of its own, or of odd strides, is laid out: the tensor-core kernels read 16 bytes at a time)
+        const bool odd = dout.scalar_type() == at::kBFloat16 && (dout.stride(0) % 8 || dout.stride(1) % 8 || dout.stride(2) % 8 || dout.stride(1) <= 0 || dout.stride(2) <= 0);
+        if (odd) laid = dout.contiguous();
+        c.p.dout = view4(odd ? laid : dout, c.keep[7]);
         c.keep[8] = THPVariable_Unpack(a[8]).contiguous();
         if (c.keep[8].scalar_type() != at::kFloat || c.keep[8].numel() != (int64_t)c.p.B * c.p.H * c.p.Lq) fail(PyExc_ValueError, "lse must be float32 [B, H, Lq]");
         c.p.lse = c.keep[8].data_ptr<float>();
