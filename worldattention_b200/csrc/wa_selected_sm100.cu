@@ -1,8 +1,8 @@
 // Gradient of attention over selected key blocks on the tensor cores of sm_100a: bf16, head_dim 128, blocks of 64 or 128 tokens.
 //
-// Two launches of one kernel.  Each owns 64 rows of one side at a time -- the first 64 key tokens, for dK and dV, the second 64 query rows,
-// for dQ -- and meets 128 rows of the other side per step: a block of 128, or two of 64 that need not be neighbours (nor, with shared
-// keys, of one query head).  With F1, F2 the owned rows and G1, G2 the met ones (keys: F = k, v and G = q, dout; queries: F = q, dout and G = k, v)
+// Two launches of one kernel.  Each owns a block of one side at a time -- the first of keys, for dK and dV, the second of queries, for dQ -- and
+// meets the blocks of the other side that are listed with it.  For blocks of 64 tokens (128: further down) a step meets two blocks,
+// which need not be neighbours (nor, with shared keys, of one query head).  With F1, F2 the owned rows and G1, G2 the met ones (keys: F = k, v and G = q, dout; queries: F = q, dout and G = k, v)
 //     S = G1 F1^T   dP = G2 F2^T                      [128 met rows x 64 owned ones]
 //     P = 2^(S c - lse)   dS = P (dP - delta)         (lse and delta of the query row: 128 of a step's, or 64 of an item's)
 //     dV^T += G2^T P   dK^T (or dQ^T) += G1^T dS      [128 channels x 64 owned rows]
@@ -132,13 +132,12 @@ struct SbList {
     }
 };
 
-template <bool KEYS, int BLK>
+template <bool KEYS>
 __global__ void __launch_bounds__(SB_THREADS, 1)
 selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
                            const __grid_constant__ CUtensorMap tm_g2, const SbParams p) {
     using Ring = SbRing<KEYS>;
     constexpr int SLOTS = Ring::SLOTS;
-    constexpr int PER = BLK / SB_OWN;                    // owned tiles of a block
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *f_s = smem, *g_s = f_s + 2 * SB_OWN_BYTES, *p_s = g_s + SLOTS * TILE_BYTES;      // p_s: [two steps][P, dS]
     SbBarriers *bar = reinterpret_cast<SbBarriers *>(p_s + 2 * Ring::FACTORS * SB_P_BYTES);
@@ -207,23 +206,15 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 tell(0, SB_END, 0, 0);
                 break;
             }
-            int item = at;
-            if (const int32_t *order = KEYS ? p.k_order : p.q_order) {
-                const int blk = order[at / PER], head = blk / (KEYS ? p.Nkv : p.Nq);      // (batch, head) of the block
-                item = head * p.owned + (blk - head * (KEYS ? p.Nkv : p.Nq)) * PER + at % PER;
-                if (item >= (head + 1) * p.owned) item = -1;                             // the last block has one tile
-            }
+            const int32_t *order = KEYS ? p.k_order : p.q_order;
+            const int item = order ? order[at] : at;
             int next_at = 0;
             if (lane == 0) next_at = (int)gridDim.x + atomicAdd(p.work_counter, 1);
-            if (item < 0) {
-                at = __shfl_sync(0xffffffffu, next_at, 0);
-                continue;
-            }
             const int tile = item % p.owned, head = item / p.owned;      // head: (batch, head) of the owned side
             const int b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
             const int hk = KEYS ? h : h / p.group;
             SbList<KEYS> list;
-            list.begin(p, (long long)head * (KEYS ? p.Nkv : p.Nq) + tile / PER, lane);
+            list.begin(p, item, lane);
             long long ahead = list.next(lane);
             if (ahead < 0) {
                 ok = tell(item, SB_EMPTY, 0, 0);
@@ -243,8 +234,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 ++items;
                 int flags = SB_FIRST;
                 while (ok && ahead >= 0) {
-                    const long long one = ahead, two = BLK == SB_OWN ? list.next(lane) : -1;
-                    ahead = BLK == SB_OWN && two < 0 ? -1 : list.next(lane);
+                    const long long one = ahead, two = list.next(lane);
+                    ahead = two < 0 ? -1 : list.next(lane);
                     if (ahead < 0) flags |= SB_LAST;
                     // rows and heads of the two halves; what is missing lies behind the last block and loads as zeros
                     const int blocks = KEYS ? p.Nq : p.Nkv;
@@ -252,9 +243,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     const int h0 = KEYS ? h * p.group + (int)(one >> 32) : hk, h1 = KEYS ? (two < 0 ? h0 : h * p.group + (int)(two >> 32)) : hk;
                     int real0 = SB_OWN, real1 = SB_OWN;
                     if (!KEYS) {
-                        const int n = p.Lkv - i0 * BLK;
-                        real0 = min(n, SB_OWN);
-                        real1 = BLK == TILE ? max(0, min(n - SB_OWN, SB_OWN)) : two < 0 ? 0 : min(p.Lkv - i1 * BLK, SB_OWN);
+                        real0 = min(p.Lkv - i0 * SB_OWN, SB_OWN);
+                        real1 = two < 0 ? 0 : min(p.Lkv - i1 * SB_OWN, SB_OWN);
                     }
                     ok = tell(item, flags, real0, real1);
                     flags = 0;
@@ -268,20 +258,16 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                             const CUtensorMap *map = g == 0 ? &tm_g1 : &tm_g2;
                             const bool with_stats = KEYS && g == 0;
                             mbar_expect_tx(full, TILE_BYTES + (with_stats ? TILE * 8 : 0));
-                            if (BLK == TILE) {
-                                tma_load_5d(dst, map, full, 0, i0 * TILE, 0, h0, b);
-                            } else {
-                                tma_load_5d(dst, map, full, 0, i0 * BLK, 0, h0, b);
-                                tma_load_5d(dst + HALF_BYTES / 2, map, full, 0, i1 * BLK, 0, h1, b);
-                                tma_load_5d(dst + HALF_BYTES, map, full, 0, i0 * BLK, 1, h0, b);
-                                tma_load_5d(dst + HALF_BYTES + HALF_BYTES / 2, map, full, 0, i1 * BLK, 1, h1, b);
-                            }
+                            tma_load_5d(dst, map, full, 0, i0 * SB_OWN, 0, h0, b);
+                            tma_load_5d(dst + HALF_BYTES / 2, map, full, 0, i1 * SB_OWN, 0, h1, b);
+                            tma_load_5d(dst + HALF_BYTES, map, full, 0, i0 * SB_OWN, 1, h0, b);
+                            tma_load_5d(dst + HALF_BYTES + HALF_BYTES / 2, map, full, 0, i1 * SB_OWN, 1, h1, b);
                             if (with_stats) {
                                 // (the statistics of step u - 2 have been read: its sums, which come after them, freed this slot)
                                 float *to = bar->stats + (steps & 1u) * 2 * TILE;
                                 const float *row = p.stats + ((long long)b * p.H) * p.padded * 2;
-                                bulk_load(to, row + (h0 * p.padded + (long long)i0 * BLK) * 2, BLK * 8, full);
-                                if (BLK != TILE) bulk_load(to + TILE, row + (h1 * p.padded + (long long)i1 * BLK) * 2, BLK * 8, full);
+                                bulk_load(to, row + (h0 * p.padded + (long long)i0 * SB_OWN) * 2, SB_OWN * 8, full);
+                                bulk_load(to + TILE, row + (h1 * p.padded + (long long)i1 * SB_OWN) * 2, SB_OWN * 8, full);
                             }
                         }
                         __syncwarp();
@@ -529,36 +515,436 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     if (warp == SB_WORKERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
+// ---- blocks of 128 tokens ---------------------------------------------------------------------------
+// An item owns a whole block, and the roles of the operands change:
+//     S = F1 G1^T   dP = F2 G2^T               [128 owned rows x 128 met ones]
+//     dV += P G2   dK (or dQ) += dS G1         [128 owned rows x 128 channels]
+// P and dS go back to tensor memory over the scores that they were made from and are first operands from there; shared memory holds nothing but
+// tiles, its reads (two tiles for 128 columns of a score product, one for a sum) are half those of the kernel above for the same
+// work, and a met tile is loaded half as often.  A warp writes its 32 columns of P as 16 words over the first half of its own 32 columns of S, so
+// that no warp waits for another's reads; the products take each K step's address from there.
+// Tensor memory: S, dP, dV and dK; or S, two of dP, and dQ.  Scores of step u + 1 follow as soon as their columns are free: behind the sum that
+// read P or dS, or, for dQ's S, behind the workers' reads.
+template <bool KEYS>
+struct SwBarriers {
+    float stats[2][2 * TILE];         // keys: of the met rows, per step; 64 rows' (-normaliser), their deltas, and the same of the others
+    uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
+    uint64_t f_full, f_empty, stats_full[2], stats_empty[2];
+    uint64_t full[5], empty[5];
+    uint64_t s_full, s_free, p_full;
+    uint64_t dp_full[2], dp_free[2], ds_full[2];
+    uint64_t acc_full, acc_empty;
+    uint32_t tmem_base;
+    int abort_flag;
+    SbDesc desc[SB_DESCS];
+};
+constexpr int SW_SLOTS = 5;
+constexpr int SW_SMEM = (2 + SW_SLOTS) * TILE_BYTES + 3072;
+static_assert(sizeof(SwBarriers<true>) <= 3072 && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
+
+template <bool KEYS>
+__global__ void __launch_bounds__(SB_THREADS, 1)
+selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
+                          const __grid_constant__ CUtensorMap tm_g2, const SbParams p) {
+    constexpr int DPS = KEYS ? 1 : 2;                    // buffers of dP
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *f_s = smem, *g_s = f_s + 2 * TILE_BYTES;
+    SwBarriers<KEYS> *bar = reinterpret_cast<SwBarriers<KEYS> *>(g_s + SW_SLOTS * TILE_BYTES);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    volatile int *abort_flag = &bar->abort_flag;
+    const FailSink sink{p.error_flag, p.status_mirror};
+
+    if (threadIdx.x == 0) {
+        bar->abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;
+        if (bar->abort_flag) report_failure(sink, 498);
+        for (int i = 0; i < SB_DESCS; ++i) {
+            mbar_init(&bar->desc_full[i], 1);
+            mbar_init(&bar->desc_empty[i], 2 + SB_WORKERS);
+        }
+        mbar_init(&bar->f_full, 1);
+        mbar_init(&bar->f_empty, 1);
+        for (int i = 0; i < SW_SLOTS; ++i) {
+            mbar_init(&bar->full[i], 1);
+            mbar_init(&bar->empty[i], 1);
+        }
+        mbar_init(&bar->s_full, 1);
+        mbar_init(&bar->s_free, KEYS ? 1 : SB_WORKERS);  // the sum that read P; the workers that read S
+        mbar_init(&bar->p_full, SB_WORKERS);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar->stats_full[i], 1);
+            mbar_init(&bar->stats_empty[i], SB_WORKERS);
+            mbar_init(&bar->dp_full[i], 1);
+            mbar_init(&bar->dp_free[i], 1);
+            mbar_init(&bar->ds_full[i], SB_WORKERS);
+        }
+        mbar_init(&bar->acc_full, 1);
+        mbar_init(&bar->acc_empty, SB_WORKERS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == SB_WORKERS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem_base;
+    const uint32_t tm_s = tmem, tm_dp = tmem + TILE, tm_sum1 = tmem + 2 * TILE, tm_sum2 = tmem + 3 * TILE;       // (dQ: the second dP lies at tm_sum1)
+    auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+
+    if (warp == SB_WORKERS) {
+        // ================= lists and loads =================
+        const bool leader = elect_one();
+        uint32_t descs = 0, tiles = 0, items = 0, steps = 0;
+        bool ok = true;
+        int at = blockIdx.x;
+        auto tell = [&](int item, int flags, int real) {
+            const uint32_t d = descs % SB_DESCS;
+            if (!wait(&bar->desc_empty[d], ((descs / SB_DESCS) & 1u) ^ 1u, 431)) return false;
+            if (leader) {
+                bar->desc[d].item = item;
+                bar->desc[d].flags = flags;
+                bar->desc[d].real[0] = real;
+                mbar_arrive(&bar->desc_full[d]);
+            }
+            __syncwarp();
+            ++descs;
+            return true;
+        };
+        while (ok) {
+            if (at >= p.items) {
+                tell(0, SB_END, 0);
+                break;
+            }
+            const int32_t *order = KEYS ? p.k_order : p.q_order;
+            const int item = order ? order[at] : at;
+            int next_at = 0;
+            if (lane == 0) next_at = (int)gridDim.x + atomicAdd(p.work_counter, 1);
+            const int tile = item % p.owned, head = item / p.owned;
+            const int b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
+            const int hk = KEYS ? h : h / p.group;
+            SbList<KEYS> list;
+            list.begin(p, item, lane);
+            long long ahead = list.next(lane);
+            if (ahead < 0) {
+                ok = tell(item, SB_EMPTY, 0);
+            } else {
+                ok = wait(&bar->f_empty, (items & 1u) ^ 1u, 432);
+                if (ok && leader) {
+                    mbar_expect_tx(&bar->f_full, 2 * TILE_BYTES);
+                    tma_load_5d(f_s, &tm_f1, &bar->f_full, 0, tile * TILE, 0, h, b);
+                    tma_load_5d(f_s + TILE_BYTES, &tm_f2, &bar->f_full, 0, tile * TILE, 0, h, b);
+                }
+                __syncwarp();
+                ++items;
+                int flags = SB_FIRST;
+                while (ok && ahead >= 0) {
+                    const int i0 = (int)(ahead & 0xffffffff), h0 = KEYS ? h * p.group + (int)(ahead >> 32) : hk;
+                    ahead = list.next(lane);
+                    if (ahead < 0) flags |= SB_LAST;
+                    ok = tell(item, flags, KEYS ? TILE : min(p.Lkv - i0 * TILE, TILE));
+                    flags = 0;
+#pragma unroll
+                    for (int g = 0; g < 2 && ok; ++g) {
+                        const uint32_t slot = tiles % SW_SLOTS;
+                        ok = wait(&bar->empty[slot], ((tiles / SW_SLOTS) & 1u) ^ 1u, 433);
+                        if (ok && leader) {
+                            mbar_expect_tx(&bar->full[slot], TILE_BYTES);
+                            tma_load_5d(g_s + slot * TILE_BYTES, g == 0 ? &tm_g1 : &tm_g2, &bar->full[slot], 0, i0 * TILE, 0, h0, b);
+                        }
+                        __syncwarp();
+                        ++tiles;
+                    }
+                    if (KEYS && ok) {      // (behind the tiles: it waits for the workers to be through with step u - 2, which the next tiles would as well)
+                        const uint32_t s = steps & 1u;
+                        ok = wait(&bar->stats_empty[s], ((steps >> 1) & 1u) ^ 1u, 434);
+                        if (ok && leader) {
+                            mbar_expect_tx(&bar->stats_full[s], TILE * 8);
+                            bulk_load(bar->stats[s], p.stats + (((long long)b * p.H + h0) * p.padded + (long long)i0 * TILE) * 2, TILE * 8, &bar->stats_full[s]);
+                        }
+                        __syncwarp();
+                    }
+                    ++steps;
+                }
+            }
+            at = __shfl_sync(0xffffffffu, next_at, 0);
+        }
+        if (*abort_flag) {      // given up: copies on their way land within microseconds, the block's shared memory is kept for a millisecond
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) { }
+        }
+    } else if (warp == SB_WORKERS + 1) {
+        // ================= scores =================
+        const bool leader = elect_one();
+        constexpr uint32_t SCORE = instr_desc(false, TILE);
+        uint32_t descs = 0, items = 0, steps = 0;
+        bool ok = true;
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 441);
+            if (!ok) break;
+            const int flags = bar->desc[d].flags;
+            __syncwarp();
+            if (leader) mbar_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+            if (flags & SB_EMPTY) continue;
+            if (flags & SB_FIRST) {
+                ok = wait(&bar->f_full, items & 1u, 442);
+                ++items;
+            }
+            const uint32_t buf = steps % DPS;
+#pragma unroll
+            for (int g = 0; g < 2 && ok; ++g) {
+                const uint32_t slot = (2 * steps + g) % SW_SLOTS;
+                ok = wait(&bar->full[slot], ((2 * steps + g) / SW_SLOTS) & 1u, 443);
+                if (ok) ok = g == 0 ? wait(&bar->s_free, (steps & 1u) ^ 1u, 444) : wait(&bar->dp_free[buf], ((steps / DPS) & 1u) ^ 1u, 445);
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t f = smem_desc(smem_u32(f_s + g * TILE_BYTES), 16, 1024), m = smem_desc(smem_u32(g_s + slot * TILE_BYTES), 16, 1024);
+                    const uint32_t to = g == 0 ? tm_s : tm_dp + buf * TILE;
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk) {
+                        const uint64_t off = (uint64_t)(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4);
+                        mma_ss(to, f + off, m + off, SCORE, kk > 0);
+                    }
+                    tc_commit(g == 0 ? &bar->s_full : &bar->dp_full[buf]);
+                    if (!KEYS && g == 1) tc_commit(&bar->empty[slot]);       // values take no part in dQ's sum
+                    if (g == 1 && (flags & SB_LAST)) tc_commit(&bar->f_empty);
+                }
+                __syncwarp();
+            }
+            ++steps;
+        }
+    } else if (warp == SB_WORKERS + 2) {
+        // ================= sums =================
+        const bool leader = elect_one();
+        constexpr uint32_t SUM = instr_desc(true, TILE);
+        uint32_t descs = 0, items = 0, steps = 0;
+        bool ok = true;
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 451);
+            if (!ok) break;
+            const int flags = bar->desc[d].flags;
+            __syncwarp();
+            if (leader) mbar_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+            if (flags & SB_EMPTY) continue;
+            const bool fresh = flags & SB_FIRST;
+            if (fresh) {
+                ok = wait(&bar->acc_empty, (items & 1u) ^ 1u, 452);
+                ++items;
+            }
+            const uint32_t buf = steps % DPS, s1 = (2 * steps) % SW_SLOTS, s2 = (2 * steps + 1) % SW_SLOTS;
+            auto add = [&](uint32_t to, uint32_t factor, uint32_t slot) {       // factor: 8 words a K step, two steps of each 32 columns
+                const uint64_t m = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024);
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                    mma_ts(to, factor + (kk >> 1) * 32 + (kk & 1) * 8, m + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
+            };
+            if (KEYS) {
+                if (ok) ok = wait(&bar->p_full, steps & 1u, 453);
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
+                    add(tm_sum1, tm_s, s2);
+                    tc_commit(&bar->s_free);
+                }
+                __syncwarp();
+            }
+            if (ok) ok = wait(&bar->ds_full[buf], (steps / DPS) & 1u, 454);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+                add(tm_sum2, tm_dp + buf * TILE, s1);
+                tc_commit(&bar->dp_free[buf]);
+                tc_commit(&bar->empty[s1]);
+                if (KEYS) tc_commit(&bar->empty[s2]);      // (dS was made from dP, which has read it too)
+                if (flags & SB_LAST) tc_commit(&bar->acc_full);
+            }
+            __syncwarp();
+            ++steps;
+        }
+    } else {
+        // ================= P, dS and the finished sums =================
+        // a thread has one owned row (tensor-memory lane) and 32 met ones (columns)
+        const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
+        const uint32_t at = (((uint32_t)(quarter * 32)) << 16) + part * 32;
+        uint32_t descs = 0, steps = 0, items = 0;
+        bool ok = true;
+        float2 norm = make_float2(0.f, 0.f), delta = norm;        // queries: of the row
+        const float2 c = make_float2(p.scale_log2, p.scale_log2);
+        auto place = [&](int item, int &b, int &h, int &token) {
+            const int heads = KEYS ? p.Hkv : p.H, head = item / p.owned;
+            b = head / heads;
+            h = head - b * heads;
+            token = (item - head * p.owned) * TILE + row;
+        };
+        // 32 channels of the row
+        auto put = [&](int item, const uint32_t (&v)[32], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
+            int b, h, token;
+            place(item, b, h, token);
+            if (token >= (KEYS ? p.Lkv : p.Lq)) return;
+            uint4 *out = reinterpret_cast<uint4 *>(to + b * sb + (long long)token * sl + h * sh + part * 32);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]) * scale, __uint_as_float(v[8 * q + 2 * e + 1]) * scale);
+                    w[e] = *reinterpret_cast<const uint32_t *>(&x);
+                }
+                out[q] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        };
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 461);
+            if (!ok) break;
+            const int item = bar->desc[d].item, flags = bar->desc[d].flags, real = bar->desc[d].real[0];
+            warp_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+            uint32_t v[32];
+            if (flags & SB_EMPTY) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0u;
+                if (KEYS) put(item, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
+                put(item, v, p.d2, p.d2b, p.d2l, p.d2h, 1.0f);
+                continue;
+            }
+            if (!KEYS && (flags & SB_FIRST)) {
+                int b, h, token;
+                place(item, b, h, token);
+                const float *st = p.stats + ((long long)b * p.H + h) * p.padded * 2 + selected_stat(token);
+                norm = make_float2(st[0], st[0]);
+                delta = make_float2(-st[64], -st[64]);
+            }
+            const uint32_t s2 = steps & 1u, buf = steps % DPS;
+            const float *st = bar->stats[s2] + (part >> 1) * TILE + (part & 1) * 32;       // keys: of the 32 met rows
+            if (KEYS) ok = wait(&bar->stats_full[s2], (steps >> 1) & 1u, 462);
+            if (ok) ok = wait(&bar->s_full, steps & 1u, 463);
+            if (!ok) break;
+            tc_fence_after();
+            float2 pr[16];
+            TMEM_LD32(tm_s + at, v);
+            tmem_wait_ld32(v);
+            if (!KEYS) {
+                tc_fence_before();
+                warp_arrive(&bar->s_free);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float4 n4 = KEYS ? *reinterpret_cast<const float4 *>(st + 2 * j) : make_float4(norm.x, norm.x, norm.x, norm.x);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 z = __ffma2_rn(make_float2(__uint_as_float(v[2 * (j + e)]), __uint_as_float(v[2 * (j + e) + 1])), c,
+                                                e == 0 ? make_float2(n4.x, n4.y) : make_float2(n4.z, n4.w));
+                    pr[j + e] = make_float2(ex2(z.x), ex2(z.y));
+                }
+            }
+            uint32_t w[16];
+            auto pack = [&]() {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const __nv_bfloat162 x = __floats2bfloat162_rn(pr[j].x, pr[j].y);
+                    w[j] = *reinterpret_cast<const uint32_t *>(&x);
+                }
+            };
+            if (KEYS) {
+                pack();
+                TMEM_ST16(tm_s + at, w);
+                tmem_wait_st();
+                tc_fence_before();
+                warp_arrive(&bar->p_full);
+            } else if (real < TILE) {      // tokens that are no keys (the last block)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (part * 32 + 2 * j >= real) pr[j].x = 0.f;
+                    if (part * 32 + 2 * j + 1 >= real) pr[j].y = 0.f;
+                }
+            }
+            ok = wait(&bar->dp_full[buf], (steps / DPS) & 1u, 464);
+            if (!ok) break;
+            tc_fence_after();
+            TMEM_LD32(tm_dp + buf * TILE + at, v);
+            tmem_wait_ld32(v);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float4 d4 = KEYS ? *reinterpret_cast<const float4 *>(st + SB_OWN + 2 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 x = make_float2(__uint_as_float(v[2 * (j + e)]), __uint_as_float(v[2 * (j + e) + 1]));
+                    const float2 dl = KEYS ? (e == 0 ? make_float2(-d4.x, -d4.y) : make_float2(-d4.z, -d4.w)) : delta;
+                    pr[j + e] = __fmul2_rn(pr[j + e], __fadd2_rn(x, dl));
+                }
+            }
+            pack();
+            TMEM_ST16(tm_dp + buf * TILE + at, w);
+            tmem_wait_st();
+            tc_fence_before();
+            if (KEYS) warp_arrive(&bar->stats_empty[s2]);
+            warp_arrive(&bar->ds_full[buf]);
+            ++steps;
+            if (flags & SB_LAST) {
+                ok = wait(&bar->acc_full, items & 1u, 465);
+                ++items;
+                if (!ok) break;
+                tc_fence_after();
+                if (KEYS) {
+                    TMEM_LD32(tm_sum1 + at, v);
+                    tmem_wait_ld32(v);
+                    put(item, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
+                }
+                TMEM_LD32(tm_sum2 + at, v);
+                tmem_wait_ld32(v);
+                tc_fence_before();
+                warp_arrive(&bar->acc_empty);
+                put(item, v, p.d2, p.d2b, p.d2l, p.d2h, p.scale);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == SB_WORKERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
 static bool aligned_view(const wa_tensor4 *t) {
     return t->ptr && (uintptr_t)t->ptr % 16 == 0 && t->stride_h % 8 == 0 && t->stride_l % 8 == 0 && t->stride_b % 8 == 0 && t->stride_h > 0 && t->stride_l > 0;
 }
 
-template <bool KEYS, int BLK>
+template <bool KEYS, int BLK>      // BLK: 64, or 128 for the kernel that owns whole blocks of 128
 static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t stream) {
     const char *what = "wa_selected_backward(tcgen05)";
+    constexpr int OWN = BLK == TILE ? TILE : SB_OWN, SMEM = BLK == TILE ? SW_SMEM : SbRing<KEYS>::SMEM;
     const wa_tensor4 &f1 = KEYS ? p->k : p->q, &f2 = KEYS ? p->v : p->dout, &g1 = KEYS ? p->q : p->k, &g2 = KEYS ? p->dout : p->v;
     const int Lf = KEYS ? p->Lkv : p->Lq, Hf = KEYS ? p->Hkv : p->H, Lg = KEYS ? p->Lq : p->Lkv, Hg = KEYS ? p->H : p->Hkv;
     CUtensorMap maps[4];
     int rc;
-    if ((rc = selected_sm100_map(&maps[0], &f1, p->B, Lf, Hf, "the owned rows", SB_OWN, 2))) return rc;
-    if ((rc = selected_sm100_map(&maps[1], &f2, p->B, Lf, Hf, "the owned rows", SB_OWN, 2))) return rc;
+    if ((rc = selected_sm100_map(&maps[0], &f1, p->B, Lf, Hf, "the owned rows", OWN, 2))) return rc;
+    if ((rc = selected_sm100_map(&maps[1], &f2, p->B, Lf, Hf, "the owned rows", OWN, 2))) return rc;
     if ((rc = selected_sm100_map(&maps[2], &g1, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
     if ((rc = selected_sm100_map(&maps[3], &g2, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
-    const auto kernel = selected_grad_sm100_kernel<KEYS, BLK>;
+    const auto kernel = BLK == TILE ? selected_grad_wide_kernel<KEYS> : selected_grad_sm100_kernel<KEYS>;
     static PerDeviceOnce attr_set;
     if (!attr_set.done()) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SbRing<KEYS>::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
-    kp.owned = ceil_div(Lf, SB_OWN);
-    kp.items = (KEYS ? kp.k_order : kp.q_order) ? p->B * Hf * ceil_div(Lf, BLK) * (BLK / SB_OWN) : p->B * Hf * kp.owned;
+    kp.owned = ceil_div(Lf, OWN);
+    kp.items = p->B * Hf * kp.owned;
     const wa_tensor4 &d2 = KEYS ? p->dk : p->dq;
     kp.d1 = (__nv_bfloat16 *)p->dv.ptr; kp.d1b = p->dv.stride_b; kp.d1l = p->dv.stride_l; kp.d1h = p->dv.stride_h;
     kp.d2 = (__nv_bfloat16 *)d2.ptr; kp.d2b = d2.stride_b; kp.d2l = d2.stride_l; kp.d2h = d2.stride_h;
     kp.work_counter += KEYS ? 0 : 1;
     const int sms = sm_count();
-    const cudaError_t e = launch_dependent(kernel, dim3(kp.items < sms ? kp.items : sms), dim3(SB_THREADS), SbRing<KEYS>::SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
+    const cudaError_t e = launch_dependent(kernel, dim3(kp.items < sms ? kp.items : sms), dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
@@ -567,7 +953,8 @@ static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t s
 
 bool selected_sm100_backward_supported(const wa_selected_params *p) {
     using namespace sm100;
-    return selected_sm100_tensors(p) && aligned_view(&p->dout) && (long long)p->B * p->H * (ceil_div(p->Lq, SB_OWN) + 1ll) <= (1 << 24) &&
+    return selected_sm100_tensors(p) && aligned_view(&p->dout) && aligned_view(&p->dq) && aligned_view(&p->dk) && aligned_view(&p->dv) &&
+           (long long)p->B * p->H * (ceil_div(p->Lq, SB_OWN) + 1ll) <= (1 << 24) &&
            (long long)p->B * p->Hkv * (ceil_div(p->Lkv, SB_OWN) + 1ll) <= (1 << 24);
 }
 size_t selected_sm100_backward_bytes(const wa_selected_params *) { return 256; }       // two work counters and the failure flag
