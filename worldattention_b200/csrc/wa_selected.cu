@@ -358,7 +358,7 @@ selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int 
             const bool seen = there && natural[u] != -INFINITY;
             float *to = stats + (b[u] * H + h[u]) * padded * 2 + selected_stat(l[u]);
             to[0] = seen ? -1.4426950408889634f * natural[u] : -INFINITY;
-            to[64] = seen ? sum[u] : 0.f;
+            to[64] = seen ? -sum[u] : 0.f;
         }
     }
 }
@@ -537,7 +537,7 @@ selected_grad_kernel(const SelectedGrad p) {
                 const float2 row = st[KEYS ? buf * T + g : f];
                 const bool there = first + f < own_real && now.from + g < now.end;
                 s[i][j] = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
-                dp[i][j] = there ? s[i][j] * (dp[i][j] - row.y) * p.scale : 0.f;
+                dp[i][j] = there ? s[i][j] * (dp[i][j] + row.y) * p.scale : 0.f;
             }
         const auto add = [&](float4 (&acc)[R][NM], const float (&factor)[R][C], const float *x) {
             __syncwarp();

@@ -42,7 +42,7 @@ struct SbDesc {
 };
 
 struct SbBarriers {
-    // 64 rows' (-normaliser) and their deltas.  keys: of the met rows, [two steps][two]; queries: of the owned rows, [four items] -- when an
+    // 64 rows' (-normaliser) and their (-delta).  keys: of the met rows, [two steps][two]; queries: of the owned rows, [four items] -- when an
     // item's are loaded, the warps may still be two items behind
     float stats[4 * TILE];
     uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
@@ -437,13 +437,13 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             }
             if ((steps & 1u) == (uint32_t)group && ok) {
                 const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
-                // (-normaliser, delta) of the met row, or of the owned rows: 64 of one, 64 of the other
+                // (-normaliser, -delta) of the met row, or of the owned rows: 64 of one, 64 of the other
                 const float *st = bar->stats + (KEYS ? buf * 2 * TILE + (row >> 6) * TILE + (row & 63) : ((items - 1) & 3u) * TILE);
                 float2 norm = make_float2(0.f, 0.f), delta = norm;
                 if (KEYS) {
                     ok = wait(&bar->full[slot], ((2 * steps) / SLOTS) & 1u, 424);
                     norm = make_float2(st[0], st[0]);
-                    delta = make_float2(-st[SB_OWN], -st[SB_OWN]);
+                    delta = make_float2(st[SB_OWN], st[SB_OWN]);
                 }
                 // queries: rows that are no keys
                 const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
@@ -469,7 +469,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 #pragma unroll
                         for (int e = 0; e < 4; e += 2) {
                             const float2 n = e == 0 ? make_float2(n4.x, n4.y) : make_float2(n4.z, n4.w);
-                            const float2 d = KEYS ? delta : e == 0 ? make_float2(-d4.x, -d4.y) : make_float2(-d4.z, -d4.w);
+                            const float2 d = KEYS ? delta : e == 0 ? make_float2(d4.x, d4.y) : make_float2(d4.z, d4.w);
                             const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[j + e]), __uint_as_float(x[j + e + 1])), c, n);
                             float2 pr = make_float2(ex2(z.x), ex2(z.y));
                             float2 ds = __fmul2_rn(pr, __fadd2_rn(make_float2(__uint_as_float(y[j + e]), __uint_as_float(y[j + e + 1])), d));
@@ -523,30 +523,36 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 // tiles, its reads (two tiles for 128 columns of a score product, one for a sum) are half those of the kernel above for the same
 // work, and a met tile is loaded half as often.  A warp writes its 32 columns of P as 16 words over the first half of its own 32 columns of S, so
 // that no warp waits for another's reads; the products take each K step's address from there.
+// Finished sums leave through the ring of tiles: at an item's end the loading warp gives the workers a slot for each, they leave it as bf16 there, and a
+// warp of its own stores it and gives the slot back.  (Stored by the workers themselves, 32 rows of 16 or 32 bytes at a time, an item's end took
+// 8000 cycles, three steps' time; lists of a chunk's keys are five steps long.)
 // Tensor memory: S, dP, dV and dK; or S, two of dP, and dQ.  Scores of step u + 1 follow as soon as their columns are free: behind the sum that
 // read P or dS, or, for dQ's S, behind the workers' reads.
 template <bool KEYS>
 struct SwBarriers {
-    float stats[2][2 * TILE];         // keys: of the met rows, per step; 64 rows' (-normaliser), their deltas, and the same of the others
+    float stats[2][2 * TILE];         // keys: of the met rows, per step; 64 rows' (-normaliser), their (-delta), and the same of the others
     uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
     uint64_t f_full, f_empty, stats_full[2], stats_empty[2];
     uint64_t full[5], empty[5];
     uint64_t s_full, s_free, p_full;
     uint64_t dp_full[2], dp_free[2], ds_full[2];
-    uint64_t acc_full, acc_empty;
+    uint64_t acc_full, acc_empty, staged[SB_DESCS];
     uint32_t tmem_base;
     int abort_flag;
     SbDesc desc[SB_DESCS];
 };
 constexpr int SW_SLOTS = 5;
+constexpr int SW_THREADS = SB_THREADS + 32;
 constexpr int SW_SMEM = (2 + SW_SLOTS) * TILE_BYTES + 3072;
 static_assert(sizeof(SwBarriers<true>) <= 3072 && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
 
 template <bool KEYS>
-__global__ void __launch_bounds__(SB_THREADS, 1)
+__global__ void __launch_bounds__(SW_THREADS, 1)
 selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
-                          const __grid_constant__ CUtensorMap tm_g2, const SbParams p) {
+                          const __grid_constant__ CUtensorMap tm_g2, const __grid_constant__ CUtensorMap tm_d1, const __grid_constant__ CUtensorMap tm_d2,
+                          const SbParams p) {
     constexpr int DPS = KEYS ? 1 : 2;                    // buffers of dP
+    constexpr int OUTS = KEYS ? 2 : 1;                   // sums of an item: slots that it takes at its end
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *f_s = smem, *g_s = f_s + 2 * TILE_BYTES;
     SwBarriers<KEYS> *bar = reinterpret_cast<SwBarriers<KEYS> *>(g_s + SW_SLOTS * TILE_BYTES);
@@ -559,7 +565,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         if (bar->abort_flag) report_failure(sink, 498);
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
-            mbar_init(&bar->desc_empty[i], 2 + SB_WORKERS);
+            mbar_init(&bar->desc_empty[i], 3 + SB_WORKERS);
+            mbar_init(&bar->staged[i], SB_WORKERS);
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
@@ -627,8 +634,19 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             SbList<KEYS> list;
             list.begin(p, item, lane);
             long long ahead = list.next(lane);
+            auto grant = [&]() {      // slots for the item's sums
+#pragma unroll
+                for (int g = 0; g < OUTS && ok; ++g) {
+                    const uint32_t slot = tiles % SW_SLOTS;
+                    ok = wait(&bar->empty[slot], ((tiles / SW_SLOTS) & 1u) ^ 1u, 435);
+                    if (ok && leader) mbar_arrive(&bar->full[slot]);
+                    __syncwarp();
+                    ++tiles;
+                }
+            };
             if (ahead < 0) {
                 ok = tell(item, SB_EMPTY, 0);
+                grant();
             } else {
                 ok = wait(&bar->f_empty, (items & 1u) ^ 1u, 432);
                 if (ok && leader) {
@@ -667,6 +685,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     }
                     ++steps;
                 }
+                grant();
             }
             at = __shfl_sync(0xffffffffu, next_at, 0);
         }
@@ -678,7 +697,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         // ================= scores =================
         const bool leader = elect_one();
         constexpr uint32_t SCORE = instr_desc(false, TILE);
-        uint32_t descs = 0, items = 0, steps = 0;
+        uint32_t descs = 0, items = 0, steps = 0, tiles = 0;
         bool ok = true;
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -689,7 +708,10 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (leader) mbar_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
-            if (flags & SB_EMPTY) continue;
+            if (flags & SB_EMPTY) {
+                tiles += OUTS;
+                continue;
+            }
             if (flags & SB_FIRST) {
                 ok = wait(&bar->f_full, items & 1u, 442);
                 ++items;
@@ -697,8 +719,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             const uint32_t buf = steps % DPS;
 #pragma unroll
             for (int g = 0; g < 2 && ok; ++g) {
-                const uint32_t slot = (2 * steps + g) % SW_SLOTS;
-                ok = wait(&bar->full[slot], ((2 * steps + g) / SW_SLOTS) & 1u, 443);
+                const uint32_t slot = (tiles + g) % SW_SLOTS;
+                ok = wait(&bar->full[slot], ((tiles + g) / SW_SLOTS) & 1u, 443);
                 if (ok) ok = g == 0 ? wait(&bar->s_free, (steps & 1u) ^ 1u, 444) : wait(&bar->dp_free[buf], ((steps / DPS) & 1u) ^ 1u, 445);
                 if (!ok) break;
                 tc_fence_after();
@@ -717,12 +739,13 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                 __syncwarp();
             }
             ++steps;
+            tiles += 2 + (flags & SB_LAST ? OUTS : 0);
         }
     } else if (warp == SB_WORKERS + 2) {
         // ================= sums =================
         const bool leader = elect_one();
         constexpr uint32_t SUM = instr_desc(true, TILE);
-        uint32_t descs = 0, items = 0, steps = 0;
+        uint32_t descs = 0, items = 0, steps = 0, tiles = 0;
         bool ok = true;
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -733,13 +756,16 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (leader) mbar_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
-            if (flags & SB_EMPTY) continue;
+            if (flags & SB_EMPTY) {
+                tiles += OUTS;
+                continue;
+            }
             const bool fresh = flags & SB_FIRST;
             if (fresh) {
                 ok = wait(&bar->acc_empty, (items & 1u) ^ 1u, 452);
                 ++items;
             }
-            const uint32_t buf = steps % DPS, s1 = (2 * steps) % SW_SLOTS, s2 = (2 * steps + 1) % SW_SLOTS;
+            const uint32_t buf = steps % DPS, s1 = tiles % SW_SLOTS, s2 = (tiles + 1) % SW_SLOTS;
             auto add = [&](uint32_t to, uint32_t factor, uint32_t slot) {       // factor: 8 words a K step, two steps of each 32 columns
                 const uint64_t m = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024);
 #pragma unroll
@@ -768,38 +794,86 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             }
             __syncwarp();
             ++steps;
+            tiles += 2 + (flags & SB_LAST ? OUTS : 0);
         }
+    } else if (warp == SB_WORKERS + 3) {
+        // ================= stores =================
+        uint32_t descs = 0, tiles = 0, items = 0;
+        bool ok = true;
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 456);
+            if (!ok) break;
+            const int item = bar->desc[d].item, flags = bar->desc[d].flags;
+            if (!(flags & (SB_EMPTY | SB_END))) tiles += 2;
+            if (flags & (SB_LAST | SB_EMPTY)) {
+                ok = wait(&bar->staged[items % SB_DESCS], (items / SB_DESCS) & 1u, 457);
+                if (!ok) break;
+                if (lane == 0) {
+                    const int tile = item % p.owned, head = item / p.owned, b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
+#pragma unroll
+                    for (int g = 0; g < OUTS; ++g)      // (rows behind the last one are clipped by the map)
+                        tma_store_5d(g + 1 < OUTS ? &tm_d1 : &tm_d2, g_s + (tiles + g) % SW_SLOTS * TILE_BYTES, 0, tile * TILE, 0, h, b);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+#pragma unroll
+                    for (int g = 0; g < OUTS; ++g) mbar_arrive(&bar->empty[(tiles + g) % SW_SLOTS]);
+                }
+                __syncwarp();
+                tiles += OUTS;
+                ++items;
+            }
+            // only now: a ring of descriptions is then also a bound on the items that are staged and not yet stored
+            warp_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // all stores have landed before the block exits
+        __syncwarp();
     } else {
         // ================= P, dS and the finished sums =================
         // a thread has one owned row (tensor-memory lane) and 32 met ones (columns)
         const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t at = (((uint32_t)(quarter * 32)) << 16) + part * 32;
-        uint32_t descs = 0, steps = 0, items = 0;
+        uint32_t descs = 0, steps = 0, items = 0, tiles = 0, done = 0;      // done: items with and without steps
         bool ok = true;
         float2 norm = make_float2(0.f, 0.f), delta = norm;        // queries: of the row
         const float2 c = make_float2(p.scale_log2, p.scale_log2);
-        auto place = [&](int item, int &b, int &h, int &token) {
-            const int heads = KEYS ? p.Hkv : p.H, head = item / p.owned;
-            b = head / heads;
-            h = head - b * heads;
-            token = (item - head * p.owned) * TILE + row;
-        };
-        // 32 channels of the row
-        auto put = [&](int item, const uint32_t (&v)[32], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
-            int b, h, token;
-            place(item, b, h, token);
-            if (token >= (KEYS ? p.Lkv : p.Lq)) return;
-            uint4 *out = reinterpret_cast<uint4 *>(to + b * sb + (long long)token * sl + h * sh + part * 32);
+        // an item's sums (or zeros) to the slots that it was given: [half of the channels][row][64 channels], pieces of 16 bytes swizzled by row
+        auto finish = [&](bool some) {
+#pragma unroll 1
+            for (int g = 0; g < OUTS; ++g, ++tiles) {
+                const bool last = g + 1 == OUTS;
+                const uint32_t slot = tiles % SW_SLOTS;
+                uint32_t v[32];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]) * scale, __uint_as_float(v[8 * q + 2 * e + 1]) * scale);
-                    w[e] = *reinterpret_cast<const uint32_t *>(&x);
+                for (int j = 0; j < 32; ++j) v[j] = 0u;
+                if (some) {
+                    TMEM_LD32((last ? tm_sum2 : tm_sum1) + at, v);
+                    tmem_wait_ld32(v);
+                    if (last) {
+                        tc_fence_before();
+                        warp_arrive(&bar->acc_empty);
+                    }
                 }
-                out[q] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (!wait(&bar->full[slot], (tiles / SW_SLOTS) & 1u, 466)) return false;
+                const float scale = last ? p.scale : 1.0f;
+                uint8_t *to = g_s + slot * TILE_BYTES + (part >> 1) * HALF_BYTES + row * 128;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v[8 * q + 2 * e]) * scale, __uint_as_float(v[8 * q + 2 * e + 1]) * scale);
+                        w[e] = *reinterpret_cast<const uint32_t *>(&x);
+                    }
+                    *reinterpret_cast<uint4 *>(to + ((((part & 1) * 4 + q) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            warp_arrive(&bar->staged[done % SB_DESCS]);
+            ++done;
+            return true;
         };
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -809,21 +883,17 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             warp_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
-            uint32_t v[32];
             if (flags & SB_EMPTY) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0u;
-                if (KEYS) put(item, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
-                put(item, v, p.d2, p.d2b, p.d2l, p.d2h, 1.0f);
+                ok = finish(false);
                 continue;
             }
             if (!KEYS && (flags & SB_FIRST)) {
-                int b, h, token;
-                place(item, b, h, token);
-                const float *st = p.stats + ((long long)b * p.H + h) * p.padded * 2 + selected_stat(token);
+                const int head = item / p.owned;
+                const float *st = p.stats + (long long)head * p.padded * 2 + selected_stat((item - head * p.owned) * TILE + row);
                 norm = make_float2(st[0], st[0]);
-                delta = make_float2(-st[64], -st[64]);
+                delta = make_float2(st[64], st[64]);
             }
+            uint32_t v[32];
             const uint32_t s2 = steps & 1u, buf = steps % DPS;
             const float *st = bar->stats[s2] + (part >> 1) * TILE + (part & 1) * 32;       // keys: of the 32 met rows
             if (KEYS) ok = wait(&bar->stats_full[s2], (steps >> 1) & 1u, 462);
@@ -879,7 +949,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float2 x = make_float2(__uint_as_float(v[2 * (j + e)]), __uint_as_float(v[2 * (j + e) + 1]));
-                    const float2 dl = KEYS ? (e == 0 ? make_float2(-d4.x, -d4.y) : make_float2(-d4.z, -d4.w)) : delta;
+                    const float2 dl = KEYS ? (e == 0 ? make_float2(d4.x, d4.y) : make_float2(d4.z, d4.w)) : delta;
                     pr[j + e] = __fmul2_rn(pr[j + e], __fadd2_rn(x, dl));
                 }
             }
@@ -890,21 +960,13 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (KEYS) warp_arrive(&bar->stats_empty[s2]);
             warp_arrive(&bar->ds_full[buf]);
             ++steps;
+            tiles += 2;
             if (flags & SB_LAST) {
                 ok = wait(&bar->acc_full, items & 1u, 465);
                 ++items;
                 if (!ok) break;
                 tc_fence_after();
-                if (KEYS) {
-                    TMEM_LD32(tm_sum1 + at, v);
-                    tmem_wait_ld32(v);
-                    put(item, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
-                }
-                TMEM_LD32(tm_sum2 + at, v);
-                tmem_wait_ld32(v);
-                tc_fence_before();
-                warp_arrive(&bar->acc_empty);
-                put(item, v, p.d2, p.d2b, p.d2l, p.d2h, p.scale);
+                ok = finish(true);
             }
         }
         tc_fence_before();
@@ -930,10 +992,11 @@ static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t s
     if ((rc = selected_sm100_map(&maps[1], &f2, p->B, Lf, Hf, "the owned rows", OWN, 2))) return rc;
     if ((rc = selected_sm100_map(&maps[2], &g1, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
     if ((rc = selected_sm100_map(&maps[3], &g2, p->B, Lg, Hg, "the met rows", BLK, BLK == TILE ? 2 : 1))) return rc;
-    const auto kernel = BLK == TILE ? selected_grad_wide_kernel<KEYS> : selected_grad_sm100_kernel<KEYS>;
     static PerDeviceOnce attr_set;
     if (!attr_set.done()) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        cudaError_t e;
+        if constexpr (BLK == TILE) e = cudaFuncSetAttribute(selected_grad_wide_kernel<KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        else e = cudaFuncSetAttribute(selected_grad_sm100_kernel<KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
@@ -944,7 +1007,16 @@ static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t s
     kp.d2 = (__nv_bfloat16 *)d2.ptr; kp.d2b = d2.stride_b; kp.d2l = d2.stride_l; kp.d2h = d2.stride_h;
     kp.work_counter += KEYS ? 0 : 1;
     const int sms = sm_count();
-    const cudaError_t e = launch_dependent(kernel, dim3(kp.items < sms ? kp.items : sms), dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
+    const dim3 grid(kp.items < sms ? kp.items : sms);
+    cudaError_t e;
+    if constexpr (BLK == TILE) {
+        CUtensorMap outs[2];
+        if ((rc = selected_sm100_map(&outs[0], KEYS ? &p->dv : &p->dq, p->B, Lf, Hf, "a gradient", TILE, 2))) return rc;
+        if ((rc = selected_sm100_map(&outs[1], KEYS ? &p->dk : &p->dq, p->B, Lf, Hf, "a gradient", TILE, 2))) return rc;
+        e = launch_dependent(selected_grad_wide_kernel<KEYS>, grid, dim3(SW_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], outs[0], outs[1], kp);
+    } else {
+        e = launch_dependent(selected_grad_sm100_kernel<KEYS>, grid, dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
+    }
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
