@@ -175,3 +175,26 @@ def test_streams_graphs_gradients_and_refusals():
         with pytest.raises(ValueError, match=word):
             bad()
     assert _same(c, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("frame,block,window,dropped", [(130, 64, 7, 3), (130, 64, 6, 3), (390, 128, 21, 3), (65, 64, 5, 1), (40, 64, 4, 2), (64, 64, 3, 2), (130, 128, 5, 4)])
+def test_the_window_rolls_as_through_clones(frame, block, window, dropped):
+    from worldattention_b200.causal_dit import roll_window
+    from worldattention_b200.hsa import HSAAttention
+    hsa = HSAAttention(2, 128, block_size=block, proj_segment_len=frame)
+    for size in (window * frame, window * frame - frame // 3):          # a whole window, and one whose last frame is cut short: refused
+        coarse = hsa.coarse_cache_size(window * frame)
+        cache = {n: _filled((1, rows, 2, 128), torch.bfloat16, i) for i, (n, rows) in enumerate((("k", window * frame), ("v", window * frame), ("k_coarse", coarse), ("v_coarse", coarse)))}
+        evict, keep = dropped * frame, size - dropped * frame
+        want = {n: t.clone() for n, t in cache.items()}
+        if size % frame:
+            with pytest.raises(ValueError, match="segment-aligned"):
+                roll_window(cache, hsa, evict, keep)
+        else:
+            c0, c1 = hsa.token_range_to_coarse(evict, evict + keep)
+            for name, a, n in (("k", evict, keep), ("v", evict, keep), ("k_coarse", c0, c1 - c0), ("v_coarse", c0, c1 - c0)):
+                want[name][:, :n] = cache[name][:, a:a + n].clone()
+            roll_window(cache, hsa, evict, keep)
+        for n in cache:
+            assert _same(cache[n], want[n]), n

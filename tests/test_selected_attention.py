@@ -327,6 +327,34 @@ def test_a_layer_of_operators_trains():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [16, 128])
+def test_block_sparse_attention_carries_gradients(dtype, D):
+    """The reference's names and layout (`[B, H, N, D]`, padded blocks), from a map and from lists; the values are those without gradients."""
+    from worldattention_b200.hsa import block_sparse_attention_reference
+    from worldattention_b200.hsa.block_sparse_triton import block_sparse_attention, map_to_index
+    g = torch.Generator(device=dev()).manual_seed(D)
+    B, H, nq, nk, block = 2, 3, 2, 4, 64
+    q, k, v, dout = (x.transpose(1, 2).contiguous() for x in _inputs(g, B, nq * block, nk * block, H, H, D, dtype))
+    sizes = torch.tensor([64, 64, 64, 10], dtype=torch.int32, device=dev())
+    block_map = torch.rand(B, H, nq, nk, generator=g, device=dev()) < 0.5
+    block_map[0, 1, 1] = False
+    index, num = map_to_index(block_map)
+    with torch.no_grad():
+        want = block_sparse_attention(q, k, v, block_sizes=sizes, block_map=block_map)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = block_sparse_attention(*leaves, block_sizes=sizes, block_map=block_map)
+    assert torch.equal(out.detach(), want) and out.requires_grad
+    grads = torch.autograd.grad(out, leaves, dout)
+    t = lambda x: x.transpose(1, 2)  # noqa: E731
+    exact = _exact(t(q), t(k), t(v), _mask(index, num, block, nq * block, nk * block, sizes), t(dout))
+    _check({n: t(x) for n, x in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads))}, {n: e for n, e in exact.items() if n != "lse"})
+    out, lse = block_sparse_attention_reference(leaves[0], k, v, index.long(), num.long(), sizes.long(), block, return_lse=True)
+    assert torch.equal(out.detach(), want) and torch.equal(torch.autograd.grad(out, leaves[0], dout)[0], grads[0]) and lse.shape == (B, H, nq * block)
+    assert not block_sparse_attention_reference(q, k, v, index, num, sizes, block).requires_grad
+
+
+@pytest.mark.gpu
 def test_refusals():
     from worldattention_b200.hsa import selected_attention
     g = torch.Generator(device=dev()).manual_seed(10)

@@ -32,6 +32,7 @@ import torch.nn.functional as F
 
 from . import _lib, rope
 from .hkv.cache import HKVCache
+from .hkv.pages import move_pages
 from .hkv.retrieval import query_index
 from .hkv.rope import temporal_band
 from .hsa.attention import HSAAttention
@@ -116,6 +117,15 @@ class _LayerNorm(nn.LayerNorm):   # model.py:89-103: float32 statistics, no affi
         return F.layer_norm(x.float(), self.normalized_shape, w, b, self.eps).type_as(x)
 
 
+def roll_window(cache: dict, hsa: HSAAttention, evict: int, keep: int) -> None:
+    """Drop the oldest `evict` tokens of a full window (causal_model.py:331-360): the `keep` tokens behind them and their compressed
+    slots move to the front, in place.  A page is what is dropped, and every page takes the next one's place; the last may be shorter."""
+    c0, c1 = hsa.token_range_to_coarse(evict, evict + keep)      # (whole segments, so that there are as many pages of slots as of tokens)
+    tensors = [cache["k"][:, :evict + keep], cache["v"][:, :evict + keep], cache["k_coarse"][:, :c1], cache["v_coarse"][:, :c1]]
+    n = -(-(evict + keep) // evict)
+    move_pages(tensors, range(n - 1), range(1, n), (evict, evict, c0, c0))
+
+
 class _SelfAttention(nn.Module):
     """causal_model.py:65-111, 143-543, KV-cache branch, HSA backend, no sink tokens."""
 
@@ -136,12 +146,7 @@ class _SelfAttention(nn.Module):
         v = self.v(x).view(b, s, cfg.heads, cfg.head_dim)
         hsa = self.hsa_attention
         if plan["roll"]:
-            # the window is full: drop the oldest frames (causal_model.py:331-360).  Source and destination overlap,
-            # so each tensor goes through one scratch copy of the kept rows.
-            ev, keep = plan["evict"], plan["keep"]
-            c0, c1 = hsa.token_range_to_coarse(ev, ev + keep)
-            for name, a, n in (("k", ev, keep), ("v", ev, keep), ("k_coarse", c0, c1 - c0), ("v_coarse", c0, c1 - c0)):
-                cache[name][:, :n] = cache[name][:, a:a + n].clone()
+            roll_window(cache, hsa, plan["evict"], plan["keep"])
         hsa.append_kv(k, v, cache["k"], cache["v"], cache["k_coarse"], cache["v_coarse"], position=plan["write"])
         end = plan["write"] + s
         c_end = hsa.token_range_to_coarse(0, end)[1]

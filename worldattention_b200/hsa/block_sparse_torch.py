@@ -10,13 +10,17 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from .selected import selected_attention
 
 __all__ = ["block_sparse_attention_reference"]
 
 
 def block_sparse_attention_reference(q, k, v, q2k_index, q2k_num, block_sizes, block_size: int,
                                      return_lse: bool = False):
-    """Attention over selected blocks for `[B, H, N, D]` inputs padded to `block_size`."""
+    """Attention over selected blocks for `[B, H, N, D]` inputs padded to `block_size`.
+
+    With gradients enabled and asked for, the result carries them to q, k and v (`selected_attention`: lists are then taken as
+    sets, an id named twice counts once and one that is no key block not at all; there are no gradients above head_dim 256)."""
     dev = _lib.require_cuda(q, k, v, q2k_index, q2k_num, block_sizes)
     bsz, heads, q_tokens, head_dim = q.shape
     kv_tokens = k.shape[2]
@@ -24,6 +28,11 @@ def block_sparse_attention_reference(q, k, v, q2k_index, q2k_num, block_sizes, b
         raise ValueError("q and k/v must be padded to a multiple of block_size")
     k = k.to(q.dtype)
     v = v.to(q.dtype)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = selected_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), q2k_index.to(torch.int32), q2k_num.to(torch.int32),
+                                      block_size, block_sizes=block_sizes.to(torch.int32), return_lse=True)
+        out = out.transpose(1, 2)
+        return (out, lse) if return_lse else out
     out = torch.empty((bsz, heads, q_tokens, head_dim), device=dev, dtype=q.dtype)
     lse = torch.empty((bsz, heads, q_tokens), device=dev, dtype=torch.float32) if return_lse else None
     index = q2k_index.to(torch.int32).contiguous()

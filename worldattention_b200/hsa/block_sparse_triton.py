@@ -1,9 +1,10 @@
-"""Inference entry points of the reference's Triton backend, served by the CUDA library.
+"""Entry points of the reference's Triton backend, served by the CUDA library.
 
 `block_sparse_attention(q, k, v, *, block_sizes, q2k_index, q2k_num, block_map)` and
 `map_to_index(block_map)` keep the signatures of wan/modules/hsa/block_sparse_triton.py:44-57,
 371-382.  No Triton is involved: the module name is kept only so that code importing the
-reference's backend module keeps working.  Forward only (the backward kernels are training code).
+reference's backend module keeps working.  Gradients reach q, k and v where they are asked for
+(block_sparse_triton.py:142-382), through `selected_attention`.
 """
 from __future__ import annotations
 
