@@ -11,6 +11,9 @@
 #include <ATen/core/CachingHostAllocator.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -52,7 +55,12 @@ volatile int *status_words[MAX_DEVICES] = {nullptr};
 struct PyFailure {};   // a Python exception is set
 
 [[noreturn]] void fail(PyObject *type, const std::string &msg) {
-    PyErr_SetString(type, msg.c_str());
+    if (PyGILState_Check()) {
+        PyErr_SetString(type, msg.c_str());
+    } else {                                // a thread of the autograd engine (its Python thread state outlives this scope)
+        pybind11::gil_scoped_acquire gil;
+        PyErr_SetString(type, msg.c_str());
+    }
     throw PyFailure();
 }
 
@@ -520,13 +528,9 @@ struct SelectedCall {
     c10::Device dev{c10::kCUDA, 0};
     bool nothing = false;              // no query or no key: no launch
 
-    explicit SelectedCall(PyObject *const *a) {
+    SelectedCall(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes) {
         bool seen = false;
-        const char *names[] = {"q", "k", "v", "index", "num"};
-        for (int i = 0; i < 5; ++i) require_cuda(tensor(a[i], names[i]), dev, seen);
-        const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &v = THPVariable_Unpack(a[2]);
-        const Tensor &index = THPVariable_Unpack(a[3]), &num = THPVariable_Unpack(a[4]);
-        const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
+        for (const Tensor *t : {&q, &k, &v, &index, &num}) require_cuda(*t, dev, seen);
         if (sizes) require_cuda(*sizes, dev, seen);
         if (q.dim() != 4 || k.dim() != 4 || v.dim() != 4) fail(PyExc_ValueError, "q, k and v must be [B, L, H, D] tensors");
         const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), D = q.size(3), Lkv = k.size(1), Hkv = k.size(2);
@@ -537,7 +541,6 @@ struct SelectedCall {
         if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) fail(PyExc_ValueError, "q, k and v must have one dtype");
         dtype_code(q.scalar_type());
         if (H == 0 || Hkv == 0 || H % Hkv) fail(PyExc_ValueError, std::to_string(H) + " query heads do not divide among " + std::to_string(Hkv) + " key heads");
-        const int block = small_integer(a[5], "block_size");
         if (block <= 0) fail(PyExc_ValueError, "block_size must be positive, got " + std::to_string(block));
         const int64_t nq = (Lq + block - 1) / block, nkv = (Lkv + block - 1) / block;
         if (index.dim() != 4 || index.size(0) != B || index.size(1) != H || index.size(2) != nq || num.dim() != 3 || num.size(0) != B || num.size(1) != H || num.size(2) != nq)
@@ -571,25 +574,106 @@ struct SelectedCall {
 };
 wa_tensor4 result4(const Tensor &t) { return wa_tensor4{t.data_ptr(), dtype_code(t.scalar_type()), 0, t.stride(0), t.stride(1), t.stride(2)}; }
 
-// -> (out [B, Lq, H, D], lse float32 [B, H, Lq])
-PyObject *selected_forward(PyObject *const *a, Py_ssize_t n) {
-    expect_args(n, 7);
-    SelectedCall c(a);
+// -> out [B, Lq, H, D], lse float32 [B, H, Lq]
+std::pair<Tensor, Tensor> selected_run(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes) {
+    SelectedCall c(q, k, v, index, num, block, sizes);
     raise_if_failed(c.dev.index());
     c10::cuda::CUDAGuard guard(c.dev);
-    const Tensor &q = THPVariable_Unpack(a[0]);
     const auto options = q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+    if (c.nothing)
+        return {at::zeros(q.sizes(), q.options().requires_grad(false)), at::full({c.p.B, c.p.H, c.p.Lq}, -INFINITY, q.options().dtype(at::kFloat).requires_grad(false))};
+    Tensor out = at::empty(q.sizes(), options), lse = at::empty({c.p.B, c.p.H, c.p.Lq}, options.dtype(at::kFloat));
+    c.p.out = result4(out);
+    c.p.lse = lse.data_ptr<float>();
+    const Tensor ws = c.workspace_for(false);
+    check(f_selected_forward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+    return {out, lse};
+}
+
+// -> dq, dk, dv
+std::vector<Tensor> selected_gradients(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes,
+                                       const Tensor &out, const Tensor &lse, const Tensor &dout) {
+    SelectedCall c(q, k, v, index, num, block, sizes);
+    raise_if_failed(c.dev.index());
+    bool seen = true;
+    for (const Tensor *t : {&out, &lse, &dout}) require_cuda(*t, c.dev, seen);
+    c10::cuda::CUDAGuard guard(c.dev);
+    if (out.sizes() != q.sizes() || dout.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || dout.scalar_type() != q.scalar_type())
+        fail(PyExc_ValueError, "out and dout must have q's shape and dtype");
+    std::vector<Tensor> grad(3);
+    for (int i = 0; i < 3; ++i) {
+        const Tensor &x = i == 0 ? q : k;
+        const auto options = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+        grad[i] = c.nothing ? at::zeros(x.sizes(), x.options().requires_grad(false)) : at::empty(x.sizes(), options);
+    }
+    if (c.nothing) return grad;
+    if (lse.scalar_type() != at::kFloat || lse.numel() != (int64_t)c.p.B * c.p.H * c.p.Lq) fail(PyExc_ValueError, "lse must be float32 [B, H, Lq]");
+    // (a gradient without memory of its own, or of odd strides, is laid out: the tensor-core kernels read 16 bytes at a time)
+    const bool odd = dout.scalar_type() == at::kBFloat16 && (dout.stride(0) % 8 || dout.stride(1) % 8 || dout.stride(2) % 8 || dout.stride(1) <= 0 || dout.stride(2) <= 0);
+    const Tensor laid = odd ? dout.contiguous() : dout;
+    c.p.out = view4(out, c.keep[6]);
+    c.p.dout = view4(laid, c.keep[7]);
+    c.keep[8] = lse.contiguous();
+    c.p.lse = c.keep[8].data_ptr<float>();
+    c.p.dq = result4(grad[0]); c.p.dk = result4(grad[1]); c.p.dv = result4(grad[2]);
+    const Tensor ws = c.workspace_for(true);
+    check(f_selected_backward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+    return grad;
+}
+
+// Autograd nodes live here because a Python one costs a step 60 us: its backward takes the interpreter lock on the engine's thread.
+[[noreturn]] void rethrow_on_engine() {       // what `fail` left on this thread, as an exception that the engine carries to the caller
+    pybind11::gil_scoped_acquire gil;
+    python_error e;
+    e.persist();
+    throw std::move(e);
+}
+
+struct SelectedNode : torch::autograd::Function<SelectedNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index,
+                                                  const Tensor &num, int64_t block, const std::optional<Tensor> &sizes) {
+        auto [out, lse] = selected_run(q, k, v, index, num, (int)block, sizes ? &*sizes : nullptr);
+        ctx->save_for_backward({q, k, v, index, num, sizes ? *sizes : Tensor(), out, lse});
+        ctx->saved_data["block"] = block;
+        ctx->mark_non_differentiable({lse});
+        ctx->set_materialize_grads(false);
+        return {out, lse};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        torch::autograd::variable_list result(7);
+        if (!grads[0].defined()) return result;
+        const auto s = ctx->get_saved_variables();
+        torch::autograd::variable_list three;
+        try {
+            at::NoGradGuard no_grad;
+            three = selected_gradients(s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["block"].toInt(), s[5].defined() ? &s[5] : nullptr, s[6], s[7], grads[0].detach());
+        } catch (const PyFailure &) {
+            rethrow_on_engine();
+        }
+        if (at::GradMode::is_enabled()) {     // (create_graph: these gradients have no gradient)
+            for (Tensor &t : three) t.requires_grad_();
+            const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 3);
+            three = (*error)(std::move(three));
+        }
+        for (int i = 0; i < 3; ++i)
+            if (ctx->needs_input_grad(i)) result[i] = three[i];
+        return result;
+    }
+};
+
+// q, k, v, index, num, block, block_sizes|None -> (out, lse), with a graph where gradients are asked for
+PyObject *selected_attention(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 7);
+    const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &index = tensor(a[3], "index"), &num = tensor(a[4], "num");
+    const int block = small_integer(a[5], "block_size");
+    const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
     Tensor out, lse;
-    if (c.nothing) {
-        out = at::zeros(q.sizes(), q.options().requires_grad(false));
-        lse = at::full({c.p.B, c.p.H, c.p.Lq}, -INFINITY, q.options().dtype(at::kFloat).requires_grad(false));
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+        auto both = SelectedNode::apply(q, k, v, index, num, (int64_t)block, sizes ? std::optional<Tensor>(*sizes) : std::nullopt);
+        out = std::move(both[0]);
+        lse = std::move(both[1]);
     } else {
-        out = at::empty(q.sizes(), options);
-        lse = at::empty({c.p.B, c.p.H, c.p.Lq}, options.dtype(at::kFloat));
-        c.p.out = result4(out);
-        c.p.lse = lse.data_ptr<float>();
-        const Tensor ws = c.workspace_for(false);
-        check(f_selected_forward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+        std::tie(out, lse) = selected_run(q, k, v, index, num, block, sizes);
     }
     PyObject *pair = PyTuple_New(2);
     if (!pair) throw PyFailure();
@@ -598,64 +682,23 @@ PyObject *selected_forward(PyObject *const *a, Py_ssize_t n) {
     return pair;
 }
 
-// ..., out, lse, dout -> (dq, dk, dv)
-PyObject *selected_backward(PyObject *const *a, Py_ssize_t n) {
-    expect_args(n, 10);
-    SelectedCall c(a);
-    raise_if_failed(c.dev.index());
-    bool seen = true;
-    const char *names[] = {"out", "lse", "dout"};
-    for (int i = 0; i < 3; ++i) require_cuda(tensor(a[7 + i], names[i]), c.dev, seen);
-    c10::cuda::CUDAGuard guard(c.dev);
-    const Tensor &q = THPVariable_Unpack(a[0]), &k = THPVariable_Unpack(a[1]), &out = THPVariable_Unpack(a[7]), &dout = THPVariable_Unpack(a[9]);
-    if (out.sizes() != q.sizes() || dout.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || dout.scalar_type() != q.scalar_type())
-        fail(PyExc_ValueError, "out and dout must have q's shape and dtype");
-    Tensor grad[3], laid;
-    for (int i = 0; i < 3; ++i) {
-        const Tensor &x = i == 0 ? q : k;
-        const auto options = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
-        grad[i] = c.nothing ? at::zeros(x.sizes(), x.options().requires_grad(false)) : at::empty(x.sizes(), options);
-    }
-    if (!c.nothing) {
-        c.p.out = view4(out, c.keep[6]);
-        // (a gradient without memory of its own, or of odd strides, is laid out: the tensor-core kernels read 16 bytes at a time)
-        const bool odd = dout.scalar_type() == at::kBFloat16 && (dout.stride(0) % 8 || dout.stride(1) % 8 || dout.stride(2) % 8 || dout.stride(1) <= 0 || dout.stride(2) <= 0);
-        if (odd) laid = dout.contiguous();
-        c.p.dout = view4(odd ? laid : dout, c.keep[7]);
-        c.keep[8] = THPVariable_Unpack(a[8]).contiguous();
-        if (c.keep[8].scalar_type() != at::kFloat || c.keep[8].numel() != (int64_t)c.p.B * c.p.H * c.p.Lq) fail(PyExc_ValueError, "lse must be float32 [B, H, Lq]");
-        c.p.lse = c.keep[8].data_ptr<float>();
-        c.p.dq = result4(grad[0]); c.p.dk = result4(grad[1]); c.p.dv = result4(grad[2]);
-        const Tensor ws = c.workspace_for(true);
-        check(f_selected_backward(&c.p, at::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
-    }
-    PyObject *three = PyTuple_New(3);
-    if (!three) throw PyFailure();
-    for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(three, i, THPVariable_Wrap(std::move(grad[i])));
-    return three;
-}
-
-// ---- axial_rope(tensors, positions int32 [L, A] or [B, L, A], table float32 [rows, pairs, 2], pairs of each axis, interleaved, inverse) -> list of tensors ----
-PyObject *axial_rope(PyObject *const *a, Py_ssize_t n) {
-    expect_args(n, 6);
-    const Sequence xs(a[0], "expected a tensor or a tuple of tensors"), axes(a[3], "axes must be a sequence of integers");
-    const Tensor &pos0 = tensor(a[1], "positions"), &table0 = tensor(a[2], "table");
-    constexpr int MOST = 4;
+// ---- axial_rope(tensors, positions int32 [L, A] or [B, L, A], table float32 [rows, pairs, 2], pairs of each axis, interleaved) -> list of tensors ----
+std::vector<Tensor> axial_run(at::TensorList xs, const Tensor &pos0, const Tensor &table0, const std::vector<int64_t> &axes, bool interleaved, bool inverse) {
+    constexpr size_t MOST = 4;
     if (xs.size() < 1 || xs.size() > MOST) fail(PyExc_ValueError, "expected one to four tensors, got " + std::to_string(xs.size()));
     c10::Device dev(c10::kCUDA, 0);
     bool seen = false;
-    for (Py_ssize_t t = 0; t < xs.size(); ++t) require_cuda(tensor(xs[t], "every element"), dev, seen);
+    for (const Tensor &x : xs) require_cuda(x, dev, seen);
     require_cuda(pos0, dev, seen);
     require_cuda(table0, dev, seen);
-    const Tensor &x0 = THPVariable_Unpack(xs[0]);
+    const Tensor &x0 = xs[0];
     if (x0.dim() != 4) fail(PyExc_ValueError, "expected [B, L, H, D] tensors, got shape " + shape_of(x0));
-    const int64_t B = x0.size(0), L = x0.size(1), D = x0.size(3);
+    const int64_t B = x0.size(0), L = x0.size(1), D = x0.size(3), A = (int64_t)axes.size();
     if (B > INT_MAX || L > INT_MAX || D > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
-    const int64_t A = axes.size();
     int pairs[8];
     if (A < 1 || A > 8) fail(PyExc_ValueError, "expected one to eight axes, got " + std::to_string(A));
     int64_t sum = 0;
-    for (int64_t i = 0; i < A; ++i) sum += pairs[i] = small_integer(axes[i], "axes");
+    for (int64_t i = 0; i < A; ++i) sum += pairs[i] = (int)axes[i];
     if (table0.dim() != 3 || table0.size(2) != 2 || table0.size(0) < 1 || table0.scalar_type() != at::kFloat)
         fail(PyExc_ValueError, "table must be float32 [rows, pairs, 2], got shape " + shape_of(table0));
     if (table0.size(1) != sum || 2 * sum > D)
@@ -668,22 +711,73 @@ PyObject *axial_rope(PyObject *const *a, Py_ssize_t n) {
     const Tensor pos = pos0.stride(-1) == 1 || A == 1 ? pos0 : pos0.contiguous(), table = table0.contiguous();
     wa_tensor4 in[MOST], out[MOST];
     int32_t heads[MOST];
-    Tensor keep[MOST], result[MOST];
-    for (Py_ssize_t t = 0; t < xs.size(); ++t) {
-        const Tensor &x = THPVariable_Unpack(xs[t]);
+    Tensor keep[MOST];
+    std::vector<Tensor> result(xs.size());
+    for (size_t t = 0; t < xs.size(); ++t) {
+        const Tensor &x = xs[t];
         if (x.dim() != 4 || x.size(0) != B || x.size(1) != L || x.size(3) != D || x.scalar_type() != x0.scalar_type())
             fail(PyExc_ValueError, "the tensors must share batch, length, head_dim and dtype, got shapes " + shape_of(x0) + " and " + shape_of(x));
         if (x.size(2) > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
         in[t] = view4(x, keep[t]);
         result[t] = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-        out[t] = wa_tensor4{result[t].data_ptr(), in[t].dtype, 0, result[t].stride(0), result[t].stride(1), result[t].stride(2)};
+        out[t] = result4(result[t]);
         heads[t] = (int32_t)x.size(2);
     }
     check(f_axial(in, out, heads, (int)xs.size(), (int)B, (int)L, (int)D, pos.data_ptr<int32_t>(), shared ? 0 : pos.stride(0), pos.stride(-2), pairs, (int)A,
-                  table.data_ptr<float>(), (int)std::min<int64_t>(table.size(0), INT_MAX), a[4] == Py_True, a[5] == Py_True, stream));
-    PyObject *list = PyList_New(xs.size());
+                  table.data_ptr<float>(), (int)std::min<int64_t>(table.size(0), INT_MAX), interleaved, inverse, stream));
+    return result;
+}
+
+std::vector<Tensor> axial_turn(const std::vector<Tensor> &xs, const Tensor &pos, const Tensor &table, const std::vector<int64_t> &axes, bool interleaved, bool inverse);
+
+struct AxialNode : torch::autograd::Function<AxialNode> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &pos, const Tensor &table, std::vector<int64_t> axes,
+                                                  bool interleaved, bool inverse, at::TensorList xs) {
+        ctx->save_for_backward({pos, table});
+        ctx->saved_data["axes"] = axes;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["inverse"] = inverse;
+        ctx->set_materialize_grads(false);
+        return axial_run(xs, pos, table, axes, interleaved, inverse);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        const auto s = ctx->get_saved_variables();
+        torch::autograd::variable_list result(5 + grads.size());
+        std::vector<Tensor> there;
+        std::vector<size_t> at;
+        for (size_t i = 0; i < grads.size(); ++i)
+            if (grads[i].defined() && ctx->needs_input_grad(2 + i)) {      // (counts tensors: positions, table, then these)
+                there.push_back(grads[i]);
+                at.push_back(5 + i);
+            }
+        if (there.empty()) return result;
+        try {
+            const auto turned = axial_turn(there, s[0], s[1], ctx->saved_data["axes"].toIntVector(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool());
+            for (size_t i = 0; i < at.size(); ++i) result[at[i]] = turned[i];
+        } catch (const PyFailure &) {
+            rethrow_on_engine();
+        }
+        return result;
+    }
+};
+
+std::vector<Tensor> axial_turn(const std::vector<Tensor> &xs, const Tensor &pos, const Tensor &table, const std::vector<int64_t> &axes, bool interleaved, bool inverse) {
+    if (at::GradMode::is_enabled() && std::any_of(xs.begin(), xs.end(), [](const Tensor &x) { return x.requires_grad(); }))
+        return AxialNode::apply(pos, table, axes, interleaved, inverse, at::TensorList(xs));
+    return axial_run(xs, pos, table, axes, interleaved, inverse);
+}
+
+PyObject *axial_rope(PyObject *const *a, Py_ssize_t n) {
+    expect_args(n, 5);
+    const Sequence given(a[0], "expected a tensor or a tuple of tensors"), pairs(a[3], "axes must be a sequence of integers");
+    std::vector<Tensor> xs;
+    for (Py_ssize_t t = 0; t < given.size(); ++t) xs.push_back(tensor(given[t], "every element"));
+    std::vector<int64_t> axes;
+    for (Py_ssize_t i = 0; i < pairs.size(); ++i) axes.push_back(small_integer(pairs[i], "axes"));
+    std::vector<Tensor> result = axial_turn(xs, tensor(a[1], "positions"), tensor(a[2], "table"), axes, a[4] == Py_True, false);
+    PyObject *list = PyList_New((Py_ssize_t)result.size());
     if (!list) throw PyFailure();
-    for (Py_ssize_t t = 0; t < xs.size(); ++t) PyList_SET_ITEM(list, t, THPVariable_Wrap(std::move(result[t])));
+    for (size_t t = 0; t < result.size(); ++t) PyList_SET_ITEM(list, (Py_ssize_t)t, THPVariable_Wrap(std::move(result[t])));
     return list;
 }
 
@@ -840,6 +934,9 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
         return F(args, n);
     } catch (const PyFailure &) {
         return nullptr;
+    } catch (python_error &e) {
+        e.restore();
+        return nullptr;
     } catch (const c10::OutOfMemoryError &e) {
         PyErr_SetString(py_out_of_memory, e.what_without_backtrace());
         return nullptr;
@@ -854,7 +951,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 #define WA_ENTRY(name) {#name, (PyCFunction)(void (*)(void))entry<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {WA_ENTRY(bind), WA_ENTRY(hsa_forward), WA_ENTRY(run_forward), WA_ENTRY(qk_norm_rope), WA_ENTRY(append_kv), WA_ENTRY(ln_modulate),
-                         WA_ENTRY(gated_residual), WA_ENTRY(axial_rope), WA_ENTRY(selected_forward), WA_ENTRY(selected_backward), WA_ENTRY(move_pages), WA_ENTRY(tensor_table), WA_ENTRY(read_on_stream), {nullptr, nullptr, 0, nullptr}};
+                         WA_ENTRY(gated_residual), WA_ENTRY(axial_rope), WA_ENTRY(selected_attention), WA_ENTRY(move_pages), WA_ENTRY(tensor_table), WA_ENTRY(read_on_stream), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1164,6 +1164,7 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
 // ---- launch preparation as a kernel of its own (used when the routing kernel has not done it) --------
 __global__ void __launch_bounds__(1024)
 schedule_kernel(const int32_t *__restrict__ num, int rows, int Nkv, SchedJob job) {
+    pdl_wait();
     if (blockIdx.x > 0) {
         convert_gate_slice(job, (blockIdx.x - 1) * 1024, 1024);
         return;
@@ -1533,7 +1534,8 @@ int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, co
         attr_set.mark();
     }
     const int rows = p->B * p->H * Nq, q_items = pair ? (Nq + 1) / 2 : Nq, n_items = p->B * p->H * q_items;
-    schedule_kernel<<<1, 1024, 0, stream>>>(num, rows, Nkv, job);
+    const cudaError_t se = launch_dependent(schedule_kernel, dim3(1), dim3(1024), 0, stream, num, rows, Nkv, job);
+    if (se != cudaSuccess) return fail((int)se, "%s: %s", what, cudaGetErrorString(se));
     if ((rc = check_launch(what))) return rc;
     Params kp{};
     kp.both = (const int32_t *)(ws + w.both);

@@ -18,8 +18,10 @@ struct SelectedPlan {
 };
 
 // Statistics of the query rows, 64 rows together: 64 times minus the log-sum-exp in powers of two, then 64 times minus the sum of dout * out.  Rows that are no
-// query's (behind the last one, and a block more) have an infinite normaliser, which makes their probabilities zero.
-inline size_t selected_stats_rows(const wa_selected_params *p, int Nq) { return align_up((size_t)(Nq + 1) * p->block_size, 64); }
+// query's (behind the last one, and a block more for the tensor-core kernels' blocks) have an infinite normaliser, which makes their probabilities zero.
+inline size_t selected_stats_rows(const wa_selected_params *p, int Nq) {
+    return align_up(p->block_size <= 128 ? (size_t)(Nq + 1) * p->block_size : (size_t)p->Lq, 64);
+}
 __host__ __device__ inline long long selected_stat(long long row) { return (row >> 6) * 128 + (row & 63); }      // the sum lies 64 behind
 
 // bf16, head_dim 128, blocks of 64 or 128 tokens.  wa_hsa_sm100.cu:

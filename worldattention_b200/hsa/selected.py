@@ -13,26 +13,6 @@ from .. import _lib
 __all__ = ["selected_attention"]
 
 
-class _SelectedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, index, num, block_size, block_sizes):
-        out, lse = _lib.host().selected_forward(q, k, v, index, num, block_size, block_sizes)
-        ctx.save_for_backward(q, k, v, index, num, block_sizes, out, lse)
-        ctx.block_size = block_size
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
-        if dout is None:
-            return (None,) * 7
-        q, k, v, index, num, block_sizes, out, lse = ctx.saved_tensors
-        grads = _lib.host().selected_backward(q, k, v, index, num, ctx.block_size, block_sizes, out, lse, dout)
-        return tuple(g if needed else None for g, needed in zip(grads, ctx.needs_input_grad)) + (None,) * 4
-
-
 def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index: torch.Tensor, num: torch.Tensor, block_size: int, *,
                        block_sizes: torch.Tensor | None = None, return_lse: bool = False):
     """Softmax attention of each query block over the key blocks listed for it -> `[B, Lq, H, D]`; differentiable in q, k and v.
@@ -48,8 +28,5 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     probabilities and dS are rounded to bf16 where they are factors of a product.  Equal calls give equal bits, gradients included.  The
     gradient of the gradient is not offered.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _SelectedAttention.apply(q, k, v, index, num, block_size, block_sizes)
-    else:
-        out, lse = _lib.host().selected_forward(q, k, v, index, num, block_size, block_sizes)
+    out, lse = _lib.host().selected_attention(q, k, v, index, num, block_size, block_sizes)
     return (out, lse) if return_lse else out

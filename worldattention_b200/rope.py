@@ -60,29 +60,6 @@ def causal_rope_apply(x: torch.Tensor, grid_sizes, freqs: torch.Tensor, start_fr
     return qk_norm_rope(x, None, 0.0, grid_sizes, freqs, start_frame)
 
 
-class _AxialRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, positions, table, axes, interleaved, inverse, *xs):
-        ctx.save_for_backward(positions, table)
-        ctx.how = axes, interleaved, inverse
-        ctx.set_materialize_grads(False)
-        return tuple(_lib.host().axial_rope(xs, positions, table, axes, interleaved, inverse))
-
-    @staticmethod
-    def backward(ctx, *grads):
-        positions, table = ctx.saved_tensors
-        axes, interleaved, inverse = ctx.how
-        there = [g for g, needed in zip(grads, ctx.needs_input_grad[5:]) if g is not None and needed]
-        turned = iter(_turn(there, positions, table, axes, interleaved, not inverse) if there else ())
-        return (None,) * 5 + tuple(next(turned) if g is not None and needed else None for g, needed in zip(grads, ctx.needs_input_grad[5:]))
-
-
-def _turn(xs, positions, table, axes, interleaved, inverse):
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-        return _AxialRope.apply(positions, table, axes, interleaved, inverse, *xs)
-    return _lib.host().axial_rope(xs, positions, table, axes, interleaved, inverse)
-
-
 def axial_rope(x, positions: torch.Tensor, table: torch.Tensor, *, axes=None, interleaved: bool = True):
     """Rotary embedding of `[B, L, H, D]` tokens at positions of their own on several axes; differentiable in `x`.
 
@@ -111,5 +88,5 @@ def axial_rope(x, positions: torch.Tensor, table: torch.Tensor, *, axes=None, in
         if n not in (1, 3):
             raise ValueError(f"axes is needed for {n} axes: how many pairs does each of them turn?")
         axes = (pairs,) if n == 1 else (pairs - 2 * (pairs // 3), pairs // 3, pairs // 3)
-    out = _turn(xs, positions, table, tuple(axes), bool(interleaved), False)
+    out = _lib.host().axial_rope(xs, positions, table, axes, bool(interleaved))
     return out[0] if alone else tuple(out)
