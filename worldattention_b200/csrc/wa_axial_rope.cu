@@ -27,6 +27,7 @@ struct AxialRope {
     long long psb, psl;               // elements between samples (0: the same for all) and between tokens
     const float2 *table;              // [rows, pairs] (cos, sin)
     float sign;                       // of the angle
+    int wide;                         // two neighbouring pairs of a row are 16 bytes: an even number of pairs, an aligned table
     int groups, groups_of[AR_TENSORS];     // vector form: head groups of all tensors and of each
 };
 
@@ -58,13 +59,29 @@ __device__ __forceinline__ void ar_turns(const AxialRope &p, const int32_t *pos,
         const int r0 = __ldg(pos + a0), r1 = __ldg(pos + a1), border = p.end[a0];
         const bool in0 = (unsigned)r0 < (unsigned)p.rows, in1 = (unsigned)r1 < (unsigned)p.rows;
         const float2 *t0 = p.table + (long long)(in0 ? r0 : 0) * p.pairs + first, *t1 = p.table + (long long)(in1 ? r1 : 0) * p.pairs + first;
+        if (p.wide) {          // two pairs a load; the second of two may be another axis'
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool one = first + i < border;
-            turn[i] = make_float2(1.f, 0.f);
-            if (first + i <= last) turn[i] = __ldg((one ? t0 : t1) + i);
-            turn[i].y *= p.sign;
-            if (!(one ? in0 : in1) && first + i <= last) turn[i] = make_float2(NAN, NAN);
+            for (int i = 0; i < N; i += 2) {
+                const bool one = first + i < border, next = first + i + 1 < border;
+                float4 t = make_float4(1.f, 0.f, 1.f, 0.f);
+                if (first + i <= last) t = __ldg(reinterpret_cast<const float4 *>((one ? t0 : t1) + i));
+                if (one && !next) {
+                    const float2 u = __ldg(t1 + i + 1);
+                    t.z = u.x;
+                    t.w = u.y;
+                }
+                turn[i] = (one ? in0 : in1) ? make_float2(t.x, t.y * p.sign) : make_float2(NAN, NAN);
+                turn[i + 1] = (next ? in0 : in1) ? make_float2(t.z, t.w * p.sign) : make_float2(NAN, NAN);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool one = first + i < border;
+                turn[i] = make_float2(1.f, 0.f);
+                if (first + i <= last) turn[i] = __ldg((one ? t0 : t1) + i);
+                turn[i].y *= p.sign;
+                if (!(one ? in0 : in1) && first + i <= last) turn[i] = make_float2(NAN, NAN);
+            }
         }
     } else {
 #pragma unroll
@@ -217,6 +234,7 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
     }
     WA_REQUIRE(pairs > 0, WA_ERR_ARG, "%s: no axis has a pair", what);
     p.pairs = (int)pairs;
+    p.wide = pairs % 2 == 0 && (uintptr_t)table % 16 == 0;
     const int dtype = x[0].dtype;
     WA_REQUIRE(valid_dtype(dtype), WA_ERR_ARG, "%s: bad dtype %d", what, dtype);
     const int n = 16 / (int)dtype_size(dtype), unit = interleaved ? D : (int)pairs;      // channels of a vector; of what a head's lanes share

@@ -315,27 +315,24 @@ static int launch_few_rows(const wa_selected_params *p, cudaStream_t stream) {
 // four rows are on their way at a time.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
-selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, long long all, float *__restrict__ stats) {
+selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, unsigned all, float *__restrict__ stats) {
     constexpr int WIDE = LANES ? LANES : 32, AT_ONCE = LANES ? 4 : 1, N = 16 / sizeof(T), EACH = 256 / WIDE;
     pdl_wait();
-    const int sub = threadIdx.x / WIDE, lane = threadIdx.x % WIDE;
-    long long row[AT_ONCE];                       // (b, token, h), heads innermost as in memory
-    long long b[AT_ONCE];
+    const int sub = threadIdx.x / WIDE, lane = threadIdx.x % WIDE, b = blockIdx.y;
+    unsigned row[AT_ONCE];                        // (token, h) of the sample, heads innermost as in memory
     int h[AT_ONCE], l[AT_ONCE];
     float sum[AT_ONCE], natural[AT_ONCE];
     uint4 x[AT_ONCE], y[AT_ONCE];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-        row[u] = ((long long)blockIdx.x * AT_ONCE + u) * EACH + sub;
-        const long long token = row[u] / H;
-        h[u] = (int)(row[u] - token * H);
-        b[u] = token / padded;
-        l[u] = (int)(token - b[u] * padded);
+        row[u] = (blockIdx.x * AT_ONCE + u) * EACH + sub;
+        l[u] = (int)(row[u] / (unsigned)H);
+        h[u] = (int)(row[u] - (unsigned)l[u] * (unsigned)H);
         sum[u] = 0.f;
         if (row[u] >= all || l[u] >= Lq) continue;
-        natural[u] = __ldg(lse + (b[u] * H + h[u]) * Lq + l[u]);
-        const T *o = (const T *)out.ptr + b[u] * out.sb + (long long)l[u] * out.sl + (long long)h[u] * out.sh;
-        const T *g = (const T *)dout.ptr + b[u] * dout.sb + (long long)l[u] * dout.sl + (long long)h[u] * dout.sh;
+        natural[u] = __ldg(lse + ((long long)b * H + h[u]) * Lq + l[u]);
+        const T *o = (const T *)out.ptr + b * out.sb + (long long)l[u] * out.sl + (long long)h[u] * out.sh;
+        const T *g = (const T *)dout.ptr + b * dout.sb + (long long)l[u] * dout.sl + (long long)h[u] * dout.sh;
         if (LANES) {
             x[u] = __ldg(reinterpret_cast<const uint4 *>(o) + lane);
             y[u] = __ldg(reinterpret_cast<const uint4 *>(g) + lane);
@@ -356,7 +353,7 @@ selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int 
         if (lane == 0 && row[u] < all) {
             // a row behind the last one, or one that nothing is listed for: no key sees it
             const bool seen = there && natural[u] != -INFINITY;
-            float *to = stats + (b[u] * H + h[u]) * padded * 2 + selected_stat(l[u]);
+            float *to = stats + ((long long)b * H + h[u]) * padded * 2 + selected_stat(l[u]);
             to[0] = seen ? -1.4426950408889634f * natural[u] : -INFINITY;
             to[64] = seen ? -sum[u] : 0.f;
         }
@@ -371,10 +368,11 @@ static int launch_stats(const wa_selected_params *p, int padded, float *stats, c
         return (uintptr_t)t.ptr % 16 == 0 && t.stride_b % n == 0 && t.stride_l % n == 0 && t.stride_h % n == 0;
     };
     const int bytes = p->D * (int)sizeof(T), lanes = pieces(p->out) && pieces(p->dout) && (bytes == 512 || bytes == 256 || bytes == 128) ? bytes / 16 : 0;
-    const long long all = (long long)p->B * p->H * padded, each = lanes ? 4 * (256 / lanes) : 8, ctas = (all + each - 1) / each;
-    WA_REQUIRE(ctas < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+    const long long all = (long long)p->H * padded, each = lanes ? 4 * (256 / lanes) : 8;
+    WA_REQUIRE(all + 1024 < (1ll << 32), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
     const auto kernel = lanes == 32 ? selected_stats_kernel<T, 32> : lanes == 16 ? selected_stats_kernel<T, 16> : lanes == 8 ? selected_stats_kernel<T, 8> : selected_stats_kernel<T, 0>;
-    const cudaError_t e = launch_dependent(kernel, dim3((unsigned)ctas), dim3(256), 0, stream, make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq, p->D, padded, all, stats);
+    const cudaError_t e = launch_dependent(kernel, dim3((unsigned)((all + each - 1) / each), p->B), dim3(256), 0, stream, make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq,
+                                           p->D, padded, (unsigned)all, stats);
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
@@ -384,7 +382,8 @@ static int launch_stats(const wa_selected_params *p, int padded, float *stats, c
 // 128).  A warp has T / 8 of the owned rows to itself: its lanes take T / 32 met rows each for the scores and dP, P and dS go through
 // shared memory of the warp's own, and for the sums a lane has 4 channels of each 128.  So an owned row is one address for all lanes, a met row one for
 // each, both 16 bytes: 16 wavefronts of shared memory for 64 multiply-adds of a warp (scores), 24 for 128 (sums), below what the multiply-adds take.
-// (16 x 16 threads with 2 x 2 scores each were bound by shared memory: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64 a row: TIMES)
+// (16 x 16 threads with 2 x 2 scores each were bound by shared memory: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64 a row: dK/dV
+// 187 us and dQ 143, now 161 and 119, heaviest first 141 and 85)
 // The next rows to meet are on their way while some are at work: asynchronous copies of aligned float32 rows, plain loads of anything else.
 struct SelectedGrad {
     View4 q, k, v, dout;
@@ -619,11 +618,13 @@ static int launch_grad(SelectedGrad p, int B, int Hkv, cudaStream_t stream) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------
-// Heaviest first where there are more items than SMs but their tensors fit L2 side by side: the order over all heads mixes the heads, which larger calls
-// pay for with what the CTAs of one head would find in L2.  (Three frames of 390 tokens, 12 heads, float32: TIMES2; TIMES3)
+// Heaviest first where there are more items than SMs and their tensors about fit L2 side by side: the order over all heads mixes the heads, which larger
+// calls pay for with what the CTAs of one head would find in L2.  Both gradients with counts between zero and 32 blocks of 64 (16 of 128), 12 heads, bf16,
+// as they come -> ordered, its launch included: 1200 tokens 51.5 -> 46.2 us, 4680 170 -> 153 (133 -> 110), 9360 (115 MB) 301 -> 293 (224 -> 195), 18 720
+// 549 -> 584 (387 -> 374).  Float32: three frames of 390 tokens 282 -> 230, its forward 103 -> 77; 2900 tokens 1240 -> 971, 450 -> 354.
 static bool selected_ordered(const wa_selected_params *p, const SelectedPlan &w) {
     const long long bytes = 2ll * dtype_size(p->q.dtype) * p->B * p->D * ((long long)p->H * p->Lq + (long long)p->Hkv * p->Lkv);
-    return (long long)p->B * p->H * w.Nq > sm_count() && (long long)p->B * p->H * w.Nq <= (1 << 20) && (long long)p->B * p->Hkv * w.Nkv <= (1 << 20) && bytes <= 64ll << 20;
+    return (long long)p->B * p->H * w.Nq > sm_count() && (long long)p->B * p->H * w.Nq <= (1 << 20) && (long long)p->B * p->Hkv * w.Nkv <= (1 << 20) && bytes <= 128ll << 20;
 }
 
 static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
