@@ -247,6 +247,21 @@ def test_equal_calls_equal_bits_streams_and_graphs(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("block", [64, 128])
+@pytest.mark.parametrize("q_len,kv_len,S", [(128, 8192, 60), (1, 20000, 30), (256, 4000, 31), (4096, 256, 2), (2500, 130, 1)])
+def test_items_of_one_step_and_items_of_many(block, q_len, kv_len, S):
+    """Key blocks that one query block lists, or none, and query blocks with one: every hand-over between items, on repeated calls."""
+    g = torch.Generator(device=dev()).manual_seed(q_len + block)
+    q, k, v, dout = _inputs(g, 1, q_len, kv_len, 6, 3, 128, torch.bfloat16)
+    index, num = _lists(g, 1, 6, -(-q_len // block), -(-kv_len // block), S, "ragged")
+    first = _run(q, k, v, index, num, block, dout)
+    _check(first, _exact(q, k, v, _mask(index, num, block, q_len, kv_len), dout))
+    for _ in range(4):
+        again = _run(q, k, v, index, num, block, dout)
+        assert all(torch.equal(again[n], first[n]) for n in first)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     from worldattention_b200.hsa import selected_attention
     g = torch.Generator(device=dev()).manual_seed(7)

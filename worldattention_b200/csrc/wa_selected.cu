@@ -14,38 +14,49 @@ namespace wa {
 // atomically, which is the same in any order.
 constexpr int SL_WARPS = 8, SL_WORDS = 1024;   // lists of a CTA; words of a bitmap up to which it has so many (32 768 key blocks)
 
-__global__ void __launch_bounds__(SL_WARPS * 32)
-selected_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__ num, long long lists, int Nq, int Nkv, int stride, int H, int group,
-                      int words, int row_words, int32_t *__restrict__ clean, int32_t *__restrict__ clean_num, uint32_t *__restrict__ rows) {
-    extern __shared__ uint32_t sl_bits[];
-    pdl_wait();
+struct SelectedLists {
+    const int32_t *index, *num;
+    long long lists;
+    int Nq, Nkv, stride, H, group, words, row_words, warps;      // warps: lists of a CTA
+    int32_t *clean, *clean_num;
+    uint32_t *rows;                                              // or null
+};
+
+__device__ __forceinline__ void selected_list(const SelectedLists &p, uint32_t *all_bits, int cta) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long list = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
-    if (list >= lists) return;
-    uint32_t *bits = sl_bits + (size_t)warp * words;
-    for (int w = lane; w < words; w += 32) bits[w] = 0u;
+    const long long list = (long long)cta * p.warps + warp;
+    if (warp >= p.warps || list >= p.lists) return;
+    uint32_t *bits = all_bits + (size_t)warp * p.words;
+    for (int w = lane; w < p.words; w += 32) bits[w] = 0u;
     __syncwarp();
-    const int n = max(0, min(num[list], stride));
-    const long long bh = list / Nq;
-    const int i = (int)(list - bh * Nq), h = (int)(bh % H), hh = h % group;
-    const long long bhk = bh / H * (H / group) + h / group;
+    const int n = max(0, min(p.num[list], p.stride));
+    const long long bh = list / p.Nq;
+    const int i = (int)(list - bh * p.Nq), h = (int)(bh % p.H), hh = h % p.group;
+    const long long bhk = bh / p.H * (p.H / p.group) + h / p.group;
     int at = 0;
     for (int c = 0; c < n; c += 32) {
-        const int id = c + lane < n ? index[list * stride + c + lane] : -1;
-        const bool there = (unsigned)id < (unsigned)Nkv;
+        const int id = c + lane < n ? p.index[list * p.stride + c + lane] : -1;
+        const bool there = (unsigned)id < (unsigned)p.Nkv;
         const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1 - lane);
         const bool take = there && lane == __ffs(same) - 1 && !((bits[id >> 5] >> (id & 31)) & 1u);
         __syncwarp();
         const unsigned all = __ballot_sync(0xffffffffu, take);
         if (take) {
-            clean[list * stride + at + __popc(all & ((1u << lane) - 1u))] = id;
+            p.clean[list * p.stride + at + __popc(all & ((1u << lane) - 1u))] = id;
             atomicOr(&bits[id >> 5], 1u << (id & 31));
-            if (rows) atomicOr(&rows[((bhk * Nkv + id) * group + hh) * row_words + (i >> 5)], 1u << (i & 31));
+            if (p.rows) atomicOr(&p.rows[((bhk * p.Nkv + id) * p.group + hh) * p.row_words + (i >> 5)], 1u << (i & 31));
         }
         at += __popc(all);
         __syncwarp();
     }
-    if (lane == 0) clean_num[list] = at;
+    if (lane == 0) p.clean_num[list] = at;
+}
+
+__global__ void __launch_bounds__(SL_WARPS * 32)
+selected_lists_kernel(const SelectedLists p) {
+    extern __shared__ uint32_t sl_bits[];
+    pdl_wait();
+    selected_list(p, sl_bits, blockIdx.x);
 }
 
 // ---- work order of the gradient ------------------------------------------------------------------------
@@ -312,12 +323,18 @@ static int launch_few_rows(const wa_selected_params *p, cudaStream_t stream) {
 
 // ---- row statistics of the gradient -----------------------------------------------------------------
 // See selected_stat.  Reads dout and out once: `LANES` lanes take a row, 16 bytes each (LANES = 0: a warp, one channel at a time, any layout), and
-// four rows are on their way at a time.
+// four rows are on their way at a time.  The first CTAs of the launch clean the lists, which nothing here needs.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256)
-selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, unsigned all, float *__restrict__ stats) {
-    constexpr int WIDE = LANES ? LANES : 32, AT_ONCE = LANES ? 4 : 1, N = 16 / sizeof(T), EACH = 256 / WIDE;
+selected_prepare_kernel(const SelectedLists lists, unsigned list_ctas, View4 out, View4 dout, const float *__restrict__ lse, int H, int Lq, int D, int padded, unsigned all,
+                        float *__restrict__ stats) {
+    extern __shared__ uint32_t sl_bits[];
     pdl_wait();
+    if (blockIdx.x < list_ctas) {
+        if (blockIdx.y == 0) selected_list(lists, sl_bits, blockIdx.x);
+        return;
+    }
+    constexpr int WIDE = LANES ? LANES : 32, AT_ONCE = LANES ? 4 : 1, N = 16 / sizeof(T), EACH = 256 / WIDE;
     const int sub = threadIdx.x / WIDE, lane = threadIdx.x % WIDE, b = blockIdx.y;
     unsigned row[AT_ONCE];                        // (token, h) of the sample, heads innermost as in memory
     int h[AT_ONCE], l[AT_ONCE];
@@ -325,7 +342,7 @@ selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int 
     uint4 x[AT_ONCE], y[AT_ONCE];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-        row[u] = (blockIdx.x * AT_ONCE + u) * EACH + sub;
+        row[u] = ((blockIdx.x - list_ctas) * AT_ONCE + u) * EACH + sub;
         l[u] = (int)(row[u] / (unsigned)H);
         h[u] = (int)(row[u] - (unsigned)l[u] * (unsigned)H);
         sum[u] = 0.f;
@@ -361,18 +378,27 @@ selected_stats_kernel(View4 out, View4 dout, const float *__restrict__ lse, int 
 }
 
 template <typename T>
-static int launch_stats(const wa_selected_params *p, int padded, float *stats, cudaStream_t stream) {
+static int launch_prepare(const wa_selected_params *p, const SelectedLists &lists, int padded, float *stats, cudaStream_t stream) {
     const char *what = "wa_selected_backward";
     const auto pieces = [](const wa_tensor4 &t) {       // rows of whole 16-byte pieces
         constexpr int n = 16 / sizeof(T);
         return (uintptr_t)t.ptr % 16 == 0 && t.stride_b % n == 0 && t.stride_l % n == 0 && t.stride_h % n == 0;
     };
     const int bytes = p->D * (int)sizeof(T), lanes = pieces(p->out) && pieces(p->dout) && (bytes == 512 || bytes == 256 || bytes == 128) ? bytes / 16 : 0;
-    const long long all = (long long)p->H * padded, each = lanes ? 4 * (256 / lanes) : 8;
-    WA_REQUIRE(all + 1024 < (1ll << 32), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
-    const auto kernel = lanes == 32 ? selected_stats_kernel<T, 32> : lanes == 16 ? selected_stats_kernel<T, 16> : lanes == 8 ? selected_stats_kernel<T, 8> : selected_stats_kernel<T, 0>;
-    const cudaError_t e = launch_dependent(kernel, dim3((unsigned)((all + each - 1) / each), p->B), dim3(256), 0, stream, make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq,
-                                           p->D, padded, (unsigned)all, stats);
+    const long long all = (long long)p->H * padded, each = lanes ? 4 * (256 / lanes) : 8, list_ctas = (lists.lists + lists.warps - 1) / lists.warps;
+    WA_REQUIRE(all + 1024 < (1ll << 32) && list_ctas + (all + each - 1) / each < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+    const auto kernel = lanes == 32 ? selected_prepare_kernel<T, 32> : lanes == 16 ? selected_prepare_kernel<T, 16> : lanes == 8 ? selected_prepare_kernel<T, 8> : selected_prepare_kernel<T, 0>;
+    const size_t smem = (size_t)lists.warps * lists.words * sizeof(uint32_t);
+    static PerDeviceOnce attr_set;
+    if (smem > 48 * 1024 && !attr_set.done()) {
+        for (auto k : {selected_prepare_kernel<T, 32>, selected_prepare_kernel<T, 16>, selected_prepare_kernel<T, 8>, selected_prepare_kernel<T, 0>}) {
+            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024);
+            if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
+        }
+        attr_set.mark();
+    }
+    const cudaError_t e = launch_dependent(kernel, dim3((unsigned)(list_ctas + (all + each - 1) / each), p->B), dim3(256), smem, stream, lists, (unsigned)list_ctas,
+                                           make_view(&p->out), make_view(&p->dout), p->lse, p->H, p->Lq, p->D, padded, (unsigned)all, stats);
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
@@ -645,14 +671,14 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     if (selected_ordered(p, w)) w.q_order = c, c = align_up(c + lists * sizeof(int32_t), 256);
     if (backward) {
         w.rows = c; c = align_up(c + (size_t)p->B * p->H * w.Nkv * w.row_words * sizeof(uint32_t), 256);
+        w.counters = c; c += SELECTED_COUNTERS;
         if (selected_ordered(p, w)) {
             w.k_order = c; c = align_up(c + (size_t)p->B * p->Hkv * w.Nkv * sizeof(int32_t), 256);
         }
         w.stats = c; c = align_up(c + (size_t)p->B * p->H * selected_stats_rows(p, w.Nq) * 2 * sizeof(float), 256);
     }
     w.tuned = c;
-    if (backward ? selected_sm100_backward_supported(p) : selected_sm100_forward_supported(p))
-        c = align_up(c + (backward ? selected_sm100_backward_bytes(p) : selected_sm100_forward_bytes(p)), 256);
+    if (!backward && selected_sm100_forward_supported(p)) c = align_up(c + selected_sm100_forward_bytes(p), 256);
     w.total = c;
     return w;
 }
@@ -687,25 +713,28 @@ static int selected_order(const wa_selected_params *p, const SelectedPlan &w, bo
     return check_launch(what);
 }
 
-static int selected_lists(const wa_selected_params *p, const SelectedPlan &w, bool backward, char *ws, cudaStream_t stream, const char *what) {
-    const long long lists = (long long)p->B * p->H * w.Nq;
-    uint32_t *rows = backward ? (uint32_t *)(ws + w.rows) : nullptr;
-    if (rows) {
-        const cudaError_t e = cudaMemsetAsync(rows, 0, (size_t)p->B * p->H * w.Nkv * w.row_words * sizeof(uint32_t), stream);
-        if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
-    }
-    const int warps = w.words <= SL_WORDS ? SL_WARPS : 1;
-    const size_t smem = (size_t)warps * w.words * sizeof(uint32_t);
+static SelectedLists selected_lists(const wa_selected_params *p, const SelectedPlan &w, bool backward, char *ws) {
+    SelectedLists l{};
+    l.index = p->index; l.num = p->num;
+    l.lists = (long long)p->B * p->H * w.Nq;
+    l.Nq = w.Nq; l.Nkv = w.Nkv; l.stride = p->index_stride; l.H = p->H; l.group = w.group; l.words = w.words; l.row_words = w.row_words;
+    l.warps = w.words <= SL_WORDS ? SL_WARPS : 1;
+    l.clean = (int32_t *)(ws + w.index); l.clean_num = (int32_t *)(ws + w.num);
+    l.rows = backward ? (uint32_t *)(ws + w.rows) : nullptr;
+    return l;
+}
+
+static int launch_lists(const SelectedLists &l, cudaStream_t stream, const char *what) {
+    const size_t smem = (size_t)l.warps * l.words * sizeof(uint32_t);
     static PerDeviceOnce attr_set;
     if (smem > 48 * 1024 && !attr_set.done()) {
         const cudaError_t e = cudaFuncSetAttribute(selected_lists_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
-    const long long ctas = (lists + warps - 1) / warps;
+    const long long ctas = (l.lists + l.warps - 1) / l.warps;
     WA_REQUIRE(ctas < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: too many query blocks", what);
-    const cudaError_t e = launch_dependent(selected_lists_kernel, dim3((unsigned)ctas), dim3(warps * 32), smem, stream, p->index, p->num, lists, w.Nq, w.Nkv,
-                                           p->index_stride, p->H, w.group, w.words, w.row_words, (int32_t *)(ws + w.index), (int32_t *)(ws + w.num), rows);
+    const cudaError_t e = launch_dependent(selected_lists_kernel, dim3((unsigned)ctas), dim3(l.warps * 32), smem, stream, l);
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }
@@ -730,7 +759,7 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     WA_REQUIRE((uintptr_t)p->workspace % 256 == 0, WA_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", what);
     if (selected_few_rows(p)) return launch_few_rows(p, stream);
     char *ws = (char *)p->workspace;
-    if ((rc = selected_lists(p, w, false, ws, stream, what))) return rc;
+    if ((rc = launch_lists(selected_lists(p, w, false, ws), stream, what))) return rc;
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
     if (selected_sm100_forward_supported(p)) return selected_sm100_forward(p, index, num, ws + w.tuned, stream);
     const bool ordered = p->D == 128 && selected_ordered(p, w);       // (the kernel of other head_dims takes its rows as they come)
@@ -748,21 +777,24 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
     WA_REQUIRE(p->workspace && p->workspace_bytes >= w.total, WA_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes, got %zu", what, w.total, p->workspace_bytes);
     WA_REQUIRE((uintptr_t)p->workspace % 256 == 0, WA_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", what);
     char *ws = (char *)p->workspace;
-    if ((rc = selected_lists(p, w, true, ws, stream, what))) return rc;
+    // the bits that the lists set, and the counters of the tensor-core kernels behind them
+    const cudaError_t me = cudaMemsetAsync(ws + w.rows, 0, w.counters + SELECTED_COUNTERS - w.rows, stream);
+    if (me != cudaSuccess) return fail((int)me, "%s: %s", what, cudaGetErrorString(me));
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
     const uint32_t *rows = (const uint32_t *)(ws + w.rows);
     float *stats = (float *)(ws + w.stats);
     const size_t stats_rows = selected_stats_rows(p, w.Nq);
     WA_REQUIRE(stats_rows < (1ull << 31), WA_ERR_UNSUPPORTED, "%s: too many tokens", what);
     const int padded = (int)stats_rows;
-    if ((rc = p->q.dtype == WA_BF16 ? launch_stats<__nv_bfloat16>(p, padded, stats, stream) : launch_stats<float>(p, padded, stats, stream))) return rc;
+    const SelectedLists lists = selected_lists(p, w, true, ws);
+    if ((rc = p->q.dtype == WA_BF16 ? launch_prepare<__nv_bfloat16>(p, lists, padded, stats, stream) : launch_prepare<float>(p, lists, padded, stats, stream))) return rc;
     int32_t *q_order = nullptr, *k_order = nullptr;
     if (selected_ordered(p, w)) {
         q_order = (int32_t *)(ws + w.q_order);
         k_order = (int32_t *)(ws + w.k_order);
         if ((rc = selected_order(p, w, true, ws, stream, what))) return rc;
     }
-    if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, q_order, k_order, ws + w.tuned, stream);
+    if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, q_order, k_order, (int *)(ws + w.counters), stream);
     SelectedGrad g{};
     g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v); g.dout = make_view(&p->dout);
     g.dq = p->dq.ptr; g.dqb = p->dq.stride_b; g.dql = p->dq.stride_l; g.dqh = p->dq.stride_h;

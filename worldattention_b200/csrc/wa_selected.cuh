@@ -11,9 +11,10 @@ struct SelectedPlan {
     int Nq, Nkv, group, words, row_words;      // query / key blocks, query heads of a key head, words of a bit per key block / per query block
     size_t index, num;                         // [B, H, Nq, index_stride] clean lists, [B, H, Nq] their lengths
     size_t rows;                               // backward: [B, Hkv, Nkv, group, row_words] which query blocks of which head list a key block
+    size_t counters;                           // backward: zeroed together with `rows`, which it follows (see selected_sm100_backward)
     size_t stats;                              // backward: [B, H, selected_stats_rows] statistics of a query row, see selected_stat
     size_t q_order, k_order;                   // backward: query blocks and key blocks, heaviest first (not in every call)
-    size_t tuned;                              // what the tensor-core kernels need
+    size_t tuned;                              // forward: what the tensor-core kernel needs
     size_t total;
 };
 
@@ -33,8 +34,8 @@ int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, co
 int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int H, const char *name, int rows, int halves);
 // wa_selected_sm100.cu:
 bool selected_sm100_backward_supported(const wa_selected_params *p);
-size_t selected_sm100_backward_bytes(const wa_selected_params *p);
+constexpr size_t SELECTED_COUNTERS = 256;      // two work counters and the failure flag
 int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats,
-                            const int32_t *q_order, const int32_t *k_order, void *workspace, cudaStream_t stream);
+                            const int32_t *q_order, const int32_t *k_order, int *counters, cudaStream_t stream);
 
 }  // namespace wa

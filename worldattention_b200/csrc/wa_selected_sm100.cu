@@ -774,6 +774,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             };
             if (KEYS) {
                 if (ok) ok = wait(&bar->p_full, steps & 1u, 453);
+                if (ok) ok = wait(&bar->full[s2], ((tiles + 1) / SW_SLOTS) & 1u, 455);       // (P needs its query rows only, not yet those of dout)
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
@@ -1029,13 +1030,10 @@ bool selected_sm100_backward_supported(const wa_selected_params *p) {
            (long long)p->B * p->H * (ceil_div(p->Lq, SB_OWN) + 1ll) <= (1 << 24) &&
            (long long)p->B * p->Hkv * (ceil_div(p->Lkv, SB_OWN) + 1ll) <= (1 << 24);
 }
-size_t selected_sm100_backward_bytes(const wa_selected_params *) { return 256; }       // two work counters and the failure flag
 
 int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, const int32_t *num, const uint32_t *rows, const float *stats,
-                            const int32_t *q_order, const int32_t *k_order, void *workspace, cudaStream_t stream) {
+                            const int32_t *q_order, const int32_t *k_order, int *counters, cudaStream_t stream) {
     using namespace sm100;
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
-    if (e != cudaSuccess) return fail((int)e, "wa_selected_backward(tcgen05): %s", cudaGetErrorString(e));
     SbParams kp{};
     kp.H = p->H; kp.Hkv = p->Hkv; kp.group = p->H / p->Hkv; kp.Lq = p->Lq; kp.Lkv = p->Lkv;
     kp.Nq = ceil_div(p->Lq, p->block_size); kp.Nkv = ceil_div(p->Lkv, p->block_size);
@@ -1044,7 +1042,7 @@ int selected_sm100_backward(const wa_selected_params *p, const int32_t *index, c
     kp.index = index; kp.num = num; kp.rows = rows; kp.stats = stats; kp.q_order = q_order; kp.k_order = k_order;
     kp.scale = (float)pow((double)TILE, -0.5);
     kp.scale_log2 = (float)(pow((double)TILE, -0.5) * 1.4426950408889634);
-    kp.work_counter = (int *)workspace;
+    kp.work_counter = counters;
     kp.error_flag = kp.work_counter + 2;
     kp.status_mirror = p->status_mirror;
     int rc;
