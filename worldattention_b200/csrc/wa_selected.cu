@@ -403,19 +403,21 @@ static int launch_prepare(const wa_selected_params *p, const SelectedLists &list
     return check_launch(what);
 }
 
-// ---- gradient, any shape ------------------------------------------------------------------------------
-// One CTA owns T rows of one side -- dQ: queries, dK/dV: keys -- and meets the rows of the other side T at a time (T = 64, 32 for head_dim above
-// 128).  A warp has T / 8 of the owned rows to itself: its lanes take T / 32 met rows each for the scores and dP, P and dS go through
-// shared memory of the warp's own, and for the sums a lane has 4 channels of each 128.  So an owned row is one address for all lanes, a met row one for
-// each, both 16 bytes: 16 wavefronts of shared memory for 64 multiply-adds of a warp (scores), 24 for 128 (sums), below what the multiply-adds take.
-// (16 x 16 threads with 2 x 2 scores each were bound by shared memory: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64 a row: dK/dV
-// 187 us and dQ 143, now 161 and 119, heaviest first 141 and 85)
+// ---- any shape -----------------------------------------------------------------------------------------
+// Forward and gradient with multiply-adds, for what the tensor-core kernels do not take.  One CTA owns TF rows of one side -- forward and dQ: queries,
+// dK/dV: keys -- and meets the rows of the other side TG at a time.  A warp has TF / 8 of the owned rows to itself: its lanes take TG / 32 met
+// rows each for the scores, P and dS go through shared memory of the warp's own, and for the sums a lane has CH channels (the width is 32 CH:
+// 64, 128 or 256).  So an owned row is one address for all lanes, a met row one for each, both 16 bytes: with 64 and 64 rows 16 wavefronts of shared
+// memory for 64 multiply-adds of a warp (scores), 24 for 128 (sums), below what the multiply-adds take.  (16 x 16 threads with 2 x 2 scores each were
+// bound by shared memory: three frames of 390 tokens, 12 heads, 3 of 19 blocks of 64 a row: dK/dV 187 us and dQ 143, now 161 and 119, heaviest first
+// 141 and 85.)  Where 64 owned rows leave SMs without a CTA there are 32 or 16 to a CTA, see selected_own.
 // The next rows to meet are on their way while some are at work: asynchronous copies of aligned float32 rows, plain loads of anything else.
-struct SelectedGrad {
+struct SelectedAny {
     View4 q, k, v, dout;
-    void *dq, *dk, *dv;
+    void *out, *dq, *dk, *dv;
+    float *lse;
     int dtype;
-    long long dqb, dql, dqh, dkb, dkl, dkh, dvb, dvl, dvh;
+    long long ob, ol, oh, dqb, dql, dqh, dkb, dkl, dkh, dvb, dvl, dvh;
     int H, group, Lq, Lkv, D, block, stride, Nq, Nkv, row_words, padded, tiles;
     int async;                        // rows of whole 16-byte pieces of float32
     const int32_t *index, *num, *block_sizes;
@@ -424,32 +426,58 @@ struct SelectedGrad {
     const float *stats;
     float scale;
 };
-template <int T, int NM, bool KEYS>      // NM: 128-column steps of head_dim
+enum { SG_FORWARD, SG_QUERIES, SG_KEYS };
+
+// channels of a lane: CH neighbouring ones, or four of each half of 256
+template <int CH>
+__device__ __forceinline__ void sg_channels(const float *row, int lane, float (&y)[CH]) {
+    if constexpr (CH == 2) {
+        const float2 v = *reinterpret_cast<const float2 *>(row + 2 * lane);
+        y[0] = v.x, y[1] = v.y;
+    } else {
+#pragma unroll
+        for (int m = 0; m < CH / 4; ++m) {
+            const float4 v = *reinterpret_cast<const float4 *>(row + 128 * m + 4 * lane);
+            y[4 * m] = v.x, y[4 * m + 1] = v.y, y[4 * m + 2] = v.z, y[4 * m + 3] = v.w;
+        }
+    }
+}
+template <int CH>
+__device__ __forceinline__ int sg_channel(int lane, int u) { return CH == 2 ? 2 * lane + u : 128 * (u >> 2) + 4 * lane + (u & 3); }
+
+template <int TF, int TG, int CH>
+constexpr size_t sg_smem(int what) {
+    return (size_t)(((what == SG_FORWARD ? 1 : 2) * TF + 4 * TG) * (32 * CH + 4) + TF * (TG + 4)) * 4 + 2 * (size_t)(TF > TG ? TF : TG) * 8;
+}
+
+template <int TF, int TG, int CH, int WHAT>
 __global__ void __launch_bounds__(256)
-selected_grad_kernel(const SelectedGrad p) {
-    constexpr int W = 128 * NM, LD = W + 4, R = T / 8, C = T / 32, LP = T + 4;      // R: owned rows of a warp, C: met rows of a lane
-    extern __shared__ __align__(16) float sg_smem[];
-    float *f1 = sg_smem, *f2 = f1 + T * LD, *met = f2 + T * LD;               // owned: q, dout or k, v; met: [two buffers][the other two]
-    float *factors = met + 4 * T * LD;                                        // P, then dS
-    float2 *st = reinterpret_cast<float2 *>(factors + T * LP);                // [two buffers] statistics of the query rows
+selected_any_kernel(const SelectedAny p) {
+    constexpr bool KEYS = WHAT == SG_KEYS, FORWARD = WHAT == SG_FORWARD;
+    constexpr int W = 32 * CH, LD = W + 4, R = TF / 8, C = TG / 32, LP = TG + 4;      // R: owned rows of a warp, C: met rows of a lane
+    constexpr int ST = TF > TG ? TF : TG;
+    extern __shared__ __align__(16) float sg_smem_[];
+    float *f1 = sg_smem_, *f2 = f1 + TF * LD, *met = FORWARD ? f2 : f2 + TF * LD;     // owned: q (and dout) or k, v; met: [two buffers][the other two]
+    float *factors = met + 4 * TG * LD;                                                // P, then dS
+    float2 *st = reinterpret_cast<float2 *>(factors + TF * LP);                        // [two buffers] statistics of the query rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = KEYS ? p.Nkv : p.Nq, heads = KEYS ? p.H / p.group : p.H;
     const int32_t *order = KEYS ? p.k_order : p.q_order;
     const int item = order ? order[blockIdx.x / p.tiles] : blockIdx.x / p.tiles, own_head = item / blocks;
-    const int blk = item - own_head * blocks, first = blk * p.block + (blockIdx.x % p.tiles) * T, b = own_head / heads, h = own_head - b * heads;
+    const int blk = item - own_head * blocks, first = blk * p.block + (blockIdx.x % p.tiles) * TF, b = own_head / heads, h = own_head - b * heads;
     const int hk = KEYS ? h : h / p.group;
     const auto keys_of = [&](int id) {       // real tokens of a key block
         const int n = min(p.block, p.Lkv - id * p.block);
         return p.block_sizes ? max(0, min(n, p.block_sizes[id])) : n;
     };
-    const int own_end = min(min(first + T, (blk + 1) * p.block), KEYS ? p.Lkv : p.Lq);       // rows to write
-    const int own_real = KEYS ? min(own_end, blk * p.block + keys_of(blk)) : own_end;         // rows that count
+    const int own_end = min(min(first + TF, (blk + 1) * p.block), KEYS ? p.Lkv : p.Lq);       // rows to write
+    const int own_real = KEYS ? min(own_end, blk * p.block + keys_of(blk)) : own_end;          // rows that count
     if (first >= own_end) return;
 
-    const auto bring = [&](float *to, const View4 &x, int head, int from, int end) {
+    const auto bring = [&](float *to, const View4 &x, int head, int from, int end, int rows) {
         const long long base = b * x.sb + (long long)head * x.sh;
         if (p.async) {
-            for (int e = threadIdx.x; e < T * (W / 4); e += 256) {
+            for (int e = threadIdx.x; e < rows * (W / 4); e += 256) {
                 const int r = e / (W / 4), d = e % (W / 4) * 4;
                 const bool there = from + r < end && d < p.D;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + r * LD + d)),
@@ -457,22 +485,22 @@ selected_grad_kernel(const SelectedGrad p) {
             }
         } else {
 #pragma unroll 4
-            for (int e = threadIdx.x; e < T * W; e += 256) {
+            for (int e = threadIdx.x; e < rows * W; e += 256) {
                 const int r = e / W, d = e % W;
                 to[r * LD + d] = from + r < end && d < p.D ? load_elem(x.ptr, x.dtype, base + (long long)(from + r) * x.sl + d) : 0.f;
             }
         }
     };
-    const auto bring_stats = [&](float2 *to, int head, int from, int end) {
+    const auto bring_stats = [&](float2 *to, int head, int from, int end, int rows) {
         const float *stats = p.stats + ((long long)b * p.H + head) * p.padded * 2;
-        for (int r = threadIdx.x; r < T; r += 256)
+        for (int r = threadIdx.x; r < rows; r += 256)
             to[r] = from + r < end ? make_float2(stats[selected_stat(from + r)], stats[selected_stat(from + r) + 64]) : make_float2(-INFINITY, 0.f);
     };
-    bring(f1, KEYS ? p.k : p.q, h, first, own_real);
-    bring(f2, KEYS ? p.v : p.dout, h, first, own_real);
-    if (!KEYS) bring_stats(st, h, first, own_real);
+    bring(f1, KEYS ? p.k : p.q, h, first, own_real, TF);
+    if (!FORWARD) bring(f2, KEYS ? p.v : p.dout, h, first, own_real, TF);
+    if (WHAT == SG_QUERIES) bring_stats(st, h, first, own_real, TF);
 
-    // the rows to meet, T at a time: those of the listed blocks in the order of the list
+    // the rows to meet, TG at a time: those of the listed blocks in the order of the list
     struct Rows { int h, from, end; };
     int at = -1, left_from = 0, left_end = 0, head = 0;
     uint32_t word = 0;
@@ -498,21 +526,25 @@ selected_grad_kernel(const SelectedGrad p) {
                 left_end = left_from + keys_of(id);
             }
         }
-        to = Rows{head, left_from, min(left_from + T, left_end)};
-        left_from += T;
+        to = Rows{head, left_from, min(left_from + TG, left_end)};
+        left_from += TG;
         return true;
     };
     const auto bring_met = [&](int buf, const Rows &r) {
-        bring(met + 2 * buf * T * LD, KEYS ? p.q : p.k, KEYS ? r.h : hk, r.from, r.end);
-        bring(met + (2 * buf + 1) * T * LD, KEYS ? p.dout : p.v, KEYS ? r.h : hk, r.from, r.end);
-        if (KEYS) bring_stats(st + buf * T, r.h, r.from, r.end);
+        bring(met + 2 * buf * TG * LD, KEYS ? p.q : p.k, KEYS ? r.h : hk, r.from, r.end, TG);
+        bring(met + (2 * buf + 1) * TG * LD, KEYS ? p.dout : p.v, KEYS ? r.h : hk, r.from, r.end, TG);
+        if (KEYS) bring_stats(st + buf * ST, r.h, r.from, r.end, TG);
     };
 
-    float4 sum1[R][NM], sum2[R][NM];         // of the owned rows: dV (KEYS), dK or dQ
+    float sum1[R][CH], sum2[R][CH];         // of the owned rows: dV (KEYS); dK, dQ or the result
+    float top[R], total[R];                 // forward: running maximum of a row, and this lane's part of the sum
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+        top[i] = -INFINITY;
+        total[i] = 0.f;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) sum1[i][m] = sum2[i][m] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < CH; ++u) sum1[i][u] = sum2[i][u] = 0.f;
+    }
     const float to_log2 = p.scale * 1.4426950408889634f;
     const int depth = (p.D + 3) & ~3;
 
@@ -526,7 +558,7 @@ selected_grad_kernel(const SelectedGrad p) {
         asm volatile("cp.async.commit_group;" ::: "memory");
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
-        const float *g1 = met + 2 * buf * T * LD, *g2 = g1 + T * LD;
+        const float *g1 = met + 2 * buf * TG * LD, *g2 = g1 + TG * LD;
         float s[R][C], dp[R][C];
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -552,19 +584,40 @@ selected_grad_kernel(const SelectedGrad p) {
             }
         };
         dots(s, f1, g1);
-        dots(dp, f2, g2);
+        if (!FORWARD) dots(dp, f2, g2);
         float *mine = factors + warp * R * LP;
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int i = 0; i < R; ++i) {
+            if (FORWARD) {
+                float high = top[i];
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-                const int f = warp * R + i, g = lane + 32 * j;
-                const float2 row = st[KEYS ? buf * T + g : f];
-                const bool there = first + f < own_real && now.from + g < now.end;
-                s[i][j] = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
-                dp[i][j] = there ? s[i][j] * (dp[i][j] + row.y) * p.scale : 0.f;
+                for (int j = 0; j < C; ++j) {
+                    s[i][j] = now.from + lane + 32 * j < now.end ? s[i][j] * to_log2 : -INFINITY;
+                    high = fmaxf(high, s[i][j]);
+                }
+                high = warp_max(high);
+                const float from = high == -INFINITY ? 0.f : high, back = exp2f(top[i] - from);      // (nothing seen yet: 2^-inf = 0)
+                top[i] = high;
+                total[i] *= back;
+#pragma unroll
+                for (int u = 0; u < CH; ++u) sum2[i][u] *= back;
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    s[i][j] = exp2f(s[i][j] - from);
+                    total[i] += s[i][j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; ++j) {
+                    const int f = warp * R + i, g = lane + 32 * j;
+                    const float2 row = st[KEYS ? buf * ST + g : f];
+                    const bool there = first + f < own_real && now.from + g < now.end;
+                    s[i][j] = there ? exp2f(fmaf(s[i][j], to_log2, row.x)) : 0.f;
+                    dp[i][j] = there ? s[i][j] * (dp[i][j] + row.y) * p.scale : 0.f;
+                }
             }
-        const auto add = [&](float4 (&acc)[R][NM], const float (&factor)[R][C], const float *x) {
+        }
+        const auto add = [&](float (&acc)[R][CH], const float (&factor)[R][C], const float *x) {
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < R; ++i)
@@ -572,48 +625,54 @@ selected_grad_kernel(const SelectedGrad p) {
                 for (int j = 0; j < C; ++j) mine[i * LP + lane + 32 * j] = factor[i][j];
             __syncwarp();
 #pragma unroll 2
-            for (int g = 0; g < T; g += 4) {
-                float4 y[4][NM];
+            for (int g = 0; g < TG; g += 4) {
+                float y[4][CH];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int m = 0; m < NM; ++m) y[u][m] = *reinterpret_cast<const float4 *>(x + (g + u) * LD + 128 * m + 4 * lane);
+                for (int u = 0; u < 4; ++u) sg_channels<CH>(x + (g + u) * LD, lane, y[u]);
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     const float4 a = *reinterpret_cast<const float4 *>(mine + i * LP + g);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const float c = u == 0 ? a.x : u == 1 ? a.y : u == 2 ? a.z : a.w;
-#pragma unroll
-                        for (int m = 0; m < NM; ++m) {
-                            acc[i][m].x = fmaf(c, y[u][m].x, acc[i][m].x);
-                            acc[i][m].y = fmaf(c, y[u][m].y, acc[i][m].y);
-                            acc[i][m].z = fmaf(c, y[u][m].z, acc[i][m].z);
-                            acc[i][m].w = fmaf(c, y[u][m].w, acc[i][m].w);
-                        }
+                    for (int m = 0; m < CH; ++m) {
+                        acc[i][m] = fmaf(a.x, y[0][m], acc[i][m]);
+                        acc[i][m] = fmaf(a.y, y[1][m], acc[i][m]);
+                        acc[i][m] = fmaf(a.z, y[2][m], acc[i][m]);
+                        acc[i][m] = fmaf(a.w, y[3][m], acc[i][m]);
                     }
                 }
             }
         };
-        if (KEYS) add(sum1, s, g2);
-        add(sum2, dp, g1);
+        if (FORWARD) {
+            add(sum2, s, g2);
+        } else {
+            if (KEYS) add(sum1, s, g2);
+            add(sum2, dp, g1);
+        }
         __syncthreads();
     }
-    const auto write = [&](const float4 (&acc)[R][NM], void *to, long long sb, long long sl, long long sh) {
+    const auto write = [&](const float (&acc)[R][CH], void *to, long long sb, long long sl, long long sh) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int r = first + warp * R + i;
             if (r >= own_end) continue;
 #pragma unroll
-            for (int m = 0; m < NM; ++m) {
-                const float v[4] = {acc[i][m].x, acc[i][m].y, acc[i][m].z, acc[i][m].w};
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (128 * m + 4 * lane + u < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + 128 * m + 4 * lane + u, v[u]);
+            for (int u = 0; u < CH; ++u) {
+                const int d = sg_channel<CH>(lane, u);
+                if (d < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + d, acc[i][u]);
             }
         }
     };
-    if (KEYS) {
+    if (FORWARD) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float all = warp_sum(total[i]);
+            const int r = first + warp * R + i;
+#pragma unroll
+            for (int u = 0; u < CH; ++u) sum2[i][u] = all == 0.f ? 0.f : sum2[i][u] / all;
+            if (p.lse && lane == 0 && r < own_end) p.lse[((long long)b * p.H + h) * p.Lq + r] = all == 0.f ? -INFINITY : (top[i] + log2f(all)) * 0.6931471805599453f;
+        }
+        write(sum2, p.out, p.ob, p.ol, p.oh);
+    } else if (KEYS) {
         write(sum1, p.dv, p.dvb, p.dvl, p.dvh);
         write(sum2, p.dk, p.dkb, p.dkl, p.dkh);
     } else {
@@ -621,26 +680,40 @@ selected_grad_kernel(const SelectedGrad p) {
     }
 }
 
-template <int T, int NM>
-static int launch_grad(SelectedGrad p, int B, int Hkv, cudaStream_t stream) {
-    const char *what = "wa_selected_backward";
-    constexpr size_t smem = (size_t)(6 * T * (128 * NM + 4) + T * (T + 4)) * 4 + 2 * T * 8;
+template <int TF, int TG, int CH, int WHAT>
+static int launch_any(SelectedAny p, long long items, cudaStream_t stream, const char *what) {
+    constexpr size_t smem = sg_smem<TF, TG, CH>(WHAT);
     static_assert(smem <= 227 * 1024, "shared memory budget exceeded");
     static PerDeviceOnce attr_set;
     if (!attr_set.done()) {
-        cudaError_t e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(selected_grad_kernel<T, NM, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(selected_any_kernel<TF, TG, CH, WHAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         attr_set.mark();
     }
-    p.tiles = ceil_div(p.block, T);
-    const long long kx = (long long)B * Hkv * p.Nkv * p.tiles, qx = (long long)B * p.H * p.Nq * p.tiles;
-    WA_REQUIRE(kx < (1ll << 31) && qx < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: grid too large", what);
-    int rc;
-    selected_grad_kernel<T, NM, true><<<(unsigned)kx, 256, smem, stream>>>(p);
-    if ((rc = check_launch(what))) return rc;
-    selected_grad_kernel<T, NM, false><<<(unsigned)qx, 256, smem, stream>>>(p);
+    p.tiles = ceil_div(p.block, TF);
+    const long long ctas = items * p.tiles;
+    WA_REQUIRE(ctas < (1ll << 31), WA_ERR_UNSUPPORTED, "%s: grid too large", what);
+    selected_any_kernel<TF, TG, CH, WHAT><<<(unsigned)ctas, 256, smem, stream>>>(p);
     return check_launch(what);
+}
+
+// Owned rows of a CTA: 64 where that gives every SM one, else 32, else 16.  A CTA of 16 rows needs OWN16 of the time of one of 64 for a quarter of its work (its
+// warps read a met row for two owned ones instead of eight).  TIMES6
+static int selected_own(long long rows, int block, int limit) {
+    const int sms = sm_count();
+    int own = limit;
+    while (own > 16 && (own > block || rows / own < sms)) own >>= 1;
+    return own;
+}
+
+template <int WHAT>
+static int run_any(const SelectedAny &p, int B, cudaStream_t stream, const char *what) {
+    const int heads = WHAT == SG_KEYS ? p.H / p.group : p.H, blocks = WHAT == SG_KEYS ? p.Nkv : p.Nq;
+    const long long items = (long long)B * heads * blocks;
+    const int own = selected_own((long long)B * heads * (WHAT == SG_KEYS ? p.Lkv : p.Lq), p.block, p.D <= 128 ? 64 : 32);
+    if (p.D <= 64) return own == 64 ? launch_any<64, 64, 2, WHAT>(p, items, stream, what) : own == 32 ? launch_any<32, 64, 2, WHAT>(p, items, stream, what) : launch_any<16, 64, 2, WHAT>(p, items, stream, what);
+    if (p.D <= 128) return own == 64 ? launch_any<64, 64, 4, WHAT>(p, items, stream, what) : own == 32 ? launch_any<32, 64, 4, WHAT>(p, items, stream, what) : launch_any<16, 64, 4, WHAT>(p, items, stream, what);
+    return own == 32 ? launch_any<32, 32, 8, WHAT>(p, items, stream, what) : launch_any<16, 32, 8, WHAT>(p, items, stream, what);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -739,6 +812,23 @@ static int launch_lists(const SelectedLists &l, cudaStream_t stream, const char 
     return check_launch(what);
 }
 
+static bool whole_pieces(const wa_tensor4 &t) {      // float32 rows of whole 16-byte pieces
+    return t.dtype == WA_F32 && (uintptr_t)t.ptr % 16 == 0 && t.stride_b % 4 == 0 && t.stride_l % 4 == 0 && t.stride_h % 4 == 0;
+}
+
+static SelectedAny selected_any(const wa_selected_params *p, const SelectedPlan &w, char *ws) {
+    SelectedAny g{};
+    g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v);
+    g.out = p->out.ptr; g.ob = p->out.stride_b; g.ol = p->out.stride_l; g.oh = p->out.stride_h;
+    g.lse = p->lse;
+    g.dtype = p->q.dtype;
+    g.H = p->H; g.group = w.group; g.Lq = p->Lq; g.Lkv = p->Lkv; g.D = p->D; g.block = p->block_size; g.stride = p->index_stride; g.Nq = w.Nq; g.Nkv = w.Nkv;
+    g.index = (const int32_t *)(ws + w.index); g.num = (const int32_t *)(ws + w.num); g.block_sizes = p->block_sizes;
+    g.scale = (float)(1.0 / sqrt((double)p->D));
+    g.async = p->D % 4 == 0 && whole_pieces(p->q) && whole_pieces(p->k) && whole_pieces(p->v);
+    return g;
+}
+
 }  // namespace wa
 
 using namespace wa;
@@ -762,10 +852,16 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     if ((rc = launch_lists(selected_lists(p, w, false, ws), stream, what))) return rc;
     const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
     if (selected_sm100_forward_supported(p)) return selected_sm100_forward(p, index, num, ws + w.tuned, stream);
-    const bool ordered = p->D == 128 && selected_ordered(p, w);       // (the kernel of other head_dims takes its rows as they come)
+    const bool ordered = selected_ordered(p, w);
     if (ordered && (rc = selected_order(p, w, false, ws, stream, what))) return rc;
+    const int32_t *order = ordered ? (const int32_t *)(ws + w.q_order) : nullptr;
+    if (p->D != 128 && !p->block_sizes) {      // (with block sizes the kernels and the bits of wa_block_sparse_forward)
+        SelectedAny g = selected_any(p, w, ws);
+        g.q_order = order;
+        return run_any<SG_FORWARD>(g, p->B, stream, what);
+    }
     return block_sparse_run(&p->q, &p->k, &p->v, &p->out, p->B, p->H, p->Lq, p->Lkv, p->D, p->block_size, index, num, p->index_stride, p->block_sizes, 0, 0,
-                            p->lse, ordered ? (const int32_t *)(ws + w.q_order) : nullptr, false, stream, w.group);
+                            p->lse, order, false, stream, w.group);
 }
 
 extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) {
@@ -795,19 +891,14 @@ extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) 
         if ((rc = selected_order(p, w, true, ws, stream, what))) return rc;
     }
     if (selected_sm100_backward_supported(p)) return selected_sm100_backward(p, index, num, rows, stats, q_order, k_order, (int *)(ws + w.counters), stream);
-    SelectedGrad g{};
-    g.q = make_view(&p->q); g.k = make_view(&p->k); g.v = make_view(&p->v); g.dout = make_view(&p->dout);
+    SelectedAny g = selected_any(p, w, ws);
+    g.dout = make_view(&p->dout);
     g.dq = p->dq.ptr; g.dqb = p->dq.stride_b; g.dql = p->dq.stride_l; g.dqh = p->dq.stride_h;
     g.dk = p->dk.ptr; g.dkb = p->dk.stride_b; g.dkl = p->dk.stride_l; g.dkh = p->dk.stride_h;
     g.dv = p->dv.ptr; g.dvb = p->dv.stride_b; g.dvl = p->dv.stride_l; g.dvh = p->dv.stride_h;
-    g.dtype = p->q.dtype;
-    g.H = p->H; g.group = w.group; g.Lq = p->Lq; g.Lkv = p->Lkv; g.D = p->D; g.block = p->block_size; g.stride = p->index_stride;
-    g.Nq = w.Nq; g.Nkv = w.Nkv; g.row_words = w.row_words; g.padded = padded;
-    g.index = index; g.num = num; g.block_sizes = p->block_sizes; g.rows = rows; g.stats = stats; g.q_order = q_order; g.k_order = k_order;
-    g.scale = (float)(1.0 / sqrt((double)p->D));
-    const auto pieces = [](const wa_tensor4 &t) {
-        return t.dtype == WA_F32 && (uintptr_t)t.ptr % 16 == 0 && t.stride_b % 4 == 0 && t.stride_l % 4 == 0 && t.stride_h % 4 == 0;
-    };
-    g.async = p->D % 4 == 0 && pieces(p->q) && pieces(p->k) && pieces(p->v) && pieces(p->dout);
-    return p->D <= 128 ? launch_grad<64, 1>(g, p->B, p->Hkv, stream) : launch_grad<32, 2>(g, p->B, p->Hkv, stream);
+    g.row_words = w.row_words; g.padded = padded;
+    g.rows = rows; g.stats = stats; g.q_order = q_order; g.k_order = k_order;
+    g.async = g.async && whole_pieces(p->dout);
+    if ((rc = run_any<SG_KEYS>(g, p->B, stream, what))) return rc;
+    return run_any<SG_QUERIES>(g, p->B, stream, what);
 }
