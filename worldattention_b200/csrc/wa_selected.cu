@@ -697,20 +697,23 @@ static int launch_any(SelectedAny p, long long items, cudaStream_t stream, const
     return check_launch(what);
 }
 
-// Owned rows of a CTA: 64 where that gives every SM one, else 32, else 16.  A CTA of 16 rows needs OWN16 of the time of one of 64 for a quarter of its work (its
-// warps read a met row for two owned ones instead of eight).  TIMES6
-static int selected_own(long long rows, int block, int limit) {
-    const int sms = sm_count();
-    int own = limit;
-    while (own > 16 && (own > block || rows / own < sms)) own >>= 1;
-    return own;
+// Owned rows of a CTA: 64, 32 or 16, whichever is done first.  A CTA of 32 rows takes 0.65 of the time of one of 64, one of 16 0.52 (its warps read a met row for
+// two owned ones instead of eight), and as many rounds as its SMs take; head_dim 64 leaves room for two on an SM.  head_dim 128, 12 heads, 10 blocks of 64
+// listed, forward and dQ with 64 rows -> as chosen: 64 queries 95 and 135 us -> 51 and 68 (16 rows); 700 97 and 137 (64 rows; with 32 125 and 176).
+static int selected_own(long long rows, int block, int limit, int resident) {
+    const long long room = (long long)sm_count() * resident;
+    const auto cost = [&](int own) { return ((rows + own - 1) / own + room - 1) / room * (own == 64 ? 20 : own == 32 ? 13 : 11); };
+    int best = 16;
+    for (int own = 32; own <= limit; own <<= 1)
+        if (own < 2 * block && cost(own) <= cost(best)) best = own;
+    return best;
 }
 
 template <int WHAT>
 static int run_any(const SelectedAny &p, int B, cudaStream_t stream, const char *what) {
     const int heads = WHAT == SG_KEYS ? p.H / p.group : p.H, blocks = WHAT == SG_KEYS ? p.Nkv : p.Nq;
     const long long items = (long long)B * heads * blocks;
-    const int own = selected_own((long long)B * heads * (WHAT == SG_KEYS ? p.Lkv : p.Lq), p.block, p.D <= 128 ? 64 : 32);
+    const int own = selected_own((long long)B * heads * (WHAT == SG_KEYS ? p.Lkv : p.Lq), p.block, p.D <= 128 ? 64 : 32, p.D <= 64 ? 2 : 1);
     if (p.D <= 64) return own == 64 ? launch_any<64, 64, 2, WHAT>(p, items, stream, what) : own == 32 ? launch_any<32, 64, 2, WHAT>(p, items, stream, what) : launch_any<16, 64, 2, WHAT>(p, items, stream, what);
     if (p.D <= 128) return own == 64 ? launch_any<64, 64, 4, WHAT>(p, items, stream, what) : own == 32 ? launch_any<32, 64, 4, WHAT>(p, items, stream, what) : launch_any<16, 64, 4, WHAT>(p, items, stream, what);
     return own == 32 ? launch_any<32, 32, 8, WHAT>(p, items, stream, what) : launch_any<16, 32, 8, WHAT>(p, items, stream, what);
@@ -855,7 +858,9 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     const bool ordered = selected_ordered(p, w);
     if (ordered && (rc = selected_order(p, w, false, ws, stream, what))) return rc;
     const int32_t *order = ordered ? (const int32_t *)(ws + w.q_order) : nullptr;
-    if (p->D != 128 && !p->block_sizes) {      // (with block sizes the kernels and the bits of wa_block_sparse_forward)
+    // (With block sizes the kernels and the bits of wa_block_sparse_forward.  Float32 with head_dim 128 there: 12 heads of 1170 tokens 71 -> 62 us here, 64 queries over
+    // 10 blocks 109 -> 51; bf16 values are its matrix instructions' own.)
+    if (!p->block_sizes && (p->D != 128 || p->q.dtype == WA_F32)) {
         SelectedAny g = selected_any(p, w, ws);
         g.q_order = order;
         return run_any<SG_FORWARD>(g, p->B, stream, what);
