@@ -697,15 +697,17 @@ static int launch_any(SelectedAny p, long long items, cudaStream_t stream, const
     return check_launch(what);
 }
 
-// Owned rows of a CTA: 64, 32 or 16, whichever is done first.  A CTA of 32 rows takes 0.65 of the time of one of 64, one of 16 0.52 (its warps read a met row for
-// two owned ones instead of eight), and as many rounds as its SMs take; head_dim 64 leaves room for two on an SM.  head_dim 128, 12 heads, 10 blocks of 64
-// listed, forward and dQ with 64 rows -> as chosen: 64 queries 95 and 135 us -> 51 and 68 (16 rows); 700 97 and 137 (64 rows; with 32 125 and 176).
+// Owned rows of a CTA: 64, 32 or 16, whichever is done first, of about equal ones the larger (it reads the met rows less often; 1170 tokens of 12
+// heads, up to six blocks listed: forward, dQ and dK/dV 61, 85 and 125 us with 64, 71, 95 and 118 with 32).  A CTA of 32 rows takes 0.65 of the time of one of
+// 64, one of 16 0.52 (its warps read a met row for two owned ones instead of eight), and as many rounds as its SMs take; head_dim 64 leaves room for two on
+// an SM.  head_dim 128, 12 heads, 10 blocks of 64 listed, forward and dQ with 64 rows -> as chosen: 64 queries 95 and 135 us -> 51 and 68 (16 rows); 700
+// 97 and 137 (64 rows; with 32 125 and 176).
 static int selected_own(long long rows, int block, int limit, int resident) {
     const long long room = (long long)sm_count() * resident;
     const auto cost = [&](int own) { return ((rows + own - 1) / own + room - 1) / room * (own == 64 ? 20 : own == 32 ? 13 : 11); };
     int best = 16;
     for (int own = 32; own <= limit; own <<= 1)
-        if (own < 2 * block && cost(own) <= cost(best)) best = own;
+        if (own < 2 * block && cost(own) * 9 <= cost(best) * 10) best = own;
     return best;
 }
 
@@ -858,8 +860,8 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     const bool ordered = selected_ordered(p, w);
     if (ordered && (rc = selected_order(p, w, false, ws, stream, what))) return rc;
     const int32_t *order = ordered ? (const int32_t *)(ws + w.q_order) : nullptr;
-    // (With block sizes the kernels and the bits of wa_block_sparse_forward.  Float32 with head_dim 128 there: 12 heads of 1170 tokens 71 -> 62 us here, 64 queries over
-    // 10 blocks 109 -> 51; bf16 values are its matrix instructions' own.)
+    // (With block sizes the kernels and the bits of wa_block_sparse_forward.  Without, it keeps bf16 with head_dim 128, which has matrix instructions there; float32 with
+    // that head_dim, there -> here: 12 heads of 1170 tokens 71 -> 61 us, 64 queries over 10 blocks 109 -> 51.)
     if (!p->block_sizes && (p->D != 128 || p->q.dtype == WA_F32)) {
         SelectedAny g = selected_any(p, w, ws);
         g.q_order = order;

@@ -15,6 +15,11 @@
 // issues the loads, one issues the scores' products and one the sums'.  Tensor memory holds two steps' scores and the sums of two owned
 // tiles (2 x 128 + 2 x 128 columns).
 //
+// What bounds it: all four products read both operands from shared memory, and one of 128 x 64 x 16 takes 48 cycles of that for 32 of the tensor cores. The
+// two issuing warps are held by their products for 1350 and 1340 of the 2500 cycles of a step (dK/dV; sixteen workers, two steps in flight, hide the rest):
+// 32 760 tokens over themselves, 32 of 512 blocks a row, 12 heads: dK/dV 920 us, dQ 728.  One issuing warp for both took 1323 and 986, eight workers 998
+// and 819.  Roundings: P and dS to bf16 as factors of products, sums in float32, gradients once at the end.
+//
 // Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
 #include "wa_selected.cuh"
 #include "wa_sm100_ptx.cuh"
@@ -526,6 +531,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 // Finished sums leave through the ring of tiles: at an item's end the loading warp gives the workers a slot for each, they leave it as bf16 there, and a
 // warp of its own stores it and gives the slot back.  (Stored by the workers themselves, 32 rows of 16 or 32 bytes at a time, an item's end took
 // 8000 cycles, three steps' time; lists of a chunk's keys are five steps long.)
+// What bounds it: dQ by the rate of the products (the issuing warps are held for 2400 of 2600 cycles a step, the forward kernel's rate), dK/dV by that
+// and by the ends of items.  4680 queries, 32 of 256 blocks a row, 12 heads: dK/dV 237 us, dQ 145 (299 and 217 before the two changes above).
 // Tensor memory: S, dP, dV and dK; or S, two of dP, and dQ.  Scores of step u + 1 follow as soon as their columns are free: behind the sum that
 // read P or dS, or, for dQ's S, behind the workers' reads.
 template <bool KEYS>
