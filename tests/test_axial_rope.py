@@ -152,6 +152,17 @@ def test_captured_and_on_another_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int64, torch.uint16, torch.uint32, torch.uint64])
+def test_positions_of_every_integer_type(dtype):
+    from worldattention_b200.rope import axial_rope
+    rows = 40000                                                                # more than 8 and 16 bits with a sign hold
+    table = torch.view_as_real(_table(rows, 16, dev())).float()
+    x = torch.randn(2, 9, 3, 32, device=dev())
+    pos = torch.randint(0, 128, (2, 9, 1), device=dev(), dtype=torch.int32)
+    assert torch.equal(axial_rope(x, pos.to(dtype), table), axial_rope(x, pos, table))
+
+
+@pytest.mark.gpu
 def test_refusals():
     from worldattention_b200.rope import axial_rope
     x, table = torch.randn(2, 5, 3, 16, device=dev()), _table(9, 8, dev())

@@ -82,7 +82,8 @@ def axial_rope(x, positions: torch.Tensor, table: torch.Tensor, *, axes=None, in
     if positions.dtype != torch.int32:
         if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
             raise ValueError(f"positions must be integers, got {positions.dtype}")
-        positions = positions.clamp(-1, table.shape[0]).int()        # (what lies outside the table stays outside)
+        # what lies outside the table stays outside; clamped in 64 bits, since the types of 8 and 16 bits cannot hold the bounds
+        positions = positions.long().clamp(-1, min(table.shape[0], 2 ** 31 - 1)).int()
     if axes is None:
         pairs, n = table.shape[1], positions.shape[-1]
         if n not in (1, 3):
