@@ -370,6 +370,26 @@ def test_block_sparse_attention_carries_gradients(dtype, D):
 
 
 @pytest.mark.gpu
+def test_a_gradient_tells_of_an_earlier_launch_that_gave_up():
+    from worldattention_b200 import _lib
+    from worldattention_b200.hsa import selected_attention
+    g = torch.Generator(device=dev()).manual_seed(12)
+    q, k, v, dout = _inputs(g, 1, 70, 130, 4, 2, 128, torch.bfloat16)
+    index, num = _lists(g, 1, 4, 2, 3, 2, "full")
+    q.requires_grad_()
+    out = selected_attention(q, k, v, index, num, 64)
+    torch.cuda.synchronize()
+    word = _lib.status_word(dev())
+    word.fill_(455)                                   # as a launch would have left it; the engine's thread does not hold the interpreter lock
+    with pytest.raises(RuntimeError, match="wait site 455"):
+        out.backward(dout)
+    assert int(word) == 0
+    out = selected_attention(q, k, v, index, num, 64)
+    out.backward(dout)
+    assert bool(q.grad.any())
+
+
+@pytest.mark.gpu
 def test_refusals():
     from worldattention_b200.hsa import selected_attention
     g = torch.Generator(device=dev()).manual_seed(10)

@@ -161,6 +161,7 @@ volatile int *status_word(int dev) {
 }
 void raise_if_failed(int dev) {
     if (*status_word(dev) == 0) return;
+    pybind11::gil_scoped_acquire gil;       // (a gradient's call comes from a thread of the autograd engine)
     PyObject *r = PyObject_CallFunction(py_raise_if_failed, "i", dev);
     if (!r) throw PyFailure();
     Py_DECREF(r);
