@@ -178,6 +178,19 @@ def test_refusals():
             call()
 
 
+@pytest.mark.gpu
+def test_a_learned_table_is_refused_instead_of_left_without_its_gradient():
+    from worldattention_b200.rope import axial_rope
+    x, pos = torch.randn(2, 5, 3, 16, device=dev()), torch.zeros(5, 1, device=dev(), dtype=torch.int32)
+    real = torch.randn(9, 8, 2, device=dev(), requires_grad=True)
+    for table in (real, torch.view_as_complex(real), real.double()):
+        for y in (x, x.detach().requires_grad_()):
+            with pytest.raises(ValueError, match="gradient"):
+                axial_rope(y, pos, table)
+    with torch.no_grad():
+        axial_rope(x, pos, real)
+
+
 def test_no_cpu_path():
     from worldattention_b200.rope import axial_rope
     with pytest.raises(RuntimeError, match="CUDA"):

@@ -763,6 +763,7 @@ struct AxialNode : torch::autograd::Function<AxialNode> {
 };
 
 std::vector<Tensor> axial_turn(const std::vector<Tensor> &xs, const Tensor &pos, const Tensor &table, const std::vector<int64_t> &axes, bool interleaved, bool inverse) {
+    if (at::GradMode::is_enabled() && table.requires_grad()) fail(PyExc_ValueError, "the table has no gradient: it must not require one");
     if (at::GradMode::is_enabled() && std::any_of(xs.begin(), xs.end(), [](const Tensor &x) { return x.requires_grad(); }))
         return AxialNode::apply(pos, table, axes, interleaved, inverse, at::TensorList(xs));
     return axial_run(xs, pos, table, axes, interleaved, inverse);

@@ -69,7 +69,8 @@ def axial_rope(x, positions: torch.Tensor, table: torch.Tensor, *, axes=None, in
     in every call.  `axes` says how many consecutive pairs each axis turns (default: all of them for one axis, and for three
     the time, height and width bands of `causal_rope_apply`).  A pair is two neighbouring channels, or with `interleaved=False`
     channels i and i + pairs.  Channels behind `2 * pairs` are copied.  A token whose position on an axis lies outside the
-    table gets NaN in the pairs of that axis (nothing is read back to the host to refuse it).
+    table gets NaN in the pairs of that axis (nothing is read back to the host to refuse it).  The table has no gradient; one that
+    requires a gradient is refused.
 
     Float32 arithmetic, rounded once.  New tensors are returned, contiguous; a tuple for a tuple.
     """
