@@ -33,6 +33,37 @@ def test_moves_that_cannot_be_made_are_refused_before_any_launch():
         assert rc == _lib.WA_ERR_ARG and word in said, (dst, src, rc, said)
 
 
+def test_caches_packed_into_one_tensor_are_apart():
+    """By a brute-force look at every byte, on moves of a page to itself: nothing is launched."""
+    from worldattention_b200 import _lib
+    rng = random.Random(3)
+
+    def views(t, shape, names):             # [B, tokens] views of rows of 16 bytes within one contiguous tensor of these axes
+        strides, at = {}, 16
+        for n, size in reversed(list(zip(names, shape))):
+            strides[n] = at
+            at *= size
+        size = dict(zip(names, shape))
+        return [_lib.PageTensor(4096 + i * strides["n"], strides["b"], strides["t"], size["t"], 16, size["b"], 1) for i in range(size["n"])]
+    for names in (("b", "n", "t"), ("n", "b", "t"), ("b", "t", "n"), ("t", "b", "n"), ("t", "n", "b"), ("n", "t", "b")):
+        for shape in ((2, 2, 8), (3, 4, 1), (1, 2, 5), (70, 2, 3), (2, 1, 1), (5, 2, 80)):
+            rc, said = _refused(views(None, shape, names), [0], [0])
+            assert rc == 0, (names, shape, said)
+    agreed = 0
+    for _ in range(3000):
+        one = lambda: _lib.PageTensor(4096 + 16 * rng.randrange(40), 16 * rng.randrange(0, 25), 16 * rng.randrange(0, 25), rng.randrange(1, 4), 16 * rng.randrange(1, 4),  # noqa: E731
+                                      rng.randrange(1, 4), 1)
+        pair = [one(), one()]
+        taken = [sorted(x.ptr + b * x.batch_stride + t * x.token_stride + r for b in range(x.batch) for t in range(x.tokens) for r in range(x.row_bytes)) for x in pair]
+        whole = all(len(set(y)) == len(y) for y in taken)
+        rc, said = _refused(pair, [0], [0])
+        if not whole or set(taken[0]) & set(taken[1]):
+            assert rc == _lib.WA_ERR_ARG, [(x.ptr, x.batch_stride, x.token_stride, x.tokens, x.row_bytes, x.batch) for x in pair]
+        else:
+            agreed += rc == 0
+    assert agreed > 100
+
+
 def test_python_refuses_what_is_no_cuda_cache():
     from worldattention_b200.hkv import move_pages
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -198,3 +229,13 @@ def test_the_window_rolls_as_through_clones(frame, block, window, dropped):
             roll_window(cache, hsa, evict, keep)
         for n in cache:
             assert _same(cache[n], want[n]), n
+
+
+@pytest.mark.gpu
+def test_keys_and_values_of_a_sample_one_behind_the_other():
+    from worldattention_b200.hkv import move_pages
+    both = _filled((2, 2, 40, 3, 8), torch.bfloat16, 9)                       # [B, keys and values, tokens, H, D]
+    k, v = both[:, 0], both[:, 1]
+    want = [_want(x, [0, 1, 2], [1, 3, None], 10) for x in (k, v)]
+    move_pages((k, v), [0, 1, 2], [1, 3, None], 10)
+    assert all(_same(a, b) for a, b in zip((k, v), want))

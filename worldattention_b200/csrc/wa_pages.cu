@@ -219,26 +219,41 @@ static bool rows_apart(const wa_page_tensor &x) {
     return n_outer <= 1 || outer >= (n_inner > 1 ? (n_inner - 1) * inner : 0) + x.row_bytes;
 }
 
-// Tensors that lie apart, or whose rows alternate (keys and values of a token side by side, two samples of one cache).
-static bool tensors_apart(const wa_page_tensor *tensors, int n) {
-    struct Span { uintptr_t from, to; const wa_page_tensor *x; };
+// Tensors that lie apart, or whose rows alternate (keys and values of a token side by side, two samples of one cache).  `most` > 1: looked at
+// sample by sample where a tensor has no more (keys and values of a sample one behind the other).
+static bool tensors_apart(const wa_page_tensor *tensors, int n, int most) {
+    struct Span {
+        uintptr_t from, to;
+        int64_t row, step[2], count[2];
+    };
     std::vector<Span> spans;
     for (int t = 0; t < n; ++t) {
         const wa_page_tensor &x = tensors[t];
         if (x.tokens * x.row_bytes * x.batch == 0) continue;
-        const uintptr_t from = (uintptr_t)x.ptr;
-        spans.push_back({from, from + (uintptr_t)((x.batch - 1) * x.batch_stride + (x.tokens - 1) * x.token_stride + x.row_bytes), &x});
+        int64_t step[2] = {x.token_stride, x.batch_stride}, count[2] = {x.tokens, x.batch};
+        if (count[0] <= 1 || (count[1] > 1 && step[1] < step[0])) std::swap(step[0], step[1]), std::swap(count[0], count[1]);
+        // slices of the outer axis one by one (they do not overlap, see above), or all at once
+        const int64_t slices = count[1] <= most ? count[1] : 1, each = count[1] / slices;
+        for (int64_t i = 0; i < slices; ++i) {
+            const uintptr_t from = (uintptr_t)x.ptr + (uintptr_t)(slices > 1 ? i * step[1] : 0);
+            const uintptr_t bytes = (uintptr_t)((count[0] - 1) * step[0] + (each > 1 ? (each - 1) * step[1] : 0) + x.row_bytes);
+            spans.push_back({from, from + bytes, x.row_bytes, {step[0], step[1]}, {count[0], each}});
+        }
     }
     std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
     for (size_t i = 0; i < spans.size(); ++i)
         for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to; ++j) {
-            const wa_page_tensor &a = *spans[i].x, &b = *spans[j].x;
-            const int64_t step = a.tokens > 1 ? a.token_stride : b.token_stride;
-            if (step <= 0 || (a.tokens > 1 && a.token_stride != step) || (b.tokens > 1 && b.token_stride != step) || (a.batch > 1 && a.batch_stride % step) ||
-                (b.batch > 1 && b.batch_stride % step))
-                return false;
-            const int64_t off = (int64_t)((spans[j].from - spans[i].from) % (uintptr_t)step);
-            if (off < a.row_bytes || off + b.row_bytes > step) return false;
+            const Span &a = spans[i], &b = spans[j];
+            int64_t step = 0;                       // the smallest that is taken; all others are multiples of it, or the two count as one
+            for (const Span *x : {&a, &b})
+                for (int k = 0; k < 2; ++k)
+                    if (x->count[k] > 1 && (step == 0 || x->step[k] < step)) step = x->step[k];
+            if (step <= 0) return false;
+            for (const Span *x : {&a, &b})
+                for (int k = 0; k < 2; ++k)
+                    if (x->count[k] > 1 && x->step[k] % step) return false;
+            const int64_t off = (int64_t)((b.from - a.from) % (uintptr_t)step);
+            if (off < a.row || off + b.row > step) return false;
         }
     return true;
 }
@@ -260,7 +275,7 @@ static int move_pages(const wa_page_tensor *tensors, int n_tensors, const int32_
         whole = std::min(whole, x.tokens / x.page_tokens);
         bits |= (uintptr_t)x.ptr | (uintptr_t)x.batch_stride | (uintptr_t)x.token_stride | (uintptr_t)x.row_bytes;
     }
-    WA_REQUIRE(tensors_apart(tensors, n_tensors), WA_ERR_ARG, "%s: two tensors share memory", what);
+    WA_REQUIRE(tensors_apart(tensors, n_tensors, 1) || tensors_apart(tensors, n_tensors, 4096), WA_ERR_ARG, "%s: two tensors share memory", what);
     int most = 0;
     for (int i = 0; i < n; ++i) {
         WA_REQUIRE(dst[i] >= 0 && dst[i] < pages && src[i] >= -1 && src[i] < pages, WA_ERR_ARG, "%s: move %d of page %d to page %d leaves the %lld pages of a tensor",
