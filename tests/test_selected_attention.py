@@ -370,6 +370,37 @@ def test_block_sparse_attention_carries_gradients(dtype, D):
 
 
 @pytest.mark.gpu
+def test_a_step_is_not_captured_over_an_eager_graph_of_its_leaves():
+    from worldattention_b200.hsa import selected_attention
+    from worldattention_b200.rope import axial_rope
+    g = torch.Generator(device=dev()).manual_seed(13)
+    q, k, v, dout = _inputs(g, 1, 70, 130, 4, 4, 128, torch.bfloat16)
+    index, num = _lists(g, 1, 4, 2, 3, 2, "full")
+    pos, table = torch.zeros(70, 1, dtype=torch.int32, device=dev()), torch.ones(1, 64, 2, device=dev())
+    q.requires_grad_()
+    attend, turn = lambda q: selected_attention(q, k, v, index, num, 64), lambda q: axial_rope(q, pos, table)  # noqa: E731
+    for call in (attend, lambda q: attend(q.view(q.shape)), turn, lambda q: turn(q[:, :])):
+        for eager in (attend, turn, lambda q: q * 2):
+            alive = eager(q)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    call(q)
+            del alive
+    want = torch.autograd.grad(attend(q), q, dout)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = attend(q)                             # on a side stream it may be alive
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(q).backward(dout)
+    graph.replay()
+    assert torch.equal(q.grad, want)
+    del alive
+
+
+@pytest.mark.gpu
 def test_a_gradient_tells_of_an_earlier_launch_that_gave_up():
     from worldattention_b200 import _lib
     from worldattention_b200.hsa import selected_attention

@@ -630,6 +630,23 @@ std::vector<Tensor> selected_gradients(const Tensor &q, const Tensor &k, const T
     throw std::move(e);
 }
 
+// A captured backward pass ends at its leaves.  A leaf that an eager graph still leads to keeps that graph's stream; where that is the default
+// stream, the engine makes it wait for the captured one, which is no legal step of a capture and ends the process.  So such a call is
+// refused while that can still be an exception.  Leaves are looked for directly and through views and other nodes of one input.
+void refuse_captured_over_eager(at::TensorList xs) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    for (const Tensor &x : xs) {
+        if (!x.requires_grad()) continue;
+        std::shared_ptr<torch::autograd::Node> node = x.grad_fn() ? x.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(x);
+        while (node && node->num_outputs() == 1) node = node->next_edge(0).function;
+        if (!node || node->num_outputs() != 0) continue;
+        const auto stream = node->stream();
+        if (stream && *stream == at::cuda::getDefaultCUDAStream(x.device().index()).unwrap())
+            fail(PyExc_RuntimeError, "a training step cannot be captured while an eager graph of the same leaves, made on the default stream, is alive: drop its "
+                                     "results first, or make it on a side stream");
+    }
+}
+
 struct SelectedNode : torch::autograd::Function<SelectedNode> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index,
                                                   const Tensor &num, int64_t block, const std::optional<Tensor> &sizes) {
@@ -670,6 +687,7 @@ PyObject *selected_attention(PyObject *const *a, Py_ssize_t n) {
     const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
     Tensor out, lse;
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+        refuse_captured_over_eager({q, k, v});
         auto both = SelectedNode::apply(q, k, v, index, num, (int64_t)block, sizes ? std::optional<Tensor>(*sizes) : std::nullopt);
         out = std::move(both[0]);
         lse = std::move(both[1]);
@@ -764,8 +782,10 @@ struct AxialNode : torch::autograd::Function<AxialNode> {
 
 std::vector<Tensor> axial_turn(const std::vector<Tensor> &xs, const Tensor &pos, const Tensor &table, const std::vector<int64_t> &axes, bool interleaved, bool inverse) {
     if (at::GradMode::is_enabled() && table.requires_grad()) fail(PyExc_ValueError, "the table has no gradient: it must not require one");
-    if (at::GradMode::is_enabled() && std::any_of(xs.begin(), xs.end(), [](const Tensor &x) { return x.requires_grad(); }))
+    if (at::GradMode::is_enabled() && std::any_of(xs.begin(), xs.end(), [](const Tensor &x) { return x.requires_grad(); })) {
+        refuse_captured_over_eager(xs);
         return AxialNode::apply(pos, table, axes, interleaved, inverse, at::TensorList(xs));
+    }
     return axial_run(xs, pos, table, axes, interleaved, inverse);
 }
 
