@@ -370,6 +370,21 @@ def test_block_sparse_attention_carries_gradients(dtype, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D,block", [(torch.bfloat16, 128, 64), (torch.bfloat16, 128, 128), (torch.float32, 128, 64), (torch.float32, 48, 64)])
+def test_rows_that_list_only_blocks_without_a_key(dtype, D, block):
+    g = torch.Generator(device=dev()).manual_seed(14)
+    q, k, v, dout = _inputs(g, 1, 3 * block, 4 * block, 2, 2, D, dtype)
+    index = torch.tensor([[0, 0], [1, 0], [2, 3]], device=dev(), dtype=torch.int32).expand(1, 2, 3, 2).contiguous()
+    num = torch.full((1, 2, 3), 2, device=dev(), dtype=torch.int32)
+    sizes = torch.tensor([0, block, block // 2, 5], device=dev(), dtype=torch.int32)
+    want = _exact(q, k, v, _mask(index, num, block, 3 * block, 4 * block, sizes), dout)
+    dout[:, :block], dout[:, 1] = math.nan, math.inf          # the first rows see no key: they have no part in the gradients
+    got = _run(q, k, v, index, num, block, dout, block_sizes=sizes)
+    _check(got, want)
+    assert not bool(got["dq"][:, :block].any()) and not bool(got["dk"][:, :block].any()) and not bool(got["dv"][:, :block].any())
+
+
+@pytest.mark.gpu
 def test_a_step_is_not_captured_over_an_eager_graph_of_its_leaves():
     from worldattention_b200.hsa import selected_attention
     from worldattention_b200.rope import axial_rope

@@ -9,13 +9,13 @@
 namespace wa {
 
 // ---- lists ---------------------------------------------------------------------------------------
-// A warp per list: ids outside the key blocks and repeated ones are dropped, the others keep their order (a router's best block
-// first).  For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set
+// A warp per list: ids outside the key blocks, of blocks without a key and repeated ones are dropped, the others keep their order (a router's best
+// block first).  So a row without a key has an empty list, and whatever its dout holds meets no product.  For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set
 // atomically, which is the same in any order.
 constexpr int SL_WARPS = 8, SL_WORDS = 1024;   // lists of a CTA; words of a bitmap up to which it has so many (32 768 key blocks)
 
 struct SelectedLists {
-    const int32_t *index, *num;
+    const int32_t *index, *num, *sizes;                          // sizes: keys of each key block, or null
     long long lists;
     int Nq, Nkv, stride, H, group, words, row_words, warps;      // warps: lists of a CTA
     int32_t *clean, *clean_num;
@@ -36,7 +36,7 @@ __device__ __forceinline__ void selected_list(const SelectedLists &p, uint32_t *
     int at = 0;
     for (int c = 0; c < n; c += 32) {
         const int id = c + lane < n ? p.index[list * p.stride + c + lane] : -1;
-        const bool there = (unsigned)id < (unsigned)p.Nkv;
+        const bool there = (unsigned)id < (unsigned)p.Nkv && (!p.sizes || __ldg(p.sizes + id) > 0);
         const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1 - lane);
         const bool take = there && lane == __ffs(same) - 1 && !((bits[id >> 5] >> (id & 31)) & 1u);
         __syncwarp();
@@ -793,7 +793,7 @@ static int selected_order(const wa_selected_params *p, const SelectedPlan &w, bo
 
 static SelectedLists selected_lists(const wa_selected_params *p, const SelectedPlan &w, bool backward, char *ws) {
     SelectedLists l{};
-    l.index = p->index; l.num = p->num;
+    l.index = p->index; l.num = p->num; l.sizes = p->block_sizes;
     l.lists = (long long)p->B * p->H * w.Nq;
     l.Nq = w.Nq; l.Nkv = w.Nkv; l.stride = p->index_stride; l.H = p->H; l.group = w.group; l.words = w.words; l.row_words = w.row_words;
     l.warps = w.words <= SL_WORDS ? SL_WARPS : 1;
