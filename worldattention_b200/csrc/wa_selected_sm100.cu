@@ -177,7 +177,10 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
+    if (KEYS) {        // (dQ waits at its end: see wa_selected_backward)
+        pdl_wait();
+        pdl_release_dependents();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -518,6 +521,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     __syncthreads();
     tc_fence_after();
     if (warp == SB_WORKERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (!KEYS) pdl_wait();
 }
 
 // ---- blocks of 128 tokens ---------------------------------------------------------------------------
@@ -599,7 +603,10 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
+    if (KEYS) {        // (dQ waits at its end: see wa_selected_backward)
+        pdl_wait();
+        pdl_release_dependents();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -982,6 +989,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
     __syncthreads();
     tc_fence_after();
     if (warp == SB_WORKERS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (!KEYS) pdl_wait();
 }
 
 static bool aligned_view(const wa_tensor4 *t) {
