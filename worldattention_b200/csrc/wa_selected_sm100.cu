@@ -15,8 +15,9 @@
 // issues the loads, one issues the scores' products and one the sums'.  Tensor memory holds two steps' scores and the sums of two owned
 // tiles (2 x 128 + 2 x 128 columns).
 //
-// What bounds it: all four products read both operands from shared memory, and one of 128 x 64 x 16 takes 48 cycles of that for 32 of the tensor cores. The
-// two issuing warps are held by their products for 1350 and 1340 of the 2500 cycles of a step (dK/dV; sixteen workers, two steps in flight, hide the rest):
+// What bounds it: shared memory, 128 bytes a cycle.  All products read both operands there, one of 128 x 64 x 16 for 48 cycles (32 of the tensor
+// cores), so a step's take 1536 cycles of it (dQ: 1152), its tiles' arrival 512 and the factors' 256 (128): 2300 of the 2500 cycles that a step of
+// dK/dV lasts, 1790 of dQ's 2030.  Sixteen workers and two steps in flight hide the rest.
 // 32 760 tokens over themselves, 32 of 512 blocks a row, 12 heads: dK/dV 920 us, dQ 728.  One issuing warp for both took 1323 and 986, eight workers 998
 // and 819.  Roundings: P and dS to bf16 as factors of products, sums in float32, gradients once at the end.
 //
