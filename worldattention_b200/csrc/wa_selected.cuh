@@ -13,7 +13,7 @@ struct SelectedPlan {
     size_t rows;                               // backward: [B, Hkv, Nkv, group, row_words] which query blocks of which head list a key block
     size_t counters;                           // backward: zeroed together with `rows`, which it follows (see selected_sm100_backward)
     size_t stats;                              // backward: [B, H, selected_stats_rows] statistics of a query row, see selected_stat
-    size_t q_order, k_order;                   // backward: query blocks and key blocks, heaviest first (not in every call)
+    size_t q_order, k_order;                   // query blocks, and backward key blocks, heaviest first (not in every call)
     size_t tuned;                              // forward: what the tensor-core kernel needs
     size_t total;
 };

@@ -153,6 +153,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 
     if (threadIdx.x == 0) {
         bar->abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;
+        if (bar->abort_flag) report_failure(sink, 498);
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
             mbar_init(&bar->desc_empty[i], 2 + SB_WORKERS);       // the warps that issue products, and the workers
