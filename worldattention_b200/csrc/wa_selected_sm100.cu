@@ -11,8 +11,8 @@
 // way they are.  The met rows' lists: bits per key block, or the clean ids of a query block.  Every sum is made in one CTA in
 // the order of its list: no atomics, equal calls give equal bits; the price is that S and dP are computed in both launches.
 //
-// One persistent CTA of nineteen warps per SM: sixteen turn scores into P and dS and write finished sums out, one walks the lists and
-// issues the loads, one issues the scores' products and one the sums'.  Tensor memory holds two steps' scores and the sums of two owned
+// One persistent CTA of twenty warps per SM: sixteen turn scores into P and dS and sums into bf16, one walks the lists and issues the loads, one
+// issues the scores' products, one the sums' and one stores finished sums.  Tensor memory holds two steps' scores and the sums of two owned
 // tiles (2 x 128 + 2 x 128 columns).
 //
 // What bounds it: shared memory, 128 bytes a cycle.  All products read both operands there, one of 128 x 64 x 16 for 48 cycles (32 of the tensor
@@ -33,7 +33,7 @@ constexpr int SB_OWN_BYTES = SB_OWN * TILE * 2;         // 16 KB: [half of the c
 constexpr int SB_P_BYTES = TILE * SB_OWN * 2;           // 16 KB: [met row][64 owned rows]
 constexpr int SB_DESCS = 4;
 constexpr int SB_WORKERS = 16;                          // warps that make P and dS
-constexpr int SB_THREADS = (SB_WORKERS + 3) * 32;
+constexpr int SB_THREADS = (SB_WORKERS + 4) * 32;
 
 template <bool KEYS> struct SbRing {
     static constexpr int SLOTS = KEYS ? 4 : 5;          // met tiles (32 KB each): G1 and G2 of a step take one each
@@ -55,7 +55,7 @@ struct SbBarriers {
     uint64_t f_full, f_empty, stats_full[4];
     uint64_t full[5], empty[5];
     uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
-    uint64_t acc_full[2], acc_empty[2];
+    uint64_t acc_full[2], acc_empty[2], staged[2], stored[2];
     uint32_t tmem_base;
     int abort_flag;
     SbDesc desc[SB_DESCS];
@@ -141,7 +141,8 @@ struct SbList {
 template <bool KEYS>
 __global__ void __launch_bounds__(SB_THREADS, 1)
 selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
-                           const __grid_constant__ CUtensorMap tm_g2, const SbParams p) {
+                           const __grid_constant__ CUtensorMap tm_g2, const __grid_constant__ CUtensorMap tm_d1, const __grid_constant__ CUtensorMap tm_d2,
+                           const SbParams p) {
     using Ring = SbRing<KEYS>;
     constexpr int SLOTS = Ring::SLOTS;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -156,7 +157,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         if (bar->abort_flag) report_failure(sink, 498);
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
-            mbar_init(&bar->desc_empty[i], 2 + SB_WORKERS);       // the warps that issue products, and the workers
+            mbar_init(&bar->desc_empty[i], 3 + SB_WORKERS);       // the warps that issue products or store, and the workers
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
@@ -171,7 +172,9 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             mbar_init(&bar->p_full[i], SB_WORKERS / 2);
             mbar_init(&bar->p_free[i], 1);
             mbar_init(&bar->acc_full[i], 1);
-            mbar_init(&bar->acc_empty[i], SB_WORKERS);
+            mbar_init(&bar->acc_empty[i], SB_WORKERS / 2);
+            mbar_init(&bar->staged[i], SB_WORKERS / 2);
+            mbar_init(&bar->stored[i], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -371,57 +374,101 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-                if (KEYS) add(acc, s2, factors);
+                // (the factors were made from both scores: those have read their tiles too.  The tile that is loaded next goes free first)
                 add(acc + SB_OWN, s1, factors + (KEYS ? SB_P_BYTES : 0));
-                // (the factors were made from both scores: those have read their tiles too)
                 tc_commit(&bar->empty[s1]);
-                if (KEYS) tc_commit(&bar->empty[s2]);
+                if (KEYS) {
+                    add(acc, s2, factors);
+                    tc_commit(&bar->empty[s2]);
+                }
                 tc_commit(&bar->p_free[buf]);
                 if (flags & SB_LAST) tc_commit(&bar->acc_full[last]);
             }
             __syncwarp();
             ++steps;
         }
+    } else if (warp == SB_WORKERS + 3) {
+        // ================= stores =================
+        uint32_t descs = 0, steps = 0, done0 = 0, done1 = 0;       // done: sums that each group of workers has staged
+        bool ok = true;
+        auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
+        while (ok) {
+            const uint32_t d = descs % SB_DESCS;
+            ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 427);
+            if (!ok) break;
+            const int item = bar->desc[d].item, flags = bar->desc[d].flags;
+            warp_arrive(&bar->desc_empty[d]);
+            ++descs;
+            if (flags & SB_END) break;
+            if (flags & SB_EMPTY) continue;
+            const uint32_t buf = steps & 1u;
+            ++steps;
+            if (!(flags & SB_LAST)) continue;
+            ok = wait(&bar->staged[buf], (buf ? done1 : done0) & 1u, 428);
+            if (!ok) break;
+            if (buf) ++done1;
+            else ++done0;
+            if (lane == 0) {
+                const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H, b = head / heads, h = head - b * heads;
+                const uint8_t *from = p_s + buf * Ring::FACTORS * SB_P_BYTES;
+                // (rows behind the last one are clipped by the map)
+                if (KEYS) tma_store_5d(&tm_d1, from, 0, tile * SB_OWN, 0, h, b);
+                tma_store_5d(&tm_d2, from + (KEYS ? SB_P_BYTES : 0), 0, tile * SB_OWN, 0, h, b);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                mbar_arrive(&bar->stored[buf]);
+            }
+            __syncwarp();
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // all stores have landed before the block exits
+        __syncwarp();
     } else {
         // ================= P, dS and the finished sums =================
         // Two groups of eight warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
         // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and 32 of its 64 columns, 16 at a time.
-        // Finished sums are written by all warps, 16 columns each.
+        // The group that took an item's last step leaves the finished sums, as bf16, where that step's factors were, and a warp of its own stores them: it
+        // would only wait otherwise.  (Stored by all workers from registers, 64 bytes of a row at a time, the sums of an item held either group
+        // up for 3900 cycles, dQ's for 2100: one and a half steps.)
         const int quarter = warp & 3, half = (warp >> 2) & 1, group = warp >> 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
-        uint32_t descs = 0, steps = 0, items = 0;
-        int waiting = -1;                  // item whose sums are still to be written out
-        uint32_t written = 0;
+        uint32_t descs = 0, steps = 0, items = 0, staged = 0;       // staged: sums that this group has left
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
-        // one of an item's sums: channel `row` of 16 owned rows to memory, 64 consecutive bytes per warp and owned row
-        auto put = [&](int item, const uint32_t (&v)[16], __nv_bfloat16 *to, long long sb, long long sl, long long sh, float scale) {
+        // zeros for channel `row` of 16 owned rows
+        auto clear = [&](int item, __nv_bfloat16 *to, long long sb, long long sl, long long sh) {
             const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H;
             const int b = head / heads, h = head - b * heads, first = tile * SB_OWN + part * 16;
             const int n = min(16, (KEYS ? p.Lkv : p.Lq) - first);
             __nv_bfloat16 *at = to + b * sb + (long long)first * sl + h * sh + row;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                if (j < n) at[j * sl] = __float2bfloat16_rn(__uint_as_float(v[j]) * scale);
+                if (j < n) at[j * sl] = __float2bfloat16_rn(0.f);
         };
-        auto finish = [&]() {
-            const uint32_t a = written & 1u;
-            if (!wait(&bar->acc_full[a], (written >> 1) & 1u, 421)) return false;
+        // the sums of the item that ends with this group's step: [half of the channels][owned row][64 channels], pieces of 16 bytes swizzled by row
+        auto finish = [&](uint32_t buf) {
+            const uint32_t it = items - 1, a = it & 1u;
+            if (!wait(&bar->acc_full[a], (it >> 1) & 1u, 421)) return false;       // (the sums of this step have read its factors, too)
             tc_fence_after();
-            uint32_t v[16];
-            const uint32_t acc = tm_acc + a * 2 * SB_OWN + part * 16 + lane_addr;
-            if (KEYS) {
-                TMEM_LD16(acc, v);
+            uint8_t *to = p_s + buf * Ring::FACTORS * SB_P_BYTES + (row >> 6) * (SB_OWN_BYTES / 2) + (row & 7) * 2;
+            const int piece = (row & 63) >> 3;
+#pragma unroll 1
+            for (int g = 0; g < 2 * Ring::FACTORS; ++g) {
+                const int col = half * 32 + (g & 1) * 16, of = KEYS ? g >> 1 : 1;       // dV, then dK; or dQ
+                uint32_t v[16];
+                TMEM_LD16(tm_acc + (a * 2 + of) * SB_OWN + col + lane_addr, v);
                 tmem_wait_ld16(v);
-                put(waiting, v, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
+                if (g + 1 == 2 * Ring::FACTORS) {
+                    tc_fence_before();
+                    warp_arrive(&bar->acc_empty[a]);
+                }
+                const float scale = of ? p.scale : 1.0f;
+                uint8_t *at = to + (KEYS ? of * SB_P_BYTES : 0) + col * 128;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16 *>(at + j * 128 + ((piece ^ (j & 7)) << 4)) = __float2bfloat16_rn(__uint_as_float(v[j]) * scale);
             }
-            TMEM_LD16(acc + SB_OWN, v);
-            tmem_wait_ld16(v);
-            tc_fence_before();
-            warp_arrive(&bar->acc_empty[a]);
-            put(waiting, v, p.d2, p.d2b, p.d2l, p.d2h, p.scale);
-            ++written;
-            waiting = -1;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            warp_arrive(&bar->staged[buf]);
+            ++staged;
             return true;
         };
         while (ok) {
@@ -431,14 +478,10 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             const SbDesc desc = bar->desc[d];
             warp_arrive(&bar->desc_empty[d]);
             ++descs;
-            if (desc.flags & SB_END) {
-                if (waiting >= 0) finish();
-                break;
-            }
+            if (desc.flags & SB_END) break;
             if (desc.flags & SB_EMPTY) {
-                uint32_t zero[16] = {};
-                if (KEYS) put(desc.item, zero, p.d1, p.d1b, p.d1l, p.d1h, 1.0f);
-                put(desc.item, zero, p.d2, p.d2b, p.d2l, p.d2h, 1.0f);
+                if (KEYS) clear(desc.item, p.d1, p.d1b, p.d1l, p.d1h);
+                clear(desc.item, p.d2, p.d2b, p.d2l, p.d2h);
                 continue;
             }
             if (desc.flags & SB_FIRST) {
@@ -457,8 +500,9 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 }
                 // queries: rows that are no keys
                 const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
-                // the sums of step u - 2 have read the factors that lie here
+                // the sums of step u - 2 have read the factors that lie here, and a store what was left since
                 if (ok) ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
+                if (ok) ok = wait(&bar->stored[buf], (staged & 1u) ^ 1u, 429);
                 if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 426);
                 if (!ok) break;
                 tc_fence_after();
@@ -510,13 +554,9 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&bar->p_full[buf]);
-                if (waiting >= 0) ok = finish();
+                if (desc.flags & SB_LAST) ok = finish(buf);
             }
             ++steps;
-            if (desc.flags & SB_LAST) {
-                if (ok && waiting >= 0) ok = finish();       // (an item of one step, which the other group took)
-                waiting = desc.item;
-            }
         }
         tc_fence_before();
     }
@@ -555,12 +595,11 @@ struct SwBarriers {
     SbDesc desc[SB_DESCS];
 };
 constexpr int SW_SLOTS = 5;
-constexpr int SW_THREADS = SB_THREADS + 32;
 constexpr int SW_SMEM = (2 + SW_SLOTS) * TILE_BYTES + 3072;
 static_assert(sizeof(SwBarriers<true>) <= 3072 && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
 
 template <bool KEYS>
-__global__ void __launch_bounds__(SW_THREADS, 1)
+__global__ void __launch_bounds__(SB_THREADS, 1)
 selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __grid_constant__ CUtensorMap tm_f2, const __grid_constant__ CUtensorMap tm_g1,
                           const __grid_constant__ CUtensorMap tm_g2, const __grid_constant__ CUtensorMap tm_d1, const __grid_constant__ CUtensorMap tm_d2,
                           const SbParams p) {
@@ -1027,13 +1066,13 @@ static int launch_owned(const wa_selected_params *p, SbParams kp, cudaStream_t s
     const int sms = sm_count();
     const dim3 grid(kp.items < sms ? kp.items : sms);
     cudaError_t e;
+    CUtensorMap outs[2];
+    if ((rc = selected_sm100_map(&outs[0], KEYS ? &p->dv : &p->dq, p->B, Lf, Hf, "a gradient", OWN, 2))) return rc;
+    if ((rc = selected_sm100_map(&outs[1], KEYS ? &p->dk : &p->dq, p->B, Lf, Hf, "a gradient", OWN, 2))) return rc;
     if constexpr (BLK == TILE) {
-        CUtensorMap outs[2];
-        if ((rc = selected_sm100_map(&outs[0], KEYS ? &p->dv : &p->dq, p->B, Lf, Hf, "a gradient", TILE, 2))) return rc;
-        if ((rc = selected_sm100_map(&outs[1], KEYS ? &p->dk : &p->dq, p->B, Lf, Hf, "a gradient", TILE, 2))) return rc;
-        e = launch_dependent(selected_grad_wide_kernel<KEYS>, grid, dim3(SW_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], outs[0], outs[1], kp);
+        e = launch_dependent(selected_grad_wide_kernel<KEYS>, grid, dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], outs[0], outs[1], kp);
     } else {
-        e = launch_dependent(selected_grad_sm100_kernel<KEYS>, grid, dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], kp);
+        e = launch_dependent(selected_grad_sm100_kernel<KEYS>, grid, dim3(SB_THREADS), SMEM, stream, maps[0], maps[1], maps[2], maps[3], outs[0], outs[1], kp);
     }
     if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
