@@ -36,7 +36,12 @@ constexpr int SB_WORKERS = 16;                          // warps that make P and
 constexpr int SB_THREADS = (SB_WORKERS + 4) * 32;
 
 template <bool KEYS> struct SbRing {
-    static constexpr int SLOTS = KEYS ? 4 : 5;          // met tiles (32 KB each): G1 and G2 of a step take one each
+    // met tiles (32 KB each): G1 and G2 of a step take one each, of slots of their own.  dQ gives G2's back with the scores, and two are enough to load
+    // the next while this one is read; three of G1's then keep the loads off the way from one step's sums to the next but one's scores
+    // (five slots in turn, window: dQ 693 us)
+    static constexpr int SLOTS1 = KEYS ? 2 : 3, SLOTS2 = 2, SLOTS = SLOTS1 + SLOTS2;
+    static __device__ __forceinline__ uint32_t slot(int g, uint32_t step) { return g == 0 ? step % SLOTS1 : SLOTS1 + step % SLOTS2; }
+    static __device__ __forceinline__ uint32_t parity(int g, uint32_t step) { return (g == 0 ? step / SLOTS1 : step / SLOTS2) & 1u; }
     static constexpr int FACTORS = KEYS ? 2 : 1;        // P and dS, or dS alone
     static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + 2 * FACTORS * SB_P_BYTES + 3072;
 };
@@ -196,7 +201,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     if (warp == SB_WORKERS) {
         // ================= lists and loads =================
         const bool leader = elect_one();
-        uint32_t descs = 0, tiles = 0, items = 0, steps = 0;       // so many so far
+        uint32_t descs = 0, items = 0, steps = 0;       // so many so far
         bool ok = true;
         int at = blockIdx.x;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
@@ -263,8 +268,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     flags = 0;
 #pragma unroll
                     for (int g = 0; g < 2 && ok; ++g) {
-                        const uint32_t slot = tiles % SLOTS;
-                        ok = wait(&bar->empty[slot], ((tiles / SLOTS) & 1u) ^ 1u, 403);
+                        const uint32_t slot = Ring::slot(g, steps);
+                        ok = wait(&bar->empty[slot], Ring::parity(g, steps) ^ 1u, 403);
                         if (ok && leader) {
                             uint8_t *dst = g_s + slot * TILE_BYTES;
                             uint64_t *full = &bar->full[slot];
@@ -284,7 +289,6 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                             }
                         }
                         __syncwarp();
-                        ++tiles;
                     }
                     ++steps;
                 }
@@ -321,8 +325,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             const uint32_t buf = steps & 1u;
 #pragma unroll
             for (int g = 0; g < 2 && ok; ++g) {
-                const uint32_t slot = (2 * steps + g) % SLOTS;
-                ok = wait(&bar->full[slot], ((2 * steps + g) / SLOTS) & 1u, 413);
+                const uint32_t slot = Ring::slot(g, steps);
+                ok = wait(&bar->full[slot], Ring::parity(g, steps), 413);
                 if (ok && g == 0) ok = wait(&bar->s_free[buf], ((steps >> 1) & 1u) ^ 1u, 414);      // the scores of step u - 2 have been read
                 if (!ok) break;
                 tc_fence_after();
@@ -362,7 +366,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 ok = wait(&bar->acc_empty[items & 1u], ((items >> 1) & 1u) ^ 1u, 416);
                 ++items;
             }
-            const uint32_t buf = steps & 1u, s1 = (2 * steps) % SLOTS, s2 = (2 * steps + 1) % SLOTS, last = (items - 1) & 1u;
+            const uint32_t buf = steps & 1u, s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps), last = (items - 1) & 1u;
             const uint32_t acc = tm_acc + last * 2 * SB_OWN;
             uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES;
             auto add = [&](uint32_t to, uint32_t slot, const uint8_t *factor) {
@@ -489,12 +493,12 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 ++items;
             }
             if ((steps & 1u) == (uint32_t)group && ok) {
-                const uint32_t buf = steps & 1u, slot = (2 * steps) % SLOTS;
+                const uint32_t buf = steps & 1u;
                 // (-normaliser, -delta) of the met row, or of the owned rows: 64 of one, 64 of the other
                 const float *st = bar->stats + (KEYS ? buf * 2 * TILE + (row >> 6) * TILE + (row & 63) : ((items - 1) & 3u) * TILE);
                 float2 norm = make_float2(0.f, 0.f), delta = norm;
                 if (KEYS) {
-                    ok = wait(&bar->full[slot], ((2 * steps) / SLOTS) & 1u, 424);
+                    ok = wait(&bar->full[Ring::slot(0, steps)], Ring::parity(0, steps), 424);
                     norm = make_float2(st[0], st[0]);
                     delta = make_float2(st[SB_OWN], st[SB_OWN]);
                 }
