@@ -36,31 +36,31 @@ constexpr int SB_WORKERS = 16;                          // warps that make P and
 constexpr int SB_THREADS = (SB_WORKERS + 4) * 32;
 
 template <bool KEYS> struct SbRing {
-    // met tiles (32 KB each): G1 and G2 of a step take one each, of slots of their own.  dQ gives G2's back with the scores, and two are enough to load
-    // the next while this one is read; three of G1's then keep the loads off the way from one step's sums to the next but one's scores
-    // (five slots in turn, window: dQ 693 us)
-    static constexpr int SLOTS1 = KEYS ? 2 : 3, SLOTS2 = 2, SLOTS = SLOTS1 + SLOTS2;
+    // met tiles (32 KB each): G1 and G2 of a step take one each, of slots of their own.  G2 goes first (dQ: with the scores; keys: its sum is issued first),
+    // and two are enough to load the next while this one is read; three of G1's then keep the loads off the way from one step's sums to the next
+    // but one's scores (five slots in turn, window: dQ 693 us)
+    static constexpr int SLOTS1 = 3, SLOTS2 = 2, SLOTS = SLOTS1 + SLOTS2;
     static __device__ __forceinline__ uint32_t slot(int g, uint32_t step) { return g == 0 ? step % SLOTS1 : SLOTS1 + step % SLOTS2; }
     static __device__ __forceinline__ uint32_t parity(int g, uint32_t step) { return (g == 0 ? step / SLOTS1 : step / SLOTS2) & 1u; }
-    static constexpr int FACTORS = KEYS ? 2 : 1;        // P and dS, or dS alone
-    static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + 2 * FACTORS * SB_P_BYTES + 3072;
+    static constexpr int FACTORS = 2;                   // P and dS of one step, or dS of two
+    static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + FACTORS * SB_P_BYTES + 3072;
 };
 
 enum { SB_FIRST = 1, SB_LAST = 2, SB_EMPTY = 4, SB_END = 8 };
 struct SbDesc {
     int item, flags;
-    int real[2];         // queries' launch: real tokens of the met rows 0..63 and 64..127
+    int of[2];           // of the met rows 0..63 and 64..127: queries' launch: how many are tokens; keys': their place among the rows of `stats`
 };
 
 struct SbBarriers {
-    // 64 rows' (-normaliser) and their (-delta).  keys: of the met rows, [two steps][two]; queries: of the owned rows, [four items] -- when an
-    // item's are loaded, the warps may still be two items behind
+    // queries: 64 (-normaliser) and 64 (-delta) of the owned rows, [four items] -- when an item's are loaded, the warps may still be two items behind
     float stats[4 * TILE];
     uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
     uint64_t f_full, f_empty, stats_full[4];
     uint64_t full[5], empty[5];
     uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
-    uint64_t acc_full[2], acc_empty[2], staged[2], stored[2];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t staged[4];                // of four items: one may be staged while the one three before it is being stored, whose slot the next would need
     uint32_t tmem_base;
     int abort_flag;
     SbDesc desc[SB_DESCS];
@@ -151,8 +151,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
     using Ring = SbRing<KEYS>;
     constexpr int SLOTS = Ring::SLOTS;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *f_s = smem, *g_s = f_s + 2 * SB_OWN_BYTES, *p_s = g_s + SLOTS * TILE_BYTES;      // p_s: [two steps][P, dS]
-    SbBarriers *bar = reinterpret_cast<SbBarriers *>(p_s + 2 * Ring::FACTORS * SB_P_BYTES);
+    uint8_t *f_s = smem, *g_s = f_s + 2 * SB_OWN_BYTES, *p_s = g_s + SLOTS * TILE_BYTES;      // p_s: [P, dS], or [two steps] dS
+    SbBarriers *bar = reinterpret_cast<SbBarriers *>(p_s + Ring::FACTORS * SB_P_BYTES);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     volatile int *abort_flag = &bar->abort_flag;
     const FailSink sink{p.error_flag, p.status_mirror};
@@ -166,7 +166,10 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(&bar->stats_full[i], 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bar->stats_full[i], 1);
+            mbar_init(&bar->staged[i], SB_WORKERS / 2);
+        }
         for (int i = 0; i < SLOTS; ++i) {
             mbar_init(&bar->full[i], 1);
             mbar_init(&bar->empty[i], 1);
@@ -178,8 +181,6 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             mbar_init(&bar->p_free[i], 1);
             mbar_init(&bar->acc_full[i], 1);
             mbar_init(&bar->acc_empty[i], SB_WORKERS / 2);
-            mbar_init(&bar->staged[i], SB_WORKERS / 2);
-            mbar_init(&bar->stored[i], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -205,14 +206,14 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         bool ok = true;
         int at = blockIdx.x;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
-        auto tell = [&](int item, int flags, int real0, int real1) {
+        auto tell = [&](int item, int flags, int of0, int of1) {
             const uint32_t d = descs % SB_DESCS;
             if (!wait(&bar->desc_empty[d], ((descs / SB_DESCS) & 1u) ^ 1u, 401)) return false;
             if (leader) {
                 bar->desc[d].item = item;
                 bar->desc[d].flags = flags;
-                bar->desc[d].real[0] = real0;
-                bar->desc[d].real[1] = real1;
+                bar->desc[d].of[0] = of0;
+                bar->desc[d].of[1] = of1;
                 mbar_arrive(&bar->desc_full[d]);
             }
             __syncwarp();
@@ -259,12 +260,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     const int blocks = KEYS ? p.Nq : p.Nkv;
                     const int i0 = (int)(one & 0xffffffff), i1 = two < 0 ? blocks : (int)(two & 0xffffffff);
                     const int h0 = KEYS ? h * p.group + (int)(one >> 32) : hk, h1 = KEYS ? (two < 0 ? h0 : h * p.group + (int)(two >> 32)) : hk;
-                    int real0 = SB_OWN, real1 = SB_OWN;
-                    if (!KEYS) {
-                        real0 = min(p.Lkv - i0 * SB_OWN, SB_OWN);
-                        real1 = two < 0 ? 0 : min(p.Lkv - i1 * SB_OWN, SB_OWN);
-                    }
-                    ok = tell(item, flags, real0, real1);
+                    if (KEYS) ok = tell(item, flags, (int)((b * p.H + h0) * p.padded) + i0 * SB_OWN, (int)((b * p.H + h1) * p.padded) + i1 * SB_OWN);
+                    else ok = tell(item, flags, min(p.Lkv - i0 * SB_OWN, SB_OWN), two < 0 ? 0 : min(p.Lkv - i1 * SB_OWN, SB_OWN));
                     flags = 0;
 #pragma unroll
                     for (int g = 0; g < 2 && ok; ++g) {
@@ -274,19 +271,11 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                             uint8_t *dst = g_s + slot * TILE_BYTES;
                             uint64_t *full = &bar->full[slot];
                             const CUtensorMap *map = g == 0 ? &tm_g1 : &tm_g2;
-                            const bool with_stats = KEYS && g == 0;
-                            mbar_expect_tx(full, TILE_BYTES + (with_stats ? TILE * 8 : 0));
+                            mbar_expect_tx(full, TILE_BYTES);
                             tma_load_5d(dst, map, full, 0, i0 * SB_OWN, 0, h0, b);
                             tma_load_5d(dst + HALF_BYTES / 2, map, full, 0, i1 * SB_OWN, 0, h1, b);
                             tma_load_5d(dst + HALF_BYTES, map, full, 0, i0 * SB_OWN, 1, h0, b);
                             tma_load_5d(dst + HALF_BYTES + HALF_BYTES / 2, map, full, 0, i1 * SB_OWN, 1, h1, b);
-                            if (with_stats) {
-                                // (the statistics of step u - 2 have been read: its sums, which come after them, freed this slot)
-                                float *to = bar->stats + (steps & 1u) * 2 * TILE;
-                                const float *row = p.stats + ((long long)b * p.H) * p.padded * 2;
-                                bulk_load(to, row + (h0 * p.padded + (long long)i0 * SB_OWN) * 2, SB_OWN * 8, full);
-                                bulk_load(to + TILE, row + (h1 * p.padded + (long long)i1 * SB_OWN) * 2, SB_OWN * 8, full);
-                            }
                         }
                         __syncwarp();
                     }
@@ -368,7 +357,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             }
             const uint32_t buf = steps & 1u, s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps), last = (items - 1) & 1u;
             const uint32_t acc = tm_acc + last * 2 * SB_OWN;
-            uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES;
+            const uint8_t *factors = p_s + (KEYS ? 0 : buf * SB_P_BYTES);
             auto add = [&](uint32_t to, uint32_t slot, const uint8_t *factor) {
                 const uint64_t a = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024), f = smem_desc(smem_u32(factor), HALF_BYTES, 1024);
 #pragma unroll
@@ -378,13 +367,13 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-                // (the factors were made from both scores: those have read their tiles too.  The tile that is loaded next goes free first)
-                add(acc + SB_OWN, s1, factors + (KEYS ? SB_P_BYTES : 0));
-                tc_commit(&bar->empty[s1]);
+                // (the factors were made from both scores: those have read their tiles too)
                 if (KEYS) {
                     add(acc, s2, factors);
                     tc_commit(&bar->empty[s2]);
                 }
+                add(acc + SB_OWN, s1, factors + (KEYS ? SB_P_BYTES : 0));
+                if (!(flags & SB_LAST)) tc_commit(&bar->empty[s1]);       // (the item's sums are left in its last slot: it is free when they are stored)
                 tc_commit(&bar->p_free[buf]);
                 if (flags & SB_LAST) tc_commit(&bar->acc_full[last]);
             }
@@ -393,7 +382,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         }
     } else if (warp == SB_WORKERS + 3) {
         // ================= stores =================
-        uint32_t descs = 0, steps = 0, done0 = 0, done1 = 0;       // done: sums that each group of workers has staged
+        uint32_t descs = 0, steps = 0, items = 0;
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
         while (ok) {
@@ -405,22 +394,21 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             ++descs;
             if (flags & SB_END) break;
             if (flags & SB_EMPTY) continue;
-            const uint32_t buf = steps & 1u;
+            const uint32_t slot = Ring::slot(0, steps);
             ++steps;
             if (!(flags & SB_LAST)) continue;
-            ok = wait(&bar->staged[buf], (buf ? done1 : done0) & 1u, 428);
+            ok = wait(&bar->staged[items & 3u], (items >> 2) & 1u, 428);
             if (!ok) break;
-            if (buf) ++done1;
-            else ++done0;
+            ++items;
             if (lane == 0) {
                 const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H, b = head / heads, h = head - b * heads;
-                const uint8_t *from = p_s + buf * Ring::FACTORS * SB_P_BYTES;
+                const uint8_t *from = g_s + slot * TILE_BYTES;
                 // (rows behind the last one are clipped by the map)
                 if (KEYS) tma_store_5d(&tm_d1, from, 0, tile * SB_OWN, 0, h, b);
-                tma_store_5d(&tm_d2, from + (KEYS ? SB_P_BYTES : 0), 0, tile * SB_OWN, 0, h, b);
+                tma_store_5d(&tm_d2, from + (KEYS ? SB_OWN_BYTES : 0), 0, tile * SB_OWN, 0, h, b);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                mbar_arrive(&bar->stored[buf]);
+                mbar_arrive(&bar->empty[slot]);
             }
             __syncwarp();
         }
@@ -430,12 +418,12 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         // ================= P, dS and the finished sums =================
         // Two groups of eight warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
         // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and 32 of its 64 columns, 16 at a time.
-        // The group that took an item's last step leaves the finished sums, as bf16, where that step's factors were, and a warp of its own stores them: it
+        // The group that took an item's last step leaves the finished sums, as bf16, in that step's slot, and a warp of its own stores them: it
         // would only wait otherwise.  (Stored by all workers from registers, 64 bytes of a row at a time, the sums of an item held either group
         // up for 3900 cycles, dQ's for 2100: one and a half steps.)
         const int quarter = warp & 3, half = (warp >> 2) & 1, group = warp >> 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
-        uint32_t descs = 0, steps = 0, items = 0, staged = 0;       // staged: sums that this group has left
+        uint32_t descs = 0, steps = 0, items = 0;
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
         // zeros for channel `row` of 16 owned rows
@@ -449,30 +437,29 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 if (j < n) at[j * sl] = __float2bfloat16_rn(0.f);
         };
         // the sums of the item that ends with this group's step: [half of the channels][owned row][64 channels], pieces of 16 bytes swizzled by row
-        auto finish = [&](uint32_t buf) {
+        auto finish = [&](uint32_t slot) {
             const uint32_t it = items - 1, a = it & 1u;
-            if (!wait(&bar->acc_full[a], (it >> 1) & 1u, 421)) return false;       // (the sums of this step have read its factors, too)
+            if (!wait(&bar->acc_full[a], (it >> 1) & 1u, 421)) return false;       // (the sums of this step have read its tiles, too)
             tc_fence_after();
-            uint8_t *to = p_s + buf * Ring::FACTORS * SB_P_BYTES + (row >> 6) * (SB_OWN_BYTES / 2) + (row & 7) * 2;
+            uint8_t *to = g_s + slot * TILE_BYTES + (row >> 6) * (SB_OWN_BYTES / 2) + (row & 7) * 2;
             const int piece = (row & 63) >> 3;
 #pragma unroll 1
-            for (int g = 0; g < 2 * Ring::FACTORS; ++g) {
+            for (int g = 0; g < (KEYS ? 4 : 2); ++g) {
                 const int col = half * 32 + (g & 1) * 16, of = KEYS ? g >> 1 : 1;       // dV, then dK; or dQ
                 uint32_t v[16];
                 TMEM_LD16(tm_acc + (a * 2 + of) * SB_OWN + col + lane_addr, v);
                 tmem_wait_ld16(v);
-                if (g + 1 == 2 * Ring::FACTORS) {
+                if (g + 1 == (KEYS ? 4 : 2)) {
                     tc_fence_before();
                     warp_arrive(&bar->acc_empty[a]);
                 }
                 const float scale = of ? p.scale : 1.0f;
-                uint8_t *at = to + (KEYS ? of * SB_P_BYTES : 0) + col * 128;
+                uint8_t *at = to + (KEYS ? of * SB_OWN_BYTES : 0) + col * 128;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16 *>(at + j * 128 + ((piece ^ (j & 7)) << 4)) = __float2bfloat16_rn(__uint_as_float(v[j]) * scale);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(&bar->staged[buf]);
-            ++staged;
+            warp_arrive(&bar->staged[it & 3u]);
             return true;
         };
         while (ok) {
@@ -495,28 +482,34 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             if ((steps & 1u) == (uint32_t)group && ok) {
                 const uint32_t buf = steps & 1u;
                 // (-normaliser, -delta) of the met row, or of the owned rows: 64 of one, 64 of the other
-                const float *st = bar->stats + (KEYS ? buf * 2 * TILE + (row >> 6) * TILE + (row & 63) : ((items - 1) & 3u) * TILE);
+                const float *st = bar->stats + ((items - 1) & 3u) * TILE;
+                const int of = row < SB_OWN ? desc.of[0] : desc.of[1];
                 float2 norm = make_float2(0.f, 0.f), delta = norm;
-                if (KEYS) {
-                    ok = wait(&bar->full[Ring::slot(0, steps)], Ring::parity(0, steps), 424);
-                    norm = make_float2(st[0], st[0]);
-                    delta = make_float2(st[SB_OWN], st[SB_OWN]);
+                if (KEYS) {        // (on their way while the scores are)
+                    const float *at = p.stats + (long long)of * 2 + (row & 63);
+                    norm.x = norm.y = __ldg(at);
+                    delta.x = delta.y = __ldg(at + SB_OWN);
                 }
                 // queries: rows that are no keys
-                const bool real = KEYS || (row < SB_OWN ? row < desc.real[0] : row - SB_OWN < desc.real[1]);
-                // the sums of step u - 2 have read the factors that lie here, and a store what was left since
-                if (ok) ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
-                if (ok) ok = wait(&bar->stored[buf], (staged & 1u) ^ 1u, 429);
+                const bool real = KEYS || (row & 63) < of;
                 if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 426);
                 if (!ok) break;
                 tc_fence_after();
-                uint8_t *factors = p_s + buf * Ring::FACTORS * SB_P_BYTES + row * 128;
                 const uint32_t s_at = tm_s + buf * SB_OWN + lane_addr, dp_at = tm_dp + buf * SB_OWN + lane_addr;
                 const float2 c = make_float2(p.scale_log2, p.scale_log2);
-                uint32_t sv[16], dv[16];
-                // 16 columns: P and dS to shared memory, two 16-byte pieces of each, swizzled by row
-                auto turn = [&](const uint32_t (&x)[16], const uint32_t (&y)[16], int col) {
-                    uint32_t pw[8], dw[8];
+                uint32_t pw[2][8], dw[2][8];       // P (keys) and dS as pairs of bf16
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int col = half * 32 + n * 16;
+                    uint32_t x[16], y[16];
+                    TMEM_LD16(s_at + col, x);
+                    TMEM_LD16(dp_at + col, y);
+                    tmem_wait_ld16(x);
+                    tmem_wait_ld16(y);
+                    if (n == 1) {
+                        tc_fence_before();
+                        warp_arrive(&bar->s_free[buf]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         float4 n4 = make_float4(norm.x, norm.x, norm.x, norm.x), d4;
@@ -526,39 +519,33 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                         }
 #pragma unroll
                         for (int e = 0; e < 4; e += 2) {
-                            const float2 n = e == 0 ? make_float2(n4.x, n4.y) : make_float2(n4.z, n4.w);
+                            const float2 nn = e == 0 ? make_float2(n4.x, n4.y) : make_float2(n4.z, n4.w);
                             const float2 d = KEYS ? delta : e == 0 ? make_float2(d4.x, d4.y) : make_float2(d4.z, d4.w);
-                            const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[j + e]), __uint_as_float(x[j + e + 1])), c, n);
+                            const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[j + e]), __uint_as_float(x[j + e + 1])), c, nn);
                             float2 pr = make_float2(ex2(z.x), ex2(z.y));
                             float2 ds = __fmul2_rn(pr, __fadd2_rn(make_float2(__uint_as_float(y[j + e]), __uint_as_float(y[j + e + 1])), d));
                             if (!KEYS && !real) ds = make_float2(0.f, 0.f);
                             const __nv_bfloat162 hp = __floats2bfloat162_rn(pr.x, pr.y), hd = __floats2bfloat162_rn(ds.x, ds.y);
-                            if (KEYS) pw[(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
-                            dw[(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hd);
+                            if (KEYS) pw[n][(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hp);
+                            dw[n][(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hd);
                         }
                     }
+                }
+                // the sums of the step before (keys), or of the one before that, have read the factors that lie here.  (Keys: on a barrier for every other step,
+                // so that a group cannot mistake the end of the step before that for it: it has waited for the one before its last step.)
+                ok = KEYS ? wait(&bar->p_free[buf ^ 1u], ((steps - 1u) >> 1) & 1u, 425) : wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
+                if (!ok) break;
+                uint8_t *factors = p_s + (KEYS ? 0 : buf * SB_P_BYTES) + row * 128;
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint8_t *to = factors + ((((col >> 3) + q) ^ (row & 7)) << 4);
-                        if (KEYS) *reinterpret_cast<uint4 *>(to) = make_uint4(pw[4 * q], pw[4 * q + 1], pw[4 * q + 2], pw[4 * q + 3]);
-                        *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dw[4 * q], dw[4 * q + 1], dw[4 * q + 2], dw[4 * q + 3]);
-                    }
-                };
-#pragma unroll 1
-                for (int col = half * 32; col < half * 32 + 32; col += 16) {
-                    TMEM_LD16(s_at + col, sv);
-                    TMEM_LD16(dp_at + col, dv);
-                    tmem_wait_ld16(sv);
-                    tmem_wait_ld16(dv);
-                    if (col & 16) {
-                        tc_fence_before();
-                        warp_arrive(&bar->s_free[buf]);
-                    }
-                    turn(sv, dv, col);
+                for (int q = 0; q < 4; ++q) {      // 16-byte pieces, swizzled by row
+                    uint8_t *to = factors + (((half * 4 + q) ^ (row & 7)) << 4);
+                    const uint32_t *pq = &pw[q >> 1][4 * (q & 1)], *dq = &dw[q >> 1][4 * (q & 1)];
+                    if (KEYS) *reinterpret_cast<uint4 *>(to) = make_uint4(pq[0], pq[1], pq[2], pq[3]);
+                    *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dq[0], dq[1], dq[2], dq[3]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&bar->p_full[buf]);
-                if (desc.flags & SB_LAST) ok = finish(buf);
+                if (desc.flags & SB_LAST) ok = finish(Ring::slot(0, steps));
             }
             ++steps;
         }
@@ -671,7 +658,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (leader) {
                 bar->desc[d].item = item;
                 bar->desc[d].flags = flags;
-                bar->desc[d].real[0] = real;
+                bar->desc[d].of[0] = real;
                 mbar_arrive(&bar->desc_full[d]);
             }
             __syncwarp();
@@ -939,7 +926,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             const uint32_t d = descs % SB_DESCS;
             ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 461);
             if (!ok) break;
-            const int item = bar->desc[d].item, flags = bar->desc[d].flags, real = bar->desc[d].real[0];
+            const int item = bar->desc[d].item, flags = bar->desc[d].flags, real = bar->desc[d].of[0];
             warp_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
