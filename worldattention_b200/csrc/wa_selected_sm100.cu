@@ -61,6 +61,7 @@ struct SbBarriers {
     uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
     uint64_t acc_full[2], acc_empty[2];
     uint64_t staged[4];                // of four items: one may be staged while the one three before it is being stored, whose slot the next would need
+    uint64_t stored[2];                // queries: of each group
     uint32_t tmem_base;
     int abort_flag;
     SbDesc desc[SB_DESCS];
@@ -179,6 +180,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             mbar_init(&bar->s_free[i], SB_WORKERS / 2);
             mbar_init(&bar->p_full[i], SB_WORKERS / 2);
             mbar_init(&bar->p_free[i], 1);
+            mbar_init(&bar->stored[i], 1);
             mbar_init(&bar->acc_full[i], 1);
             mbar_init(&bar->acc_empty[i], SB_WORKERS / 2);
         }
@@ -373,7 +375,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     tc_commit(&bar->empty[s2]);
                 }
                 add(acc + SB_OWN, s1, factors + (KEYS ? SB_P_BYTES : 0));
-                if (!(flags & SB_LAST)) tc_commit(&bar->empty[s1]);       // (the item's sums are left in its last slot: it is free when they are stored)
+                if (!KEYS || !(flags & SB_LAST)) tc_commit(&bar->empty[s1]);       // (keys: the item's sums are left in its last slot, free when they are stored)
                 tc_commit(&bar->p_free[buf]);
                 if (flags & SB_LAST) tc_commit(&bar->acc_full[last]);
             }
@@ -394,7 +396,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             ++descs;
             if (flags & SB_END) break;
             if (flags & SB_EMPTY) continue;
-            const uint32_t slot = Ring::slot(0, steps);
+            const uint32_t buf = steps & 1u, slot = Ring::slot(0, steps);
             ++steps;
             if (!(flags & SB_LAST)) continue;
             ok = wait(&bar->staged[items & 3u], (items >> 2) & 1u, 428);
@@ -402,13 +404,13 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             ++items;
             if (lane == 0) {
                 const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H, b = head / heads, h = head - b * heads;
-                const uint8_t *from = g_s + slot * TILE_BYTES;
+                const uint8_t *from = KEYS ? g_s + slot * TILE_BYTES : p_s + buf * SB_P_BYTES;
                 // (rows behind the last one are clipped by the map)
                 if (KEYS) tma_store_5d(&tm_d1, from, 0, tile * SB_OWN, 0, h, b);
                 tma_store_5d(&tm_d2, from + (KEYS ? SB_OWN_BYTES : 0), 0, tile * SB_OWN, 0, h, b);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                mbar_arrive(&bar->empty[slot]);
+                mbar_arrive(KEYS ? &bar->empty[slot] : &bar->stored[buf]);
             }
             __syncwarp();
         }
@@ -418,12 +420,12 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         // ================= P, dS and the finished sums =================
         // Two groups of eight warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
         // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and 32 of its 64 columns, 16 at a time.
-        // The group that took an item's last step leaves the finished sums, as bf16, in that step's slot, and a warp of its own stores them: it
-        // would only wait otherwise.  (Stored by all workers from registers, 64 bytes of a row at a time, the sums of an item held either group
+        // The group that took an item's last step leaves the finished sums, as bf16, in that step's slot, or where its dS was, and a warp of its own stores
+        // them: it would only wait otherwise.  (dQ's in the slot, too, one of three: window 614 -> 632 us.)  (Stored by all workers from registers, 64 bytes of a row at a time, the sums of an item held either group
         // up for 3900 cycles, dQ's for 2100: one and a half steps.)
         const int quarter = warp & 3, half = (warp >> 2) & 1, group = warp >> 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
-        uint32_t descs = 0, steps = 0, items = 0;
+        uint32_t descs = 0, steps = 0, items = 0, staged = 0;       // staged: by this group
         bool ok = true;
         auto wait = [&](uint64_t *b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag, sink, code)); };
         // zeros for channel `row` of 16 owned rows
@@ -437,11 +439,11 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 if (j < n) at[j * sl] = __float2bfloat16_rn(0.f);
         };
         // the sums of the item that ends with this group's step: [half of the channels][owned row][64 channels], pieces of 16 bytes swizzled by row
-        auto finish = [&](uint32_t slot) {
+        auto finish = [&](uint8_t *to) {
             const uint32_t it = items - 1, a = it & 1u;
-            if (!wait(&bar->acc_full[a], (it >> 1) & 1u, 421)) return false;       // (the sums of this step have read its tiles, too)
+            if (!wait(&bar->acc_full[a], (it >> 1) & 1u, 421)) return false;       // (the sums of this step have read its tiles and factors, too)
             tc_fence_after();
-            uint8_t *to = g_s + slot * TILE_BYTES + (row >> 6) * (SB_OWN_BYTES / 2) + (row & 7) * 2;
+            to += (row >> 6) * (SB_OWN_BYTES / 2) + (row & 7) * 2;
             const int piece = (row & 63) >> 3;
 #pragma unroll 1
             for (int g = 0; g < (KEYS ? 4 : 2); ++g) {
@@ -460,6 +462,7 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&bar->staged[it & 3u]);
+            ++staged;
             return true;
         };
         while (ok) {
@@ -492,12 +495,25 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                 }
                 // queries: rows that are no keys
                 const bool real = KEYS || (row & 63) < of;
+                if (!KEYS) {       // the sums of step u - 2 have read the factors that lie here, and a store what was left since
+                    if (ok) ok = wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
+                    if (ok) ok = wait(&bar->stored[buf], (staged & 1u) ^ 1u, 424);
+                }
                 if (ok) ok = wait(&bar->s_full[buf], (steps >> 1) & 1u, 426);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t s_at = tm_s + buf * SB_OWN + lane_addr, dp_at = tm_dp + buf * SB_OWN + lane_addr;
                 const float2 c = make_float2(p.scale_log2, p.scale_log2);
                 uint32_t pw[2][8], dw[2][8];       // P (keys) and dS as pairs of bf16
+                uint8_t *factors = p_s + (KEYS ? 0 : buf * SB_P_BYTES) + row * 128;
+                auto leave = [&](int n) {          // 16 columns, 16-byte pieces swizzled by row
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint8_t *to = factors + (((half * 4 + 2 * n + q) ^ (row & 7)) << 4);
+                        if (KEYS) *reinterpret_cast<uint4 *>(to) = make_uint4(pw[n][4 * q], pw[n][4 * q + 1], pw[n][4 * q + 2], pw[n][4 * q + 3]);
+                        *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dw[n][4 * q], dw[n][4 * q + 1], dw[n][4 * q + 2], dw[n][4 * q + 3]);
+                    }
+                };
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int col = half * 32 + n * 16;
@@ -530,22 +546,19 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                             dw[n][(j + e) >> 1] = *reinterpret_cast<const uint32_t *>(&hd);
                         }
                     }
+                    if (!KEYS) leave(n);
                 }
-                // the sums of the step before (keys), or of the one before that, have read the factors that lie here.  (Keys: on a barrier for every other step,
-                // so that a group cannot mistake the end of the step before that for it: it has waited for the one before its last step.)
-                ok = KEYS ? wait(&bar->p_free[buf ^ 1u], ((steps - 1u) >> 1) & 1u, 425) : wait(&bar->p_free[buf], ((steps >> 1) & 1u) ^ 1u, 425);
-                if (!ok) break;
-                uint8_t *factors = p_s + (KEYS ? 0 : buf * SB_P_BYTES) + row * 128;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {      // 16-byte pieces, swizzled by row
-                    uint8_t *to = factors + (((half * 4 + q) ^ (row & 7)) << 4);
-                    const uint32_t *pq = &pw[q >> 1][4 * (q & 1)], *dq = &dw[q >> 1][4 * (q & 1)];
-                    if (KEYS) *reinterpret_cast<uint4 *>(to) = make_uint4(pq[0], pq[1], pq[2], pq[3]);
-                    *reinterpret_cast<uint4 *>(to + (KEYS ? SB_P_BYTES : 0)) = make_uint4(dq[0], dq[1], dq[2], dq[3]);
+                if (KEYS) {
+                    // the sums of the step before have read the factors that lie here.  (On a barrier for every other step, so that a group cannot mistake the
+                    // end of the step before that for it: it has waited for the one before its last step.)
+                    ok = wait(&bar->p_free[buf ^ 1u], ((steps - 1u) >> 1) & 1u, 425);
+                    if (!ok) break;
+                    leave(0);
+                    leave(1);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&bar->p_full[buf]);
-                if (desc.flags & SB_LAST) ok = finish(Ring::slot(0, steps));
+                if (desc.flags & SB_LAST) ok = finish(KEYS ? g_s + Ring::slot(0, steps) * TILE_BYTES : p_s + buf * SB_P_BYTES);
             }
             ++steps;
         }
