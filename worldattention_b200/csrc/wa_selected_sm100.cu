@@ -578,8 +578,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 // tiles, its reads (two tiles for 128 columns of a score product, one for a sum) are half those of the kernel above for the same
 // work, and a met tile is loaded half as often.  A warp writes its 32 columns of P as 16 words over the first half of its own 32 columns of S, so
 // that no warp waits for another's reads; the products take each K step's address from there.
-// Finished sums leave through the ring of tiles: at an item's end the loading warp gives the workers a slot for each, they leave it as bf16 there, and a
-// warp of its own stores it and gives the slot back.  (Stored by the workers themselves, 32 rows of 16 or 32 bytes at a time, an item's end took
+// Finished sums leave through the last step's slots, of which G1's and G2's are kept as above: the workers leave them there as bf16, and a warp of its own stores
+// them and gives the slots back.  (Stored by the workers themselves, 32 rows of 16 or 32 bytes at a time, an item's end took
 // 8000 cycles, three steps' time; lists of a chunk's keys are five steps long.)
 // What bounds it: dQ by the rate of the products (the issuing warps are held for 2400 of 2600 cycles a step, the forward kernel's rate), dK/dV by that
 // and by the ends of items.  4680 queries, 32 of 256 blocks a row, 12 heads: dK/dV 237 us, dQ 145 (299 and 217 before the two changes above).
@@ -598,8 +598,7 @@ struct SwBarriers {
     int abort_flag;
     SbDesc desc[SB_DESCS];
 };
-constexpr int SW_SLOTS = 5;
-constexpr int SW_SMEM = (2 + SW_SLOTS) * TILE_BYTES + 3072;
+constexpr int SW_SMEM = (2 + SbRing<true>::SLOTS) * TILE_BYTES + 3072;
 static_assert(sizeof(SwBarriers<true>) <= 3072 && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
 
 template <bool KEYS>
@@ -608,10 +607,10 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                           const __grid_constant__ CUtensorMap tm_g2, const __grid_constant__ CUtensorMap tm_d1, const __grid_constant__ CUtensorMap tm_d2,
                           const SbParams p) {
     constexpr int DPS = KEYS ? 1 : 2;                    // buffers of dP
-    constexpr int OUTS = KEYS ? 2 : 1;                   // sums of an item: slots that it takes at its end
+    using Ring = SbRing<KEYS>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *f_s = smem, *g_s = f_s + 2 * TILE_BYTES;
-    SwBarriers<KEYS> *bar = reinterpret_cast<SwBarriers<KEYS> *>(g_s + SW_SLOTS * TILE_BYTES);
+    SwBarriers<KEYS> *bar = reinterpret_cast<SwBarriers<KEYS> *>(g_s + Ring::SLOTS * TILE_BYTES);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     volatile int *abort_flag = &bar->abort_flag;
     const FailSink sink{p.error_flag, p.status_mirror};
@@ -626,7 +625,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
-        for (int i = 0; i < SW_SLOTS; ++i) {
+        for (int i = 0; i < Ring::SLOTS; ++i) {
             mbar_init(&bar->full[i], 1);
             mbar_init(&bar->empty[i], 1);
         }
@@ -662,7 +661,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
     if (warp == SB_WORKERS) {
         // ================= lists and loads =================
         const bool leader = elect_one();
-        uint32_t descs = 0, tiles = 0, items = 0, steps = 0;
+        uint32_t descs = 0, items = 0, steps = 0;
         bool ok = true;
         int at = blockIdx.x;
         auto tell = [&](int item, int flags, int real) {
@@ -693,19 +692,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             SbList<KEYS> list;
             list.begin(p, item, lane);
             long long ahead = list.next(lane);
-            auto grant = [&]() {      // slots for the item's sums
-#pragma unroll
-                for (int g = 0; g < OUTS && ok; ++g) {
-                    const uint32_t slot = tiles % SW_SLOTS;
-                    ok = wait(&bar->empty[slot], ((tiles / SW_SLOTS) & 1u) ^ 1u, 435);
-                    if (ok && leader) mbar_arrive(&bar->full[slot]);
-                    __syncwarp();
-                    ++tiles;
-                }
-            };
             if (ahead < 0) {
                 ok = tell(item, SB_EMPTY, 0);
-                grant();
             } else {
                 ok = wait(&bar->f_empty, (items & 1u) ^ 1u, 432);
                 if (ok && leader) {
@@ -724,14 +712,13 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     flags = 0;
 #pragma unroll
                     for (int g = 0; g < 2 && ok; ++g) {
-                        const uint32_t slot = tiles % SW_SLOTS;
-                        ok = wait(&bar->empty[slot], ((tiles / SW_SLOTS) & 1u) ^ 1u, 433);
+                        const uint32_t slot = Ring::slot(g, steps);
+                        ok = wait(&bar->empty[slot], Ring::parity(g, steps) ^ 1u, 433);
                         if (ok && leader) {
                             mbar_expect_tx(&bar->full[slot], TILE_BYTES);
                             tma_load_5d(g_s + slot * TILE_BYTES, g == 0 ? &tm_g1 : &tm_g2, &bar->full[slot], 0, i0 * TILE, 0, h0, b);
                         }
                         __syncwarp();
-                        ++tiles;
                     }
                     if (KEYS && ok) {      // (behind the tiles: it waits for the workers to be through with step u - 2, which the next tiles would as well)
                         const uint32_t s = steps & 1u;
@@ -744,7 +731,6 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     }
                     ++steps;
                 }
-                grant();
             }
             at = __shfl_sync(0xffffffffu, next_at, 0);
         }
@@ -756,7 +742,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         // ================= scores =================
         const bool leader = elect_one();
         constexpr uint32_t SCORE = instr_desc(false, TILE);
-        uint32_t descs = 0, items = 0, steps = 0, tiles = 0;
+        uint32_t descs = 0, items = 0, steps = 0;
         bool ok = true;
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -767,10 +753,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (leader) mbar_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
-            if (flags & SB_EMPTY) {
-                tiles += OUTS;
-                continue;
-            }
+            if (flags & SB_EMPTY) continue;
             if (flags & SB_FIRST) {
                 ok = wait(&bar->f_full, items & 1u, 442);
                 ++items;
@@ -778,8 +761,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             const uint32_t buf = steps % DPS;
 #pragma unroll
             for (int g = 0; g < 2 && ok; ++g) {
-                const uint32_t slot = (tiles + g) % SW_SLOTS;
-                ok = wait(&bar->full[slot], ((tiles + g) / SW_SLOTS) & 1u, 443);
+                const uint32_t slot = Ring::slot(g, steps);
+                ok = wait(&bar->full[slot], Ring::parity(g, steps), 443);
                 if (ok) ok = g == 0 ? wait(&bar->s_free, (steps & 1u) ^ 1u, 444) : wait(&bar->dp_free[buf], ((steps / DPS) & 1u) ^ 1u, 445);
                 if (!ok) break;
                 tc_fence_after();
@@ -798,13 +781,12 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                 __syncwarp();
             }
             ++steps;
-            tiles += 2 + (flags & SB_LAST ? OUTS : 0);
         }
     } else if (warp == SB_WORKERS + 2) {
         // ================= sums =================
         const bool leader = elect_one();
         constexpr uint32_t SUM = instr_desc(true, TILE);
-        uint32_t descs = 0, items = 0, steps = 0, tiles = 0;
+        uint32_t descs = 0, items = 0, steps = 0;
         bool ok = true;
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -815,16 +797,13 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (leader) mbar_arrive(&bar->desc_empty[d]);
             ++descs;
             if (flags & SB_END) break;
-            if (flags & SB_EMPTY) {
-                tiles += OUTS;
-                continue;
-            }
+            if (flags & SB_EMPTY) continue;
             const bool fresh = flags & SB_FIRST;
             if (fresh) {
                 ok = wait(&bar->acc_empty, (items & 1u) ^ 1u, 452);
                 ++items;
             }
-            const uint32_t buf = steps % DPS, s1 = tiles % SW_SLOTS, s2 = (tiles + 1) % SW_SLOTS;
+            const uint32_t buf = steps % DPS, s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps);
             auto add = [&](uint32_t to, uint32_t factor, uint32_t slot) {       // factor: 8 words a K step, two steps of each 32 columns
                 const uint64_t m = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024);
 #pragma unroll
@@ -833,7 +812,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             };
             if (KEYS) {
                 if (ok) ok = wait(&bar->p_full, steps & 1u, 453);
-                if (ok) ok = wait(&bar->full[s2], ((tiles + 1) / SW_SLOTS) & 1u, 455);       // (P needs its query rows only, not yet those of dout)
+                if (ok) ok = wait(&bar->full[s2], Ring::parity(1, steps), 455);       // (P needs its query rows only, not yet those of dout)
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
@@ -846,43 +825,43 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (!ok) break;
             tc_fence_after();
             if (leader) {
+                // (An item's sums are left in its last step's slots: those are free when they are stored.)
+                if (KEYS && !(flags & SB_LAST)) tc_commit(&bar->empty[s2]);      // free with dV's sum: dS was made from dP, which has read it too
                 add(tm_sum2, tm_dp + buf * TILE, s1);
                 tc_commit(&bar->dp_free[buf]);
-                tc_commit(&bar->empty[s1]);
-                if (KEYS) tc_commit(&bar->empty[s2]);      // (dS was made from dP, which has read it too)
-                if (flags & SB_LAST) tc_commit(&bar->acc_full);
+                if (!(flags & SB_LAST)) tc_commit(&bar->empty[s1]);
+                else tc_commit(&bar->acc_full);
             }
             __syncwarp();
             ++steps;
-            tiles += 2 + (flags & SB_LAST ? OUTS : 0);
         }
     } else if (warp == SB_WORKERS + 3) {
         // ================= stores =================
-        uint32_t descs = 0, tiles = 0, items = 0;
+        uint32_t descs = 0, steps = 0, items = 0;
         bool ok = true;
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
             ok = wait(&bar->desc_full[d], (descs / SB_DESCS) & 1u, 456);
             if (!ok) break;
             const int item = bar->desc[d].item, flags = bar->desc[d].flags;
-            if (!(flags & (SB_EMPTY | SB_END))) tiles += 2;
-            if (flags & (SB_LAST | SB_EMPTY)) {
+            if (flags & SB_LAST) {
                 ok = wait(&bar->staged[items % SB_DESCS], (items / SB_DESCS) & 1u, 457);
                 if (!ok) break;
                 if (lane == 0) {
                     const int tile = item % p.owned, head = item / p.owned, b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
-#pragma unroll
-                    for (int g = 0; g < OUTS; ++g)      // (rows behind the last one are clipped by the map)
-                        tma_store_5d(g + 1 < OUTS ? &tm_d1 : &tm_d2, g_s + (tiles + g) % SW_SLOTS * TILE_BYTES, 0, tile * TILE, 0, h, b);
+                    const uint32_t s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps);
+                    // (rows behind the last one are clipped by the map)
+                    if (KEYS) tma_store_5d(&tm_d1, g_s + s2 * TILE_BYTES, 0, tile * TILE, 0, h, b);
+                    tma_store_5d(&tm_d2, g_s + s1 * TILE_BYTES, 0, tile * TILE, 0, h, b);
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-#pragma unroll
-                    for (int g = 0; g < OUTS; ++g) mbar_arrive(&bar->empty[(tiles + g) % SW_SLOTS]);
+                    if (KEYS) mbar_arrive(&bar->empty[s2]);
+                    mbar_arrive(&bar->empty[s1]);
                 }
                 __syncwarp();
-                tiles += OUTS;
                 ++items;
             }
+            if (!(flags & (SB_EMPTY | SB_END))) ++steps;
             // only now: a ring of descriptions is then also a bound on the items that are staged and not yet stored
             warp_arrive(&bar->desc_empty[d]);
             ++descs;
@@ -895,30 +874,23 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         // a thread has one owned row (tensor-memory lane) and 32 met ones (columns)
         const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t at = (((uint32_t)(quarter * 32)) << 16) + part * 32;
-        uint32_t descs = 0, steps = 0, items = 0, tiles = 0, done = 0;      // done: items with and without steps
+        uint32_t descs = 0, steps = 0, items = 0;
         bool ok = true;
         float2 norm = make_float2(0.f, 0.f), delta = norm;        // queries: of the row
         const float2 c = make_float2(p.scale_log2, p.scale_log2);
-        // an item's sums (or zeros) to the slots that it was given: [half of the channels][row][64 channels], pieces of 16 bytes swizzled by row
-        auto finish = [&](bool some) {
+        // an item's sums to its last step's slots: [half of the channels][row][64 channels], pieces of 16 bytes swizzled by row
+        auto finish = [&]() {
 #pragma unroll 1
-            for (int g = 0; g < OUTS; ++g, ++tiles) {
-                const bool last = g + 1 == OUTS;
-                const uint32_t slot = tiles % SW_SLOTS;
+            for (int g = KEYS ? 1 : 0; g >= 0; --g) {      // dV to G2's slot, dK or dQ to G1's
                 uint32_t v[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0u;
-                if (some) {
-                    TMEM_LD32((last ? tm_sum2 : tm_sum1) + at, v);
-                    tmem_wait_ld32(v);
-                    if (last) {
-                        tc_fence_before();
-                        warp_arrive(&bar->acc_empty);
-                    }
+                TMEM_LD32((g == 0 ? tm_sum2 : tm_sum1) + at, v);
+                tmem_wait_ld32(v);
+                if (g == 0) {
+                    tc_fence_before();
+                    warp_arrive(&bar->acc_empty);
                 }
-                if (!wait(&bar->full[slot], (tiles / SW_SLOTS) & 1u, 466)) return false;
-                const float scale = last ? p.scale : 1.0f;
-                uint8_t *to = g_s + slot * TILE_BYTES + (part >> 1) * HALF_BYTES + row * 128;
+                const float scale = g == 0 ? p.scale : 1.0f;
+                uint8_t *to = g_s + Ring::slot(g, steps) * TILE_BYTES + (part >> 1) * HALF_BYTES + row * 128;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t w[4];
@@ -931,9 +903,15 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(&bar->staged[done % SB_DESCS]);
-            ++done;
-            return true;
+            warp_arrive(&bar->staged[(items - 1) % SB_DESCS]);
+        };
+        // zeros for a quarter of the channels of 32 of an item's rows
+        auto clear = [&](int item, __nv_bfloat16 *to, long long sb, long long sl, long long sh) {
+            const int tile = item % p.owned, head = item / p.owned, heads = KEYS ? p.Hkv : p.H, b = head / heads, l = tile * TILE + row;
+            if (l >= (KEYS ? p.Lkv : p.Lq)) return;
+            uint4 *out = reinterpret_cast<uint4 *>(to + b * sb + (long long)l * sl + (head - b * heads) * sh + part * 32);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) out[q] = make_uint4(0u, 0u, 0u, 0u);
         };
         while (ok) {
             const uint32_t d = descs % SB_DESCS;
@@ -944,7 +922,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             ++descs;
             if (flags & SB_END) break;
             if (flags & SB_EMPTY) {
-                ok = finish(false);
+                if (KEYS) clear(item, p.d1, p.d1b, p.d1l, p.d1h);
+                clear(item, p.d2, p.d2b, p.d2l, p.d2h);
                 continue;
             }
             if (!KEYS && (flags & SB_FIRST)) {
@@ -1019,15 +998,14 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             tc_fence_before();
             if (KEYS) warp_arrive(&bar->stats_empty[s2]);
             warp_arrive(&bar->ds_full[buf]);
-            ++steps;
-            tiles += 2;
             if (flags & SB_LAST) {
                 ok = wait(&bar->acc_full, items & 1u, 465);
                 ++items;
                 if (!ok) break;
                 tc_fence_after();
-                ok = finish(true);
+                finish();
             }
+            ++steps;
         }
         tc_fence_before();
     }
