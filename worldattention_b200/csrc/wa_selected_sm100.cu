@@ -593,7 +593,7 @@ struct SwBarriers {
     uint64_t full[5], empty[5];
     uint64_t s_full, s_free, p_full;
     uint64_t dp_full[2], dp_free[2], ds_full[2];
-    uint64_t acc_full, acc_empty, staged[SB_DESCS];
+    uint64_t acc_full[2], acc_empty[2], staged[2][SB_DESCS];   // of dK or dQ, and of dV
     uint32_t tmem_base;
     int abort_flag;
     SbDesc desc[SB_DESCS];
@@ -621,7 +621,8 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         for (int i = 0; i < SB_DESCS; ++i) {
             mbar_init(&bar->desc_full[i], 1);
             mbar_init(&bar->desc_empty[i], 3 + SB_WORKERS);
-            mbar_init(&bar->staged[i], SB_WORKERS);
+            mbar_init(&bar->staged[0][i], SB_WORKERS);
+            mbar_init(&bar->staged[1][i], SB_WORKERS);
         }
         mbar_init(&bar->f_full, 1);
         mbar_init(&bar->f_empty, 1);
@@ -638,9 +639,9 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             mbar_init(&bar->dp_full[i], 1);
             mbar_init(&bar->dp_free[i], 1);
             mbar_init(&bar->ds_full[i], SB_WORKERS);
+            mbar_init(&bar->acc_full[i], 1);
+            mbar_init(&bar->acc_empty[i], SB_WORKERS);
         }
-        mbar_init(&bar->acc_full, 1);
-        mbar_init(&bar->acc_empty, SB_WORKERS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == SB_WORKERS) {
@@ -799,10 +800,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (flags & SB_END) break;
             if (flags & SB_EMPTY) continue;
             const bool fresh = flags & SB_FIRST;
-            if (fresh) {
-                ok = wait(&bar->acc_empty, (items & 1u) ^ 1u, 452);
-                ++items;
-            }
+            if (fresh) ++items;
             const uint32_t buf = steps % DPS, s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps);
             auto add = [&](uint32_t to, uint32_t factor, uint32_t slot) {       // factor: 8 words a K step, two steps of each 32 columns
                 const uint64_t m = smem_desc(smem_u32(g_s + slot * TILE_BYTES), HALF_BYTES, 1024);
@@ -811,6 +809,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     mma_ts(to, factor + (kk >> 1) * 32 + (kk & 1) * 8, m + (uint64_t)((kk * 2048) >> 4), SUM, !(fresh && kk == 0));
             };
             if (KEYS) {
+                if (fresh) ok = wait(&bar->acc_empty[1], items & 1u, 452);
                 if (ok) ok = wait(&bar->p_full, steps & 1u, 453);
                 if (ok) ok = wait(&bar->full[s2], Ring::parity(1, steps), 455);       // (P needs its query rows only, not yet those of dout)
                 if (!ok) break;
@@ -818,9 +817,11 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                 if (leader) {
                     add(tm_sum1, tm_s, s2);
                     tc_commit(&bar->s_free);
+                    if (flags & SB_LAST) tc_commit(&bar->acc_full[1]);
                 }
                 __syncwarp();
             }
+            if (fresh && ok) ok = wait(&bar->acc_empty[0], items & 1u, 452);
             if (ok) ok = wait(&bar->ds_full[buf], (steps / DPS) & 1u, 454);
             if (!ok) break;
             tc_fence_after();
@@ -830,7 +831,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                 add(tm_sum2, tm_dp + buf * TILE, s1);
                 tc_commit(&bar->dp_free[buf]);
                 if (!(flags & SB_LAST)) tc_commit(&bar->empty[s1]);
-                else tc_commit(&bar->acc_full);
+                else tc_commit(&bar->acc_full[0]);
             }
             __syncwarp();
             ++steps;
@@ -845,20 +846,20 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             if (!ok) break;
             const int item = bar->desc[d].item, flags = bar->desc[d].flags;
             if (flags & SB_LAST) {
-                ok = wait(&bar->staged[items % SB_DESCS], (items / SB_DESCS) & 1u, 457);
-                if (!ok) break;
-                if (lane == 0) {
-                    const int tile = item % p.owned, head = item / p.owned, b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
-                    const uint32_t s1 = Ring::slot(0, steps), s2 = Ring::slot(1, steps);
-                    // (rows behind the last one are clipped by the map)
-                    if (KEYS) tma_store_5d(&tm_d1, g_s + s2 * TILE_BYTES, 0, tile * TILE, 0, h, b);
-                    tma_store_5d(&tm_d2, g_s + s1 * TILE_BYTES, 0, tile * TILE, 0, h, b);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    if (KEYS) mbar_arrive(&bar->empty[s2]);
-                    mbar_arrive(&bar->empty[s1]);
+                const int tile = item % p.owned, head = item / p.owned, b = head / (KEYS ? p.Hkv : p.H), h = head - b * (KEYS ? p.Hkv : p.H);
+#pragma unroll
+                for (int g = KEYS ? 1 : 0; g >= 0 && ok; --g) {
+                    ok = wait(&bar->staged[g][items % SB_DESCS], (items / SB_DESCS) & 1u, 457);
+                    if (ok && lane == 0) {
+                        const uint32_t slot = Ring::slot(g, steps);
+                        tma_store_5d(g == 1 ? &tm_d1 : &tm_d2, g_s + slot * TILE_BYTES, 0, tile * TILE, 0, h, b);       // (rows behind the last one are clipped by the map)
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        mbar_arrive(&bar->empty[slot]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (!ok) break;
                 ++items;
             }
             if (!(flags & (SB_EMPTY | SB_END))) ++steps;
@@ -881,14 +882,14 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
         // an item's sums to its last step's slots: [half of the channels][row][64 channels], pieces of 16 bytes swizzled by row
         auto finish = [&]() {
 #pragma unroll 1
-            for (int g = KEYS ? 1 : 0; g >= 0; --g) {      // dV to G2's slot, dK or dQ to G1's
+            for (int g = KEYS ? 1 : 0; g >= 0; --g) {      // dV to G2's slot, while dK's products run; dK or dQ to G1's
+                if (!wait(&bar->acc_full[g], items & 1u, 465)) return false;
+                tc_fence_after();
                 uint32_t v[32];
                 TMEM_LD32((g == 0 ? tm_sum2 : tm_sum1) + at, v);
                 tmem_wait_ld32(v);
-                if (g == 0) {
-                    tc_fence_before();
-                    warp_arrive(&bar->acc_empty);
-                }
+                tc_fence_before();
+                warp_arrive(&bar->acc_empty[g]);
                 const float scale = g == 0 ? p.scale : 1.0f;
                 uint8_t *to = g_s + Ring::slot(g, steps) * TILE_BYTES + (part >> 1) * HALF_BYTES + row * 128;
 #pragma unroll
@@ -901,9 +902,11 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     }
                     *reinterpret_cast<uint4 *>(to + ((((part & 1) * 4 + q) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                warp_arrive(&bar->staged[g][items % SB_DESCS]);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            warp_arrive(&bar->staged[(items - 1) % SB_DESCS]);
+            ++items;
+            return true;
         };
         // zeros for a quarter of the channels of 32 of an item's rows
         auto clear = [&](int item, __nv_bfloat16 *to, long long sb, long long sl, long long sh) {
@@ -998,13 +1001,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
             tc_fence_before();
             if (KEYS) warp_arrive(&bar->stats_empty[s2]);
             warp_arrive(&bar->ds_full[buf]);
-            if (flags & SB_LAST) {
-                ok = wait(&bar->acc_full, items & 1u, 465);
-                ++items;
-                if (!ok) break;
-                tc_fence_after();
-                finish();
-            }
+            if (flags & SB_LAST) ok = finish();
             ++steps;
         }
         tc_fence_before();
