@@ -15,11 +15,12 @@
 // issues the scores' products, one the sums' and one stores finished sums.  Tensor memory holds two steps' scores and the sums of two owned
 // tiles (2 x 128 + 2 x 128 columns).
 //
-// What bounds it: shared memory, 128 bytes a cycle.  All products read both operands there, one of 128 x 64 x 16 for 48 cycles (32 of the tensor
-// cores), so a step's take 1536 cycles of it (dQ: 1152), its tiles' arrival 512 and the factors' 256 (128): 2300 of the 2500 cycles that a step of
-// dK/dV lasts, 1790 of dQ's 2030.  Sixteen workers and two steps in flight hide the rest.
-// 32 760 tokens over themselves, 32 of 512 blocks a row, 12 heads: dK/dV 920 us, dQ 728.  One issuing warp for both took 1323 and 986, eight workers 998
-// and 819.  Roundings: P and dS to bf16 as factors of products, sums in float32, gradients once at the end.
+// What bounds it: the tensor pipe, and how long a step takes from load to sum.  A product of 128 x 64 x 16 keeps the pipe for 48 cycles (32 would do, but both
+// operands come from shared memory), a step's for 1536 (dQ: 1152) of the 2080 (1600) that it lasts: 72 % of the time.  Two steps are in flight, and each is
+// a chain of a tile's arrival (1100), the scores (770), P and dS (1100) and the sums.
+// 32 760 tokens over themselves, 32 of 512 blocks a row, 12 heads: dK/dV 805 us, dQ 610.  One issuing warp for both took 1323 and 986, eight workers 998
+// and 819, five slots in turn and sums stored by the workers 920 and 708.  Tried since: a second loading warp 809
+// and 628, owned tiles loaded one by one 815 and 643, the next item's list read ahead 843 and 602.  Roundings: P and dS to bf16 as factors of products, sums in float32, gradients once at the end.
 //
 // Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
 #include "wa_selected.cuh"
@@ -581,8 +582,9 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
 // Finished sums leave through the last step's slots, of which G1's and G2's are kept as above: the workers leave them there as bf16, and a warp of its own stores
 // them and gives the slots back.  (Stored by the workers themselves, 32 rows of 16 or 32 bytes at a time, an item's end took
 // 8000 cycles, three steps' time; lists of a chunk's keys are five steps long.)
-// What bounds it: dQ by the rate of the products (the issuing warps are held for 2400 of 2600 cycles a step, the forward kernel's rate), dK/dV by that
-// and by the ends of items.  4680 queries, 32 of 256 blocks a row, 12 heads: dK/dV 237 us, dQ 145 (299 and 217 before the two changes above).
+// What bounds it: as above; the tensor pipe is busy 66 % of the time for dQ, and 50 % for dK/dV, whose items are short (five steps): each ends with a
+// chain of sums, reads, stores and the next one's tiles.  4680 queries, 32 of 256 blocks a row, 12 heads: dK/dV 230 us, dQ 145 (131 behind the other; 299
+// and 217 before the two changes above).  Tried: an item's sums left in the next item's first step 255 us.
 // Tensor memory: S, dP, dV and dK; or S, two of dP, and dQ.  Scores of step u + 1 follow as soon as their columns are free: behind the sum that
 // read P or dS, or, for dQ's S, behind the workers' reads.
 template <bool KEYS>
