@@ -33,6 +33,7 @@ constexpr int SB_OWN = 64;                              // owned rows of an item
 constexpr int SB_OWN_BYTES = SB_OWN * TILE * 2;         // 16 KB: [half of the channels][row][64 channels]
 constexpr int SB_P_BYTES = TILE * SB_OWN * 2;           // 16 KB: [met row][64 owned rows]
 constexpr int SB_DESCS = 4;
+constexpr int SB_BARRIER_BYTES = 3 * 1024;
 constexpr int SB_WORKERS = 16;                          // warps that make P and dS
 constexpr int SB_THREADS = (SB_WORKERS + 4) * 32;
 
@@ -44,7 +45,7 @@ template <bool KEYS> struct SbRing {
     static __device__ __forceinline__ uint32_t slot(int g, uint32_t step) { return g == 0 ? step % SLOTS1 : SLOTS1 + step % SLOTS2; }
     static __device__ __forceinline__ uint32_t parity(int g, uint32_t step) { return (g == 0 ? step / SLOTS1 : step / SLOTS2) & 1u; }
     static constexpr int FACTORS = 2;                   // P and dS of one step, or dS of two
-    static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + FACTORS * SB_P_BYTES + 3072;
+    static constexpr int SMEM = 2 * SB_OWN_BYTES + SLOTS * TILE_BYTES + FACTORS * SB_P_BYTES + SB_BARRIER_BYTES;
 };
 
 enum { SB_FIRST = 1, SB_LAST = 2, SB_EMPTY = 4, SB_END = 8 };
@@ -67,7 +68,7 @@ struct SbBarriers {
     int abort_flag;
     SbDesc desc[SB_DESCS];
 };
-static_assert(sizeof(SbBarriers) <= 3072, "barrier block exceeds its shared-memory budget");
+static_assert(sizeof(SbBarriers) <= SB_BARRIER_BYTES, "barrier block exceeds its shared-memory budget");
 static_assert(SbRing<true>::SMEM <= 227 * 1024 && SbRing<false>::SMEM <= 227 * 1024, "shared memory budget exceeded");
 
 struct SbParams {
@@ -600,8 +601,8 @@ struct SwBarriers {
     int abort_flag;
     SbDesc desc[SB_DESCS];
 };
-constexpr int SW_SMEM = (2 + SbRing<true>::SLOTS) * TILE_BYTES + 3072;
-static_assert(sizeof(SwBarriers<true>) <= 3072 && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
+constexpr int SW_SMEM = (2 + SbRing<true>::SLOTS) * TILE_BYTES + SB_BARRIER_BYTES;
+static_assert(sizeof(SwBarriers<true>) <= SB_BARRIER_BYTES && SW_SMEM <= 227 * 1024, "shared memory budget exceeded");
 
 template <bool KEYS>
 __global__ void __launch_bounds__(SB_THREADS, 1)
