@@ -1076,10 +1076,11 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 // `both` receives the number of common blocks (lower half) and the item's sparse tiles (upper half).  The CTA that finishes
 // last makes the work order from the latter (unless SchedJob::by_counts): what an item costs is its tiles, and two query blocks that
 // share their blocks have far fewer of them than their counts say.
+// `counts`, if any: lists are sets, an id that is no block or is named again does not count, and the lengths that are left go there.
 constexpr int PL_WARPS = 8;
 __global__ void __launch_bounds__(PL_WARPS * 32)
 pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__ num, int Nq, int Nkv, int stride, int q_items, int n_items,
-                  int32_t *__restrict__ lists, int32_t *both, int ctas, SchedJob job) {
+                  int32_t *__restrict__ lists, int32_t *both, int ctas, int32_t *__restrict__ counts, SchedJob job) {
     extern __shared__ uint32_t pl_smem[];
     __shared__ int hist[SCHED_BINS], warp_tot[32], last_cta;
     const int words = (Nkv + 31) >> 5, lane = threadIdx.x & 31;
@@ -1095,10 +1096,10 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
         auto id_of = [&](int side, int i) { return max(0, min(index[(row0 + side) * stride + i], Nkv - 1)); };
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-            n[side] = side == 0 || two ? max(0, min(num[row0 + side], Nkv)) : 0;
+            n[side] = side == 0 || two ? max(0, min(num[row0 + side], counts ? stride : Nkv)) : 0;
             for (int i = lane; i < n[side]; i += 32) {
-                const int id = id_of(side, i);
-                atomicOr(&bits[side][id >> 5], 1u << (id & 31));
+                const int id = counts ? index[(row0 + side) * stride + i] : id_of(side, i);
+                if ((unsigned)id < (unsigned)Nkv) atomicOr(&bits[side][id >> 5], 1u << (id & 31));
             }
         }
         __syncwarp();
@@ -1112,6 +1113,11 @@ pair_lists_kernel(const int32_t *__restrict__ index, const int32_t *__restrict__
             distinct[0] += __shfl_xor_sync(0xffffffffu, distinct[0], o);
             distinct[1] += __shfl_xor_sync(0xffffffffu, distinct[1], o);
             shared += __shfl_xor_sync(0xffffffffu, shared, o);
+        }
+        if (counts) {
+            n[0] = distinct[0];
+            n[1] = distinct[1];
+            if (lane < 1 + two) counts[row0 + lane] = lane == 0 ? n[0] : n[1];
         }
         const bool plain = distinct[0] != n[0] || distinct[1] != n[1];
         const int n_both = plain ? 0 : shared;
@@ -1390,7 +1396,7 @@ int hsa_sm100_launch(const wa_hsa_params *p, int Lc, const wa_tensor4 *kc, const
     if (pair) {
         const size_t smem = (size_t)PL_WARPS * 2 * ((Nkv + 31) / 32) * sizeof(uint32_t);   // at most 32 KB beside 17 KB for the order
         const cudaError_t e = launch_dependent(pair_lists_kernel, dim3(ceil_div(n_items, PL_WARPS)), dim3(PL_WARPS * 32), smem, stream, index, num, Nq,
-                                               Nkv, Nkv, q_items, n_items, lists, both, n_items < max_grid() ? n_items : max_grid(), job);
+                                               Nkv, Nkv, q_items, n_items, lists, both, n_items < max_grid() ? n_items : max_grid(), (int32_t *)nullptr, job);
         if (e != cudaSuccess) return fail((int)e, "wa_hsa_forward(pairs): %s", cudaGetErrorString(e));
         if ((rc = check_launch("wa_hsa_forward(pairs)"))) return rc;
         index = lists;
@@ -1503,7 +1509,9 @@ bool selected_sm100_tensors(const wa_selected_params *p) {
 bool selected_sm100_forward_supported(const wa_selected_params *p) { return selected_sm100_tensors(p) && sm100::view_ok(&p->out); }
 size_t selected_sm100_forward_bytes(const wa_selected_params *p) { return sm100::selected_ws(p).total; }
 
-int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, void *workspace, cudaStream_t stream) {
+bool selected_sm100_cleans(const wa_selected_params *p) { return sm100::selected_paired(p); }
+
+int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, int32_t *counts, void *workspace, cudaStream_t stream) {
     using namespace sm100;
     const char *what = "wa_selected_forward(tcgen05)";
     const SelectedWs w = selected_ws(p);
@@ -1543,10 +1551,11 @@ int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, co
         const size_t smem = (size_t)PL_WARPS * 2 * ((Nkv + 31) / 32) * sizeof(uint32_t);
         const cudaError_t e = launch_dependent(pair_lists_kernel, dim3(ceil_div(n_items, PL_WARPS)), dim3(PL_WARPS * 32), smem, stream, index, num, Nq, Nkv,
                                                p->index_stride, q_items, n_items, (int32_t *)(ws + w.lists), (int32_t *)(ws + w.both),
-                                               n_items < max_grid() ? n_items : max_grid(), job);
+                                               n_items < max_grid() ? n_items : max_grid(), counts, job);
         if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
         if ((rc = check_launch(what))) return rc;
         index = (const int32_t *)(ws + w.lists);
+        num = counts;
     }
     kp.B = p->B; kp.H = p->H; kp.Lq = p->Lq; kp.Lkv = p->Lkv; kp.Nq = Nq; kp.Nkv = Nkv;
     kp.n_items = n_items; kp.q_items = q_items; kp.blk = blk;

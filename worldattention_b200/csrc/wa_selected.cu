@@ -875,9 +875,11 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     WA_REQUIRE((uintptr_t)p->workspace % 256 == 0, WA_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", what);
     if (selected_few_rows(p)) return launch_few_rows(p, stream);
     char *ws = (char *)p->workspace;
+    int32_t *index = (int32_t *)(ws + w.index), *num = (int32_t *)(ws + w.num);
+    const bool tuned = selected_sm100_forward_supported(p);
+    if (tuned && selected_sm100_cleans(p)) return selected_sm100_forward(p, p->index, p->num, num, ws + w.tuned, stream);
     if ((rc = launch_lists(selected_lists(p, w, false, ws), stream, what))) return rc;
-    const int32_t *index = (const int32_t *)(ws + w.index), *num = (const int32_t *)(ws + w.num);
-    if (selected_sm100_forward_supported(p)) return selected_sm100_forward(p, index, num, ws + w.tuned, stream);
+    if (tuned) return selected_sm100_forward(p, index, num, nullptr, ws + w.tuned, stream);
     const bool ordered = selected_ordered(p, w);
     if (ordered && (rc = selected_order(p, w, false, ws, stream, what))) return rc;
     const int32_t *order = ordered ? (const int32_t *)(ws + w.q_order) : nullptr;

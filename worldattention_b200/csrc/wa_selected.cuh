@@ -29,7 +29,9 @@ __host__ __device__ inline long long selected_stat(long long row) { return (row 
 bool selected_sm100_tensors(const wa_selected_params *p);                 // q, k, v, blocks and device
 bool selected_sm100_forward_supported(const wa_selected_params *p);
 size_t selected_sm100_forward_bytes(const wa_selected_params *p);
-int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, void *workspace, cudaStream_t stream);
+bool selected_sm100_cleans(const wa_selected_params *p);                  // the call's own lists will do, which are cleaned on the way to lists of pairs
+// `counts` [B, H, Nq]: lengths of those
+int selected_sm100_forward(const wa_selected_params *p, const int32_t *index, const int32_t *num, int32_t *counts, void *workspace, cudaStream_t stream);
 // a [B, L, H, 128] view as a map of boxes of `rows` tokens and one or both halves of the channels
 int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int H, const char *name, int rows, int halves);
 // wa_selected_sm100.cu:
