@@ -470,6 +470,10 @@ selected_any_kernel(const SelectedAny p) {
     constexpr bool KEYS = WHAT == SG_KEYS, FORWARD = WHAT == SG_FORWARD;
     constexpr int W = 32 * CH, LD = W + 4, R = TF / 8, C = TG / 32, LP = TG + 4;      // R: owned rows of a warp, C: met rows of a lane
     constexpr int ST = TF > TG ? TF : TG;
+    // Two multiply-adds an instruction where a warp has eight rows: issue slots count beside shared memory there (12 heads of 1170 tokens, dK/dV 127 -> 118 us;
+    // eight of 1500, head_dim 64, dQ 158 -> 151, its forward 83 -> 79).  With fewer rows the chains get too long (64 queries, dQ 81 -> 85), and so they do
+    // in the forward of head_dim 128 (62 -> 65).
+    constexpr bool TWO = TF == 64 && (WHAT != SG_FORWARD || CH == 2);
     extern __shared__ __align__(16) float sg_smem_[];
     float *f1 = sg_smem_, *f2 = f1 + TF * LD, *met = FORWARD ? f2 : f2 + TF * LD;     // owned: q (and dout) or k, v; met: [two buffers][the other two]
     float *factors = met + 4 * TG * LD;                                                // P, then dS
@@ -584,6 +588,33 @@ selected_any_kernel(const SelectedAny p) {
 #pragma unroll
             for (int j = 0; j < C; ++j) s[i][j] = dp[i][j] = 0.f;
         const auto dots = [&](float (&acc)[R][C], const float *f, const float *g) {
+            if constexpr (TWO) {               // of even and of odd channels
+                float2 two[R][C];
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int j = 0; j < C; ++j) two[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
+                for (int d = 0; d < depth; d += 4) {
+                    float4 y[C];
+#pragma unroll
+                    for (int j = 0; j < C; ++j) y[j] = *reinterpret_cast<const float4 *>(g + (lane + 32 * j) * LD + d);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        const float4 x = *reinterpret_cast<const float4 *>(f + (warp * R + i) * LD + d);
+#pragma unroll
+                        for (int j = 0; j < C; ++j) {
+                            two[i][j] = __ffma2_rn(make_float2(x.x, x.y), make_float2(y[j].x, y[j].y), two[i][j]);
+                            two[i][j] = __ffma2_rn(make_float2(x.z, x.w), make_float2(y[j].z, y[j].w), two[i][j]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int j = 0; j < C; ++j) acc[i][j] = two[i][j].x + two[i][j].y;
+                return;
+            }
 #pragma unroll 2
             for (int d = 0; d < depth; d += 4) {
                 float4 y[C];
@@ -651,12 +682,25 @@ selected_any_kernel(const SelectedAny p) {
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     const float4 a = *reinterpret_cast<const float4 *>(mine + i * LP + g);
+                    if constexpr (TWO) {
 #pragma unroll
-                    for (int m = 0; m < CH; ++m) {
-                        acc[i][m] = fmaf(a.x, y[0][m], acc[i][m]);
-                        acc[i][m] = fmaf(a.y, y[1][m], acc[i][m]);
-                        acc[i][m] = fmaf(a.z, y[2][m], acc[i][m]);
-                        acc[i][m] = fmaf(a.w, y[3][m], acc[i][m]);
+                        for (int m = 0; m < CH; m += 2) {
+                            float2 t = make_float2(acc[i][m], acc[i][m + 1]);
+                            t = __ffma2_rn(make_float2(a.x, a.x), make_float2(y[0][m], y[0][m + 1]), t);
+                            t = __ffma2_rn(make_float2(a.y, a.y), make_float2(y[1][m], y[1][m + 1]), t);
+                            t = __ffma2_rn(make_float2(a.z, a.z), make_float2(y[2][m], y[2][m + 1]), t);
+                            t = __ffma2_rn(make_float2(a.w, a.w), make_float2(y[3][m], y[3][m + 1]), t);
+                            acc[i][m] = t.x;
+                            acc[i][m + 1] = t.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < CH; ++m) {
+                            acc[i][m] = fmaf(a.x, y[0][m], acc[i][m]);
+                            acc[i][m] = fmaf(a.y, y[1][m], acc[i][m]);
+                            acc[i][m] = fmaf(a.z, y[2][m], acc[i][m]);
+                            acc[i][m] = fmaf(a.w, y[3][m], acc[i][m]);
+                        }
                     }
                 }
             }
