@@ -262,6 +262,42 @@ def test_items_of_one_step_and_items_of_many(block, q_len, kv_len, S):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("block", [64, 128])
+def test_what_follows_the_gradients_sees_all_of_them(dtype, block):
+    """The second launch of the gradient is short here and begins before the first one's end: a copy behind it, on this stream, on another one or in a graph."""
+    from worldattention_b200.hsa import selected_attention
+    g = torch.Generator(device=dev()).manual_seed(15)
+    q, k, v, dout = _inputs(g, 1, 70, 20000, 6, 3, 128, dtype)
+    index, num = _lists(g, 1, 6, -(-70 // block), -(-20000 // block), -(-20000 // block), "full")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    side = torch.cuda.Stream()
+
+    def step():
+        grads = torch.autograd.grad(selected_attention(*leaves, index, num, block), leaves, dout)
+        return grads, [x.clone() for x in grads]
+    for _ in range(3):
+        grads, copies = step()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            far = [x.clone() for x in grads]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(grads, copies, far))
+    want = [x.clone() for x in grads]
+    del grads, copies, far
+    leaves = [x.detach().requires_grad_() for x in leaves]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads, copies = step()
+    for _ in range(2):
+        for x in (*grads, *copies):
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) and torch.equal(y, z) for x, y, z in zip(want, grads, copies))
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     from worldattention_b200.hsa import selected_attention
     g = torch.Generator(device=dev()).manual_seed(7)
