@@ -119,7 +119,8 @@ template <> struct ArVec<float> {
 
 // `INTER`: a pair is two neighbouring channels, and a lane's vector holds whole pairs.  Otherwise a pair is channels i and i + pairs,
 // and a lane takes the two vectors that hold its pairs' halves.  Channels behind the turned ones are copied.
-template <typename T, bool INTER>
+// `ALL`: of neighbouring pairs every one is turned, none has to be looked at (24 heads of 4680 tokens 12.6 -> 12.0 us).
+template <typename T, bool INTER, bool ALL>
 __global__ void __launch_bounds__(AR_WARPS * 32)
 axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
     using V = ArVec<T>;
@@ -160,7 +161,7 @@ axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
         if (INTER) {
 #pragma unroll
             for (int i = 0; i < TURNS; ++i) {
-                const bool turned = c * TURNS + i < p.pairs;
+                const bool turned = ALL || c * TURNS + i < p.pairs;
                 r[2 * i] = turned ? fmaf(x[2 * i], turn[i].x, -x[2 * i + 1] * turn[i].y) : x[2 * i];
                 r[2 * i + 1] = turned ? fmaf(x[2 * i], turn[i].y, x[2 * i + 1] * turn[i].x) : x[2 * i + 1];
             }
@@ -261,8 +262,11 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
     if (vec && B <= 65535 && groups <= 65535) {
         const int each = ar_groups(interleaved != 0);
         p.groups = (int)groups;
-        const auto kernel = dtype == WA_BF16 ? (interleaved ? axial_rope_vec_kernel<__nv_bfloat16, true> : axial_rope_vec_kernel<__nv_bfloat16, false>)
-                                             : (interleaved ? axial_rope_vec_kernel<float, true> : axial_rope_vec_kernel<float, false>);
+        const bool whole = 2 * pairs == D;
+        const auto kernel = dtype == WA_BF16 ? (!interleaved ? axial_rope_vec_kernel<__nv_bfloat16, false, true>
+                                                : whole ? axial_rope_vec_kernel<__nv_bfloat16, true, true> : axial_rope_vec_kernel<__nv_bfloat16, true, false>)
+                                             : (!interleaved ? axial_rope_vec_kernel<float, false, true>
+                                                : whole ? axial_rope_vec_kernel<float, true, true> : axial_rope_vec_kernel<float, true, false>);
         e = launch_dependent(kernel, dim3(ceil_div(L, AR_WARPS), (unsigned)((groups + each - 1) / each), B), dim3(AR_WARPS * 32), 0, (cudaStream_t)stream, p);
     } else {
         const long long want = (p.tokens * all_heads * (D - pairs) + 255) / 256, most = 32ll * sm_count();
