@@ -135,20 +135,29 @@ axial_rope_vec_kernel(const __grid_constant__ AxialRope p) {
     const T *src[AT_ONCE];
     T *dst[AT_ONCE];
     uint4 v[AT_ONCE], w[AT_ONCE];
+    int g = part * AT_ONCE, t = 0, h = 0;
+    const T *from = nullptr;
+    T *to = nullptr;
+    bool step = false;            // the next group is the next of the same tensor: its place is a step away
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
         src[u] = nullptr;
-        int g = part * AT_ONCE + u, t = 0;
-        if (g < p.groups) {
+        if (!step) {
             while (t < p.tensors - 1 && g >= p.groups_of[t]) g -= p.groups_of[t++];
-            const int h = g * at_once + sub;
-            if (sub < at_once && h < p.heads[t]) {
-                src[u] = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh + c * N;
-                dst[u] = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t] + c * N;
-                v[u] = *reinterpret_cast<const uint4 *>(src[u]);
-                if (!INTER) w[u] = *reinterpret_cast<const uint4 *>(src[u] + p.pairs);
-            }
+            h = g * at_once + sub;
+            from = (const T *)p.x[t].ptr + b * p.x[t].sb + l * p.x[t].sl + h * p.x[t].sh + c * N;
+            to = (T *)p.out[t] + b * p.ob[t] + l * p.ol[t] + h * p.oh[t] + c * N;
         }
+        if (sub < at_once && h < p.heads[t]) {
+            src[u] = from;
+            dst[u] = to;
+            v[u] = *reinterpret_cast<const uint4 *>(from);
+            if (!INTER) w[u] = *reinterpret_cast<const uint4 *>(from + p.pairs);
+        }
+        step = ++g < p.groups_of[t];
+        h += at_once;
+        from += at_once * p.x[t].sh;
+        to += at_once * p.oh[t];
     }
     const int32_t *pos = p.positions + b * p.psb + l * p.psl;
     float2 turn[TURNS];
