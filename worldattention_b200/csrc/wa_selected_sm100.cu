@@ -19,8 +19,9 @@
 // operands come from shared memory), a step's for 1536 (dQ: 1152) of the 2080 (1600) that it lasts: 72 % of the time.  Two steps are in flight, and each is
 // a chain of a tile's arrival (1100), the scores (770), P and dS (1100) and the sums.
 // 32 760 tokens over themselves, 32 of 512 blocks a row, 12 heads: dK/dV 805 us, dQ 610.  One issuing warp for both took 1323 and 986, eight workers 998
-// and 819, five slots in turn and sums stored by the workers 920 and 708.  Tried since: a second loading warp 809
-// and 628, owned tiles loaded one by one 815 and 643, the next item's list read ahead 843 and 602.  Roundings: P and dS to bf16 as factors of products, sums in float32, gradients once at the end.
+// and 819, five slots in turn and sums stored by the workers 920 and 708.  Tried since: a second loading warp 809 and 628, owned tiles loaded one by one 815
+// and 643, the next item's list read ahead 843 and 602.
+// Roundings: P and dS to bf16 as factors of products, as their other factors are; sums in float32; gradients once at the end.
 //
 // Every wait is bounded (about two seconds); on expiry a flag is raised, all roles leave, tensor memory is freed and the kernel returns.
 #include "wa_selected.cuh"
@@ -55,7 +56,8 @@ struct SbDesc {
 };
 
 struct SbBarriers {
-    // queries: 64 (-normaliser) and 64 (-delta) of the owned rows, [four items] -- when an item's are loaded, the warps may still be two items behind
+    // queries: 64 (-normaliser) and 64 (-delta) of the owned rows, [four items] -- when an item's are loaded, the warps may still be three items behind, but not
+    // four: the scores of the item before needed a slot that the sums of that one gave back
     float stats[4 * TILE];
     uint64_t desc_full[SB_DESCS], desc_empty[SB_DESCS];
     uint64_t f_full, f_empty, stats_full[4];
@@ -423,8 +425,8 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
         // Two groups of eight warps take the steps in turn: a step is a chain of waits, tensor-memory reads, exponentials and fences, longer than
         // its products take, and two of them overlap.  A thread has one met row (tensor-memory lane) and 32 of its 64 columns, 16 at a time.
         // The group that took an item's last step leaves the finished sums, as bf16, in that step's slot, or where its dS was, and a warp of its own stores
-        // them: it would only wait otherwise.  (dQ's in the slot, too, one of three: window 614 -> 632 us.)  (Stored by all workers from registers, 64 bytes of a row at a time, the sums of an item held either group
-        // up for 3900 cycles, dQ's for 2100: one and a half steps.)
+        // them: it would only wait otherwise.  (dQ's in the slot, too, one of three: window 614 -> 632 us.  Stored by all workers from registers, 64 bytes of
+        // a row at a time, the sums of an item held either group up for 3900 cycles, dQ's for 2100: one and a half steps.)
         const int quarter = warp & 3, half = (warp >> 2) & 1, group = warp >> 3, part = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lane_addr = ((uint32_t)(quarter * 32)) << 16;
         uint32_t descs = 0, steps = 0, items = 0, staged = 0;       // staged: by this group
