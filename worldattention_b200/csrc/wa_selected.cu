@@ -721,7 +721,7 @@ selected_any_kernel(const SelectedAny p) {
 #pragma unroll
             for (int u = 0; u < CH; ++u) {
                 const int d = sg_channel<CH>(lane, u);
-                if (d < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + d, acc[i][u]);
+                if (d < p.D) store_elem(to, p.dtype, b * sb + r * sl + h * sh + d, r < own_real ? acc[i][u] : 0.f);      // (tokens that are no keys: a met row's NaN times zero)
             }
         }
     };
