@@ -24,6 +24,7 @@ struct GenericAttnParams {
     long long osb, osl, osh;
     int H, Lq, Lkv, D;
     int kv_group = 1;   // query heads that share a key head
+    bool nan_lse = false;   // the normaliser of a row whose sum is not a number: that, not -inf (the gradient takes -inf for a row without a key)
     int q_block;    // query rows per routing block
     int q_tile;     // query rows per CTA (<= GA_QT, divides the work inside one routing block)
     int tiles_per_block;
@@ -162,7 +163,7 @@ generic_attention_kernel(GenericAttnParams p) {
             }
         }
         if (p.lse && lane == 0)
-            p.lse[((long long)b * p.H + h) * p.Lq + row] = l_i[r] > 0.f ? m_i[r] + logf(l_i[r]) : -INFINITY;
+            p.lse[((long long)b * p.H + h) * p.Lq + row] = l_i[r] > 0.f || (p.nan_lse && l_i[r] != 0.f) ? m_i[r] + logf(l_i[r]) : -INFINITY;
     }
 }
 
@@ -545,7 +546,7 @@ split_attention_kernel(GenericAttnParams p) {
                 *reinterpret_cast<float2 *>((float *)p.out + at + 8 * j) = make_float2(x, y);
             }
         }
-        if (p.lse && c2 == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l > 0.f ? m + logf(l) : -INFINITY;
+        if (p.lse && c2 == 0) p.lse[((long long)b * p.H + h) * p.Lq + row] = l > 0.f || (p.nan_lse && l != 0.f) ? m + logf(l) : -INFINITY;
     }
 }
 
@@ -892,7 +893,7 @@ using namespace wa;
 namespace wa {
 int block_sparse_run(const wa_tensor4 *q, const wa_tensor4 *k, const wa_tensor4 *v, const wa_tensor4 *out, int B, int H, int Lq, int Lkv, int D,
                      int block_size, const int32_t *index, const int32_t *num, int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
-                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream, int kv_group) {
+                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream, int kv_group, bool nan_lse) {
     const char *what = "wa_block_sparse_forward";
     int rc;
     if ((rc = check_view(q, what, "q")) || (rc = check_view(k, what, "k")) || (rc = check_view(v, what, "v")) ||
@@ -911,7 +912,7 @@ int block_sparse_run(const wa_tensor4 *q, const wa_tensor4 *k, const wa_tensor4 
     p.scale = (float)(1.0 / sqrt((double)D));
     p.lse = lse;
     p.order = order; p.ahead = ahead;
-    p.kv_group = kv_group;
+    p.kv_group = kv_group; p.nan_lse = nan_lse;
     return launch_generic_attention(p, B, ceil_div(Lq, block_size), stream, what);
 }
 
@@ -943,7 +944,7 @@ extern "C" int wa_block_sparse_forward(const wa_tensor4 *q, const wa_tensor4 *k,
                                        int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
                                        int round_output_bf16, float *lse, void *stream) {
     return block_sparse_run(q, k, v, out, B, H, Lq, Lkv, D, block_size, index, num, index_stride, block_sizes, round_inputs_bf16,
-                            round_output_bf16, lse, nullptr, false, (cudaStream_t)stream, 1);
+                            round_output_bf16, lse, nullptr, false, (cudaStream_t)stream, 1, false);
 }
 
 extern "C" int wa_linear_branch(const wa_tensor4 *q, const wa_tensor4 *k_coarse, const wa_tensor4 *v_coarse,

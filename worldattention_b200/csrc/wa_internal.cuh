@@ -236,7 +236,7 @@ int compress_sm100_launch(const wa_tensor4 *k, const wa_tensor4 *v, const wa_ten
 // writes and starts on what that leaves free, but completes only after it (head_dim 128; otherwise one after the other).
 int block_sparse_run(const wa_tensor4 *q, const wa_tensor4 *k, const wa_tensor4 *v, const wa_tensor4 *out, int B, int H, int Lq, int Lkv, int D,
                      int block_size, const int32_t *index, const int32_t *num, int index_stride, const int32_t *block_sizes, int round_inputs_bf16,
-                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream, int kv_group = 1);
+                     int round_output_bf16, float *lse, const int32_t *order, bool ahead, cudaStream_t stream, int kv_group = 1, bool nan_lse = false);
 int linear_run(const wa_tensor4 *q, const wa_tensor4 *k_coarse, const wa_tensor4 *v_coarse, const wa_tensor4 *out, int B, int H, int Lq, int Lc,
                int D, int round_output_bf16, float *lse, bool beside, cudaStream_t stream);
 

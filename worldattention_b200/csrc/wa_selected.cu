@@ -935,7 +935,7 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
         return run_any<SG_FORWARD>(g, p->B, stream, what);
     }
     return block_sparse_run(&p->q, &p->k, &p->v, &p->out, p->B, p->H, p->Lq, p->Lkv, p->D, p->block_size, index, num, p->index_stride, p->block_sizes, 0, 0,
-                            p->lse, order, false, stream, w.group);
+                            p->lse, order, false, stream, w.group, true);
 }
 
 extern "C" int wa_selected_backward(const wa_selected_params *p, void *stream_) {
