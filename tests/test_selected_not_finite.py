@@ -53,7 +53,7 @@ def _where(index, num, block, B, H, row_block):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,D,block,sizes", [(torch.float32, 128, 64, False), (torch.float32, 48, 16, False),
+@pytest.mark.parametrize("dtype,D,block,sizes", [(torch.bfloat16, 128, 64, False), (torch.bfloat16, 128, 128, False), (torch.float32, 128, 64, False), (torch.float32, 48, 16, False),
                                                  (torch.bfloat16, 128, 32, False), (torch.bfloat16, 128, 64, True), (torch.float32, 128, 64, True), (torch.bfloat16, 96, 64, True)])
 @pytest.mark.parametrize("Lq,H", [(1, 4), (8, 4), (9, 4), (333, 4), (333, 48)])
 @pytest.mark.parametrize("what", ["key nan", "key +inf", "value nan", "value inf", "query nan", "query inf", "dout nan"])

@@ -826,9 +826,12 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 // the first tile of the linear branch (above), the linear one in the combine. ----
                 lA = quad_sum(lA);
                 lB = quad_sum(lB);
-                const float invA = lA > 0.f ? 1.0f / lA : 0.f, invB = lB > 0.f ? 1.0f / lB : 0.f;
-                const float lsA = lA > 0.f ? (mA + log2f(lA)) * 0.6931471805599453f : -INFINITY;
-                const float lsB = lB > 0.f ? (mB + log2f(lB)) * 0.6931471805599453f : -INFINITY;
+                // SEL: a sum that is not a number stays one, in the result, which takes zeros where the quotient is zero, and in the normaliser, by
+                // which the gradient knows rows without a key.  (Else the accumulator, times a quotient of zero, shows it.)
+                const bool keyA = SEL ? lA != 0.f : lA > 0.f, keyB = SEL ? lB != 0.f : lB > 0.f;
+                const float invA = keyA ? 1.0f / lA : 0.f, invB = keyB ? 1.0f / lB : 0.f;
+                const float lsA = keyA ? (mA + log2f(lA)) * 0.6931471805599453f : -INFINITY;
+                const float lsB = keyB ? (mB + log2f(lB)) * 0.6931471805599453f : -INFINITY;
                 if (SEL) {
                     inv_linA = invA;
                     inv_linB = invB;
