@@ -56,7 +56,7 @@ def _where(index, num, block, B, H, row_block):
 @pytest.mark.parametrize("dtype,D,block,sizes", [(torch.bfloat16, 128, 64, False), (torch.bfloat16, 128, 128, False), (torch.float32, 128, 64, False), (torch.float32, 48, 16, False),
                                                  (torch.bfloat16, 128, 32, False), (torch.bfloat16, 128, 64, True), (torch.float32, 128, 64, True), (torch.bfloat16, 96, 64, True)])
 @pytest.mark.parametrize("Lq,H", [(1, 4), (8, 4), (9, 4), (333, 4), (333, 48)])
-@pytest.mark.parametrize("what", ["key nan", "key +inf", "value nan", "value inf", "query nan", "query inf", "dout nan"])
+@pytest.mark.parametrize("what", ["key nan", "key +inf", "key -inf", "value nan", "value inf", "query nan", "query inf", "dout nan"])
 def test_what_is_attended_to_and_no_number_shows(dtype, D, block, sizes, Lq, H, what):
     g = torch.Generator(device=dev()).manual_seed(block + Lq)
     Lkv, Hkv = 9 * block - 7, H // 2
@@ -88,3 +88,33 @@ def test_what_is_attended_to_and_no_number_shows(dtype, D, block, sizes, Lq, H, 
     want = _by_lists(q2, k2, v2, mask, dout2)
     assert kind == "dout" or not bool(torch.isfinite(want["out"]).all()) or what == "key -inf"
     _agree(_run(q2, k2, v2, index, num, block, dout2, **more), want, _exact(q, k, v, clean, dout))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scores_of_minus_infinity_before_finite_ones(dtype, block):
+    """Whole blocks whose scores are all -inf, first, last and in the middle of a list: the others are what is attended to.  A row that has nothing else is as
+    one without a key."""
+    g = torch.Generator(device=dev()).manual_seed(block)
+    Lq, Lkv, H = 4 * block + 3, 6 * block, 4
+    q, k, v, dout = _inputs(g, 1, Lq, Lkv, H, H, 128, dtype)
+    q[..., 5] = q[..., 5].abs() + 0.25
+    index = torch.tensor([[0, 2, 3], [2, 0, 3], [2, 3, 0], [0, 1, 0], [1, 0, 4]], dtype=torch.int32, device=dev()).expand(1, H, 5, 3).contiguous()
+    num = torch.tensor([3, 3, 3, 2, 1], dtype=torch.int32, device=dev()).expand(1, H, 5).contiguous()
+    mask = _mask(index, num, block, Lq, Lkv)
+    k2 = k.clone()
+    k2[:, :2 * block, :, 5] = -math.inf                        # blocks 0 and 1
+    clean = mask.clone()
+    clean[..., :2 * block] = False
+    want = _exact(q, k, v, clean, dout)
+    got = _run(q, k2, v, index, num, block, dout)
+    touched = mask[..., :2 * block].any(-1).transpose(1, 2)    # dS of zero times an infinity in the rows that list those keys
+    assert bool(torch.isnan(got["dq"][..., 5][touched & (want["lse"][0] > -math.inf).transpose(1, 2)]).all())
+    for x in (got["dq"], want["dq"][0], want["dq"][1]):
+        x[..., 5] = 0
+    for name, (value, bound) in want.items():
+        x = got[name].double()
+        assert torch.equal(torch.isfinite(x), torch.isfinite(value)), name
+        far = ((x - value).abs() - bound - 1e-30)[torch.isfinite(value)]
+        assert float(far.max()) <= 0, (name, float(far.max()))

@@ -711,6 +711,10 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                         }
                         // p = 2^(s*c - m), row sums, pack to bf16
                         float2 nmA = make_float2(-mA, -mA), nmB = make_float2(-mB, -mB);
+                        if (SEL) {      // only scores of -inf so far: probabilities of zero
+                            if (mA == -INFINITY) nmA = make_float2(0.f, 0.f);
+                            if (mB == -INFINITY) nmB = make_float2(0.f, 0.f);
+                        }
                         float2 accA = make_float2(0.f, 0.f), accB = make_float2(0.f, 0.f);
                         auto exp32 = [&](const uint32_t (&r)[16], uint32_t *pk, auto poly) {       // 32 columns of the row pair
                             exp_step<decltype(poly)::value>(r[0], r[1], r[2], r[3], sc, nmA, nmB, accA, accB, pk[0], pk[1]);
@@ -734,7 +738,7 @@ hsa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                             }
                         } else {
                             // A row that has seen no key yet and sees none here keeps sums of zero.
-                            const bool any_real = lim_lo > 0 || lim_hi > HALF;
+                            const bool any_real = SEL || lim_lo > 0 || lim_hi > HALF;      // (SEL: see above)
                             if (!any_real && mA == -INFINITY) nmA = make_float2(0.f, 0.f);
                             if (!any_real && mB == -INFINITY) nmB = make_float2(0.f, 0.f);
                             tmem_wait_ld16(lo);

@@ -557,6 +557,10 @@ selected_grad_sm100_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gr
                     // end of the step before that for it: it has waited for the one before its last step.)
                     ok = wait(&bar->p_free[buf ^ 1u], ((steps - 1u) >> 1) & 1u, 425);
                     if (!ok) break;
+                    if (__builtin_expect(norm.x == -INFINITY, 0)) {      // no query: its scores are no numbers where a key holds an infinity
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) pw[0][j] = pw[1][j] = dw[0][j] = dw[1][j] = 0u;
+                    }
                     leave(0);
                     leave(1);
                 }
@@ -714,7 +718,7 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     const int i0 = (int)(ahead & 0xffffffff), h0 = KEYS ? h * p.group + (int)(ahead >> 32) : hk;
                     ahead = list.next(lane);
                     if (ahead < 0) flags |= SB_LAST;
-                    ok = tell(item, flags, KEYS ? TILE : min(p.Lkv - i0 * TILE, TILE));
+                    ok = tell(item, flags, min((KEYS ? p.Lq : p.Lkv) - i0 * TILE, TILE));
                     flags = 0;
 #pragma unroll
                     for (int g = 0; g < 2 && ok; ++g) {
@@ -972,18 +976,19 @@ selected_grad_wide_kernel(const __grid_constant__ CUtensorMap tm_f1, const __gri
                     w[j] = *reinterpret_cast<const uint32_t *>(&x);
                 }
             };
+            if (real < TILE) {      // tokens that are none (the last block): a score of theirs is no number where the owned row holds an infinity
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (part * 32 + 2 * j >= real) pr[j].x = 0.f;
+                    if (part * 32 + 2 * j + 1 >= real) pr[j].y = 0.f;
+                }
+            }
             if (KEYS) {
                 pack();
                 TMEM_ST16(tm_s + at, w);
                 tmem_wait_st();
                 tc_fence_before();
                 warp_arrive(&bar->p_full);
-            } else if (real < TILE) {      // tokens that are no keys (the last block)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (part * 32 + 2 * j >= real) pr[j].x = 0.f;
-                    if (part * 32 + 2 * j + 1 >= real) pr[j].y = 0.f;
-                }
             }
             ok = wait(&bar->dp_full[buf], (steps / DPS) & 1u, 464);
             if (!ok) break;
