@@ -15,14 +15,13 @@
 // Page numbers and tensors travel as launch parameters: nothing is copied to the device, and the call can be captured.
 #include <algorithm>
 #include <new>
-#include <numeric>
 #include <vector>
 
 #include "wa_common.cuh"
+#include "wa_pages_plan.cuh"
 
 namespace wa {
 
-constexpr int PM_CLEAR = -1, PM_SAVED = -2, PM_SAVE = -3;      // sources that are no page: zeros, the kept piece; keep a piece of `dst`
 constexpr int PM_THREADS = 256, PM_PIECES = 4;                   // pieces of a thread, whose loads are in flight together
 
 struct PageTensor {
@@ -36,7 +35,7 @@ struct PageTensor {
 template <int TENSORS, int MOVES>
 struct PageMoves {
     PageTensor tensor[TENSORS];
-    int2 move[MOVES];                  // (destination, source)
+    PageMove move[MOVES];
     int part[MOVES + 1];               // first move of each part
     int tensors, last_of[TENSORS];     // last_of: first launch row behind each tensor's (samples of all tensors are the grid's z)
 };
@@ -68,86 +67,28 @@ move_pages_kernel(const __grid_constant__ PageMoves<TENSORS, MOVES> p) {
     int kept_rows = 0;
     const int end = p.part[blockIdx.y + 1];
     for (int i = p.part[blockIdx.y]; i < end; ++i) {
-        const int2 m = p.move[i];
-        const int page = m.y >= 0 ? m.y : m.x, mine = rows_of(page);
-        const bool load = m.y >= 0 || m.y == PM_SAVE;
+        const PageMove m = p.move[i];
+        const int page = m.from >= 0 ? m.from : m.to, mine = rows_of(page);
+        const bool load = m.from >= 0 || m.from == PM_SAVE;
         const char *src = base + (long long)page * x.page_stride;
         Piece v[PM_PIECES];
 #pragma unroll
         for (int u = 0; u < PM_PIECES; ++u) {
-            v[u] = m.y == PM_SAVED ? kept[u] : Piece{};
+            v[u] = m.from == PM_SAVED ? kept[u] : Piece{};
             if (load && row[u] < mine) v[u] = *reinterpret_cast<const Piece *>(src + at[u]);
         }
-        if (m.y == PM_SAVE) {
+        if (m.from == PM_SAVE) {
 #pragma unroll
             for (int u = 0; u < PM_PIECES; ++u) kept[u] = v[u];
             kept_rows = mine;
             continue;
         }
-        const int rows = min(m.y == PM_SAVED ? kept_rows : mine, rows_of(m.x));
-        char *dst = base + (long long)m.x * x.page_stride;
+        const int rows = min(m.from == PM_SAVED ? kept_rows : mine, rows_of(m.to));
+        char *dst = base + (long long)m.to * x.page_stride;
 #pragma unroll
         for (int u = 0; u < PM_PIECES; ++u)
             if (row[u] < rows) *reinterpret_cast<Piece *>(dst + at[u]) = v[u];
     }
-}
-
-struct PagePlan {
-    std::vector<int2> move;
-    std::vector<int> part, hole;       // of each move: its part, and the page that the kept piece may be put back to behind it (-1: none is kept)
-};
-
-// The order described above.  `pages`: one more than the largest page number.
-static PagePlan plan_moves(const int32_t *dst, const int32_t *src, int n, int pages) {
-    std::vector<int> op(pages, -1), readers(pages, 0), root(pages);
-    std::iota(root.begin(), root.end(), 0);
-    auto find = [&](int a) {
-        while (root[a] != a) a = root[a] = root[root[a]];
-        return a;
-    };
-    for (int i = 0; i < n; ++i)
-        if (dst[i] != src[i]) op[dst[i]] = i;
-    for (int i = 0; i < n; ++i)
-        if (dst[i] != src[i] && src[i] >= 0) {
-            ++readers[src[i]];
-            if (op[src[i]] >= 0) root[find(dst[i])] = find(src[i]);
-        }
-    PagePlan plan;
-    std::vector<char> done(n, 0);
-    auto emit = [&](int d, int s, int hole) {
-        plan.move.push_back(make_int2(d, s));
-        plan.part.push_back(find(d));
-        plan.hole.push_back(hole);
-    };
-    for (int i = 0; i < n; ++i) {              // from pages that nothing reads
-        int j = i;
-        while (j >= 0 && dst[j] != src[j] && !done[j] && readers[dst[j]] == 0) {
-            done[j] = 1;
-            emit(dst[j], src[j] < 0 ? PM_CLEAR : src[j], -1);
-            const int s = src[j];
-            j = s >= 0 && --readers[s] == 0 ? op[s] : -1;
-        }
-    }
-    for (int i = 0; i < n; ++i) {              // what is left are rings
-        if (done[i] || dst[i] == src[i]) continue;
-        emit(dst[i], PM_SAVE, dst[i]);
-        for (int j = i; !done[j]; j = op[src[j]]) {
-            done[j] = 1;
-            const bool closes = src[j] == dst[i];
-            emit(dst[j], closes ? PM_SAVED : src[j], closes ? -1 : src[j]);
-        }
-    }
-    // part by part, in the order above within each
-    std::vector<int> by(plan.move.size());
-    std::iota(by.begin(), by.end(), 0);
-    std::stable_sort(by.begin(), by.end(), [&](int a, int b) { return plan.part[a] < plan.part[b]; });
-    PagePlan sorted;
-    for (int i : by) {
-        sorted.move.push_back(plan.move[i]);
-        sorted.part.push_back(plan.part[i]);
-        sorted.hole.push_back(plan.hole[i]);
-    }
-    return sorted;
 }
 
 template <typename Piece, int TENSORS, int MOVES>
@@ -173,28 +114,8 @@ static int launch_moves(const wa_page_tensor *tensors, int n_tensors, const Page
         if (widest == 0 || rows == 0) continue;
         WA_REQUIRE(widest < (1ll << 31) - PM_THREADS * PM_PIECES, WA_ERR_UNSUPPORTED, "%s: pages of more than 2^31 pieces", what);
         const long long gx = (widest + PM_THREADS * PM_PIECES - 1) / (PM_THREADS * PM_PIECES);
-        int reopen = -1;                       // page that holds the kept piece of a ring that the launch before cut
-        for (int m = 0; m < total;) {
-            int n = 0, parts = 0;
-            if (reopen >= 0) p.move[n++] = make_int2(reopen, PM_SAVE);
-            reopen = -1;
-            const int begin = m;
-            int stop = std::min(total, m + MOVES - n);
-            if (stop < total && plan.hole[stop - 1] >= 0) {
-                // a ring is cut: its kept piece goes to a page that is free by then, one that is whole in every tensor
-                --stop;
-                while (stop > begin && plan.hole[stop - 1] >= whole_pages) --stop;
-                WA_REQUIRE(stop > begin, WA_ERR_UNSUPPORTED, "%s: a ring of moves through too many shortened pages", what);
-            }
-            for (; m < stop; ++m) {
-                if (m == begin || plan.part[m] != plan.part[m - 1]) p.part[parts++] = m == begin ? 0 : n;
-                p.move[n++] = plan.move[m];
-            }
-            if (m < total && plan.hole[m - 1] >= 0) {
-                reopen = plan.hole[m - 1];
-                p.move[n++] = make_int2(reopen, PM_SAVED);
-            }
-            p.part[parts] = n;
+        for (PageCut cut; cut.at < total;) {
+            const int parts = next_moves(plan, whole_pages, MOVES, cut, p.move, p.part);
             const cudaError_t e = launch_dependent(move_pages_kernel<Piece, TENSORS, MOVES>, dim3((unsigned)gx, parts, (unsigned)rows), dim3(PM_THREADS), 0, stream, p);
             if (e != cudaSuccess) return fail((int)e, "%s: %s", what, cudaGetErrorString(e));
             const int rc = check_launch(what);
@@ -287,9 +208,9 @@ static int move_pages(const wa_page_tensor *tensors, int n_tensors, const int32_
         WA_REQUIRE(!taken[dst[i]], WA_ERR_ARG, "%s: page %d is the destination of two moves", what, dst[i]);
         taken[dst[i]] = 1;
     }
-    const PagePlan plan = plan_moves(dst, src, n, most);
+    const int whole_pages = (int)std::min<int64_t>(whole, INT32_MAX);      // (`pages` or one less: whole in every tensor)
+    const PagePlan plan = plan_moves(dst, src, n, most, whole_pages);
     if (plan.move.empty()) return 0;
-    const int whole_pages = (int)std::min<int64_t>(whole, INT32_MAX);
     if (bits % 16 == 0) return launch_moves<uint4>(tensors, n_tensors, plan, whole_pages, stream, what);
     if (bits % 4 == 0) return launch_moves<uint32_t>(tensors, n_tensors, plan, whole_pages, stream, what);
     return launch_moves<unsigned char>(tensors, n_tensors, plan, whole_pages, stream, what);
