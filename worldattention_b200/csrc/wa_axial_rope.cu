@@ -30,7 +30,7 @@ struct AxialRope {
     const float2 *table;              // [rows, pairs] (cos, sin)
     float sign;                       // of the angle
     int wide;                         // two neighbouring pairs of a row are 16 bytes: an even number of pairs, an aligned table
-    int groups, groups_of[AR_TENSORS];     // vector form: head groups of all tensors and of each
+    int groups_of[AR_TENSORS];        // vector form: head groups of each tensor
 };
 
 constexpr int ar_groups(bool interleaved) { return interleaved ? 4 : 2; }        // head groups of a warp: four vectors of a lane
@@ -272,7 +272,6 @@ extern "C" int wa_axial_rope(const wa_tensor4 *x, const wa_tensor4 *out, const i
     cudaError_t e;
     if (vec && B <= 65535 && groups <= 65535) {
         const int each = ar_groups(interleaved != 0);
-        p.groups = (int)groups;
         const bool whole = 2 * pairs == D;
         const auto kernel = dtype == WA_BF16 ? (!interleaved ? axial_rope_vec_kernel<__nv_bfloat16, false, true>
                                                 : whole ? axial_rope_vec_kernel<__nv_bfloat16, true, true> : axial_rope_vec_kernel<__nv_bfloat16, true, false>)

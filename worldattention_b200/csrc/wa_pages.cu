@@ -29,7 +29,6 @@ struct PageTensor {
     long long batch_stride, row_stride, page_stride;            // bytes
     long long rows;                                             // tokens of a sample
     int page_rows, row_pieces;                                  // tokens of a page, pieces of a token
-    int batch;
 };
 
 template <int TENSORS, int MOVES>
@@ -105,7 +104,7 @@ static int launch_moves(const wa_page_tensor *tensors, int n_tensors, const Page
             WA_REQUIRE(x.batch <= 65535, WA_ERR_UNSUPPORTED, "%s: more than 65535 samples", what);
             PageTensor &y = p.tensor[p.tensors];
             y.ptr = (char *)x.ptr; y.batch_stride = x.batch_stride; y.row_stride = x.token_stride; y.page_stride = x.token_stride * x.page_tokens;
-            y.rows = x.tokens; y.page_rows = x.page_tokens; y.row_pieces = (int)(x.row_bytes / (int64_t)sizeof(Piece)); y.batch = x.batch;
+            y.rows = x.tokens; y.page_rows = x.page_tokens; y.row_pieces = (int)(x.row_bytes / (int64_t)sizeof(Piece));
             rows += x.batch;
             p.last_of[p.tensors++] = (int)rows;
             widest = std::max(widest, (long long)y.page_rows * y.row_pieces);
