@@ -152,7 +152,7 @@ int wa_block_sparse_forward(const wa_tensor4 *q, const wa_tensor4 *k, const wa_t
  * block_sparse_triton.py:142-382):  S = q k^T D^-1/2,  P = softmax of S over the tokens of the listed blocks,  out = P v, and with
  * delta = sum(dout * out)  dv = P^T dout,  dS = P (dout v^T - delta) D^-1/2,  dq = dS k,  dk = dS^T q.
  * `Hkv` divides `H`; query head h reads key head h / (H / Hkv).  Lists: `[B, H, ceil(Lq / block_size)]` rows, `index_stride` ids apart,
- * of which the first `num` count; an id that is listed twice counts once, one outside the key blocks not at all.  A
+ * of which the first `num` count; an id that is listed twice counts once, one outside the key blocks not at all (but see `as_listed`).  A
  * row without a key gives out = 0, lse = -inf and takes no part in the gradients.  `block_sizes` (device int32 per key block, or null): only the
  * first so many tokens of a block are keys.  One dtype for all tensors; sums, statistics and gradients are accumulated in float32 (bf16:
  * probabilities and dS are rounded to bf16 as factors of the products).  No atomics on values: equal calls give equal bits.
@@ -167,6 +167,8 @@ typedef struct wa_selected_params {
     void *workspace;
     size_t workspace_bytes;
     int32_t *status_mirror;             /* page-locked host word, or null: the site code of a bounded wait that ran out (401 to 499: gradient) */
+    int32_t as_listed;                  /* not 0: lists, and the values of the forward call, as wa_block_sparse_forward has them: an id that is listed twice counts
+                                         * twice, one outside the key blocks is the nearest one */
 } wa_selected_params;
 size_t wa_selected_params_size(void);
 /* 0 for arguments that the call itself refuses. */

@@ -56,7 +56,7 @@ class SelectedParams(C.Structure):  # wa_selected_params
     _fields_ = [(n, C.c_int32) for n in ("B", "H", "Hkv", "D", "Lq", "Lkv", "block_size", "index_stride")] + \
                [(n, Tensor4) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + \
                [(n, C.c_void_p) for n in ("index", "num", "block_sizes", "lse", "workspace")] + \
-               [("workspace_bytes", C.c_size_t), ("status_mirror", C.c_void_p)]
+               [("workspace_bytes", C.c_size_t), ("status_mirror", C.c_void_p), ("as_listed", C.c_int32)]
 
 
 class PageTensor(C.Structure):      # wa_page_tensor

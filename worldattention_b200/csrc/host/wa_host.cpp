@@ -522,14 +522,15 @@ int small_integer(PyObject *o, const char *what) {
     return (int)v;
 }
 
-// ---- attention over selected blocks (hsa/selected.py): q [B, Lq, H, D], k, v [B, Lkv, Hkv, D], index [B, H, Nq, S], num [B, H, Nq], block, block_sizes|None ----
+// ---- attention over selected blocks (hsa/selected.py): q [B, Lq, H, D], k, v [B, Lkv, Hkv, D], index [B, H, Nq, S], num [B, H, Nq], block, block_sizes|None,
+// lists as block_sparse_attention takes them (hsa/block_sparse_torch.py) ----
 struct SelectedCall {
     wa_selected_params p{};
     Tensor keep[9];
     c10::Device dev{c10::kCUDA, 0};
     bool nothing = false;              // no query or no key: no launch
 
-    SelectedCall(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes) {
+    SelectedCall(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes, bool as_listed) {
         bool seen = false;
         for (const Tensor *t : {&q, &k, &v, &index, &num}) require_cuda(*t, dev, seen);
         if (sizes) require_cuda(*sizes, dev, seen);
@@ -547,9 +548,10 @@ struct SelectedCall {
         if (index.dim() != 4 || index.size(0) != B || index.size(1) != H || index.size(2) != nq || num.dim() != 3 || num.size(0) != B || num.size(1) != H || num.size(2) != nq)
             fail(PyExc_ValueError, "index must be [B, H, Nq, ids] and num [B, H, Nq] with Nq = " + std::to_string(nq) + " query blocks, got " + shape_of(index) + " and " + shape_of(num));
         if (index.scalar_type() != at::kInt || num.scalar_type() != at::kInt) fail(PyExc_ValueError, "index and num must be int32");
-        if (sizes && (sizes->dim() != 1 || sizes->size(0) != nkv || sizes->scalar_type() != at::kInt))
+        if (sizes && (sizes->dim() != 1 || (as_listed ? sizes->size(0) < nkv : sizes->size(0) != nkv) || sizes->scalar_type() != at::kInt))
             fail(PyExc_ValueError, "block_sizes must be int32 [" + std::to_string(nkv) + "], got shape " + shape_of(*sizes));
         nothing = B == 0 || Lq == 0 || Lkv == 0 || D == 0 || index.size(3) == 0;
+        p.as_listed = as_listed;
         p.B = (int)B; p.H = (int)H; p.Hkv = (int)Hkv; p.D = (int)D; p.Lq = (int)Lq; p.Lkv = (int)Lkv; p.block_size = block;
         if (index.size(3) > INT_MAX) fail(PyExc_NotImplementedError, "sizes must fit 32 bits");
         p.index_stride = (int)index.size(3);
@@ -576,14 +578,17 @@ struct SelectedCall {
 wa_tensor4 result4(const Tensor &t) { return wa_tensor4{t.data_ptr(), dtype_code(t.scalar_type()), 0, t.stride(0), t.stride(1), t.stride(2)}; }
 
 // -> out [B, Lq, H, D], lse float32 [B, H, Lq]
-std::pair<Tensor, Tensor> selected_run(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes) {
-    SelectedCall c(q, k, v, index, num, block, sizes);
+std::pair<Tensor, Tensor> selected_run(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes,
+                                       bool as_listed) {
+    SelectedCall c(q, k, v, index, num, block, sizes, as_listed);
     raise_if_failed(c.dev.index());
     c10::cuda::CUDAGuard guard(c.dev);
-    const auto options = q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
-    if (c.nothing)
-        return {at::zeros(q.sizes(), q.options().requires_grad(false)), at::full({c.p.B, c.p.H, c.p.Lq}, -INFINITY, q.options().dtype(at::kFloat).requires_grad(false))};
-    Tensor out = at::empty(q.sizes(), options), lse = at::empty({c.p.B, c.p.H, c.p.Lq}, options.dtype(at::kFloat));
+    const auto options = q.options().requires_grad(false);
+    // (as listed: [B, H, Lq, D] in memory, as that call's results lie without gradients)
+    const int64_t B = c.p.B, H = c.p.H, L = c.p.Lq, D = c.p.D;
+    Tensor out = as_listed ? at::empty_strided({B, L, H, D}, {H * L * D, D, L * D, 1}, options) : at::empty(q.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    if (c.nothing) return {out.zero_(), at::full({B, H, L}, -INFINITY, options.dtype(at::kFloat))};
+    Tensor lse = at::empty({B, H, L}, options.dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
     c.p.out = result4(out);
     c.p.lse = lse.data_ptr<float>();
     const Tensor ws = c.workspace_for(false);
@@ -593,8 +598,8 @@ std::pair<Tensor, Tensor> selected_run(const Tensor &q, const Tensor &k, const T
 
 // -> dq, dk, dv
 std::vector<Tensor> selected_gradients(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index, const Tensor &num, int block, const Tensor *sizes,
-                                       const Tensor &out, const Tensor &lse, const Tensor &dout) {
-    SelectedCall c(q, k, v, index, num, block, sizes);
+                                       bool as_listed, const Tensor &out, const Tensor &lse, const Tensor &dout) {
+    SelectedCall c(q, k, v, index, num, block, sizes, as_listed);
     raise_if_failed(c.dev.index());
     bool seen = true;
     for (const Tensor *t : {&out, &lse, &dout}) require_cuda(*t, c.dev, seen);
@@ -649,22 +654,24 @@ void refuse_captured_over_eager(at::TensorList xs) {
 
 struct SelectedNode : torch::autograd::Function<SelectedNode> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &index,
-                                                  const Tensor &num, int64_t block, const std::optional<Tensor> &sizes) {
-        auto [out, lse] = selected_run(q, k, v, index, num, (int)block, sizes ? &*sizes : nullptr);
+                                                  const Tensor &num, int64_t block, const std::optional<Tensor> &sizes, bool as_listed) {
+        auto [out, lse] = selected_run(q, k, v, index, num, (int)block, sizes ? &*sizes : nullptr, as_listed);
         ctx->save_for_backward({q, k, v, index, num, sizes ? *sizes : Tensor(), out, lse});
         ctx->saved_data["block"] = block;
+        ctx->saved_data["as_listed"] = as_listed;
         ctx->mark_non_differentiable({lse});
         ctx->set_materialize_grads(false);
         return {out, lse};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
-        torch::autograd::variable_list result(7);
+        torch::autograd::variable_list result(8);
         if (!grads[0].defined()) return result;
         const auto s = ctx->get_saved_variables();
         torch::autograd::variable_list three;
         try {
             at::NoGradGuard no_grad;
-            three = selected_gradients(s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["block"].toInt(), s[5].defined() ? &s[5] : nullptr, s[6], s[7], grads[0].detach());
+            three = selected_gradients(s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["block"].toInt(), s[5].defined() ? &s[5] : nullptr,
+                                       ctx->saved_data["as_listed"].toBool(), s[6], s[7], grads[0].detach());
         } catch (const PyFailure &) {
             rethrow_on_engine();
         }
@@ -679,20 +686,21 @@ struct SelectedNode : torch::autograd::Function<SelectedNode> {
     }
 };
 
-// q, k, v, index, num, block, block_sizes|None -> (out, lse), with a graph where gradients are asked for
+// q, k, v, index, num, block, block_sizes|None, as listed -> (out, lse), with a graph where gradients are asked for
 PyObject *selected_attention(PyObject *const *a, Py_ssize_t n) {
-    expect_args(n, 7);
+    expect_args(n, 8);
     const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &index = tensor(a[3], "index"), &num = tensor(a[4], "num");
     const int block = small_integer(a[5], "block_size");
     const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
+    const bool as_listed = a[7] == Py_True;
     Tensor out, lse;
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
         refuse_captured_over_eager({q, k, v});
-        auto both = SelectedNode::apply(q, k, v, index, num, (int64_t)block, sizes ? std::optional<Tensor>(*sizes) : std::nullopt);
+        auto both = SelectedNode::apply(q, k, v, index, num, (int64_t)block, sizes ? std::optional<Tensor>(*sizes) : std::nullopt, as_listed);
         out = std::move(both[0]);
         lse = std::move(both[1]);
     } else {
-        std::tie(out, lse) = selected_run(q, k, v, index, num, block, sizes);
+        std::tie(out, lse) = selected_run(q, k, v, index, num, block, sizes, as_listed);
     }
     PyObject *pair = PyTuple_New(2);
     if (!pair) throw PyFailure();

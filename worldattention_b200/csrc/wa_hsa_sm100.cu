@@ -1510,7 +1510,7 @@ int selected_sm100_map(CUtensorMap *map, const wa_tensor4 *t, int B, int L, int 
 }
 bool selected_sm100_tensors(const wa_selected_params *p) {
     using namespace sm100;
-    return p->D == TILE && (p->block_size == TILE || p->block_size == HALF) && !p->block_sizes && view_ok(&p->q) && view_ok(&p->k) && view_ok(&p->v) &&
+    return p->D == TILE && (p->block_size == TILE || p->block_size == HALF) && !p->block_sizes && !p->as_listed && view_ok(&p->q) && view_ok(&p->k) && view_ok(&p->v) &&
            (long long)p->B * p->H * ceil_div(p->Lq, p->block_size) <= (1 << 24) && device_is_sm100() && encode_fn() != nullptr;
 }
 bool selected_sm100_forward_supported(const wa_selected_params *p) { return selected_sm100_tensors(p) && sm100::view_ok(&p->out); }

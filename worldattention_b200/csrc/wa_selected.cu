@@ -10,7 +10,7 @@ namespace wa {
 
 // ---- lists ---------------------------------------------------------------------------------------
 // A warp per list: ids outside the key blocks, of blocks without a key and repeated ones are dropped, the others keep their order (a router's best
-// block first).  So a row without a key has an empty list, and whatever its dout holds meets no product.  For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set
+// block first); `as_listed`, those of blocks without a key alone.  So a row without a key has an empty list, and whatever its dout holds meets no product.  For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set
 // atomically, which is the same in any order.
 constexpr int SL_WARPS = 8, SL_WORDS = 1024;   // lists of a CTA; words of a bitmap up to which it has so many (32 768 key blocks)
 
@@ -18,6 +18,7 @@ struct SelectedLists {
     const int32_t *index, *num, *sizes;                          // sizes: keys of each key block, or null
     long long lists;
     int Nq, Nkv, stride, H, group, words, row_words, warps;      // warps: lists of a CTA
+    int as_listed;
     int32_t *clean, *clean_num;
     uint32_t *rows;                                              // or null
 };
@@ -35,10 +36,11 @@ __device__ __forceinline__ void selected_list(const SelectedLists &p, uint32_t *
     const long long bhk = bh / p.H * (p.H / p.group) + h / p.group;
     int at = 0;
     for (int c = 0; c < n; c += 32) {
-        const int id = c + lane < n ? p.index[list * p.stride + c + lane] : -1;
+        int id = c + lane < n ? p.index[list * p.stride + c + lane] : -1;
+        if (p.as_listed && c + lane < n) id = max(0, min(id, p.Nkv - 1));
         const bool there = (unsigned)id < (unsigned)p.Nkv && (!p.sizes || __ldg(p.sizes + id) > 0);
         const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1 - lane);
-        const bool take = there && lane == __ffs(same) - 1 && !((bits[id >> 5] >> (id & 31)) & 1u);
+        const bool take = there && (p.as_listed || (lane == __ffs(same) - 1 && !((bits[id >> 5] >> (id & 31)) & 1u)));
         __syncwarp();
         const unsigned all = __ballot_sync(0xffffffffu, take);
         if (take) {
@@ -434,6 +436,7 @@ struct SelectedAny {
     long long ob, ol, oh, dqb, dql, dqh, dkb, dkl, dkh, dvb, dvl, dvh;
     int H, group, Lq, Lkv, D, block, stride, Nq, Nkv, row_words, padded, tiles;
     int async;                        // rows of whole 16-byte pieces of float32
+    int as_listed;                    // a query block's list may name a key block more than once
     const int32_t *index, *num, *block_sizes;
     const int32_t *q_order, *k_order; // or null: as they come
     const uint32_t *rows;
@@ -525,13 +528,18 @@ selected_any_kernel(const SelectedAny p) {
 
     // the rows to meet, TG at a time: those of the listed blocks in the order of the list
     struct Rows { int h, from, end; };
-    int at = -1, left_from = 0, left_end = 0, head = 0;
+    int at = -1, left_from = 0, left_end = 0, head = 0, times = 1;        // times: keys, how often the list still names this block
     uint32_t word = 0;
     const long long list = KEYS ? (long long)item * p.group * p.row_words : (long long)item;
     const int n = KEYS ? p.group * p.row_words : p.num[list];
     const auto next = [&](Rows &to) {
         while (left_from >= left_end) {
             if (KEYS) {
+                if (times > 1) {
+                    --times;
+                    left_from = (left_end - 1) / p.block * p.block;
+                    continue;
+                }
                 while (word == 0u) {
                     if (++at >= n) return false;
                     word = p.rows[list + at];
@@ -541,6 +549,12 @@ selected_any_kernel(const SelectedAny p) {
                 head = hk * p.group + at / p.row_words;
                 left_from = i * p.block;
                 left_end = min(left_from + p.block, p.Lq);
+                if (p.as_listed) {
+                    const long long row = ((long long)b * p.H + head) * p.Nq + i;
+                    unsigned named = 0;
+                    for (int e = lane; e < p.num[row]; e += 32) named += p.index[row * p.stride + e] == blk;
+                    times = (int)__reduce_add_sync(0xffffffffu, named);
+                }
             } else {
                 if (++at >= n) return false;
                 const int id = p.index[list * p.stride + at];
@@ -805,7 +819,7 @@ static SelectedPlan selected_plan(const wa_selected_params *p, bool backward) {
     w.row_words = ceil_div(w.Nq, 32);
     const size_t lists = (size_t)p->B * p->H * w.Nq;
     size_t c = 0;
-    if (!backward && selected_few_rows(p)) {       // needs none
+    if (!backward && (p->as_listed || selected_few_rows(p))) {       // needs none
         w.total = 256;
         return w;
     }
@@ -862,6 +876,7 @@ static SelectedLists selected_lists(const wa_selected_params *p, const SelectedP
     l.lists = (long long)p->B * p->H * w.Nq;
     l.Nq = w.Nq; l.Nkv = w.Nkv; l.stride = p->index_stride; l.H = p->H; l.group = w.group; l.words = w.words; l.row_words = w.row_words;
     l.warps = w.words <= SL_WORDS ? SL_WARPS : 1;
+    l.as_listed = p->as_listed;
     l.clean = (int32_t *)(ws + w.index); l.clean_num = (int32_t *)(ws + w.num);
     l.rows = backward ? (uint32_t *)(ws + w.rows) : nullptr;
     return l;
@@ -895,6 +910,7 @@ static SelectedAny selected_any(const wa_selected_params *p, const SelectedPlan 
     g.H = p->H; g.group = w.group; g.Lq = p->Lq; g.Lkv = p->Lkv; g.D = p->D; g.block = p->block_size; g.stride = p->index_stride; g.Nq = w.Nq; g.Nkv = w.Nkv;
     g.index = (const int32_t *)(ws + w.index); g.num = (const int32_t *)(ws + w.num); g.block_sizes = p->block_sizes;
     g.scale = (float)(1.0 / sqrt((double)p->D));
+    g.as_listed = p->as_listed;
     g.async = p->D % 4 == 0 && whole_pieces(p->q) && whole_pieces(p->k) && whole_pieces(p->v);
     return g;
 }
@@ -917,6 +933,9 @@ extern "C" int wa_selected_forward(const wa_selected_params *p, void *stream_) {
     const SelectedPlan w = selected_plan(p, false);
     WA_REQUIRE(p->workspace && p->workspace_bytes >= w.total, WA_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes, got %zu", what, w.total, p->workspace_bytes);
     WA_REQUIRE((uintptr_t)p->workspace % 256 == 0, WA_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", what);
+    if (p->as_listed)
+        return block_sparse_run(&p->q, &p->k, &p->v, &p->out, p->B, p->H, p->Lq, p->Lkv, p->D, p->block_size, p->index, p->num, p->index_stride, p->block_sizes, 0, 0,
+                                p->lse, nullptr, false, stream, w.group, true);
     if (selected_few_rows(p)) return launch_few_rows(p, stream);
     char *ws = (char *)p->workspace;
     int32_t *index = (int32_t *)(ws + w.index), *num = (int32_t *)(ws + w.num);

@@ -10,7 +10,6 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .selected import selected_attention
 
 __all__ = ["block_sparse_attention_reference"]
 
@@ -19,8 +18,8 @@ def block_sparse_attention_reference(q, k, v, q2k_index, q2k_num, block_sizes, b
                                      return_lse: bool = False):
     """Attention over selected blocks for `[B, H, N, D]` inputs padded to `block_size`.
 
-    With gradients enabled and asked for, the result carries them to q, k and v (`selected_attention`: lists are then taken as
-    sets, an id named twice counts once and one that is no key block not at all; there are no gradients above head_dim 256)."""
+    With gradients enabled and asked for, the result carries them to q, k and v; its values are those without.  Either way the lists
+    are taken as they are: an id named twice counts twice, one that is no key block is the nearest one."""
     dev = _lib.require_cuda(q, k, v, q2k_index, q2k_num, block_sizes)
     bsz, heads, q_tokens, head_dim = q.shape
     kv_tokens = k.shape[2]
@@ -29,8 +28,8 @@ def block_sparse_attention_reference(q, k, v, q2k_index, q2k_num, block_sizes, b
     k = k.to(q.dtype)
     v = v.to(q.dtype)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = selected_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), q2k_index.to(torch.int32), q2k_num.to(torch.int32),
-                                      block_size, block_sizes=block_sizes.to(torch.int32), return_lse=True)
+        out, lse = _lib.host().selected_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), q2k_index.to(torch.int32),
+                                                  q2k_num.to(torch.int32), block_size, block_sizes.to(torch.int32), True)
         out = out.transpose(1, 2)
         return (out, lse) if return_lse else out
     out = torch.empty((bsz, heads, q_tokens, head_dim), device=dev, dtype=q.dtype)

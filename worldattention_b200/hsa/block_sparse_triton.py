@@ -4,7 +4,7 @@
 `map_to_index(block_map)` keep the signatures of wan/modules/hsa/block_sparse_triton.py:44-57,
 371-382.  No Triton is involved: the module name is kept only so that code importing the
 reference's backend module keeps working.  Gradients reach q, k and v where they are asked for
-(block_sparse_triton.py:142-382), through `selected_attention`.
+(block_sparse_triton.py:142-382).
 """
 from __future__ import annotations
 

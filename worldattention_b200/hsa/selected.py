@@ -29,5 +29,5 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     gradient of the gradient is not offered.  A step can be captured into a CUDA graph, its backward pass included, unless an eager graph of the
     same leaves from the default stream is still alive (refused).
     """
-    out, lse = _lib.host().selected_attention(q, k, v, index, num, block_size, block_sizes)
+    out, lse = _lib.host().selected_attention(q, k, v, index, num, block_size, block_sizes, False)
     return (out, lse) if return_lse else out
