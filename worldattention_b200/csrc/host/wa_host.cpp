@@ -522,6 +522,12 @@ int small_integer(PyObject *o, const char *what) {
     return (int)v;
 }
 
+// Tangents of forward-mode derivatives are not carried: a call that has one is refused, where it would be lost without a word.
+void refuse_tangents(at::TensorList xs) {
+    for (const Tensor &x : xs)
+        if (x._fw_grad(/*level=*/0).defined()) fail(PyExc_NotImplementedError, "forward-mode derivatives are not offered: a tensor of the call has a tangent");
+}
+
 // ---- attention over selected blocks (hsa/selected.py): q [B, Lq, H, D], k, v [B, Lkv, Hkv, D], index [B, H, Nq, S], num [B, H, Nq], block, block_sizes|None,
 // lists as block_sparse_attention takes them (hsa/block_sparse_torch.py) ----
 struct SelectedCall {
@@ -693,6 +699,7 @@ PyObject *selected_attention(PyObject *const *a, Py_ssize_t n) {
     const int block = small_integer(a[5], "block_size");
     const Tensor *sizes = tensor_or_null(a[6], "block_sizes");
     const bool as_listed = a[7] == Py_True;
+    refuse_tangents({q, k, v});
     Tensor out, lse;
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
         refuse_captured_over_eager({q, k, v});
@@ -789,6 +796,8 @@ struct AxialNode : torch::autograd::Function<AxialNode> {
 };
 
 std::vector<Tensor> axial_turn(const std::vector<Tensor> &xs, const Tensor &pos, const Tensor &table, const std::vector<int64_t> &axes, bool interleaved, bool inverse) {
+    refuse_tangents(xs);
+    refuse_tangents(table);
     if (at::GradMode::is_enabled() && table.requires_grad()) fail(PyExc_ValueError, "the table has no gradient: it must not require one");
     if (at::GradMode::is_enabled() && std::any_of(xs.begin(), xs.end(), [](const Tensor &x) { return x.requires_grad(); })) {
         refuse_captured_over_eager(xs);
@@ -841,6 +850,7 @@ PyObject *move_pages(PyObject *const *a, Py_ssize_t n) {
         require_cuda(x, dev, seen);
         if (x.dim() < 2) fail(PyExc_ValueError, "expected [B, tokens, ...] tensors, got shape " + shape_of(x));
         if (lengths[t] <= 0) fail(PyExc_ValueError, "page_tokens must be positive");
+        refuse_tangents(x);
         if (x.requires_grad() && at::GradMode::is_enabled())
             fail(PyExc_RuntimeError, "pages are moved in place: a tensor that requires a gradient cannot be moved with gradients enabled");
         int64_t row = 1;
