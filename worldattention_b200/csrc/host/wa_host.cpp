@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -22,6 +23,7 @@
 #include <list>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "../../../include/worldattention_b200.h"
@@ -643,18 +645,40 @@ std::vector<Tensor> selected_gradients(const Tensor &q, const Tensor &k, const T
 
 // A captured backward pass ends at its leaves.  A leaf that an eager graph still leads to keeps that graph's stream; where that is the default
 // stream, the engine makes it wait for the captured one, which is no legal step of a capture and ends the process.  So such a call is
-// refused while that can still be an exception.  Leaves are looked for directly and through views and other nodes of one input.
+// refused while that can still be an exception: at once where a leaf is an input, or one seen through views and other nodes of one input, and in the
+// backward pass, before a gradient leaves this node, for every leaf that the pass will reach from here.
+bool capturing() { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; }
+void refuse_eager_leaf(torch::autograd::Node &node) {
+    const auto stream = node.stream();
+    if (stream && stream->device_type() == c10::kCUDA && *stream == at::cuda::getDefaultCUDAStream(stream->device_index()).unwrap())
+        fail(PyExc_RuntimeError, "a training step cannot be captured while an eager graph of the same leaves, made on the default stream, is alive: drop its "
+                                 "results first, or make it on a side stream");
+}
 void refuse_captured_over_eager(at::TensorList xs) {
-    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    if (!capturing()) return;
     for (const Tensor &x : xs) {
         if (!x.requires_grad()) continue;
         std::shared_ptr<torch::autograd::Node> node = x.grad_fn() ? x.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(x);
         while (node && node->num_outputs() == 1) node = node->next_edge(0).function;
-        if (!node || node->num_outputs() != 0) continue;
-        const auto stream = node->stream();
-        if (stream && *stream == at::cuda::getDefaultCUDAStream(x.device().index()).unwrap())
-            fail(PyExc_RuntimeError, "a training step cannot be captured while an eager graph of the same leaves, made on the default stream, is alive: drop its "
-                                     "results first, or make it on a side stream");
+        if (node && node->num_outputs() == 0) refuse_eager_leaf(*node);
+    }
+}
+void refuse_captured_backward_over_eager() {
+    if (!capturing()) return;
+    const auto *tasks = torch::autograd::get_current_graph_task_exec_info();      // empty: everything is executed
+    std::unordered_set<const torch::autograd::Node *> seen;
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo{torch::autograd::get_current_node()};
+    while (!todo.empty()) {
+        const auto node = todo.back();
+        todo.pop_back();
+        if (!node || !seen.insert(node.get()).second) continue;
+        if (seen.size() > 1 && tasks && !tasks->empty()) {
+            const auto task = tasks->find(node.get());
+            if (task == tasks->end() || !task->second.should_execute()) continue;
+            if (!task->second.needed_ && node->num_outputs() != 0) continue;      // its gradient is wanted, and none behind it
+        }
+        if (node->num_outputs() == 0) refuse_eager_leaf(*node);
+        for (const auto &edge : node->next_edges()) todo.push_back(edge.function);
     }
 }
 
@@ -675,6 +699,7 @@ struct SelectedNode : torch::autograd::Function<SelectedNode> {
         const auto s = ctx->get_saved_variables();
         torch::autograd::variable_list three;
         try {
+            refuse_captured_backward_over_eager();
             at::NoGradGuard no_grad;
             three = selected_gradients(s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["block"].toInt(), s[5].defined() ? &s[5] : nullptr,
                                        ctx->saved_data["as_listed"].toBool(), s[6], s[7], grads[0].detach());
@@ -702,7 +727,7 @@ PyObject *selected_attention(PyObject *const *a, Py_ssize_t n) {
     refuse_tangents({q, k, v});
     Tensor out, lse;
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
-        refuse_captured_over_eager({q, k, v});
+        if (!as_listed) refuse_captured_over_eager({q, k, v});      // (a forward pass alone was captured before that call carried gradients)
         auto both = SelectedNode::apply(q, k, v, index, num, (int64_t)block, sizes ? std::optional<Tensor>(*sizes) : std::nullopt, as_listed);
         out = std::move(both[0]);
         lse = std::move(both[1]);
@@ -786,6 +811,7 @@ struct AxialNode : torch::autograd::Function<AxialNode> {
             }
         if (there.empty()) return result;
         try {
+            refuse_captured_backward_over_eager();
             const auto turned = axial_turn(there, s[0], s[1], ctx->saved_data["axes"].toIntVector(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool());
             for (size_t i = 0; i < at.size(); ++i) result[at[i]] = turned[i];
         } catch (const PyFailure &) {

@@ -26,8 +26,8 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
 
     `return_lse`: also the natural-log normalisers, float32 `[B, H, Lq]` (not differentiable).  Sums and statistics are float32; in bf16 the
     probabilities and dS are rounded to bf16 where they are factors of a product.  Equal calls give equal bits, gradients included.  The
-    gradient of the gradient is not offered.  A step can be captured into a CUDA graph, its backward pass included, unless an eager graph of the
-    same leaves from the default stream is still alive (refused).
+    gradient of the gradient is not offered, nor are forward-mode derivatives.  A step can be captured into a CUDA graph, its backward pass included, unless
+    an eager graph of the same leaves from the default stream is still alive (refused).
     """
     out, lse = _lib.host().selected_attention(q, k, v, index, num, block_size, block_sizes, False)
     return (out, lse) if return_lse else out
