@@ -527,7 +527,7 @@ int small_integer(PyObject *o, const char *what) {
 // Tangents of forward-mode derivatives are not carried: a call that has one is refused, where it would be lost without a word.
 void refuse_tangents(at::TensorList xs) {
     for (const Tensor &x : xs)
-        if (x._fw_grad(/*level=*/0).defined()) fail(PyExc_NotImplementedError, "forward-mode derivatives are not offered: a tensor of the call has a tangent");
+        if (torch::autograd::impl::get_autograd_meta(x) && x._fw_grad(/*level=*/0).defined()) fail(PyExc_NotImplementedError, "forward-mode derivatives are not offered: a tensor of the call has a tangent");
 }
 
 // ---- attention over selected blocks (hsa/selected.py): q [B, Lq, H, D], k, v [B, Lkv, Hkv, D], index [B, H, Nq, S], num [B, H, Nq], block, block_sizes|None,

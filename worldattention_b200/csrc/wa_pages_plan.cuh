@@ -16,13 +16,14 @@ namespace wa {
 
 constexpr int PM_CLEAR = -1, PM_SAVED = -2, PM_SAVE = -3;      // sources that are no page: zeros, the kept piece; keep a piece of `to`
 
-struct PageMove {
+struct alignas(8) PageMove {
     int to, from;
 };
 
 struct PagePlan {
     std::vector<PageMove> move;
     std::vector<int> part, hole;       // of each move: its part, and the page that the kept piece may be put back to behind it (-1: none is kept)
+    explicit PagePlan(size_t most) { move.reserve(most), part.reserve(most), hole.reserve(most); }
 };
 
 // `pages`: one more than the largest page number.  Pages from `whole` on, at most one, may be shorter.
@@ -40,7 +41,7 @@ inline PagePlan plan_moves(const int *dst, const int *src, int n, int pages, int
             ++readers[src[i]];
             if (op[src[i]] >= 0) root[find(dst[i])] = find(src[i]);
         }
-    PagePlan plan;
+    PagePlan plan(n + n / 2);                  // (a ring of two or more is a move longer)
     std::vector<char> done(n, 0);
     auto emit = [&](int d, int s, int hole) {
         plan.move.push_back(PageMove{d, s});
@@ -70,7 +71,7 @@ inline PagePlan plan_moves(const int *dst, const int *src, int n, int pages, int
     std::vector<int> by(plan.move.size());
     std::iota(by.begin(), by.end(), 0);
     std::stable_sort(by.begin(), by.end(), [&](int a, int b) { return plan.part[a] < plan.part[b]; });
-    PagePlan sorted;
+    PagePlan sorted(by.size());
     for (int i : by) {
         sorted.move.push_back(plan.move[i]);
         sorted.part.push_back(plan.part[i]);
