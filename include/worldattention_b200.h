@@ -157,7 +157,10 @@ int wa_block_sparse_forward(const wa_tensor4 *q, const wa_tensor4 *k, const wa_t
  * first so many tokens of a block are keys.  One dtype for all tensors; sums, statistics and gradients are accumulated in float32 (bf16:
  * probabilities and dS are rounded to bf16 as factors of the products).  No atomics on values: equal calls give equal bits.
  * `lse` float32 `[B, H, Lq]`, natural logarithm: written by the forward call (or null), read by the backward call.
- * bf16 with head_dim 128 and blocks of 64 or 128 tokens runs on the tensor cores; head_dim is at most 256. */
+ * bf16 with head_dim 128 and blocks of 64 or 128 tokens runs on the tensor cores (tcgen05) where `block_sizes` is null, `as_listed` is 0 and all
+ * tensors have 16-byte aligned rows and positive strides between tokens and between heads (key heads expanded with a stride of 0 have none).  Anything else
+ * runs on multiply-adds in float32 (forward with head_dim 128, in bf16 or with `block_sizes`: warp-level matrix instructions).  head_dim is at most 256.
+ * What is attended to and no number shows in all results that depend on it, and only there. */
 typedef struct wa_selected_params {
     int32_t B, H, Hkv, D, Lq, Lkv, block_size, index_stride;
     wa_tensor4 q, k, v, out;            /* forward; backward reads all four */

@@ -4,9 +4,8 @@
 // causal_model.py:331-360) is the one that moves every page to the front.  No scratch and no order between thread blocks is needed:
 // whatever happens to one 16-byte piece of a page happens to the same piece of every page, independently of all other pieces.  So
 // a thread takes a piece (its place within a page) and runs a short list of page numbers over it: load from the source pages,
-// store to the destinations.  The host puts a list into an order in which no page is overwritten before it has been read for the last
-// time (a page that is read by several comes after them, a ring of pages keeps one piece in registers), and splits it
-// into parts that share no page that is both read and written; parts run side by side.
+// store to the destinations.  The host puts a list into an order in which that can be done and splits it into parts that run side by side
+// (wa_pages_plan.cuh).
 //
 // Bound: HBM, every moved page is read once and written once.  A thread has four pieces of one move in flight and makes the moves of a part one
 // after the other: the loads of several moves at a time touch as many more pages, which DRAM takes badly (60 tensors of 21 pages of 4.8 MB,

@@ -10,8 +10,10 @@ namespace wa {
 
 // ---- lists ---------------------------------------------------------------------------------------
 // A warp per list: ids outside the key blocks, of blocks without a key and repeated ones are dropped, the others keep their order (a router's best
-// block first); `as_listed`, those of blocks without a key alone.  So a row without a key has an empty list, and whatever its dout holds meets no product.  For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set
-// atomically, which is the same in any order.
+// block first).  `as_listed`: repeated ids stay, those outside become the nearest block, only blocks without a key are dropped.  So a row without a
+// key has an empty list, and whatever its dout holds meets no product.
+// For the gradient the same ids turned around: bit i of `rows` of a key block says that query block i lists it.  Bits are set atomically, which is
+// the same in any order; how often a list names the block is counted where it is met.
 constexpr int SL_WARPS = 8, SL_WORDS = 1024;   // lists of a CTA; words of a bitmap up to which it has so many (32 768 key blocks)
 
 struct SelectedLists {
@@ -85,8 +87,9 @@ selected_order_kernel(const int32_t *__restrict__ num, const uint32_t *__restric
 // Single tokens, or up to eight rows of one query block, bf16 with head_dim 128: no tensor-core tile would be filled, and what counts is how soon the
 // listed keys and values are read.  A cluster of up to eight CTAs shares a (batch, head)'s list.  Four tokens are half a warp's step: each
 // token's 256 bytes are its 16 lanes' 16-byte loads, four of keys and four of values on their way at a time (eight of each take the registers of
-// a third CTA per SM: 12.9 -> 18.5 us); scores by shuffles, a running maximum and sum per half warp, and the halves, warps and CTAs are joined at the end in a fixed order through shared memory and the
-// cluster's.  Every CTA cleans the list for itself (a launch less).  Float32 throughout, nothing is rounded but the result.
+// a third CTA per SM: 12.9 -> 18.5 us).  Scores by shuffles, a running maximum and sum per half warp; halves, warps and CTAs are joined at the end in
+// a fixed order, through shared memory and the cluster's.  Every CTA cleans the list for itself (a launch less).  Float32 throughout, nothing is
+// rounded but the result.
 constexpr int SR_WARPS = 8, SR_STEP = 4, SR_IDS = 1024, SR_WORDS = 1024;      // tokens of a step; longest list and bitmap (32 768 key blocks)
 
 __device__ __forceinline__ float sr_exp2(float x) {

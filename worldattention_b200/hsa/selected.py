@@ -22,7 +22,12 @@ def selected_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     `Nq = ceil(Lq / block_size)`) are the lists, as `build_block_routing` gives them: the first `num` ids of a row.  Lists are taken
     as sets: an id named twice counts once, an id that is no key block counts nothing.  Rows whose list is empty give zeros (and
     -inf as log-sum-exp) and have no part in the gradients.  `block_sizes` (int32 `[Nkv]`): only the first so many
-    tokens of a block are keys, as in `block_sparse_attention`; what lies behind them is not read.
+    tokens of a block are keys, as in `block_sparse_attention`; what lies behind them is not read, and its gradients are zero.
+
+    A NaN, or an infinite score, in what a row attends to shows in the row's result and normaliser and in the gradients that depend on it.
+
+    The tensor cores (tcgen05) take bf16 with head_dim 128 and blocks of 64 or 128 without `block_sizes`, 16-byte aligned rows and positive strides between
+    tokens and heads; other calls, key heads expanded with a stride of 0 among them, run on float32 multiply-adds, which take many times as long.
 
     `return_lse`: also the natural-log normalisers, float32 `[B, H, Lq]` (not differentiable).  Sums and statistics are float32; in bf16 the
     probabilities and dS are rounded to bf16 where they are factors of a product.  Equal calls give equal bits, gradients included.  The
